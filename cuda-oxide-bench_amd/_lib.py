@@ -55,6 +55,14 @@ SIGNATURES: dict[str, tuple] = {
     "mx_gemm_bf16_batched": (_i, [_vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _i, _ll, _ll, _ll, _vp]),
     "mx_mla_decode_absorbed": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _f, _vp, _sz, _vp]),
     "mx_mla_decode_absorbed_workspace": (_sz, [_i, _i, _i]),
+    "mx_quant_int8": (_i, [_vp, _vp, _vp, _i, _i, _i, _i, _vp]),
+    "mx_gemm_int8": (_i, [_vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _vp]),
+    "mx_linear_int8": (_i, [_vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _vp, _sz, _vp]),
+    "mx_linear_int8_workspace": (_sz, [_i, _i]),
+    "mx_kv8_append": (_i, [_vp] * 9 + [_i] * 11 + [_vp]),
+    "mx_kv8_copy_pages": (_i, [_vp] * 6 + [_i] * 5 + [_vp]),
+    "mx_gqa_kv8": (_i, [_vp] * 9 + [_i] * 11 + [_f, _i, _i, _vp, _sz, _vp]),
+    "mx_gqa_kv8_workspace": (_sz, [_i] * 7),
 }
 
 

@@ -1,0 +1,274 @@
+// The paged 8-bit cache: new keys and values quantised into it, pages copied.
+//
+// A page of a head has one scale for K and one for V, a power of two s, and holds
+// e4m3 codes with value = code * s.  When new tokens reach a page, with a = their
+// largest finite magnitude,
+//     s = max(s_old, 2^ceil(log2(a / 448)), 2^-32)   (s_old only if the page holds
+//                                                    tokens before them)
+//     kept codes = e4m3(code * s_old / s),   new codes = e4m3(x / s)
+// Both quotients are by powers of two, so they are exact in fp32 and each code is
+// rounded once, to nearest even.  e4m3 has 18 binades: a scale between two
+// powers of two would place the largest value better in its last binade, and
+// lose or gain nothing else.
+#include "kv8_common.h"
+
+namespace mx {
+namespace kv8 {
+
+constexpr float kLeast = 0x1p-32f;
+
+// 2^ceil(log2(a / 448)) for the magnitude bits of a finite bf16 / f16: 448 = 1.75 * 2^8.
+template <typename T>
+__device__ __forceinline__ float scale_for(uint32_t magnitude) {
+  const uint32_t b = __float_as_uint(T::to_f32(magnitude));
+  const int e = (int)(b >> 23) - 127 - 8 + ((b & 0x7fffffu) > 0x600000u ? 1 : 0);  // 1.75 = 1 + 0x600000 / 2^23
+  return fmaxf(__uint_as_float((uint32_t)(max(e, -32) + 127) << 23), kLeast);
+}
+
+template <typename T>
+__device__ __forceinline__ constexpr uint32_t first_nonfinite() {
+  return std::is_same<T, BF16>::value ? 0x7f80u : 0x7c00u;
+}
+
+// Two codes of finite values or NaN (|x| <= 448).
+__device__ __forceinline__ uint32_t codes2(float a, float b) {
+  return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false) & 0xffffu;
+}
+
+// One code at another scale; NaN stays the NaN that it is.
+__device__ __forceinline__ uint8_t moved(uint8_t code, float ratio) {
+  if ((code & 0x7f) == 0x7f) return code;
+  return (uint8_t)codes2(__builtin_amdgcn_cvt_f32_fp8(code, 0) * ratio, 0.f);
+}
+
+// One workgroup per (page that new tokens reach, head): it reads them once, 4 tokens
+// by 8 channels a thread, and keeps them in registers from the maximum to the
+// codes.  K's codes go out 8 bytes a token; V's pass through LDS, 4 tokens
+// packed in a dword, so that its transposed rows are written 16 bytes (16
+// tokens) at a time where they are all new.
+template <typename T, int D, int LP>
+__global__ __launch_bounds__(256) void append_kernel(const uint16_t* __restrict__ knew, const uint16_t* __restrict__ vnew,
+                                                     uint8_t* __restrict__ kc, uint8_t* __restrict__ vc,
+                                                     float* __restrict__ ks, float* __restrict__ vs,
+                                                     const int* __restrict__ table, const int* __restrict__ lens,
+                                                     const int* __restrict__ cu, int n_kv, int T_, int pages,
+                                                     int max_pages, int k_stride, int v_stride) {
+  constexpr int P = 1 << LP;
+  constexpr int UNITS = P * D / 32;  // 4 tokens x 8 channels
+  constexpr int NT = UNITS < 64 ? 64 : UNITS < 256 ? UNITS : 256;
+  constexpr int U = (UNITS + NT - 1) / NT;
+  constexpr int VROW = P + 4;  // bytes of a V row in LDS
+  __shared__ __align__(16) uint8_t vt[D * VROW];
+  __shared__ uint32_t red[2][NT / 64];
+
+  const int t = threadIdx.x;
+  const int h = blockIdx.x % n_kv, b = blockIdx.x / n_kv;
+  const int len = cut_len(lens[b], max_pages, LP);
+  const Rows rows = rows_of(cu, b, T_);
+  const int n = rows.last - rows.first;
+  if (n == 0) return;
+  const int start = len - n;  // position of the first new token; below 0 where there are more rows than tokens
+  const int j_end = (len - 1) >> LP;
+  for (int j = (max(start, 0) >> LP) + blockIdx.y; j <= j_end; j += gridDim.y) {
+    const int page = page_of(table + (size_t)b * max_pages, j << LP, LP, max_pages, pages);
+    if (page < 0) continue;
+    const int lo = max(start - (j << LP), 0), hi = min(len - (j << LP), P);  // the new tokens' slots
+    const int row0 = rows.first + (j << LP) - start;                       // the row of slot 0
+    const size_t at = (size_t)page * n_kv + h;
+
+    u32x4 x[2][U][4];
+    uint32_t mx[2] = {0, 0};
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int unit = t + u * NT, s0 = unit / (D / 8) * 4, c0 = unit % (D / 8) * 8;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const bool in = unit < UNITS && s0 + i >= lo && s0 + i < hi;
+        x[0][u][i] = x[1][u][i] = u32x4{};
+        if (in) {
+          x[0][u][i] = ld128(knew + (size_t)(row0 + s0 + i) * k_stride + h * D + c0);
+          x[1][u][i] = ld128(vnew + (size_t)(row0 + s0 + i) * v_stride + h * D + c0);
+        }
+      }
+    }
+#pragma unroll
+    for (int kv = 0; kv < 2; ++kv)
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int w = 0; w < 4; ++w) {
+            const uint32_t lo16 = x[kv][u][i][w] & 0x7fffu, hi16 = (x[kv][u][i][w] >> 16) & 0x7fffu;
+            if (lo16 < first_nonfinite<T>()) mx[kv] = max(mx[kv], lo16);
+            if (hi16 < first_nonfinite<T>()) mx[kv] = max(mx[kv], hi16);
+          }
+    const float was[2] = {ks[at], vs[at]};
+#pragma unroll
+    for (int kv = 0; kv < 2; ++kv) {
+#pragma unroll
+      for (int off = 1; off < 64; off <<= 1) mx[kv] = max(mx[kv], (uint32_t)__shfl_xor((int)mx[kv], off, 64));
+      if ((t & 63) == 0) red[kv][t >> 6] = mx[kv];
+    }
+    __syncthreads();  // also: every thread has read the page's scales
+    float now[2];
+#pragma unroll
+    for (int kv = 0; kv < 2; ++kv) {
+      uint32_t m = 0;
+#pragma unroll
+      for (int w = 0; w < NT / 64; ++w) m = max(m, red[kv][w]);
+      now[kv] = scale_for<T>(m);
+      if (lo > 0) now[kv] = fmaxf(now[kv], was[kv]);
+    }
+    if (t == 0) {
+      ks[at] = now[0];
+      vs[at] = now[1];
+    }
+    uint8_t* kp = kc + at * (P * D);
+    uint8_t* vp = vc + at * (P * D);
+
+    // codes before the new ones, where the scale grew
+    if (lo > 0 && now[0] != was[0]) {
+      const float ratio = was[0] / now[0];
+      for (int i = t; i < lo * D; i += NT) kp[i] = moved(kp[i], ratio);
+    }
+    if (lo > 0 && now[1] != was[1]) {
+      const float ratio = was[1] / now[1];
+      for (int i = t; i < lo * D; i += NT) {
+        uint8_t* p = vp + (size_t)(i % D) * P + i / D;
+        *p = moved(*p, ratio);
+      }
+    }
+
+    const float r[2] = {1.0f / now[0], 1.0f / now[1]};
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int unit = t + u * NT, s0 = unit / (D / 8) * 4, c0 = unit % (D / 8) * 8;
+      if (unit >= UNITS || s0 >= hi || s0 + 4 <= lo) continue;
+      uint32_t code[2][4][2];  // [K, V][token][8 channels]
+#pragma unroll
+      for (int kv = 0; kv < 2; ++kv)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int w = 0; w < 4; ++w) {
+            const uint32_t v = x[kv][u][i][w];
+            float a = T::to_f32(v & 0xffffu) * r[kv], c = T::to_f32(v >> 16) * r[kv];
+            if ((v & 0x7fffu) >= first_nonfinite<T>()) a = __builtin_nanf("");
+            if (((v >> 16) & 0x7fffu) >= first_nonfinite<T>()) c = __builtin_nanf("");
+            const uint32_t two = codes2(a, c);
+            code[kv][i][w >> 1] = (w & 1) ? code[kv][i][w >> 1] | two << 16 : two;
+          }
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (s0 + i >= lo && s0 + i < hi) st64(kp + (s0 + i) * D + c0, u32x2{code[0][i][0], code[0][i][1]});
+#pragma unroll
+      for (int c = 0; c < 8; ++c) {
+        uint32_t w = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w |= ((code[1][i][c >> 2] >> (8 * (c & 3))) & 0xffu) << (8 * i);
+        *reinterpret_cast<uint32_t*>(vt + (c0 + c) * VROW + s0) = w;
+      }
+    }
+    __syncthreads();
+    for (int i = t; i < D * (P / 16); i += NT) {
+      const int c = i / (P / 16), s0 = i % (P / 16) * 16;
+      if (s0 >= hi || s0 + 16 <= lo) continue;
+      const uint32_t* src = reinterpret_cast<const uint32_t*>(vt + c * VROW + s0);
+      uint8_t* dst = vp + c * P + s0;
+      if (s0 >= lo && s0 + 16 <= hi) {
+        st128(dst, u32x4{src[0], src[1], src[2], src[3]});
+      } else {
+        for (int k = max(lo - s0, 0); k < min(hi - s0, 16); ++k) dst[k] = (uint8_t)(src[k >> 2] >> (8 * (k & 3)));
+      }
+    }
+    __syncthreads();  // vt and red serve the next page
+  }
+}
+
+// Pairs of pages: PIECE bytes of a page's K or V codes per workgroup, 16 bytes a
+// thread and load; the first of a page's workgroups takes the scales too.
+constexpr int COPY_NT = 256, COPY_U = 4, PIECE = COPY_NT * COPY_U * 16;
+__global__ __launch_bounds__(COPY_NT) void copy_kernel(uint8_t* kc, uint8_t* vc, float* ks, float* vs,
+                                                       const int* __restrict__ src, const int* __restrict__ dst,
+                                                       int n_kv, uint32_t bytes, int pieces, int pages) {
+  const int i = blockIdx.x / (2 * pieces), part = blockIdx.x % (2 * pieces);
+  const int from = src[i], to = dst[i];
+  if (from < 0 || from >= pages || to < 0 || to >= pages || from == to) return;
+  const bool v = part >= pieces;
+  const uint32_t base = (uint32_t)(v ? part - pieces : part) * PIECE + threadIdx.x * 16;
+  const uint8_t* a = (v ? vc : kc) + (size_t)from * bytes;
+  uint8_t* b = (v ? vc : kc) + (size_t)to * bytes;
+  u32x4 x[COPY_U];
+#pragma unroll
+  for (int u = 0; u < COPY_U; ++u)
+    if (base + u * COPY_NT * 16 < bytes) x[u] = ld128(a + base + u * COPY_NT * 16);
+#pragma unroll
+  for (int u = 0; u < COPY_U; ++u)
+    if (base + u * COPY_NT * 16 < bytes) st128(b + base + u * COPY_NT * 16, x[u]);
+  if (part == 0)
+    for (int h = threadIdx.x; h < n_kv; h += COPY_NT) {
+      ks[(size_t)to * n_kv + h] = ks[(size_t)from * n_kv + h];
+      vs[(size_t)to * n_kv + h] = vs[(size_t)from * n_kv + h];
+    }
+}
+
+template <typename T, int D, int LP>
+static int launch_append(const void* k, const void* v, void* kc, void* vc, float* ks, float* vs, const int* table,
+                         const int* lens, const int* cu, int B, int T_, int reach, int n_kv, int pages, int max_pages,
+                         int k_stride, int v_stride, hipStream_t s) {
+  constexpr int UNITS = (D << LP) / 32;
+  constexpr int NT = UNITS < 64 ? 64 : UNITS < 256 ? UNITS : 256;
+  hipLaunchKernelGGL((append_kernel<T, D, LP>), dim3((unsigned)(B * n_kv), (unsigned)reach), dim3(NT), 0, s,
+                     (const uint16_t*)k, (const uint16_t*)v, (uint8_t*)kc, (uint8_t*)vc, ks, vs, table, lens, cu, n_kv,
+                     T_, pages, max_pages, k_stride, v_stride);
+  MX_RETURN_IF_HIP(hipGetLastError());
+  return MX_OK;
+}
+
+}  // namespace kv8
+}  // namespace mx
+
+extern "C" int mx_kv8_append(const void* k, const void* v, void* k_cache, void* v_cache, float* k_scale, float* v_scale,
+                             const int* page_table, const int* kv_lens, const int* cu, int B, int T, int max_q, int n_kv,
+                             int d, int page, int pages, int max_pages, int k_stride, int v_stride, int dtype,
+                             void* stream) {
+  using namespace mx::kv8;
+  if (!k || !v || !page_table || !kv_lens) return MX_ERR_NULL;
+  const int rc = check_cache(k_cache, v_cache, k_scale, v_scale, n_kv, d, page, pages);
+  if (rc != MX_OK) return rc;
+  if (B <= 0 || T <= 0 || max_q <= 0 || max_pages <= 0 || (!cu && T != B)) return MX_ERR_SHAPE;
+  if ((long long)B * n_kv > (1 << 24)) return MX_ERR_SHAPE;
+  if (k_stride < n_kv * d || v_stride < n_kv * d) return MX_ERR_SHAPE;
+  if (k_stride % 8 || v_stride % 8 || (((uintptr_t)k | (uintptr_t)v) & 15)) return MX_ERR_ALIGN;
+  if (dtype != MX_DTYPE_BF16 && dtype != MX_DTYPE_F16) return MX_ERR_DTYPE;
+  const int lp = log2_page(page);
+  // pages that max_q consecutive tokens can reach
+  const long long most = ((long long)(max_q < T ? max_q : T) + page - 2) / page + 1;
+  const int reach = (int)(most < 65535 ? most : 65535);
+  hipStream_t s = (hipStream_t)stream;
+#define KV8_APPEND(TT, DD, LL)                                                                                      \
+  launch_append<TT, DD, LL>(k, v, k_cache, v_cache, k_scale, v_scale, page_table, kv_lens, cu, B, T, reach, n_kv, pages, \
+                            max_pages, k_stride, v_stride, s)
+#define KV8_APPEND_P(TT, DD) \
+  (lp == 4 ? KV8_APPEND(TT, DD, 4) : lp == 5 ? KV8_APPEND(TT, DD, 5) : lp == 6 ? KV8_APPEND(TT, DD, 6) : KV8_APPEND(TT, DD, 7))
+  if (dtype == MX_DTYPE_BF16) return d == 64 ? KV8_APPEND_P(mx::BF16, 64) : KV8_APPEND_P(mx::BF16, 128);
+  return d == 64 ? KV8_APPEND_P(mx::F16, 64) : KV8_APPEND_P(mx::F16, 128);
+}
+
+extern "C" int mx_kv8_copy_pages(void* k_cache, void* v_cache, float* k_scale, float* v_scale, const int* src,
+                                 const int* dst, int n, int n_kv, int d, int page, int pages, void* stream) {
+  using namespace mx::kv8;
+  const int rc = check_cache(k_cache, v_cache, k_scale, v_scale, n_kv, d, page, pages);
+  if (rc != MX_OK) return rc;
+  if (!src || !dst) return MX_ERR_NULL;
+  if (n <= 0) return MX_ERR_SHAPE;
+  const long long bytes = (long long)n_kv * page * d;
+  const long long pieces = (bytes + PIECE - 1) / PIECE;
+  if (bytes > 0x7fffffffLL || 2 * pieces * n > 0x7fffffffLL) return MX_ERR_SHAPE;
+  hipLaunchKernelGGL(copy_kernel, dim3((unsigned)(2 * pieces * n)), dim3(COPY_NT), 0, (hipStream_t)stream,
+                     (uint8_t*)k_cache, (uint8_t*)v_cache, k_scale, v_scale, src, dst, n_kv, (uint32_t)bytes, (int)pieces,
+                     pages);
+  MX_RETURN_IF_HIP(hipGetLastError());
+  return MX_OK;
+}

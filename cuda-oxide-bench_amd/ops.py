@@ -463,3 +463,308 @@ def mla_decode_absorbed(q_nope, q_rope, kv, w_uk, w_uv, scale, out=None, workspa
     _lib.call("mx_mla_decode_absorbed", q_nope.data_ptr(), q_rope.data_ptr(), kv.data_ptr(), w_uk.data_ptr(),
               w_uv.data_ptr(), out.data_ptr(), B, Hh, T, dn, dv, float(scale), ws_ptr, ws_bytes, _stream())
     return out
+
+
+# ---------------------------------------------------------------------------
+# 8-bit serving: int8 linear layers, the paged e4m3 cache and its attention
+# ---------------------------------------------------------------------------
+def _rows(t, name, dtypes, inner):
+    """Checks of a tensor whose rows (first dimension) may lie apart, each of them contiguous; its row stride."""
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name} must be a torch.Tensor")
+    if t.dtype not in dtypes:
+        raise TypeError(f"{name} has dtype {t.dtype}, expected one of {list(dtypes)}")
+    if not t.is_cuda:
+        raise ValueError(f"{name} must be on a HIP device (got {t.device})")
+    if t.dim() != inner + 1:
+        raise ValueError(f"{name} must be {inner + 1}-D (got shape {tuple(t.shape)})")
+    if t.is_contiguous():
+        return t.numel() // t.shape[0] if t.shape[0] else 0
+    want = 1
+    for d in range(inner, 0, -1):
+        if t.shape[d] != 1 and t.stride(d) != want:
+            raise ValueError(f"each row of {name} must be contiguous (strides {t.stride()})")
+        want *= t.shape[d]
+    if t.shape[0] > 1 and t.stride(0) < want:
+        raise ValueError(f"rows of {name} overlap (strides {t.stride()})")
+    return t.stride(0) if t.shape[0] > 1 else want
+
+
+def _launch(fn, t, *args):
+    """Calls an entry point on t's device and that device's current stream (appended to args)."""
+    d = t.get_device()
+    if _C._cuda_getDevice() == d:
+        _lib.call(fn, *args, _C._cuda_getCurrentRawStream(d))
+    else:
+        with torch.cuda.device(d):
+            _lib.call(fn, *args, _C._cuda_getCurrentRawStream(d))
+
+
+def quant_int8(x, q=None, scales=None):
+    """Rows quantised to int8, one scale per row: x [M,K] bf16/f16 (rows may lie
+    apart; K % 16 == 0) -> (q [M,K] int8, scales [M] fp32), x ~= q * scale.
+    scale = max |row| / 127 (1.0 for a zero row), codes round the exact quotient
+    to nearest even.  A row with an infinity or a NaN gets scale NaN.  Rows of
+    activations give a scale per token, rows of an [N,K] weight one per channel."""
+    ldx = _rows(x, "x", _IO_DTYPES, 1)
+    M, K = x.shape
+    if M < 1 or K < 1 or K % 16:
+        raise ValueError(f"x must have rows, of a multiple of 16 values (got {tuple(x.shape)})")
+    if q is None:
+        q = torch.empty((M, K), dtype=torch.int8, device=x.device)
+    else:
+        _require(q, "q", (torch.int8,), 2)
+    if scales is None:
+        scales = torch.empty((M,), dtype=torch.float32, device=x.device)
+    else:
+        _require(scales, "scales", (torch.float32,), 1)
+    if q.shape != (M, K) or scales.shape != (M,):
+        raise ValueError(f"q must be {(M, K)} and scales {(M,)}")
+    _same_device(x, q, scales)
+    _launch("mx_quant_int8", x, x.data_ptr(), q.data_ptr(), scales.data_ptr(), M, K, ldx, _IO_DTYPES[x.dtype])
+    return q, scales
+
+
+def _check_weight(w, sw, K):
+    _require(w, "w", (torch.int8,), 2)
+    _require(sw, "sw", (torch.float32,), 1)
+    N = w.shape[0]
+    if w.shape[1] != K:
+        raise ValueError(f"inner dimensions differ: {K} vs w {tuple(w.shape)}")
+    if sw.shape[0] != N:
+        raise ValueError(f"sw must be {(N,)}, got {tuple(sw.shape)}")
+    if N < 1 or K < 16 or K % 16 or K > 131071:
+        raise ValueError(f"w must be [N, K] with K a multiple of 16 up to 131071, got {tuple(w.shape)}")
+    return N
+
+
+def gemm_int8(a, sa, w, sw, out=None, dtype=torch.bfloat16):
+    """C[m,n] = (sum_k a[m,k] w[n,k]) * sa[m] * sw[n]: a [M,K], w [N,K] int8
+    (w as a linear layer stores its weight), sa [M], sw [N] fp32.  The sum is
+    exact; C is bf16 or f16 (`dtype`, or out's).  K % 16 == 0, any M and N."""
+    _require(a, "a", (torch.int8,), 2)
+    _require(sa, "sa", (torch.float32,), 1)
+    M, K = a.shape
+    N = _check_weight(w, sw, K)
+    if M < 1 or sa.shape[0] != M:
+        raise ValueError(f"a must have rows and sa one scale for each, got {tuple(a.shape)} and {tuple(sa.shape)}")
+    if out is None:
+        if dtype not in _IO_DTYPES:
+            raise TypeError(f"dtype must be one of {list(_IO_DTYPES)}, got {dtype}")
+        out = torch.empty((M, N), dtype=dtype, device=a.device)
+    else:
+        _require(out, "out", _IO_DTYPES, 2)
+        if out.shape != (M, N):
+            raise ValueError(f"out must be {(M, N)}, got {tuple(out.shape)}")
+    _same_device(a, sa, w, sw, out)
+    _launch("mx_gemm_int8", a, a.data_ptr(), sa.data_ptr(), w.data_ptr(), sw.data_ptr(), out.data_ptr(), M, N, K,
+            _IO_DTYPES[out.dtype])
+    return out
+
+
+def linear_int8_workspace_bytes(M: int, K: int) -> int:
+    return int(_lib.load().mx_linear_int8_workspace(M, K))
+
+
+def linear_int8(x, w, sw, out=None, workspace=None):
+    """An int8 linear layer: quant_int8(x), then gemm_int8 with the weight w [N,K]
+    and its channel scales sw [N].  x [M,K] bf16/f16, rows may lie apart; the
+    result [M,N] has x's type.  Pass `workspace` (uint8, contiguous, at least
+    linear_int8_workspace_bytes) to allocate nothing but the result."""
+    ldx = _rows(x, "x", _IO_DTYPES, 1)
+    M, K = x.shape
+    N = _check_weight(w, sw, K)
+    if M < 1:
+        raise ValueError(f"x must have rows (got {tuple(x.shape)})")
+    if out is None:
+        out = torch.empty((M, N), dtype=x.dtype, device=x.device)
+    else:
+        _require(out, "out", (x.dtype,), 2)
+        if out.shape != (M, N):
+            raise ValueError(f"out must be {(M, N)}, got {tuple(out.shape)}")
+    if workspace is None:
+        workspace = torch.empty(linear_int8_workspace_bytes(M, K), dtype=torch.uint8, device=x.device)
+    else:
+        _require(workspace, "workspace", (torch.uint8,))
+    _same_device(x, w, sw, out, workspace)
+    _launch("mx_linear_int8", x, x.data_ptr(), w.data_ptr(), sw.data_ptr(), out.data_ptr(), M, N, K, ldx,
+            _IO_DTYPES[x.dtype], workspace.data_ptr(), workspace.numel())
+    return out
+
+
+class KV8Cache:
+    """A paged cache of keys and values in e4m3, a scale per page and head.
+
+    k [pages, n_kv, page, d], v [pages, n_kv, d, page] (each page of v is held
+    transposed) float8_e4m3fn; k_scale, v_scale [pages, n_kv] fp32: value = code *
+    scale.  d 64 or 128, page 16, 32, 64 or 128 tokens.  KV8Cache.empty() makes the
+    tensors; the constructor takes those that the caller has.  The checks run
+    here, once, and the tensors cannot be exchanged afterwards."""
+
+    __slots__ = ("_k", "_v", "_k_scale", "_v_scale", "_args", "_sizes", "_device")
+
+    def __init__(self, k, v, k_scale, v_scale):
+        f8, f32 = (torch.float8_e4m3fn,), (torch.float32,)
+        _require(k, "k", f8, 4)
+        _require(v, "v", f8, 4)
+        _require(k_scale, "k_scale", f32, 2)
+        _require(v_scale, "v_scale", f32, 2)
+        pages, n_kv, page, d = k.shape
+        if d not in (64, 128) or page not in (16, 32, 64, 128) or pages < 1 or n_kv < 1:
+            raise ValueError(f"k must be [pages, n_kv, page, d] with page 16, 32, 64 or 128 and d 64 or 128, got "
+                             f"{tuple(k.shape)}")
+        if v.shape != (pages, n_kv, d, page):
+            raise ValueError(f"v must be {(pages, n_kv, d, page)} (pages transposed), got {tuple(v.shape)}")
+        if k_scale.shape != (pages, n_kv) or v_scale.shape != (pages, n_kv):
+            raise ValueError(f"k_scale and v_scale must be {(pages, n_kv)}")
+        _same_device(k, v, k_scale, v_scale)
+        self._k, self._v, self._k_scale, self._v_scale = k, v, k_scale, v_scale
+        self._args = (k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr())
+        self._sizes = (pages, n_kv, page, d)
+        self._device = k.get_device()
+
+    @classmethod
+    def empty(cls, pages, n_kv, d, page=64, device="cuda"):
+        """A cache of zeros."""
+        return cls(torch.zeros((pages, n_kv, page, d), dtype=torch.uint8, device=device).view(torch.float8_e4m3fn),
+                   torch.zeros((pages, n_kv, d, page), dtype=torch.uint8, device=device).view(torch.float8_e4m3fn),
+                   torch.ones((pages, n_kv), dtype=torch.float32, device=device),
+                   torch.ones((pages, n_kv), dtype=torch.float32, device=device))
+
+    k = property(lambda self: self._k)
+    v = property(lambda self: self._v)
+    k_scale = property(lambda self: self._k_scale)
+    v_scale = property(lambda self: self._v_scale)
+    pages = property(lambda self: self._sizes[0])
+    n_kv = property(lambda self: self._sizes[1])
+    page = property(lambda self: self._sizes[2])
+    d = property(lambda self: self._sizes[3])
+
+
+_I32 = (torch.int32,)
+
+
+def _check_cache(cache):
+    if type(cache) is not KV8Cache:
+        raise TypeError(f"cache must be a KV8Cache, got {type(cache).__name__}")
+
+
+def _check_sequences(cache, T, page_table, kv_lens, cu_q, max_q):
+    """(B, table columns, cu pointer, max_q) of a call over sequences, checked."""
+    _require(page_table, "page_table", _I32, 2)
+    _require(kv_lens, "kv_lens", _I32, 1)
+    B, most = page_table.shape
+    if B < 1 or most < 1 or kv_lens.shape[0] != B:
+        raise ValueError(f"page_table must be [B, pages of a sequence] and kv_lens [B], got {tuple(page_table.shape)} "
+                         f"and {tuple(kv_lens.shape)}")
+    d = cache._device
+    if page_table.get_device() != d or kv_lens.get_device() != d:
+        raise ValueError("all tensors must be on the cache's device")
+    if cu_q is None:
+        if T != B:
+            raise ValueError(f"without cu_q there is one row per sequence: {T} rows for {B} sequences")
+        if max_q not in (None, 1):
+            raise ValueError("max_q needs cu_q")
+        return B, most, None, 1
+    _require(cu_q, "cu_q", _I32, 1)
+    if cu_q.shape[0] != B + 1:
+        raise ValueError(f"cu_q must be {(B + 1,)}, got {tuple(cu_q.shape)}")
+    if cu_q.get_device() != d:
+        raise ValueError("all tensors must be on the cache's device")
+    max_q = T if max_q is None else int(max_q)
+    if max_q < 1:
+        raise ValueError(f"max_q ({max_q}) must be positive")
+    return B, most, cu_q.data_ptr(), min(max_q, T)
+
+
+def kv8_append(k, v, cache, page_table, kv_lens, cu_q=None, max_q=None):
+    """Quantises new keys and values into a KV8Cache.
+
+    k, v [T, n_kv, d] bf16/f16, rows may lie apart (views of a fused projection).
+    Sequence b's new tokens are rows cu_q[b]:cu_q[b+1] (row b without cu_q) and its
+    last ones: kv_lens[b] counts them already.  Token t lies on page
+    page_table[b, t // page].  A page's scale grows to the smallest power of two that
+    holds the new tokens too, and the codes on it move along; one whose first token
+    is new starts anew.  max_q, the most new tokens of a sequence, sizes the
+    launch.  page_table [B, *], kv_lens [B], cu_q [B + 1]: int32."""
+    _check_cache(cache)
+    ks, vs = _rows(k, "k", _IO_DTYPES, 2), _rows(v, "v", (k.dtype,), 2)
+    T = k.shape[0]
+    B, most, cu, max_q = _check_sequences(cache, T, page_table, kv_lens, cu_q, max_q)
+    pages, n_kv, page, d = cache._sizes
+    if T < 1 or k.shape != (T, n_kv, d) or v.shape != k.shape:
+        raise ValueError(f"k and v must be [T, {n_kv}, {d}], got {tuple(k.shape)} and {tuple(v.shape)}")
+    if k.get_device() != cache._device or v.get_device() != cache._device:
+        raise ValueError("all tensors must be on the cache's device")
+    _launch("mx_kv8_append", k, k.data_ptr(), v.data_ptr(), *cache._args, page_table.data_ptr(), kv_lens.data_ptr(), cu,
+            B, T, max_q, n_kv, d, page, pages, most, ks, vs, _IO_DTYPES[k.dtype])
+
+
+def kv8_copy_pages(cache, src, dst):
+    """Page dst[i] of the cache becomes page src[i], all heads, codes and scales
+    (src, dst [n] int32): a forked sequence's last page, the moves of a compaction
+    (KVPages gives both).  A page is at most once a destination, and no
+    destination is a source; pairs with numbers that are no pages are skipped."""
+    _check_cache(cache)
+    _require(src, "src", _I32, 1)
+    _require(dst, "dst", _I32, 1)
+    n = src.shape[0]
+    if dst.shape[0] != n:
+        raise ValueError(f"src and dst must be of one length, got {n} and {dst.shape[0]}")
+    if src.get_device() != cache._device or dst.get_device() != cache._device:
+        raise ValueError("all tensors must be on the cache's device")
+    if n:
+        pages, n_kv, page, d = cache._sizes
+        _launch("mx_kv8_copy_pages", src, *cache._args, src.data_ptr(), dst.data_ptr(), n, n_kv, d, page, pages)
+
+
+def gqa_kv8_workspace_bytes(B: int, T: int, max_q: int, max_kv: int, n_q: int, n_kv: int, d: int) -> int:
+    return int(_lib.load().mx_gqa_kv8_workspace(B, T, max_q, max_kv, n_q, n_kv, d))
+
+
+def gqa_kv8(q, cache, page_table, kv_lens, cu_q=None, max_q=None, max_kv=None, causal=True, scale=None, out=None,
+            workspace=None):
+    """Grouped-query attention over a KV8Cache -> [T, n_q, d], q's type.
+
+    q [T, n_q, d] bf16/f16, rows may lie apart.  Sequence b's rows are
+    cu_q[b]:cu_q[b+1] (row b without cu_q), its tokens t < kv_lens[b] on pages
+    page_table[b, t // page]; causal: its rows are its last tokens, and each sees those
+    up to itself.  A row that sees no token gives zeros; rows of no sequence are
+    left as they are.  max_q and max_kv (the most rows and tokens of a sequence; T and
+    the table's width without them) choose the launch, not what is computed: give
+    max_kv where the table is wider than the sequences are long.  scale defaults to
+    1/sqrt(d).  Pass `workspace` (uint8, contiguous, at least gqa_kv8_workspace_bytes)
+    to allocate nothing but the result; calls that may overlap each need their own."""
+    _check_cache(cache)
+    qs = _rows(q, "q", _IO_DTYPES, 2)
+    T = q.shape[0]
+    B, most, cu, max_q = _check_sequences(cache, T, page_table, kv_lens, cu_q, max_q)
+    pages, n_kv, page, d = cache._sizes
+    n_q = q.shape[1]
+    if T < 1 or q.shape[2] != d or n_q < 1 or n_q % n_kv:
+        raise ValueError(f"q must be [T, a multiple of {n_kv}, {d}], got {tuple(q.shape)}")
+    max_kv = most * page if max_kv is None else min(int(max_kv), most * page)
+    if max_kv < 1:
+        raise ValueError(f"max_kv ({max_kv}) must be positive")
+    if scale is None:
+        scale = 1.0 / math.sqrt(d)
+    if out is None:
+        out = torch.empty((T, n_q, d), dtype=q.dtype, device=q.device)
+    else:
+        _require(out, "out", (q.dtype,), 3)
+        if out.shape != q.shape:
+            raise ValueError(f"out must be {tuple(q.shape)}")
+    if q.get_device() != cache._device or out.get_device() != cache._device:
+        raise ValueError("all tensors must be on the cache's device")
+    need = gqa_kv8_workspace_bytes(B, T, max_q, max_kv, n_q, n_kv, d)
+    if workspace is None:
+        if need:
+            workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
+    else:
+        _require(workspace, "workspace", (torch.uint8,))
+        _same_device(q, workspace)
+    ws, ws_bytes = (None, 0) if workspace is None else (workspace.data_ptr(), workspace.numel())
+    _launch("mx_gqa_kv8", q, q.data_ptr(), *cache._args, page_table.data_ptr(), kv_lens.data_ptr(), cu, out.data_ptr(),
+            B, T, max_q, max_kv, n_q, n_kv, d, page, pages, most, qs, float(scale), int(bool(causal)),
+            _IO_DTYPES[q.dtype], ws, ws_bytes)
+    return out

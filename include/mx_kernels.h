@@ -296,6 +296,122 @@ int mx_kda_decode(const void* q, const void* k, const void* v, const void* g, co
                   const float* S_in, float* S_out, void* o, int B, int H, int dk, int dv,
                   int dtype, void* stream);
 
+/*
+ * int8 quantisation of the rows of X[M,K] (bf16 or f16, leading dimension
+ * ldx >= K in elements), one scale per row:
+ *   scales[m] = max_k |X[m,k]| / 127      (fp32; 1.0 for an all-zero row)
+ *   Q[m,k]    = RNE(X[m,k] / scales[m])   (of the exact quotient: -127..127)
+ * A row that holds an infinity or a NaN gets scale NaN and codes 0, so every
+ * product with it is NaN.  Rows of activations give a scale per token, rows
+ * of an [N,K] weight one per output channel.  Requires K % 16 == 0,
+ * ldx % 8 == 0, 16-byte aligned X and Q.
+ * No counterpart in the reference (its quantised product is the fp8 one).
+ */
+int mx_quant_int8(const void* X, void* Q, float* scales, int M, int K, int ldx, int dtype, void* stream);
+
+/*
+ * int8 matrix product with a scale per token and per output channel:
+ *   C[m,n] = (sum_k A[m,k] * B[n,k]) * sA[m] * sB[n]
+ * A[M,K] and B[N,K] row-major int8 (B as a linear layer stores its weight),
+ * sA[M], sB[N] fp32, C[M,N] row-major bf16 or f16 (`dtype`).  The sum is
+ * exact (int32), converted to fp32, scaled and rounded once.  Any M and N;
+ * requires K % 16 == 0, K <= 131071 (the sum of K products of -128 fits
+ * int32) and 16-byte aligned A, B, C.
+ * No counterpart in the reference, as above.
+ */
+int mx_gemm_int8(const void* A, const float* sA, const void* B, const float* sB, void* C, int M, int N, int K,
+                 int dtype, void* stream);
+
+/*
+ * An int8 linear layer: mx_quant_int8 of X[M,K] into the workspace, then
+ * mx_gemm_int8 with the weight W[N,K] and its scales sW[N].  C has X's type.
+ * The workspace (mx_linear_int8_workspace(M, K) bytes, 16-byte aligned; 0 for
+ * invalid sizes) holds the codes and the scales; calls that may overlap each
+ * need their own.
+ */
+int mx_linear_int8(const void* X, const void* W, const float* sW, void* C, int M, int N, int K, int ldx, int dtype,
+                   void* workspace, size_t ws_bytes, void* stream);
+size_t mx_linear_int8_workspace(int M, int K);
+
+/*
+ * The paged 8-bit cache of keys and values that the mx_kv8_* entry points
+ * and mx_gqa_kv8 share:
+ *   K codes  [pages, n_kv, page, d]   e4m3fn
+ *   V codes  [pages, n_kv, d, page]   e4m3fn, each page transposed: the
+ *            attention reads consecutive keys of one channel
+ *   K, V scales [pages, n_kv]         fp32: value = code * scale
+ * d is 64 or 128, page (tokens a page) 16, 32, 64 or 128.  Token t of sequence
+ * b lies on page page_table[b * max_pages + t / page], slot t % page; kv_lens[b]
+ * counts sequence b's tokens with the new ones, which are its last.  The new
+ * rows (queries, keys, values) of all B sequences lie one behind the other:
+ * sequence b's are rows cu[b] .. cu[b+1]-1 of T, or row b alone with cu NULL
+ * (then T = B).  page_table, kv_lens and cu are int32 on the device.
+ * What the device-side numbers may hold is checked there: a length is taken
+ * as at least 0 and at most max_pages * page, row ranges are cut to 0..T, and
+ * a page number outside 0..pages-1 is never followed: its tokens are neither
+ * written nor seen.  Rows outside cu[0]..cu[B]-1 are left as they are.
+ */
+
+/*
+ * Quantises the new keys and values (k, v: [T, n_kv, d] bf16 or f16, rows
+ * k_stride / v_stride elements apart) into the cache.  For each page and head that
+ * new tokens reach, K and V on their own:
+ *   s = the smallest power of two, at least 2^-32, with max |x| <= 448 s over the
+ *       page's new tokens (finite values only); not below the page's present
+ *       scale, unless the new tokens begin at slot 0
+ *   codes already on the page move to s: e4m3fn(RNE(code * s_old / s))
+ *   new codes = e4m3fn(RNE(x / s)); an infinity or a NaN becomes NaN
+ * Powers of two: e4m3 is a floating format, so another scale gains no
+ * precision, and moving codes to a larger one then rounds nothing but the
+ * smallest codes.  Slots behind the new tokens keep what they hold.
+ * max_q: the most new tokens of a sequence, or an estimate (it sizes the
+ * launch; a sequence with more is still written whole).  No page that a
+ * sequence writes may be in another sequence's reach in the same call.
+ * Requires n_kv * B <= 2^24, strides % 8 == 0 and >= n_kv * d, 16-byte aligned
+ * k, v and codes.
+ * No counterpart in the reference (it has no cache of keys and values beyond
+ * the latent one of cutile-attn-mla).
+ */
+int mx_kv8_append(const void* k, const void* v, void* k_cache, void* v_cache, float* k_scale, float* v_scale,
+                  const int* page_table, const int* kv_lens, const int* cu, int B, int T, int max_q, int n_kv, int d,
+                  int page, int pages, int max_pages, int k_stride, int v_stride, int dtype, void* stream);
+
+/*
+ * Copies pages of the cache, all heads, codes and scales: page dst[i] becomes
+ * page src[i], i < n (int32 on the device; a pair with a number outside
+ * 0..pages-1 is skipped).  For forked sequences (the shared prefix's last,
+ * partly filled page) and compactions.  The copies run side by side: a page
+ * is at most once a destination, and no destination is a source.
+ */
+int mx_kv8_copy_pages(void* k_cache, void* v_cache, float* k_scale, float* v_scale, const int* src, const int* dst,
+                      int n, int n_kv, int d, int page, int pages, void* stream);
+
+/*
+ * Grouped-query attention over the cache.  Row i (of n_b) of sequence b,
+ * query head h:
+ *   O = softmax_t(scale * q . K[t, h / (n_q / n_kv)]) . V[t, h / (n_q / n_kv)]
+ * over the sequence's tokens t < kv_lens[b], with causal != 0 only
+ * t <= kv_lens[b] - n_b + i.  q: [T, n_q, d] bf16 or f16, rows q_stride elements
+ * apart; O: [T, n_q, d] contiguous, same type.  fp32 scores, softmax and sums;
+ * P is rounded to the I/O type for the product with V.  A row that sees no
+ * token gives zeros.  The scales of K and V may be any positive finite
+ * numbers, those of V within 2^100 of each other.
+ * max_q and max_kv: the largest number of rows and of tokens of a sequence, or
+ * estimates: they choose the kernel and its split of the keys, not what is
+ * computed.  The workspace (mx_gqa_kv8_workspace bytes for the same sizes, may
+ * be 0; 16-byte aligned) holds partial results; calls that may overlap each
+ * need their own.
+ * n_q % n_kv == 0; requires q_stride % 8 == 0 and >= n_q * d, 16-byte aligned q,
+ * O and codes.
+ * No counterpart in the reference: its attention kernels read bf16 or f16 keys and
+ * values of one length (cutile-attn-gqa/main.py:64-170).
+ */
+int mx_gqa_kv8(const void* q, const void* k_cache, const void* v_cache, const float* k_scale, const float* v_scale,
+               const int* page_table, const int* kv_lens, const int* cu, void* O, int B, int T, int max_q, int max_kv,
+               int n_q, int n_kv, int d, int page, int pages, int max_pages, int q_stride, float scale, int causal,
+               int dtype, void* workspace, size_t ws_bytes, void* stream);
+size_t mx_gqa_kv8_workspace(int B, int T, int max_q, int max_kv, int n_q, int n_kv, int d);
+
 #ifdef __cplusplus
 }
 #endif

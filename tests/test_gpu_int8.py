@@ -1,0 +1,158 @@
+"""int8 quantiser, product and linear layer on the GPU against the 64-bit oracle."""
+from __future__ import annotations
+
+import pytest
+import torch
+
+from conftest import announce
+from oracle import int8 as oracle
+
+pytestmark = pytest.mark.gpu
+
+DTYPES = [torch.bfloat16, torch.float16]
+
+
+def bound(exact: torch.Tensor, dtype) -> torch.Tensor:
+    """How far the product may be off: its rounding to `dtype` (half a step relative to the value, or half
+    the smallest f16 subnormal), after three fp32 roundings (the int32 sum's conversion, two scales)."""
+    fp32 = 3 * 2.0 ** -24
+    return exact.abs() * ((1 + fp32) * torch.finfo(dtype).eps / 2 + fp32 * 1.0001) + (
+        2.0 ** -25 if dtype == torch.float16 else 0.0)
+
+
+def rows(m, k, dtype, seed):
+    g = torch.Generator().manual_seed(seed)
+    return (torch.randn((m, k), generator=g) * torch.exp(torch.randn(k, generator=g))).to(dtype)
+
+
+def codes(m, k, seed):
+    g = torch.Generator().manual_seed(seed)
+    return (torch.randint(-128, 128, (m, k), generator=g, dtype=torch.int32).to(torch.int8),
+            torch.rand(m, generator=g) * 0.02 + 1e-4)
+
+
+def same(q, s, x):
+    qe, se = oracle.quantize_rows(x)
+    assert torch.equal(q.cpu(), qe)
+    assert torch.equal(s.cpu().view(torch.int32)[~se.isnan()], se.view(torch.int32)[~se.isnan()])
+    assert torch.equal(s.cpu().isnan(), se.isnan())
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("m,k", [(1, 16), (3, 48), (5, 4096), (2, 4112), (7, 8208), (2, 16400), (300, 1040)])
+def test_quantiser(ops, dtype, m, k):
+    announce(f"quant_int8 {m}x{k} {dtype}")
+    x = rows(m, k, dtype, m + k)
+    same(*ops.quant_int8(x.cuda()), x)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_quantiser_ties_and_special_rows(ops, dtype):
+    announce(f"quant_int8 special rows {dtype}")
+    x = torch.zeros((10, 64), dtype=dtype)
+    x[0] = torch.arange(64) - 31.5                       # scale 1 below: exact ties
+    x[0, 0] = 127
+    x[1] = (torch.arange(64) - 31.5) * 2.0 ** -8
+    x[1, 5] = -127 * 2.0 ** -8
+    x[3, 7] = float("inf")
+    x[4, 63] = float("nan")
+    x[5] = torch.finfo(dtype).max
+    x[6] = torch.finfo(dtype).smallest_normal
+    x[7, ::3] = torch.finfo(dtype).smallest_normal / 16  # subnormal
+    x[8] = -0.0
+    x[9] = torch.linspace(-1, 1, 64).to(dtype)
+    same(*ops.quant_int8(x.cuda()), x)
+
+
+def test_quantiser_strided_rows(ops):
+    announce("quant_int8 strided rows")
+    x = rows(9, 512, torch.bfloat16, 3).cuda()
+    q, s = ops.quant_int8(x[:, 128:384])
+    same(q, s, x[:, 128:384].contiguous().cpu())
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("m,n,k", [
+    (1, 1, 16), (1, 17, 48), (1, 1024, 4096), (2, 24, 144), (15, 33, 112), (16, 100, 1040), (17, 256, 256), (31, 130, 400),
+    (33, 64, 128), (48, 72, 2064), (64, 500, 640), (65, 65, 65 * 16), (100, 129, 272), (128, 128, 128), (200, 264, 528),
+    (255, 257, 144), (700, 1000, 96), (513, 771, 1552), (1024, 1024, 1024)])
+def test_product(ops, dtype, m, n, k):
+    announce(f"gemm_int8 {m}x{n}x{k} {dtype}")
+    a, sa = codes(m, k, m * 7 + k)
+    w, sw = codes(n, k, n * 5 + k)
+    exact = oracle.product(a, sa, w, sw)
+    out = torch.full((m + 2, n), float("nan"), dtype=dtype, device="cuda")
+    ops.gemm_int8(a.cuda(), sa.cuda(), w.cuda(), sw.cuda(), out=out[:m])
+    assert bool(((out[:m].cpu().double() - exact).abs() <= bound(exact, dtype)).all())
+    assert bool(out[m:].isnan().all())  # nothing behind the last row is touched
+
+
+def test_product_of_extremes(ops):
+    """The longest sum of the largest products: 131056 * 128 * 128 lies 2^18 below 2^31."""
+    announce("gemm_int8 largest sum")
+    k = 131056
+    a = torch.full((2, k), -128, dtype=torch.int8)
+    a[1] = 127
+    w = torch.full((20, k), -128, dtype=torch.int8)
+    w[3:] = 127
+    one = torch.ones
+    exact = oracle.product(a, one(2), w, one(20))
+    for rows_ in (2, 70):  # the kernel for few rows, and tiles
+        out = ops.gemm_int8(a.repeat(rows_ // 2, 1).cuda(), one(rows_).cuda(), w.cuda(), one(20).cuda())
+        assert bool(((out.cpu().double() - exact.repeat(rows_ // 2, 1)).abs() <= bound(exact, torch.bfloat16).repeat(
+            rows_ // 2, 1)).all())
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("m,n,k", [(1, 40, 256), (37, 300, 1040), (130, 260, 512)])
+def test_linear(ops, dtype, m, n, k):
+    """Against the oracle's quantiser and product, with the caller's workspace, on rows that lie apart."""
+    announce(f"linear_int8 {m}x{n}x{k} {dtype}")
+    x = rows(m, 2 * k, dtype, 11)
+    w, sw = oracle.quantize_rows(rows(n, k, dtype, 12))
+    q, sx = oracle.quantize_rows(x[:, k:].contiguous())
+    exact = oracle.product(q, sx, w, sw)
+    ws = torch.empty(ops.linear_int8_workspace_bytes(m, k), dtype=torch.uint8, device="cuda")
+    y = ops.linear_int8(x.cuda()[:, k:], w.cuda(), sw.cuda(), workspace=ws)
+    assert y.dtype == dtype
+    assert bool(((y.cpu().double() - exact).abs() <= bound(exact, dtype)).all())
+
+
+def test_linear_poisoned_row(ops):
+    announce("linear_int8 NaN row")
+    x = rows(5, 256, torch.bfloat16, 1)
+    x[2, 9], x[4, 0] = float("nan"), float("-inf")
+    w, sw = oracle.quantize_rows(rows(48, 256, torch.bfloat16, 2))
+    y = ops.linear_int8(x.cuda(), w.cuda(), sw.cuda()).cpu()
+    assert y.isnan().all(1).tolist() == [False, False, True, False, True] and not y[[0, 1, 3]].isnan().any()
+
+
+def test_streams_and_capture(ops):
+    """Two graphs of two layers with workspaces of their own, replayed on two streams between eager calls."""
+    announce("linear_int8 graphs on two streams")
+    w, sw = oracle.quantize_rows(rows(320, 512, torch.bfloat16, 5))
+    w, sw = w.cuda(), sw.cuda()
+    xs = [rows(m, 512, torch.bfloat16, m).cuda() for m in (3, 90)]
+    want = [ops.linear_int8(x, w, sw) for x in xs]
+    outs = [torch.empty_like(y) for y in want]
+    spaces = [torch.empty(ops.linear_int8_workspace_bytes(*x.shape), dtype=torch.uint8, device="cuda") for x in xs]
+    torch.cuda.synchronize()
+    graphs = []
+    for x, y, ws in zip(xs, outs, spaces):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            ops.linear_int8(x, w, sw, out=y, workspace=ws)
+        graphs.append(g)
+    streams = [torch.cuda.Stream() for _ in graphs]
+    for _ in range(3):
+        for y in outs:
+            y.fill_(float("nan"))
+        torch.cuda.synchronize()
+        for g, s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                g.replay()
+        eager = ops.linear_int8(xs[0], w, sw)
+        torch.cuda.synchronize()
+        assert torch.equal(eager, want[0])
+        for y, e in zip(outs, want):
+            assert torch.equal(y, e)
