@@ -47,21 +47,24 @@ __device__ __forceinline__ f32x4 scales4(const float* sB, int n, int N) {
 
 // ---------------------------------------------------------------------------
 // Tiles for many rows: WM x WN waves, each TM rows of A by 64 rows of B.  Whole
-// 128-byte lines of both operands go HBM -> LDS with direct loads into two
-// slots, one K step of 128 ahead of the MFMAs.
+// 128-byte lines of both operands go HBM -> LDS with direct loads into a ring of
+// NS slots, NS - 1 K steps of 128 ahead of the MFMAs.
 // ---------------------------------------------------------------------------
 constexpr int KS = 128;  // bytes of K per slot
 constexpr int TN = 64;   // B rows of a wave: 4 fragments
 constexpr int FN = 4;
 constexpr int GROUP_M = 8;
 
-template <int BM, int BN, int NW>
-struct Cfg {
+template <int BM, int BN, int NW, int NS>
+struct Tile {
   static constexpr int WN = BN / TN, WM = NW / WN;
   static constexpr int TM = BM / WM, FM = TM / 16;
   static constexpr int SLOT = (BM + BN) * KS;
-  static constexpr int LDS = 2 * SLOT;
+  static constexpr int LDS = NS * SLOT;
   static constexpr int A_LPW = BM * KS / 1024 / NW, B_LPW = BN * KS / 1024 / NW;
+  static constexpr int LPW = A_LPW + B_LPW;
+  static constexpr int PER_CU = LDS <= 80 * 1024 ? 2 : 1;  // workgroups
+  static_assert((NS - 2) * LPW < 64, "vmcnt");
   static_assert(WM * WN == NW && FM >= 1 && A_LPW >= 1 && B_LPW >= 1 && LDS <= 160 * 1024, "tile");
 };
 
@@ -71,11 +74,11 @@ struct Cfg {
 __device__ __forceinline__ int swz_a(int r) { return (r >> 1) & 7; }
 __device__ __forceinline__ int swz_b(int r) { return ((r >> 1) & 1) | (((r >> 4) & 3) << 1); }
 
-template <int BM, int BN, int NW, typename T>
-__global__ __launch_bounds__(64 * NW, NW == 8 ? 1 : 2) void gemm_int8_kernel(
+template <int BM, int BN, int NW, int NS, typename T>
+__global__ __launch_bounds__(64 * NW, (NW / 4 * Tile<BM, BN, NW, NS>::PER_CU)) void gemm_int8_kernel(
     const uint8_t* __restrict__ A, const float* __restrict__ sA, const uint8_t* __restrict__ B,
     const float* __restrict__ sB, uint16_t* __restrict__ C, int M, int N, int K) {
-  using CF = Cfg<BM, BN, NW>;
+  using CF = Tile<BM, BN, NW, NS>;
   constexpr int FM = CF::FM;
   extern __shared__ __align__(1024) unsigned char smem[];
   const int lane = threadIdx.x & 63;
@@ -112,7 +115,7 @@ __global__ __launch_bounds__(64 * NW, NW == 8 ? 1 : 2) void gemm_int8_kernel(
   const uint8_t* a_tile = A + (size_t)m0 * K;
   const uint8_t* b_tile = B + (size_t)n0 * K;
   auto issue = [&](int j) {
-    const uint32_t slot = lds0 + (j & 1) * CF::SLOT;
+    const uint32_t slot = lds0 + (j % NS) * CF::SLOT;
     const int most = (K - j * KS) / 16 - 1;  // the step's last chunk
 #pragma unroll
     for (int n = 0; n < CF::A_LPW; ++n)
@@ -140,12 +143,17 @@ __global__ __launch_bounds__(64 * NW, NW == 8 ? 1 : 2) void gemm_int8_kernel(
     for (int j = 0; j < FN; ++j) acc[i][j] = i32x4{};
   land_args(C, sA, sB);
 
-  issue(0);
+#pragma unroll
+  for (int j = 0; j < NS - 1; ++j)
+    if (j < steps) issue(j);
   for (int j = 0; j < steps; ++j) {
-    wait_vmcnt<0>();
+    if (j + NS - 2 < steps)
+      wait_vmcnt<(NS - 2) * CF::LPW>();
+    else
+      wait_vmcnt<0>();
     lds_barrier();  // step j is in LDS, and every wave is done with step j-1
-    if (j + 1 < steps) issue(j + 1);
-    const uint32_t so = (j & 1) * CF::SLOT;
+    if (j + NS - 1 < steps) issue(j + NS - 1);
+    const uint32_t so = (j % NS) * CF::SLOT;
     const int left = K - j * KS;
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
@@ -168,86 +176,169 @@ __global__ __launch_bounds__(64 * NW, NW == 8 ? 1 : 2) void gemm_int8_kernel(
   }
 
   // Lane: row m = .. + 16 i + r16, columns 16 g + 4 f + 0..3: 16 consecutive ones,
-  // 32 bytes, and the four lanes of a row a whole 128-byte line.
-  const int n = n0 + wn * TN + 16 * g;
+  // 32 bytes, and the four lanes of a row a whole 128-byte line.  Where C's rows
+  // are no multiple of 16 bytes the 16 x 64 results of a fragment row go through
+  // LDS, and out along the rows, 4 bytes a lane (2 for an odd N): stores of a
+  // lane's own columns, 2 bytes each, took 68 us for 2197x7908x336, this way 25.
+  const int nw = n0 + wn * TN, n = nw + 16 * g;
   f32x4 sb[FN];
 #pragma unroll
   for (int f = 0; f < FN; ++f) sb[f] = scales4(sB, n + 4 * f, N);
   const bool wide = (N & 7) == 0;
+  if (!wide) __syncthreads();  // the rings are free
+  unsigned char* stage = smem + wave * 2048;
 #pragma unroll
   for (int i = 0; i < FM; ++i) {
     const int m = m0 + wm * CF::TM + 16 * i + r16;
-    if (m < M && n < N) {
-      const float sa = sA[m];
+    const float sa = sA[min(m, M - 1)];
+    u32x4 row[2];
+#pragma unroll
+    for (int f = 0; f < 2; ++f) {
+      const u32x2 lo = scaled4<T>(acc[i][2 * f], sa, sb[2 * f]), hi = scaled4<T>(acc[i][2 * f + 1], sa, sb[2 * f + 1]);
+      row[f] = u32x4{lo[0], lo[1], hi[0], hi[1]};
+    }
+    if (wide) {
       uint16_t* out = C + (size_t)m * N + n;
 #pragma unroll
-      for (int f = 0; f < FN; f += 2) {
-        const u32x2 lo = scaled4<T>(acc[i][f], sa, sb[f]), hi = scaled4<T>(acc[i][f + 1], sa, sb[f + 1]);
-        if (wide) {
-          if (n + 4 * f < N) st128(out + 4 * f, u32x4{lo[0], lo[1], hi[0], hi[1]});
-        } else {
-          store4(out + 4 * f, lo, N - n - 4 * f);
-          store4(out + 4 * f + 4, hi, N - n - 4 * f - 4);
+      for (int f = 0; f < 2; ++f)
+        if (m < M && n + 8 * f < N) st128(out + 8 * f, row[f]);
+    } else {
+      const int mw = m - r16;  // the fragment's first row
+#pragma unroll
+      for (int f = 0; f < 2; ++f) st128(stage + r16 * 128 + 16 * ((2 * g + f) ^ (r16 & 7)), row[f]);
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the wave's own stage: no barrier
+      if ((N & 1) == 0) {
+#pragma unroll
+        for (int s = 0; s < 8; ++s) {
+          const int r = 2 * s + (lane >> 5), c = lane & 31;  // a dword: columns 2 c, 2 c + 1
+          const uint32_t v = *reinterpret_cast<const uint32_t*>(stage + r * 128 + 16 * ((c >> 2) ^ (r & 7)) + 4 * (c & 3));
+          if (mw + r < M && nw + 2 * c < N) *reinterpret_cast<uint32_t*>(C + (size_t)(mw + r) * N + nw + 2 * c) = v;
+        }
+      } else {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const uint16_t v =
+              *reinterpret_cast<const uint16_t*>(stage + r * 128 + 16 * ((lane >> 3) ^ (r & 7)) + 2 * (lane & 7));
+          if (mw + r < M && nw + lane < N) C[(size_t)(mw + r) * N + nw + lane] = v;
         }
       }
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     }
   }
 }
 
 // ---------------------------------------------------------------------------
-// Few rows: the weight is streamed once from HBM into registers.  A workgroup
-// takes 16 rows of B and all rows of A (16 NM at most); its waves split K and
-// meet in LDS (exact integer sums).  A lane reads 32 consecutive bytes of its
-// row, a quarter of the line that its group of four lanes reads together.
+// Few rows: the weight is streamed once.  A workgroup takes 16 FB rows of B and 16
+// FM rows of A; its four waves split K and meet in LDS (exact integer sums).
+// Each wave fills a ring of its own with direct loads of whole 128-byte lines and
+// waits for nobody: no barrier before the sums.  Loading the fragments straight
+// into registers needs no LDS, but neighbouring lanes then read different rows,
+// which the L1 takes one at a time (64x4096x7168: 21 us, and 11.5 this way).
 // ---------------------------------------------------------------------------
-template <int NM, int NW, typename T>
-__global__ __launch_bounds__(64 * NW) void gemm_int8_rows_kernel(
+constexpr int RW = 4;  // waves
+template <int FM, int FB, int PER_CU>
+struct Rows {
+  static constexpr int SLOT = 16 * (FM + FB) * KS;
+  static constexpr int LPW = 2 * (FM + FB);  // 1 KB loads of a step
+  static constexpr int FIT = 160 * 1024 / PER_CU / RW / SLOT;
+  static constexpr int NS = FIT > 8 ? 8 : FIT;
+  static constexpr int LDS = RW * NS * SLOT;
+  static_assert(NS >= 2 && (NS - 1) * LPW < 64, "vmcnt");
+  static_assert(FM * FB * 64 * 16 <= NS * SLOT, "the sums meet in the rings");
+};
+
+template <int FM, int FB, int PER_CU, typename T>
+__global__ __launch_bounds__(64 * RW) void gemm_int8_rows_kernel(
     const uint8_t* __restrict__ A, const float* __restrict__ sA, const uint8_t* __restrict__ B,
     const float* __restrict__ sB, uint16_t* __restrict__ C, int M, int N, int K) {
-  __shared__ i32x4 red[NW][NM][64];
+  using R = Rows<FM, FB, PER_CU>;
+  extern __shared__ __align__(1024) unsigned char smem[];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int r16 = lane & 15, g = lane >> 4;
-  const int n0 = blockIdx.x * 16;
-  const int m0 = blockIdx.y * 16 * NM;
+  // workgroups of the same rows of B side by side: one XCD's L2 then reads them once
+  const int tiles_m = (M + 16 * FM - 1) / (16 * FM);
+  const int id = xcd_remap(blockIdx.x, gridDim.x);
+  const int n0 = id / tiles_m * 16 * FB, m0 = id % tiles_m * 16 * FM;
   const int steps = (K + KS - 1) / KS;
-  const int k0 = (int)((long long)steps * wave / NW), k1 = (int)((long long)steps * (wave + 1) / NW);
-  const uint8_t* brow = B + (size_t)min(n0 + r16, N - 1) * K;
-  const uint8_t* arow[NM];
+  const int k0 = steps * wave / RW, k1 = steps * (wave + 1) / RW;
+
+  // rows of a slot: A's 16 FM, then B's 16 FB; lane i of load n: row 8 n + i/8, chunk
+  // (i%8) ^ swizzle.  Past M, N or K: the last row or chunk again.
+  const uint32_t ring = lds_addr(smem) + wave * R::NS * R::SLOT;
+  const int lr = lane >> 3;
+  uint32_t off[R::LPW];
 #pragma unroll
-  for (int i = 0; i < NM; ++i) arow[i] = A + (size_t)min(m0 + 16 * i + r16, M - 1) * K;
-  i32x4 acc[NM];
+  for (int n = 0; n < R::LPW; ++n) {
+    const int r = 8 * n + lr;
+    off[n] = (uint32_t)(n < 2 * FM ? min(m0 + r, M - 1) - m0 : min(n0 + r - 16 * FM, N - 1) - n0) * (uint32_t)K;
+  }
+  const uint8_t *a_rows = A + (size_t)m0 * K, *b_rows = B + (size_t)n0 * K;
+  const int ch[2] = {(lane & 7) ^ swz_a(lr), (lane & 7) ^ swz_a(8 + lr)};
+  auto issue = [&](int k, int slot) {
+    const int most = (K - k * KS) / 16 - 1;
 #pragma unroll
-  for (int i = 0; i < NM; ++i) acc[i] = i32x4{};
-  auto step = [&](int k, bool whole) {
-    u32x4 b[2], a[NM][2];
+    for (int n = 0; n < R::LPW; ++n)
+      dma16((n < 2 * FM ? a_rows : b_rows) + (size_t)k * KS, off[n] + 16 * min(ch[n & 1], most),
+            ring + slot * R::SLOT + n * 1024);
+  };
+  uint32_t at[2];
+#pragma unroll
+  for (int h = 0; h < 2; ++h) at[h] = ring + r16 * KS + 16 * ((4 * h + g) ^ swz_a(r16));
+
+  i32x4 acc[FM][FB];
+#pragma unroll
+  for (int i = 0; i < FM; ++i)
+#pragma unroll
+    for (int f = 0; f < FB; ++f) acc[i][f] = i32x4{};
+  land_args(C, sA, sB);
+
+#pragma unroll
+  for (int s = 0; s < R::NS; ++s)
+    if (k0 + s < k1) issue(k0 + s, s);
+  int slot = 0;
+  for (int k = k0; k < k1; ++k) {
+    if (k + R::NS <= k1)
+      wait_vmcnt<(R::NS - 1) * R::LPW>();
+    else
+      wait_vmcnt<0>();
+    asm volatile("" ::: "memory");  // no read before the wait
+    const uint32_t so = slot * R::SLOT;
+    const int left = K - k * KS;
+    u32x4 a[2][FM], b[2][FB];
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      const int at = k * KS + 32 * g + 16 * h;
-      const bool in = whole || at < K;
-      b[h] = in ? ld128(brow + at) : u32x4{};
 #pragma unroll
-      for (int i = 0; i < NM; ++i) a[i][h] = in ? ld128(arow[i] + at) : u32x4{};
+      for (int f = 0; f < FB; ++f) b[h][f] = lds_ld128(at[h] + so + 16 * (FM + f) * KS);
+#pragma unroll
+      for (int f = 0; f < FM; ++f) {
+        a[h][f] = lds_ld128(at[h] + so + 16 * f * KS);
+        if (64 * h + 16 * g >= left) a[h][f] = u32x4{};  // past K
+      }
     }
 #pragma unroll
     for (int h = 0; h < 2; ++h)
 #pragma unroll
-      for (int i = 0; i < NM; ++i) acc[i] = mfma_i8(b[h], a[i][h], acc[i]);
-  };
-  const int whole = min(k1, K / KS);
-  int k = k0;
-  constexpr int UN = NM <= 2 ? 4 : 2;
-#pragma unroll UN
-  for (; k < whole; ++k) step(k, true);
-  if (k < k1) step(k, false);
+      for (int i = 0; i < FM; ++i)
 #pragma unroll
-  for (int i = 0; i < NM; ++i) red[wave][i][lane] = acc[i];
+        for (int f = 0; f < FB; ++f) acc[i][f] = mfma_i8(b[h][f], a[h][i], acc[i][f]);
+    __builtin_amdgcn_sched_barrier(0);  // the slot's reads have arrived: it can be filled again
+    if (k + R::NS < k1) issue(k + R::NS, slot);
+    slot = slot + 1 == R::NS ? 0 : slot + 1;
+  }
+
   __syncthreads();
-  for (int i = wave; i < NM; i += NW) {
-    i32x4 c = red[0][i][lane];
+  i32x4* red = reinterpret_cast<i32x4*>(smem);  // [RW][FM * FB][64]
 #pragma unroll
-    for (int w = 1; w < NW; ++w) c += red[w][i][lane];
-    const int m = m0 + 16 * i + r16, n = n0 + 4 * g;
+  for (int i = 0; i < FM; ++i)
+#pragma unroll
+    for (int f = 0; f < FB; ++f) red[(wave * FM * FB + i * FB + f) * 64 + lane] = acc[i][f];
+  __syncthreads();
+  for (int i = wave; i < FM * FB; i += RW) {
+    i32x4 c = red[i * 64 + lane];
+#pragma unroll
+    for (int w = 1; w < RW; ++w) c += red[(w * FM * FB + i) * 64 + lane];
+    const int m = m0 + 16 * (i / FB) + r16, n = n0 + 16 * (i % FB) + 4 * g;
     if (m < M && n < N) {
       const u32x2 v = scaled4<T>(c, sA[m], scales4(sB, n, N));
       uint16_t* out = C + (size_t)m * N + n;
@@ -259,37 +350,75 @@ __global__ __launch_bounds__(64 * NW) void gemm_int8_rows_kernel(
   }
 }
 
-template <int BM, int BN, int NW, typename T>
-static int launch_tile(const uint8_t* A, const float* sA, const uint8_t* B, const float* sB, uint16_t* C, int M, int N,
-                       int K, hipStream_t s) {
-  using CF = Cfg<BM, BN, NW>;
-  const long long grid = (long long)((M + BM - 1) / BM) * ((N + BN - 1) / BN);
-  if (grid > 0x7fffffffLL) return MX_ERR_SHAPE;
-  constexpr auto kern = gemm_int8_kernel<BM, BN, NW, T>;
-  MX_RETURN_IF_HIP(lds_limit_once<kern>(CF::LDS));
-  hipLaunchKernelGGL(kern, dim3((unsigned)grid), dim3(64 * NW), CF::LDS, s, A, sA, B, sB, C, M, N, K);
-  MX_RETURN_IF_HIP(hipGetLastError());
-  return MX_OK;
+// ---------------------------------------------------------------------------
+// Launch choice.  What bounds every variant short of the largest products is the rate
+// at which a CU takes operand lines in, near 46 GB/s for one workgroup of a CU and 61 for two
+// side by side (measured from 1x1024x1024 to 8192^3; about 37 for the 256x256 tile,
+// whose ring holds two slots), so a variant costs
+//     start + (workgroups per CU) * (rows of A and B of a workgroup) * K / rate
+// and no less than HBM takes for the operands.  Against the best variant of each of 37
+// measured products the choice loses 2% on average.
+// ---------------------------------------------------------------------------
+struct Variant {
+  int bm, bn;
+  float start, one, many;  // us; bytes per us with one workgroup on a CU, with more
+};
+constexpr Variant kVariants[] = {
+    {16, 16, 2.3f, 46e3f, 61e3f},  {16, 32, 2.3f, 46e3f, 61e3f},  {32, 16, 2.3f, 46e3f, 61e3f},
+    {32, 32, 2.3f, 48e3f, 61e3f},  {64, 32, 2.3f, 50e3f, 50e3f},  {32, 64, 2.3f, 50e3f, 50e3f},
+    {64, 64, 3.3f, 46e3f, 61e3f},  {128, 64, 3.3f, 46e3f, 64e3f}, {64, 128, 3.3f, 46e3f, 62e3f},
+    {128, 128, 3.3f, 44e3f, 60e3f}, {256, 256, 3.3f, 37e3f, 37e3f},
+};
+constexpr int kNumVariants = sizeof(kVariants) / sizeof(kVariants[0]);
+
+static int pick(int M, int N, int K) {
+  int best = 0;
+  double least = 1e30;
+  for (int i = 0; i < kNumVariants; ++i) {
+    const Variant& v = kVariants[i];
+    const double wgs = (double)((M + v.bm - 1) / v.bm) * ((N + v.bn - 1) / v.bn);
+    const double n = wgs <= 256 ? 1 : wgs <= 8192 ? (double)(((long long)wgs + 255) / 256) : wgs / 256;
+    const double us = v.start + n * (v.bm + v.bn) * K / (n > 1 ? v.many : v.one);
+    if (us < least) least = us, best = i;
+  }
+  return best;
 }
 
-template <int NM, int NW, typename T>
-static int launch_rows(const uint8_t* A, const float* sA, const uint8_t* B, const float* sB, uint16_t* C, int M, int N,
-                       int K, hipStream_t s) {
-  const dim3 grid((unsigned)((N + 15) / 16), (unsigned)((M + 16 * NM - 1) / (16 * NM)));
-  hipLaunchKernelGGL((gemm_int8_rows_kernel<NM, NW, T>), grid, dim3(64 * NW), 0, s, A, sA, B, sB, C, M, N, K);
+template <typename Kern>
+static int launch(Kern kern, hipError_t ready, int lds, int threads, dim3 grid, const uint8_t* A, const float* sA,
+                  const uint8_t* B, const float* sB, uint16_t* C, int M, int N, int K, hipStream_t s) {
+  MX_RETURN_IF_HIP(ready);
+  hipLaunchKernelGGL(kern, grid, dim3(threads), lds, s, A, sA, B, sB, C, M, N, K);
   MX_RETURN_IF_HIP(hipGetLastError());
   return MX_OK;
 }
 
 template <typename T>
-static int dispatch(const uint8_t* A, const float* sA, const uint8_t* B, const float* sB, uint16_t* C, int M, int N,
-                    int K, hipStream_t s) {
-  if (M <= 16) return launch_rows<1, 8, T>(A, sA, B, sB, C, M, N, K, s);
-  if (M <= 32) return launch_rows<2, 8, T>(A, sA, B, sB, C, M, N, K, s);
-  if (M <= 64) return launch_rows<4, 8, T>(A, sA, B, sB, C, M, N, K, s);
-  const long long big = (long long)((M + 255) / 256) * ((N + 255) / 256);
-  if (big >= 200) return launch_tile<256, 256, 8, T>(A, sA, B, sB, C, M, N, K, s);
-  return launch_tile<128, 128, 4, T>(A, sA, B, sB, C, M, N, K, s);
+static int run(int variant, const uint8_t* A, const float* sA, const uint8_t* B, const float* sB, uint16_t* C, int M,
+               int N, int K, hipStream_t s) {
+  const Variant& v = kVariants[variant];
+  const long long tm = (M + v.bm - 1) / v.bm, tn = (N + v.bn - 1) / v.bn;
+#define ROWS(FM, FB, PER)                                                                                         \
+  launch(gemm_int8_rows_kernel<FM, FB, PER, T>, lds_limit_once<gemm_int8_rows_kernel<FM, FB, PER, T>>(Rows<FM, FB, PER>::LDS), \
+         Rows<FM, FB, PER>::LDS, 64 * RW, dim3((unsigned)(tm * tn)), A, sA, B, sB, C, M, N, K, s)
+#define TILE(BM, BN, NW, NS)                                                                                      \
+  launch(gemm_int8_kernel<BM, BN, NW, NS, T>, lds_limit_once<gemm_int8_kernel<BM, BN, NW, NS, T>>(Tile<BM, BN, NW, NS>::LDS), \
+         Tile<BM, BN, NW, NS>::LDS, 64 * NW, dim3((unsigned)(tm * tn)), A, sA, B, sB, C, M, N, K, s)
+  switch (variant) {
+    case 0: return ROWS(1, 1, 2);
+    case 1: return ROWS(1, 2, 2);
+    case 2: return ROWS(2, 1, 2);
+    case 3: return ROWS(2, 2, 2);
+    case 4: return ROWS(4, 2, 1);
+    case 5: return ROWS(2, 4, 1);
+    case 6: return TILE(64, 64, 4, 4);
+    case 7: return TILE(128, 64, 4, 3);
+    case 8: return TILE(64, 128, 4, 3);
+    case 9: return TILE(128, 128, 8, 2);
+    default: return TILE(256, 256, 8, 2);
+  }
+#undef ROWS
+#undef TILE
 }
 
 static int check(const void* A, const float* sA, const void* B, const float* sB, const void* C, int M, int N, int K,
@@ -312,8 +441,9 @@ extern "C" int mx_gemm_int8(const void* A, const float* sA, const void* B, const
   const int rc = check(A, sA, B, sB, C, M, N, K, dtype);
   if (rc != MX_OK) return rc;
   const uint8_t *a = (const uint8_t*)A, *b = (const uint8_t*)B;
-  if (dtype == MX_DTYPE_BF16) return dispatch<mx::BF16>(a, sA, b, sB, (uint16_t*)C, M, N, K, (hipStream_t)stream);
-  return dispatch<mx::F16>(a, sA, b, sB, (uint16_t*)C, M, N, K, (hipStream_t)stream);
+  const int v = pick(M, N, K);
+  if (dtype == MX_DTYPE_BF16) return run<mx::BF16>(v, a, sA, b, sB, (uint16_t*)C, M, N, K, (hipStream_t)stream);
+  return run<mx::F16>(v, a, sA, b, sB, (uint16_t*)C, M, N, K, (hipStream_t)stream);
 }
 
 // Workspace of the linear layer: the codes (256-byte multiple), then the scales.
