@@ -99,8 +99,8 @@ __global__ __launch_bounds__(64 * NW, NR == 1 ? 2 : 1) void rows_kernel(const Ar
 
   const Rows rw = rows_of(a.cu, b, a.T);
   const int n = rw.last - rw.first;
-  if (n == 0) return;
   const int len = cut_len(a.lens[b], a.max_pages, a.lp);
+  if (n == 0) return;
   const int t0 = min((long long)split * a.chunk, (long long)len);
   const int t1 = split + 1 == a.splits ? len : min(len, t0 + a.chunk);
   const int* row_pages = a.table + (size_t)b * a.max_pages;
@@ -366,8 +366,8 @@ struct Stage {
   static constexpr int K = BN * D * 2, V = D * BN * 2;
   static constexpr int BYTES = K + V;
   static constexpr int CONSTS = 2 * BYTES;            // [2][4 groups of 16 keys] x {cs, lv, iv, 0}
-  static constexpr int FLAGS = CONSTS + 2 * 4 * 16;   // [2][TW] a NaN among V's codes
-  static constexpr int LDS = FLAGS + 2 * TW * 4;
+  static constexpr int FLAGS = CONSTS + 2 * 4 * 16;   // tiles with a NaN among V's codes
+  static constexpr int LDS = FLAGS + 16;
 };
 // 16-byte slot of a row, swizzled so that the 16 lanes LDS serves together hit different
 // slots of its 256-byte window.
@@ -376,7 +376,8 @@ __device__ __forceinline__ int slot_at(int row, int slot) {
   return ROW == 256 ? slot ^ (row & 15) : slot ^ ((row >> 1) & 7);
 }
 
-template <typename T, int D>
+// WIDE: pages of 64 tokens and more, one page and one set of scales per tile.
+template <typename T, int D, bool WIDE>
 __global__ __launch_bounds__(64 * TW, 1) void tile_kernel(const Args a) {
   using L = Stage<D>;
   constexpr int DC = D / 16, DT = D / 32;
@@ -425,72 +426,91 @@ __global__ __launch_bounds__(64 * TW, 1) void tile_kernel(const Args a) {
       for (int k = 0; k < DC; ++k) qf[k] = ld128(src + 16 * k) ^ u32x4{flip, flip, flip, flip};
     }
 
-    // ---- a tile's codes: unit id < 4 D: K, row id / (D/16); else V, channel ----
+    // ---- a tile's codes: unit id < 4 D: K, row id / (D/16); else V, channel.  Page
+    // numbers are looked up a tile before the codes are loaded, those a tile before
+    // they are widened.  Past the last tile: page -1, zeros into a stage nobody reads. ----
     u32x4 raw[U];
     float rks = 0.f, rvs = 0.f;
-    int page_n[U], page_s;  // pages of the next tile to load
+    int page_n[U], page_s;
+    bool bad[U], bad_s = true;
     auto key_of = [&](int u) {
       const int id = tid + u * NT;
       return id < 4 * D ? id / (D / 16) : (id - 4 * D) % 4 * 16;
     };
+    const int last_col = a.max_pages - 1;
     auto find = [&](int tile) {
       const int at = s0 + BN * tile;
 #pragma unroll
-      for (int u = 0; u < U; ++u)
-        page_n[u] = at + key_of(u) < high ? page_of(row_pages, at + key_of(u), a.lp, a.max_pages, a.pages) : -1;
-      page_s = tid < 4 && at + 16 * tid < high ? page_of(row_pages, at + 16 * tid, a.lp, a.max_pages, a.pages) : -1;
+      for (int u = 0; u < U; ++u) page_n[u] = row_pages[min((at + key_of(u)) >> a.lp, last_col)];
+      page_s = row_pages[min((at + 16 * (tid & 3)) >> a.lp, last_col)];
     };
-    bool bad[U], bad_s;
     auto load = [&](int tile) {
       const int at = s0 + BN * tile;
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-        const int id = tid + u * NT, key = (at + key_of(u)) & (P - 1);
-        bad[u] = page_n[u] < 0;
-        const size_t page = ((size_t)max(page_n[u], 0) * a.n_kv + h) * (size_t)(D * P);
-        raw[u] = ld128(id < 4 * D ? a.kc + page + (size_t)key * D + id % (D / 16) * 16
-                                  : a.vc + page + (size_t)((id - 4 * D) / 4) * P + key);
+        const int id = tid + u * NT, key = at + key_of(u);
+        bad[u] = key >= high || (uint32_t)page_n[u] >= (uint32_t)a.pages;
+        const size_t page = ((size_t)(uint32_t)(bad[u] ? 0 : page_n[u]) * a.n_kv + h) * (size_t)(D * P);
+        raw[u] = ld128(id < 4 * D ? a.kc + page + (size_t)(key & (P - 1)) * D + id % (D / 16) * 16
+                                  : a.vc + page + (size_t)((id - 4 * D) / 4) * P + (key & (P - 1)));
       }
-      bad_s = page_s < 0;
-      rks = a.ks[(size_t)max(page_s, 0) * a.n_kv + h];
-      rvs = a.vs[(size_t)max(page_s, 0) * a.n_kv + h];
+      bad_s = at + 16 * (tid & 3) >= high || (uint32_t)page_s >= (uint32_t)a.pages;
+      const size_t page = (size_t)(uint32_t)(bad_s ? 0 : page_s) * a.n_kv + h;
+      rks = a.ks[page];
+      rvs = a.vs[page];
     };
-    auto store = [&](int tile) {
+    // Tiles from first_masked on are not seen whole by every row: at most 6, bits of *flags.
+    int* flags = reinterpret_cast<int*>(smem + L::FLAGS);
+    const int first_masked = low > s0 ? (low - s0) / BN : 0;
+    // A tile that some row does not see whole: V's codes of tokens past the last become 0,
+    // and so do NaNs, which are flagged (with a causal mask: without one every row sees
+    // every token that is there).
+    auto clean = [&](int tile) {
       const int at = s0 + BN * tile;
-      const uint32_t st = (tile & 1) * L::BYTES;
       bool nan = false;
 #pragma unroll
       for (int u = 0; u < U; ++u) {
         const int id = tid + u * NT;
-        u32x4 x = bad[u] ? u32x4{} : raw[u];
-        if (id < 4 * D) {
-          const int row = id / (D / 16), slot = id % (D / 16) * 2;
-          st128(smem + st + row * (2 * D) + 16 * slot_at<2 * D>(row, slot), widen8<T>(x[0], x[1]));
-          st128(smem + st + row * (2 * D) + 16 * slot_at<2 * D>(row, slot + 1), widen8<T>(x[2], x[3]));
-        } else {
-          const int row = (id - 4 * D) / 4, slot = (id - 4 * D) % 4 * 2;
-          if (at + BN > low) {  // some row does not see every key of the tile
-            const int left = high - at - 8 * slot;
+        if (id >= 4 * D) {
+          const int left = high - at - (id - 4 * D) % 4 * 16;
 #pragma unroll
-            for (int w = 0; w < 4; ++w) {
+          for (int w = 0; w < 4; ++w) {
 #pragma unroll
-              for (int j = 0; j < 4; ++j)
-                if (4 * w + j >= left) x[w] &= ~(0xffu << (8 * j));
-              const uint32_t bits = a.causal ? nan_bytes(x[w]) : 0u;
-              nan |= bits != 0;
-              x[w] &= ~spread(bits);
-            }
+            for (int j = 0; j < 4; ++j)
+              if (bad[u] || 4 * w + j >= left) raw[u][w] &= ~(0xffu << (8 * j));
+            const uint32_t bits = a.causal ? nan_bytes(raw[u][w]) : 0u;
+            nan |= bits != 0;
+            raw[u][w] &= ~spread(bits);
           }
-          st128(smem + st + L::K + row * (2 * BN) + 16 * slot_at<2 * BN>(row, slot), widen8<T>(x[0], x[2]));
-          st128(smem + st + L::K + row * (2 * BN) + 16 * slot_at<2 * BN>(row, slot + 1), widen8<T>(x[1], x[3]));
         }
       }
-      if (tid < 4)
-        *reinterpret_cast<f32x4*>(smem + L::CONSTS + ((tile & 1) * 4 + tid) * 16) =
-            bad_s ? f32x4{0.f, -INFINITY, 0.f, 0.f} : f32x4{c * rks, __builtin_amdgcn_logf(rvs), 1.0f / rvs, 0.f};
-      const bool any = __any(nan);
-      if (lane == 0) *reinterpret_cast<int*>(smem + L::FLAGS + ((tile & 1) * TW + wave) * 4) = any;
+      if (__any(nan) && lane == 0) atomicOr(flags, 1 << (tile - first_masked));
     };
+    // unit u of the loaded tile into the stage at byte st
+    auto store = [&](int u, int st) {
+      const int id = tid + u * NT;
+      const u32x4 x = bad[u] ? u32x4{} : raw[u];
+      if (id < 4 * D) {
+        const int row = id / (D / 16), slot = id % (D / 16) * 2;
+        st128(smem + st + row * (2 * D) + 16 * slot_at<2 * D>(row, slot), widen8<T>(x[0], x[1]));
+        st128(smem + st + row * (2 * D) + 16 * slot_at<2 * D>(row, slot + 1), widen8<T>(x[2], x[3]));
+      } else {
+        const int row = (id - 4 * D) / 4, slot = (id - 4 * D) % 4 * 2;
+        st128(smem + st + L::K + row * (2 * BN) + 16 * slot_at<2 * BN>(row, slot), widen8<T>(x[0], x[2]));
+        st128(smem + st + L::K + row * (2 * BN) + 16 * slot_at<2 * BN>(row, slot + 1), widen8<T>(x[1], x[3]));
+      }
+    };
+    auto store_consts = [&](int stage) {
+      if (tid < 4)
+        *reinterpret_cast<f32x4*>(smem + L::CONSTS + (stage * 4 + tid) * 16) =
+            bad_s ? f32x4{0.f, -INFINITY, 0.f, 0.f} : f32x4{c * rks, __builtin_amdgcn_logf(rvs), 1.0f / rvs, 0.f};
+    };
+
+    // K fragment: key row 32 t + ql, slot 2 k + g; V fragment: channel row 32 d + ql, slot
+    // 2 k + g of the tile's 16-key chunk k.  The swizzle is an xor, so slot 2 k is an xor away
+    // from slot 0: one register each, made opaque in every tile lest all of them be kept.
+    const uint32_t k_base = lds0 + ql * (2 * D) + 16 * slot_at<2 * D>(ql, g);
+    const uint32_t v_base = lds0 + L::K + ql * (2 * BN) + 16 * slot_at<2 * BN>(ql, g);
 
     f32x16 acc[DT];
 #pragma unroll
@@ -498,39 +518,80 @@ __global__ __launch_bounds__(64 * TW, 1) void tile_kernel(const Args a) {
     float m = 0.f, l = 0.f;
     bool open = true, seen = false;
 
-    __syncthreads();  // the stages are free
+    // LDS writes done, then the barrier: no wait for the loads that are under way
+    auto meet = [&] {
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      lds_barrier();
+    };
+    __syncthreads();  // the stages and flags are free
+    if (tid == 0) *flags = 0;
+    if (a.causal) __syncthreads();
     if (tiles > 0) {
       find(0);
       load(0);
       find(1);
-      store(0);
-      if (tiles > 1) load(1);
+      if (s0 + BN > low) clean(0);
+#pragma unroll
+      for (int u = 0; u < U; ++u) store(u, 0);
+      store_consts(0);
+      load(1);
       find(2);
     }
-    for (int tile = 0; tile < tiles; ++tile) {
-      __syncthreads();  // the tile's stage is written, the other one read
-      if (tile + 1 < tiles) {
-        store(tile + 1);
-        if (tile + 2 < tiles) load(tile + 2);
-        find(tile + 3);
-      }
+    auto step = [&](int tile, auto stage_tag) {
+      constexpr int STG = decltype(stage_tag)::value;
+      constexpr uint32_t st = STG * L::BYTES, other = (1 - STG) * L::BYTES;
+      meet();  // the tile's stage is written, the other one read
       const int at = s0 + BN * tile;
-      if (idle || at >= w_high) continue;
-      const uint32_t st = lds0 + (tile & 1) * L::BYTES;
+      if (at + 2 * BN > low) clean(tile + 1);
+      if (idle || at >= w_high) {  // nothing to compute: the wave's share of the next tile
+#pragma unroll
+        for (int u = 0; u < U; ++u) store(u, other);
+        store_consts(1 - STG);
+        load(tile + 2);
+        find(tile + 3);
+        return;
+      }
 
-      // ---- S^T ----
+      // ---- S^T, the next tile's codes widened and stored beside its MFMAs ----
+      __builtin_amdgcn_s_setprio(1);
       f32x16 s[2];
+      u32x4 kb[3][2];
+      uint32_t kb0 = k_base;
+      asm volatile("" : "+v"(kb0));
+      auto kread = [&](int t, int k) { return lds_ld128((kb0 ^ (32 * k)) + st + 32 * t * (2 * D)); };
 #pragma unroll
-      for (int k = 0; k < DC; ++k)
+      for (int i = 0; i < 2; ++i) {
+        kb[i][0] = kread(0, i);
+        kb[i][1] = kread(1, i);
+      }
 #pragma unroll
-        for (int t = 0; t < 2; ++t) {
-          const u32x4 kf = lds_ld128(st + (32 * t + ql) * (2 * D) + 16 * slot_at<2 * D>(ql, 2 * k + g));
-          s[t] = mfma32<T>(kf, qf[k], k ? s[t] : f32x16{});
+      for (int k = 0; k < DC; ++k) {
+        if (k + 2 < DC) {
+          kb[(k + 2) % 3][0] = kread(0, k + 2);
+          kb[(k + 2) % 3][1] = kread(1, k + 2);
         }
-      f32x4 cst[4];
 #pragma unroll
-      for (int u = 0; u < 4; ++u)
-        cst[u] = *reinterpret_cast<const f32x4*>(smem + L::CONSTS + ((tile & 1) * 4 + u) * 16);
+        for (int t = 0; t < 2; ++t) s[t] = mfma32<T>(kb[k % 3][t], qf[k], k ? s[t] : f32x16{});
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+          if (k == 1 + u * 2) store(u, other);
+        if (k == DC - 1) {
+          store_consts(1 - STG);
+          load(tile + 2);
+          find(tile + 3);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      f32x4 cst[WIDE ? 1 : 4];
+#pragma unroll
+      for (int u = 0; u < (WIDE ? 1 : 4); ++u) cst[u] = *reinterpret_cast<const f32x4*>(smem + L::CONSTS + (STG * 4 + u) * 16);
+      uint32_t vb0 = v_base;
+      asm volatile("" : "+v"(vb0));
+      auto vread = [&](int k, int d) { return lds_ld128((vb0 ^ (32 * k)) + st + 32 * d * (2 * BN)); };
+      u32x4 vb[2][DT];
+#pragma unroll
+      for (int d = 0; d < DT; ++d) vb[0][d] = vread(0, d);
+      __builtin_amdgcn_s_setprio(0);
 
       // ---- y - m, the running maximum ----
       float mx = -INFINITY;
@@ -539,11 +600,20 @@ __global__ __launch_bounds__(64 * TW, 1) void tile_kernel(const Args a) {
       for (int t = 0; t < 2; ++t)
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
-          const f32x4& k = cst[2 * t + (e >> 3)];
+          const f32x4& k = cst[WIDE ? 0 : 2 * t + (e >> 3)];
           s[t][e] = __builtin_fmaf(s[t][e], k[0], k[1] - m);
-          if (masked) s[t][e] = at + 32 * t + 8 * (e >> 2) + 4 * g + (e & 3) < limit ? s[t][e] : -INFINITY;
-          mx = fmaxf(mx, s[t][e]);
         }
+      if (masked) {
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+          for (int e = 0; e < 16; ++e)
+            s[t][e] = at + 32 * t + 8 * (e >> 2) + 4 * g + (e & 3) < limit ? s[t][e] : -INFINITY;
+      }
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) mx = fmaxf(mx, s[t][e]);
       mx = max_xor32(mx);
       const bool moved = __any(mx > kLazy);
       if (moved || open) {
@@ -551,7 +621,7 @@ __global__ __launch_bounds__(64 * TW, 1) void tile_kernel(const Args a) {
         const float shift = empty ? (met ? mx : 0.f) : moved ? fmaxf(mx, 0.f) : 0.f;
         open = __any(empty && !met);
 #pragma unroll
-        for (int u = 0; u < 4; ++u) seen |= cst[u][1] > -INFINITY && at + 16 * u < limit;
+        for (int u = 0; u < (WIDE ? 1 : 4); ++u) seen |= cst[u][1] > -INFINITY && at + 16 * u < limit;
         m += shift;
         const float corr = empty ? 1.f : __builtin_amdgcn_exp2f(-shift);
         l *= corr;
@@ -563,58 +633,81 @@ __global__ __launch_bounds__(64 * TW, 1) void tile_kernel(const Args a) {
           for (int e = 0; e < 16; ++e) s[t][e] -= shift;
       }
 
-      // ---- a NaN among V's codes that some row does not see: see rows_kernel ----
-      if (at + BN > low && a.causal) {
-        int any = 0;
+      // ---- P', O^T += V^T P'^T by chunks of 16 keys: the next chunk's exponentials and
+      // V reads run beside a chunk's MFMAs ----
 #pragma unroll
-        for (int w = 0; w < TW; ++w) any |= *reinterpret_cast<const int*>(smem + L::FLAGS + ((tile & 1) * TW + w) * 4);
-        if (any) {
-          for (int k = 0; k < 4; ++k) {
-            const int page = at + 16 * k < high ? page_of(row_pages, at + 16 * k, a.lp, a.max_pages, a.pages) : -1;
-            if (page < 0) continue;
-            const int key = at + 16 * k + 4 * g;
-            u32x4 vis, x;
-#pragma unroll
-            for (int w = 0; w < 4; ++w) {
-              const int e = key + 8 * (w >> 1) + 2 * (w & 1);
-              vis[w] = (e < limit ? one_bits<T>() : 0u) | (e + 1 < limit ? one_bits<T>() << 16 : 0u);
-            }
-#pragma unroll
-            for (int d = 0; d < DT; ++d) {
-              const uint8_t* p = a.vc + ((size_t)page * a.n_kv + h) * (size_t)(D * P) + (size_t)(32 * d + ql) * P + (key & (P - 1));
-#pragma unroll
-              for (int w = 0; w < 4; ++w) {
-                const int e = 8 * (w >> 1) + 2 * (w & 1);
-                x[w] = ((p[e] & 0x7f) == 0x7f && key + e < high ? one_bits<T>() : 0u) |
-                       ((p[e + 1] & 0x7f) == 0x7f && key + e + 1 < high ? one_bits<T>() << 16 : 0u);
-              }
-              const f32x16 cnt = mfma32<T>(x, vis, f32x16{});
-#pragma unroll
-              for (int e = 0; e < 16; ++e)
-                if (cnt[e] > 0.f) acc[d][e] = __builtin_nanf("");
-            }
-          }
-        }
-      }
-
-      // ---- P', O^T += V^T P'^T ----
+      for (int e = 0; e < 8; ++e) s[0][e] = __builtin_amdgcn_exp2f(s[0][e]);
+      __builtin_amdgcn_s_setprio(1);
+      float sum = 0.f;
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
         f32x16& x = s[k >> 1];
         const int o = 8 * (k & 1);
-        float sum = 0.f;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          x[o + e] = __builtin_amdgcn_exp2f(x[o + e]);
-          sum += x[o + e];
-        }
-        l = __builtin_fmaf(sum, cst[k][2], l);
         const u32x4 pf{T::pack2(x[o], x[o + 1]), T::pack2(x[o + 2], x[o + 3]), T::pack2(x[o + 4], x[o + 5]),
                        T::pack2(x[o + 6], x[o + 7])};
+        const float part = ((x[o] + x[o + 1]) + (x[o + 2] + x[o + 3])) + ((x[o + 4] + x[o + 5]) + (x[o + 6] + x[o + 7]));
+        if constexpr (WIDE)
+          sum += part;
+        else
+          l = __builtin_fmaf(part, cst[WIDE ? 0 : k][2], l);
+        if (k + 1 < 4) {
 #pragma unroll
-        for (int d = 0; d < DT; ++d) {
-          const u32x4 vf = lds_ld128(st + L::K + (32 * d + ql) * (2 * BN) + 16 * slot_at<2 * BN>(ql, 2 * k + g));
-          acc[d] = mfma32<T>(vf, pf, acc[d]);
+          for (int d = 0; d < DT; ++d) vb[(k + 1) & 1][d] = vread(k + 1, d);
+          const int o1 = 8 * ((k + 1) & 1);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) s[(k + 1) >> 1][o1 + e] = __builtin_amdgcn_exp2f(s[(k + 1) >> 1][o1 + e]);
+        }
+#pragma unroll
+        for (int d = 0; d < DT; ++d) acc[d] = mfma32<T>(vb[k & 1][d], pf, acc[d]);
+        if (k + 1 < 4) {
+          __builtin_amdgcn_sched_group_barrier(0x002, 4, 0);
+#pragma unroll
+          for (int d = 0; d < DT; ++d) {
+            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+            __builtin_amdgcn_sched_group_barrier(0x400, 8 / DT, 0);
+            __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+            __builtin_amdgcn_sched_group_barrier(0x002, 8 / DT, 0);
+          }
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      if constexpr (WIDE) l = __builtin_fmaf(sum, cst[0][2], l);
+      __builtin_amdgcn_s_setprio(0);
+    };
+    for (int tile = 0; tile < tiles; tile += 2) {
+      step(tile, std::integral_constant<int, 0>{});
+      if (tile + 1 < tiles) step(tile + 1, std::integral_constant<int, 1>{});
+    }
+
+    // ---- a NaN among V's codes that some row does not see: those that it does see are
+    // counted, by channel and row, with the products' own layout ----
+    if (a.causal) {
+      meet();
+      for (int flagged = *flags; flagged; flagged &= flagged - 1) {
+        const int at = s0 + BN * (first_masked + __builtin_ctz(flagged));
+        for (int k = 0; k < 4; ++k) {
+          const int page = at + 16 * k < high ? page_of(row_pages, at + 16 * k, a.lp, a.max_pages, a.pages) : -1;
+          if (page < 0) continue;
+          const int key = at + 16 * k + 4 * g;
+          u32x4 vis, x;
+#pragma unroll
+          for (int w = 0; w < 4; ++w) {
+            const int e = key + 8 * (w >> 1) + 2 * (w & 1);
+            vis[w] = (e < limit ? one_bits<T>() : 0u) | (e + 1 < limit ? one_bits<T>() << 16 : 0u);
+          }
+#pragma unroll
+          for (int d = 0; d < DT; ++d) {
+            const uint8_t* p = a.vc + ((size_t)page * a.n_kv + h) * (size_t)(D * P) + (size_t)(32 * d + ql) * P + (key & (P - 1));
+#pragma unroll
+            for (int w = 0; w < 4; ++w) {
+              const int e = 8 * (w >> 1) + 2 * (w & 1);
+              x[w] = ((p[e] & 0x7f) == 0x7f ? one_bits<T>() : 0u) | ((p[e + 1] & 0x7f) == 0x7f ? one_bits<T>() << 16 : 0u);
+            }
+            const f32x16 cnt = mfma32<T>(x, vis, f32x16{});
+#pragma unroll
+            for (int e = 0; e < 16; ++e)
+              if (cnt[e] > 0.f) acc[d][e] = __builtin_nanf("");
+          }
         }
       }
     }
@@ -723,11 +816,11 @@ static int launch_rows(const Args& a, hipStream_t s) {
   return MX_OK;
 }
 
-template <typename T, int D>
+template <typename T, int D, bool WIDE>
 static int launch_tiles(const Args& a, const Plan& p, hipStream_t s) {
   constexpr int lds = Stage<D>::LDS;
-  MX_RETURN_IF_HIP((lds_limit_once<tile_kernel<T, D>>(lds)));
-  hipLaunchKernelGGL((tile_kernel<T, D>), dim3((unsigned)(a.B * a.n_kv), (unsigned)p.tiles, (unsigned)a.splits), dim3(64 * TW),
+  MX_RETURN_IF_HIP((lds_limit_once<tile_kernel<T, D, WIDE>>(lds)));
+  hipLaunchKernelGGL((tile_kernel<T, D, WIDE>), dim3((unsigned)(a.B * a.n_kv), (unsigned)p.tiles, (unsigned)a.splits), dim3(64 * TW),
                      lds, s, a);
   MX_RETURN_IF_HIP(hipGetLastError());
   return MX_OK;
@@ -735,7 +828,7 @@ static int launch_tiles(const Args& a, const Plan& p, hipStream_t s) {
 
 template <typename T, int D>
 static int run(const Args& a, const Plan& p, hipStream_t s) {
-  const int rc = p.nr == 1 ? launch_rows<T, D, 1>(a, s) : p.nr == 2 ? launch_rows<T, D, 2>(a, s) : launch_tiles<T, D>(a, p, s);
+  const int rc = p.nr == 1 ? launch_rows<T, D, 1>(a, s) : p.nr == 2 ? launch_rows<T, D, 2>(a, s) : a.lp >= 6 ? launch_tiles<T, D, true>(a, p, s) : launch_tiles<T, D, false>(a, p, s);
   if (rc != MX_OK || p.splits == 1) return rc;
   const long long rows = (long long)a.T * a.n_q;
   hipLaunchKernelGGL((combine_kernel<T, D>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, s, a);
