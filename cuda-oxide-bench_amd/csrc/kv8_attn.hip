@@ -68,6 +68,32 @@ __device__ __forceinline__ uint32_t nan_bytes(uint32_t x) { return ((x & 0x7f7f7
 // 0xff for each byte of a nan_bytes() dword that is set.
 __device__ __forceinline__ uint32_t spread(uint32_t m) { return (m >> 7) * 0xffu; }
 
+// MFMA operands of ones and zeros, their product counts the NaNs that a row sees: which of keys
+// at .. at + 7 lie below limit, and which of 8 codes are NaN.
+template <typename T>
+__device__ __forceinline__ u32x4 visible8(int at, int limit) {
+  u32x4 v;
+#pragma unroll
+  for (int w = 0; w < 4; ++w)
+    v[w] = (at + 2 * w < limit ? one_bits<T>() : 0u) | (at + 2 * w + 1 < limit ? one_bits<T>() << 16 : 0u);
+  return v;
+}
+template <typename T>
+__device__ __forceinline__ u32x4 nans8(uint32_t lo, uint32_t hi) {
+  u32x4 v;
+#pragma unroll
+  for (int w = 0; w < 4; ++w) {
+    const uint32_t two = nan_bytes(w < 2 ? lo : hi) >> (16 * (w & 1));
+    v[w] = ((two & 0x80u) ? one_bits<T>() : 0u) | ((two & 0x8000u) ? one_bits<T>() << 16 : 0u);
+  }
+  return v;
+}
+// x of any of the lanes l, l ^ 16, l ^ 32, l ^ 48
+__device__ __forceinline__ bool any_group(bool x) {
+  const int v = (int)x | __shfl_xor((int)x, 16, 64);
+  return v | __shfl_xor(v, 32, 64);
+}
+
 // ---------------------------------------------------------------------------
 // Few rows per sequence (decode, a few speculated tokens): the cache is read once
 // from HBM into registers.  A workgroup takes one KV head of a sequence and one
@@ -245,27 +271,12 @@ __global__ __launch_bounds__(64 * NW, NR == 1 ? 2 : 1) void rows_kernel(const Ar
           // see, and take them out of the product
 #pragma unroll
           for (int i = 0; i < NR; ++i) {
-            u32x4 vis[2];
-#pragma unroll
-            for (int u = 0; u < 2; ++u)
-#pragma unroll
-              for (int w = 0; w < 4; ++w) {
-                const int e = 8 * u + 2 * w;
-                vis[u][w] = (key0 + e < limit[i] ? one_bits<T>() : 0u) | (key0 + e + 1 < limit[i] ? one_bits<T>() << 16 : 0u);
-              }
+            const u32x4 vis[2] = {visible8<T>(key0, limit[i]), visible8<T>(key0 + 8, limit[i])};
 #pragma unroll
             for (int d = 0; d < DT; ++d) {
               f32x4 cnt{};
 #pragma unroll
-              for (int u = 0; u < 2; ++u) {
-                u32x4 x;
-#pragma unroll
-                for (int w = 0; w < 4; ++w) {
-                  const uint32_t two = nan_bytes(vx[d][2 * u + (w >> 1)]) >> (16 * (w & 1));
-                  x[w] = ((two & 0x80u) ? one_bits<T>() : 0u) | ((two & 0x8000u) ? one_bits<T>() << 16 : 0u);
-                }
-                cnt = mfma16<T>(x, vis[u], cnt);
-              }
+              for (int u = 0; u < 2; ++u) cnt = mfma16<T>(nans8<T>(vx[d][2 * u], vx[d][2 * u + 1]), vis[u], cnt);
 #pragma unroll
               for (int j = 0; j < 4; ++j)
                 if (cnt[j] > 0.f) acc[i][d][j] = __builtin_nanf("");
@@ -298,8 +309,7 @@ __global__ __launch_bounds__(64 * NW, NR == 1 ? 2 : 1) void rows_kernel(const Ar
 #pragma unroll
     for (int i = 0; i < NR; ++i) {
       l[i] = sum_xor32(sum_xor16(l[i]));
-      const bool met = __shfl_xor((int)seen[i], 16, 64) | __shfl_xor((int)seen[i], 32, 64) |
-                       __shfl_xor((int)seen[i], 48, 64) | (int)seen[i];
+      const bool met = any_group(seen[i]);
       if (g == 0) {
         ml[((wave * NR + i) * 16 + r16) * 2] = met && m[i] == -INFINITY ? kNoScore : m[i];
         ml[((wave * NR + i) * 16 + r16) * 2 + 1] = l[i];
@@ -348,46 +358,52 @@ __global__ __launch_bounds__(64 * NW, NR == 1 ? 2 : 1) void rows_kernel(const Ar
 }
 
 // ---------------------------------------------------------------------------
-// Many rows per sequence (prompts and their chunks): a workgroup of 8 waves takes 256
+// Many rows per sequence (prompts and their chunks): a workgroup of TW waves takes 32 TW
 // rows (row = token * G + head of the group) of one KV head, 32 a wave, and walks
 // the keys in tiles of 64.  A tile's codes go HBM -> registers one tile ahead, are
 // widened to 16 bits once per workgroup and written to one of two LDS stages; every
-// wave then reads its 32x32x16 MFMA operands from there: K as stored, V from its
-// transposed page, in the order of keys that a score tile leaves in a lane's
-// registers, so that P' is the second product's operand as it is.
+// wave reads its MFMA operands from there.  Rows, keys and channels sit in the lanes as in
+// rows_kernel: a lane's 16 keys are a piece of one page, with one set of scales.
+//
+// 16x16x32 MFMAs: for the same products 32x32x16 ones read and write twice the
+// accumulator registers, and the power that takes costs clock.
 // ---------------------------------------------------------------------------
-constexpr int TW = 8;           // waves
-constexpr int TR = 32 * TW;     // rows of a workgroup
+#ifndef KV8_TW
+#define KV8_TW 8
+#endif
 constexpr int BN = 64;          // keys of a tile
 constexpr float kLazy = 8.0f;   // log2 units that a score may pass the running maximum by before it moves
 
 template <int D>
 struct Stage {
   static constexpr int K = BN * D * 2, V = D * BN * 2;
-  static constexpr int BYTES = K + V;
-  static constexpr int CONSTS = 2 * BYTES;            // [2][4 groups of 16 keys] x {cs, lv, iv, 0}
+  static constexpr int V_OFF = 2 * K;                 // two stages of K, three of V
+  static constexpr int CONSTS = V_OFF + 3 * V;        // [2][4 groups of 16 keys] x {cs, lv, iv, 0}
   static constexpr int FLAGS = CONSTS + 2 * 4 * 16;   // tiles with a NaN among V's codes
   static constexpr int LDS = FLAGS + 16;
 };
-// 16-byte slot of a row, swizzled so that the 16 lanes LDS serves together hit different
-// slots of its 256-byte window.
-template <int ROW>
-__device__ __forceinline__ int slot_at(int row, int slot) {
-  return ROW == 256 ? slot ^ (row & 15) : slot ^ ((row >> 1) & 7);
+// 16-byte slots of a row, swizzled so that the 16 lanes that LDS serves together hit
+// different slots of its 256-byte window.  K: a fragment's rows are 16 i + 4 t + 0..3, i = 0..3;
+// V: 16 consecutive ones.
+template <int D>
+__device__ __forceinline__ int k_slot(int row, int slot) {
+  return D == 128 ? slot ^ ((row & 3) | ((row >> 4) & 3) << 2) : slot ^ (((row >> 1) & 1) | ((row >> 4) & 3) << 1);
 }
+__device__ __forceinline__ int v_slot(int row, int slot) { return slot ^ ((row >> 1) & 7); }
 
-// WIDE: pages of 64 tokens and more, one page and one set of scales per tile.
-template <typename T, int D, bool WIDE>
-__global__ __launch_bounds__(64 * TW, 1) void tile_kernel(const Args a) {
+// WIDE: pages of 64 tokens and more.  A tile then has one page, whose address the scalar unit
+// works out; its threads add an offset that never changes.
+template <typename T, int D, int TW, bool WIDE>
+__global__ __launch_bounds__(64 * TW, 2) void tile_kernel(const Args a) {
   using L = Stage<D>;
-  constexpr int DC = D / 16, DT = D / 32;
-  constexpr int NT = 64 * TW;
+  constexpr int KC = D / 32, DT = D / 16;
+  constexpr int NT = 64 * TW, TR = 32 * TW;
   constexpr int U = D * 8 / NT;  // 16-byte units of a tile (K, then V) per thread
   static_assert(U >= 1 && U * NT == D * 8, "units");
   extern __shared__ __align__(1024) unsigned char smem[];
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int ql = lane & 31, g = lane >> 5;
+  const int r16 = lane & 15, g = lane >> 4;
   const int G = a.n_q / a.n_kv;
   const int h = blockIdx.x % a.n_kv, b = blockIdx.x / a.n_kv;
   const int split = blockIdx.z;
@@ -399,6 +415,7 @@ __global__ __launch_bounds__(64 * TW, 1) void tile_kernel(const Args a) {
   const int s0 = min((long long)split * a.chunk, (long long)len);
   const int s1 = split + 1 == a.splits ? len : min(len, s0 + a.chunk);
   const int* row_pages = a.table + (size_t)b * a.max_pages;
+  const int last_col = a.max_pages - 1;
   const float c = fabsf(a.c);
   const uint32_t flip = a.c < 0.f ? 0x80008000u : 0u;
   const uint32_t lds0 = lds_addr(smem);
@@ -412,72 +429,111 @@ __global__ __launch_bounds__(64 * TW, 1) void tile_kernel(const Args a) {
     };
     const int low = sees(0), high = min(sees(rows - 1), s1);
     const int tiles = high > s0 ? (high - s0 + BN - 1) / BN : 0;
-    const int r = 32 * wave + ql;
-    const int rr = min(r, rows - 1);
-    const int limit = min(sees(rr), s1);
-    const int w_low = sees(min(32 * wave, rows - 1)), w_high = min(sees(min(32 * wave + 31, rows - 1)), s1);
+    const int w_low = min(sees(min(32 * wave, rows - 1)), s1), w_high = min(sees(min(32 * wave + 31, rows - 1)), s1);
     const bool idle = 32 * wave >= rows;
-    const int tok = (int)((r0 + rr) / (uint32_t)G), head = h * G + (int)((r0 + rr) % (uint32_t)G);
-
-    u32x4 qf[DC];
-    {
-      const uint16_t* src = a.q + (size_t)(rw.first + tok) * a.q_stride + head * D + 8 * g;
+    int limit[2], tok[2], head[2];
+    u32x4 qf[2][KC];
 #pragma unroll
-      for (int k = 0; k < DC; ++k) qf[k] = ld128(src + 16 * k) ^ u32x4{flip, flip, flip, flip};
+    for (int i = 0; i < 2; ++i) {
+      const int rr = min(32 * wave + 16 * i + r16, rows - 1);
+      limit[i] = min(sees(rr), s1);
+      tok[i] = (int)((r0 + rr) / (uint32_t)G);
+      head[i] = h * G + (int)((r0 + rr) % (uint32_t)G);
+      const uint16_t* src = a.q + (size_t)(rw.first + tok[i]) * a.q_stride + head[i] * D + 8 * g;
+#pragma unroll
+      for (int k = 0; k < KC; ++k) qf[i][k] = ld128(src + 32 * k) ^ u32x4{flip, flip, flip, flip};
     }
 
     // ---- a tile's codes: unit id < 4 D: K, row id / (D/16); else V, channel.  Page
     // numbers are looked up a tile before the codes are loaded, those a tile before
-    // they are widened.  Past the last tile: page -1, zeros into a stage nobody reads. ----
+    // they are widened.  Past the last tile: zeros into a stage nobody reads. ----
     u32x4 raw[U];
     float rks = 0.f, rvs = 0.f;
     int page_n[U], page_s;
     bool bad[U], bad_s = true;
+    auto is_k = [&](int u) { return (u + 1) * NT <= 4 * D ? true : u * NT >= 4 * D ? false : tid + u * NT < 4 * D; };
     auto key_of = [&](int u) {
       const int id = tid + u * NT;
-      return id < 4 * D ? id / (D / 16) : (id - 4 * D) % 4 * 16;
+      return is_k(u) ? id / (D / 16) : id % 4 * 16;
     };
-    const int last_col = a.max_pages - 1;
+    auto offset_of = [&](int u, int slot) {  // of unit u in its page, slot: the token of its first byte
+      const int id = tid + u * NT;
+      return (uint32_t)(is_k(u) ? slot * D + id % (D / 16) * 16 : (id - 4 * D) / 4 * P + slot);
+    };
+    uint32_t wide_off[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) wide_off[u] = offset_of(u, key_of(u));
     auto find = [&](int tile) {
       const int at = s0 + BN * tile;
+      if constexpr (WIDE) {
+        page_s = row_pages[min(at >> a.lp, last_col)];
+      } else {
 #pragma unroll
-      for (int u = 0; u < U; ++u) page_n[u] = row_pages[min((at + key_of(u)) >> a.lp, last_col)];
-      page_s = row_pages[min((at + 16 * (tid & 3)) >> a.lp, last_col)];
+        for (int u = 0; u < U; ++u) page_n[u] = row_pages[min((at + key_of(u)) >> a.lp, last_col)];
+        page_s = row_pages[min((at + 16 * (tid & 3)) >> a.lp, last_col)];
+      }
     };
     auto load = [&](int tile) {
       const int at = s0 + BN * tile;
+      constexpr int LD = D == 128 ? 7 : 6;
+      if constexpr (WIDE) {
+        const int page = __builtin_amdgcn_readfirstlane(page_s);
+        bad_s = at >= high || (uint32_t)page >= (uint32_t)a.pages;
+        const uint32_t ph = (uint32_t)((bad_s ? 0 : page) * a.n_kv + h);
+        const uint64_t base = (uint64_t)ph << (a.lp + LD);
+        const uint32_t half = at & (P - 1);  // 64 in the second tile of a page of 128
+        const uint8_t *kp = a.kc + base + half * D, *vp = a.vc + base + half;
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const int id = tid + u * NT, key = at + key_of(u);
-        bad[u] = key >= high || (uint32_t)page_n[u] >= (uint32_t)a.pages;
-        const size_t page = ((size_t)(uint32_t)(bad[u] ? 0 : page_n[u]) * a.n_kv + h) * (size_t)(D * P);
-        raw[u] = ld128(id < 4 * D ? a.kc + page + (size_t)(key & (P - 1)) * D + id % (D / 16) * 16
-                                  : a.vc + page + (size_t)((id - 4 * D) / 4) * P + (key & (P - 1)));
+        for (int u = 0; u < U; ++u) {
+          bad[u] = bad_s || at + key_of(u) >= high;
+          raw[u] = ld128((is_k(u) ? kp : vp) + wide_off[u]);
+        }
+        rks = a.ks[ph];
+        rvs = a.vs[ph];
+        bad_s |= at + 16 * (tid & 3) >= high;
+      } else {
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          const int key = at + key_of(u);
+          bad[u] = key >= high || (uint32_t)page_n[u] >= (uint32_t)a.pages;
+          const uint64_t page = (uint64_t)(uint32_t)((bad[u] ? 0 : page_n[u]) * a.n_kv + h) << (a.lp + LD);
+          raw[u] = ld128((is_k(u) ? a.kc : a.vc) + page + offset_of(u, key & (P - 1)));
+        }
+        bad_s = at + 16 * (tid & 3) >= high || (uint32_t)page_s >= (uint32_t)a.pages;
+        const uint32_t page = (uint32_t)((bad_s ? 0 : page_s) * a.n_kv + h);
+        rks = a.ks[page];
+        rvs = a.vs[page];
       }
-      bad_s = at + 16 * (tid & 3) >= high || (uint32_t)page_s >= (uint32_t)a.pages;
-      const size_t page = (size_t)(uint32_t)(bad_s ? 0 : page_s) * a.n_kv + h;
-      rks = a.ks[page];
-      rvs = a.vs[page];
     };
-    // Tiles from first_masked on are not seen whole by every row: at most 6, bits of *flags.
+    // Before a loaded tile is stored: the codes of pages that are none become 0.  Tiles from
+    // first_masked on are not seen whole by every row: at most TR / 64 + 2 with a causal
+    // mask, bits of *flags.  There V's codes of tokens past the last become 0, and so do
+    // NaNs, which are flagged (without a causal mask every row sees every token that is
+    // there).
     int* flags = reinterpret_cast<int*>(smem + L::FLAGS);
     const int first_masked = low > s0 ? (low - s0) / BN : 0;
-    // A tile that some row does not see whole: V's codes of tokens past the last become 0,
-    // and so do NaNs, which are flagged (with a causal mask: without one every row sees
-    // every token that is there).
     auto clean = [&](int tile) {
       const int at = s0 + BN * tile;
+      const bool partial = at + BN > low;
+      bool none = false;  // a tile that is seen whole has no keys past the last
+      if constexpr (WIDE) {
+        none = bad_s;
+      } else {
+#pragma unroll
+        for (int u = 0; u < U; ++u) none |= bad[u];
+      }
+      if (!partial && !__any(none)) return;
       bool nan = false;
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-        const int id = tid + u * NT;
-        if (id >= 4 * D) {
-          const int left = high - at - (id - 4 * D) % 4 * 16;
+        if (bad[u]) raw[u] = u32x4{};
+        if (partial && !is_k(u)) {
+          const int left = high - at - key_of(u);
 #pragma unroll
           for (int w = 0; w < 4; ++w) {
 #pragma unroll
             for (int j = 0; j < 4; ++j)
-              if (bad[u] || 4 * w + j >= left) raw[u][w] &= ~(0xffu << (8 * j));
+              if (4 * w + j >= left) raw[u][w] &= ~(0xffu << (8 * j));
             const uint32_t bits = a.causal ? nan_bytes(raw[u][w]) : 0u;
             nan |= bits != 0;
             raw[u][w] &= ~spread(bits);
@@ -486,37 +542,47 @@ __global__ __launch_bounds__(64 * TW, 1) void tile_kernel(const Args a) {
       }
       if (__any(nan) && lane == 0) atomicOr(flags, 1 << (tile - first_masked));
     };
-    // unit u of the loaded tile into the stage at byte st
-    auto store = [&](int u, int st) {
-      const int id = tid + u * NT;
-      const u32x4 x = bad[u] ? u32x4{} : raw[u];
-      if (id < 4 * D) {
-        const int row = id / (D / 16), slot = id % (D / 16) * 2;
-        st128(smem + st + row * (2 * D) + 16 * slot_at<2 * D>(row, slot), widen8<T>(x[0], x[1]));
-        st128(smem + st + row * (2 * D) + 16 * slot_at<2 * D>(row, slot + 1), widen8<T>(x[2], x[3]));
-      } else {
-        const int row = (id - 4 * D) / 4, slot = (id - 4 * D) % 4 * 2;
-        st128(smem + st + L::K + row * (2 * BN) + 16 * slot_at<2 * BN>(row, slot), widen8<T>(x[0], x[2]));
-        st128(smem + st + L::K + row * (2 * BN) + 16 * slot_at<2 * BN>(row, slot + 1), widen8<T>(x[1], x[3]));
+    // unit u of the loaded tile into its stage: 16 channels of a K row are its slots 2 i,
+    // 2 i + 1, 16 keys of a V row (a lane group's) slots g (keys 0..7) and 4 + g
+    uint32_t put[U][2];
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int v = 0; v < 2; ++v) {
+        const int id = tid + u * NT;
+        const int kr = id / (D / 16), vr = (id - 4 * D) / 4;
+        put[u][v] = is_k(u) ? kr * (2 * D) + 16 * k_slot<D>(kr, id % (D / 16) * 2 + v)
+                            : L::V_OFF + vr * (2 * BN) + 16 * v_slot(vr, id % 4 + 4 * v);
       }
+    auto store = [&](int u, int k_st, int v_st) {
+      const int st = is_k(u) ? k_st : v_st;
+      st128(smem + put[u][0] + st, widen8<T>(raw[u][0], raw[u][1]));
+      st128(smem + put[u][1] + st, widen8<T>(raw[u][2], raw[u][3]));
     };
     auto store_consts = [&](int stage) {
       if (tid < 4)
         *reinterpret_cast<f32x4*>(smem + L::CONSTS + (stage * 4 + tid) * 16) =
-            bad_s ? f32x4{0.f, -INFINITY, 0.f, 0.f} : f32x4{c * rks, __builtin_amdgcn_logf(rvs), 1.0f / rvs, 0.f};
+            f32x4{bad_s ? 0.f : c * rks, bad_s ? -INFINITY : __builtin_amdgcn_logf(rvs),
+                  bad_s ? 0.f : __builtin_amdgcn_rcpf(rvs), 0.f};
     };
 
-    // K fragment: key row 32 t + ql, slot 2 k + g; V fragment: channel row 32 d + ql, slot
-    // 2 k + g of the tile's 16-key chunk k.  The swizzle is an xor, so slot 2 k is an xor away
-    // from slot 0: one register each, made opaque in every tile lest all of them be kept.
-    const uint32_t k_base = lds0 + ql * (2 * D) + 16 * slot_at<2 * D>(ql, g);
-    const uint32_t v_base = lds0 + L::K + ql * (2 * BN) + 16 * slot_at<2 * BN>(ql, g);
+    // K fragment t: key row 16 (r16 / 4) + 4 t + r16 % 4, slot 4 k + g; V fragment d:
+    // channel row 16 d + r16, slot 4 u + g.  The swizzle is an xor, so slot 4 k is an xor away
+    // from slot 0.
+    const int k_row = 16 * (r16 >> 2) + (r16 & 3);
+    const uint32_t k_base = lds0 + k_row * (2 * D) + 16 * k_slot<D>(k_row, g);
+    const uint32_t v_base = lds0 + L::V_OFF + r16 * (2 * BN) + 16 * v_slot(r16, g);
 
-    f32x16 acc[DT];
+    f32x4 acc[2][DT];
+    float m[2] = {0.f, 0.f}, l[2] = {0.f, 0.f};
+    bool open = true, seen[2] = {false, false};
+    u32x4 pf[2][2];  // P' of the tile before, 8 keys of a lane each
 #pragma unroll
-    for (int d = 0; d < DT; ++d) acc[d] = f32x16{};
-    float m = 0.f, l = 0.f;
-    bool open = true, seen = false;
+    for (int i = 0; i < 2; ++i) {
+      pf[i][0] = pf[i][1] = u32x4{};
+#pragma unroll
+      for (int d = 0; d < DT; ++d) acc[i][d] = f32x4{};
+    }
 
     // LDS writes done, then the barrier: no wait for the loads that are under way
     auto meet = [&] {
@@ -525,158 +591,188 @@ __global__ __launch_bounds__(64 * TW, 1) void tile_kernel(const Args a) {
     };
     __syncthreads();  // the stages and flags are free
     if (tid == 0) *flags = 0;
-    if (a.causal) __syncthreads();
     if (tiles > 0) {
+      // V's last stage, the first tile's "tile before": zeros
+      for (int i = tid; i < L::V / 16; i += NT) st128(smem + L::V_OFF + 2 * L::V + 16 * i, u32x4{});
       find(0);
       load(0);
       find(1);
-      if (s0 + BN > low) clean(0);
+    }
+    if (a.causal) __syncthreads();
+    if (tiles > 0) {
+      clean(0);
 #pragma unroll
-      for (int u = 0; u < U; ++u) store(u, 0);
+      for (int u = 0; u < U; ++u) store(u, 0, 0);
       store_consts(0);
       load(1);
       find(2);
     }
-    auto step = [&](int tile, auto stage_tag) {
-      constexpr int STG = decltype(stage_tag)::value;
-      constexpr uint32_t st = STG * L::BYTES, other = (1 - STG) * L::BYTES;
-      meet();  // the tile's stage is written, the other one read
-      const int at = s0 + BN * tile;
-      if (at + 2 * BN > low) clean(tile + 1);
-      if (idle || at >= w_high) {  // nothing to compute: the wave's share of the next tile
-#pragma unroll
-        for (int u = 0; u < U; ++u) store(u, other);
-        store_consts(1 - STG);
-        load(tile + 2);
-        find(tile + 3);
-        return;
-      }
+    const int mine = idle ? 0 : w_high > s0 ? (w_high - s0 + BN - 1) / BN : 0;  // tiles that the wave's rows see
 
-      // ---- S^T, the next tile's codes widened and stored beside its MFMAs ----
-      __builtin_amdgcn_s_setprio(1);
-      f32x16 s[2];
-      u32x4 kb[3][2];
-      uint32_t kb0 = k_base;
-      asm volatile("" : "+v"(kb0));
-      auto kread = [&](int t, int k) { return lds_ld128((kb0 ^ (32 * k)) + st + 32 * t * (2 * D)); };
+    // V fragment e: half u = e / DT of the keys, channels d = e % DT
+    auto vread = [&](uint32_t vb0, int e) { return lds_ld128((vb0 ^ (64 * (e / DT))) + 16 * (e % DT) * (2 * BN)); };
+    // One tile: S^T beside the next tile's widening, then the product of the tile
+    // before beside this tile's softmax, so that neither MFMAs nor VALU wait for the other.
+    // P' is taken with the maximum as it was: a tile that moves it (or meets a row's first
+    // keys) is seen at the vote behind, and its scores are then computed once more.
+    auto step = [&](int tile, int v_old, int v_new, auto masked_tag) {
+      constexpr bool MASKED = decltype(masked_tag)::value;
+      const int at = s0 + BN * tile;
+      const uint32_t kb0 = k_base + (tile & 1) * L::K, vb0 = v_base + v_old * L::V;
+      auto kread = [&](int k, int t) { return lds_ld128((kb0 ^ (64 * k)) + 4 * t * (2 * D)); };
+
+      f32x4 s[2][4];
+      u32x4 kb[2][4], vb[DT];
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        kb[i][0] = kread(0, i);
-        kb[i][1] = kread(1, i);
-      }
+      for (int t = 0; t < 4; ++t) kb[0][t] = kread(0, t);
 #pragma unroll
-      for (int k = 0; k < DC; ++k) {
-        if (k + 2 < DC) {
-          kb[(k + 2) % 3][0] = kread(0, k + 2);
-          kb[(k + 2) % 3][1] = kread(1, k + 2);
+      for (int k = 0; k < KC; ++k) {
+        if (k + 1 < KC) {
+#pragma unroll
+          for (int t = 0; t < 4; ++t) kb[(k + 1) & 1][t] = kread(k + 1, t);
+        } else {
+#pragma unroll
+          for (int d = 0; d < DT; ++d) vb[d] = vread(vb0, d);
         }
 #pragma unroll
-        for (int t = 0; t < 2; ++t) s[t] = mfma32<T>(kb[k % 3][t], qf[k], k ? s[t] : f32x16{});
+        for (int t = 0; t < 4; ++t)
+#pragma unroll
+          for (int i = 0; i < 2; ++i) s[i][t] = mfma16<T>(kb[k & 1][t], qf[i][k], k ? s[i][t] : f32x4{});
 #pragma unroll
         for (int u = 0; u < U; ++u)
-          if (k == 1 + u * 2) store(u, other);
-        if (k == DC - 1) {
-          store_consts(1 - STG);
+          if (k == u * KC / U) store(u, ((tile + 1) & 1) * L::K, v_new * L::V);
+        if (k == KC - 1) {
+          store_consts((tile + 1) & 1);
           load(tile + 2);
           find(tile + 3);
         }
         __builtin_amdgcn_sched_barrier(0);
       }
-      f32x4 cst[WIDE ? 1 : 4];
-#pragma unroll
-      for (int u = 0; u < (WIDE ? 1 : 4); ++u) cst[u] = *reinterpret_cast<const f32x4*>(smem + L::CONSTS + (STG * 4 + u) * 16);
-      uint32_t vb0 = v_base;
-      asm volatile("" : "+v"(vb0));
-      auto vread = [&](int k, int d) { return lds_ld128((vb0 ^ (32 * k)) + st + 32 * d * (2 * BN)); };
-      u32x4 vb[2][DT];
-#pragma unroll
-      for (int d = 0; d < DT; ++d) vb[0][d] = vread(0, d);
-      __builtin_amdgcn_s_setprio(0);
 
-      // ---- y - m, the running maximum ----
-      float mx = -INFINITY;
-      const bool masked = at + BN > min(w_low, s1);
-#pragma unroll
-      for (int t = 0; t < 2; ++t)
+      const f32x4 cst = *reinterpret_cast<const f32x4*>(smem + L::CONSTS + ((tile & 1) * 4 + g) * 16);
+      auto exponents = [&](int i) {  // y - m, masked; the lane's maximum
+        const float off = cst[1] - m[i];
+        float mx = -INFINITY;
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
-          const f32x4& k = cst[WIDE ? 0 : 2 * t + (e >> 3)];
-          s[t][e] = __builtin_fmaf(s[t][e], k[0], k[1] - m);
+          float x = __builtin_fmaf(s[i][e >> 2][e & 3], cst[0], off);
+          if constexpr (MASKED) x = at + 16 * g + e < limit[i] ? x : -INFINITY;
+          s[i][e >> 2][e & 3] = x;
+          mx = fmaxf(mx, x);
         }
-      if (masked) {
+        return mx;
+      };
+      u32x4 pn[2][2];
+      float sum[2];
+      auto expo = [&](int i) {
+        sum[i] = 0.f;
 #pragma unroll
-        for (int t = 0; t < 2; ++t)
+        for (int t = 0; t < 4; ++t) {
+          f32x4 p;
 #pragma unroll
-          for (int e = 0; e < 16; ++e)
-            s[t][e] = at + 32 * t + 8 * (e >> 2) + 4 * g + (e & 3) < limit ? s[t][e] : -INFINITY;
+          for (int j = 0; j < 4; ++j) p[j] = __builtin_amdgcn_exp2f(s[i][t][j]);
+          sum[i] += (p[0] + p[1]) + (p[2] + p[3]);
+          pn[i][t >> 1][2 * (t & 1)] = T::pack2(p[0], p[1]);
+          pn[i][t >> 1][2 * (t & 1) + 1] = T::pack2(p[2], p[3]);
+        }
+      };
+      float mx[2];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        mx[i] = exponents(i);
+        expo(i);
       }
 #pragma unroll
-      for (int t = 0; t < 2; ++t)
+      for (int e = 0; e < 2 * DT; ++e) {
 #pragma unroll
-        for (int e = 0; e < 16; ++e) mx = fmaxf(mx, s[t][e]);
-      mx = max_xor32(mx);
-      const bool moved = __any(mx > kLazy);
-      if (moved || open) {
-        const bool empty = open && sum_xor32(l) == 0.f, met = mx > -INFINITY;
-        const float shift = empty ? (met ? mx : 0.f) : moved ? fmaxf(mx, 0.f) : 0.f;
-        open = __any(empty && !met);
-#pragma unroll
-        for (int u = 0; u < (WIDE ? 1 : 4); ++u) seen |= cst[u][1] > -INFINITY && at + 16 * u < limit;
-        m += shift;
-        const float corr = empty ? 1.f : __builtin_amdgcn_exp2f(-shift);
-        l *= corr;
-#pragma unroll
-        for (int d = 0; d < DT; ++d) acc[d] *= corr;
-#pragma unroll
-        for (int t = 0; t < 2; ++t)
-#pragma unroll
-          for (int e = 0; e < 16; ++e) s[t][e] -= shift;
+        for (int i = 0; i < 2; ++i) acc[i][e % DT] = mfma16<T>(vb[e % DT], pf[i][e / DT], acc[i][e % DT]);
+        if (e + DT < 2 * DT) vb[e % DT] = vread(vb0, e + DT);
       }
+#pragma unroll
+      for (int e = 0; e < 4 * DT; ++e) {
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+        if (e & 1) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x002, 128 / (4 * DT), 0);
+      }
+      __builtin_amdgcn_sched_barrier(0);
 
-      // ---- P', O^T += V^T P'^T by chunks of 16 keys: the next chunk's exponentials and
-      // V reads run beside a chunk's MFMAs ----
+      const bool moved = __any(fmaxf(mx[0], mx[1]) > kLazy);
+      if (moved || open) {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) s[0][e] = __builtin_amdgcn_exp2f(s[0][e]);
-      __builtin_amdgcn_s_setprio(1);
-      float sum = 0.f;
+        for (int k = 0; k < KC; ++k)
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        f32x16& x = s[k >> 1];
-        const int o = 8 * (k & 1);
-        const u32x4 pf{T::pack2(x[o], x[o + 1]), T::pack2(x[o + 2], x[o + 3]), T::pack2(x[o + 4], x[o + 5]),
-                       T::pack2(x[o + 6], x[o + 7])};
-        const float part = ((x[o] + x[o + 1]) + (x[o + 2] + x[o + 3])) + ((x[o + 4] + x[o + 5]) + (x[o + 6] + x[o + 7]));
-        if constexpr (WIDE)
-          sum += part;
-        else
-          l = __builtin_fmaf(part, cst[WIDE ? 0 : k][2], l);
-        if (k + 1 < 4) {
+          for (int t = 0; t < 4; ++t) {
+            const u32x4 kf = kread(k, t);
 #pragma unroll
-          for (int d = 0; d < DT; ++d) vb[(k + 1) & 1][d] = vread(k + 1, d);
-          const int o1 = 8 * ((k + 1) & 1);
-#pragma unroll
-          for (int e = 0; e < 8; ++e) s[(k + 1) >> 1][o1 + e] = __builtin_amdgcn_exp2f(s[(k + 1) >> 1][o1 + e]);
-        }
-#pragma unroll
-        for (int d = 0; d < DT; ++d) acc[d] = mfma32<T>(vb[k & 1][d], pf, acc[d]);
-        if (k + 1 < 4) {
-          __builtin_amdgcn_sched_group_barrier(0x002, 4, 0);
-#pragma unroll
-          for (int d = 0; d < DT; ++d) {
-            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-            __builtin_amdgcn_sched_group_barrier(0x400, 8 / DT, 0);
-            __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
-            __builtin_amdgcn_sched_group_barrier(0x002, 8 / DT, 0);
+            for (int i = 0; i < 2; ++i) s[i][t] = mfma16<T>(kf, qf[i][k], k ? s[i][t] : f32x4{});
+            __builtin_amdgcn_sched_barrier(0);
           }
+        bool still = false;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          mx[i] = exponents(i);
+          mx[i] = max_xor32(max_xor16(mx[i]));
+          const bool empty = open && sum_xor32(sum_xor16(l[i])) == 0.f, met = mx[i] > -INFINITY;
+          const float shift = empty ? (met ? mx[i] : 0.f) : mx[i] > kLazy ? mx[i] : 0.f;
+          still |= empty && !met;
+          seen[i] |= cst[1] > -INFINITY && at + 16 * g < limit[i];
+          m[i] += shift;
+          const float corr = empty ? 1.f : __builtin_amdgcn_exp2f(-shift);
+          l[i] *= corr;
+#pragma unroll
+          for (int d = 0; d < DT; ++d) acc[i][d] *= corr;
+#pragma unroll
+          for (int e = 0; e < 16; ++e) s[i][e >> 2][e & 3] -= shift;
+          expo(i);
         }
-        __builtin_amdgcn_sched_barrier(0);
+        open = __any(still);
       }
-      if constexpr (WIDE) l = __builtin_fmaf(sum, cst[0][2], l);
-      __builtin_amdgcn_s_setprio(0);
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        l[i] = __builtin_fmaf(sum[i], cst[2], l[i]);
+        pf[i][0] = pn[i][0];
+        pf[i][1] = pn[i][1];
+      }
     };
-    for (int tile = 0; tile < tiles; tile += 2) {
-      step(tile, std::integral_constant<int, 0>{});
-      if (tile + 1 < tiles) step(tile + 1, std::integral_constant<int, 1>{});
+    auto last = [&](int v_old) {  // the product of the wave's last tile
+      const uint32_t vb0 = v_base + v_old * L::V;
+#pragma unroll
+      for (int e = 0; e < 2 * DT; ++e) {
+        const u32x4 vf = vread(vb0, e);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) acc[i][e % DT] = mfma16<T>(vf, pf[i][e / DT], acc[i][e % DT]);
+      }
+    };
+    // tiles that every row of the wave sees whole, those that some rows see in part, and
+    // those that only other waves need: three loops, so that each has one path
+    int v_old = 2, v_now = 0, v_new = 1;  // V's stages of the tile before, this one and the next
+    auto next = [&] {
+      const int v = v_old;
+      v_old = v_now;
+      v_now = v_new;
+      v_new = v;
+    };
+    const int whole = w_low > s0 ? min((w_low - s0) / BN, mine) : 0;
+    int tile = 0;
+    for (; tile < whole; ++tile, next()) {
+      meet();  // the tile's stages are written; K's other one and V's next are read
+      clean(tile + 1);
+      step(tile, v_old, v_new, std::false_type{});
+    }
+    for (; tile < mine; ++tile, next()) {
+      meet();
+      clean(tile + 1);
+      step(tile, v_old, v_new, std::true_type{});
+    }
+    if (mine > 0) last(v_old);
+    for (; tile < tiles; ++tile, next()) {
+      meet();
+      clean(tile + 1);
+#pragma unroll
+      for (int u = 0; u < U; ++u) store(u, ((tile + 1) & 1) * L::K, v_new * L::V);
+      store_consts((tile + 1) & 1);
+      load(tile + 2);
+      find(tile + 3);
     }
 
     // ---- a NaN among V's codes that some row does not see: those that it does see are
@@ -684,61 +780,53 @@ __global__ __launch_bounds__(64 * TW, 1) void tile_kernel(const Args a) {
     if (a.causal) {
       meet();
       for (int flagged = *flags; flagged; flagged &= flagged - 1) {
-        const int at = s0 + BN * (first_masked + __builtin_ctz(flagged));
-        for (int k = 0; k < 4; ++k) {
-          const int page = at + 16 * k < high ? page_of(row_pages, at + 16 * k, a.lp, a.max_pages, a.pages) : -1;
-          if (page < 0) continue;
-          const int key = at + 16 * k + 4 * g;
-          u32x4 vis, x;
+        const int key = s0 + BN * (first_masked + __builtin_ctz(flagged)) + 16 * g;  // the lane's keys
+        const int page = key < high ? page_of(row_pages, key, a.lp, a.max_pages, a.pages) : -1;
+        const uint8_t* p = a.vc + ((size_t)max(page, 0) * a.n_kv + h) * (size_t)(D * P) + (size_t)r16 * P + (key & (P - 1));
 #pragma unroll
-          for (int w = 0; w < 4; ++w) {
-            const int e = key + 8 * (w >> 1) + 2 * (w & 1);
-            vis[w] = (e < limit ? one_bits<T>() : 0u) | (e + 1 < limit ? one_bits<T>() << 16 : 0u);
-          }
+        for (int u = 0; u < 2; ++u) {
+          u32x4 vis[2];
 #pragma unroll
+          for (int i = 0; i < 2; ++i) vis[i] = visible8<T>(key + 8 * u, limit[i]);
           for (int d = 0; d < DT; ++d) {
-            const uint8_t* p = a.vc + ((size_t)page * a.n_kv + h) * (size_t)(D * P) + (size_t)(32 * d + ql) * P + (key & (P - 1));
+            const u32x2 v = page < 0 ? u32x2{} : ld64(p + (size_t)16 * d * P + 8 * u);
+            const u32x4 x = nans8<T>(v[0], v[1]);
 #pragma unroll
-            for (int w = 0; w < 4; ++w) {
-              const int e = 8 * (w >> 1) + 2 * (w & 1);
-              x[w] = ((p[e] & 0x7f) == 0x7f ? one_bits<T>() : 0u) | ((p[e + 1] & 0x7f) == 0x7f ? one_bits<T>() << 16 : 0u);
+            for (int i = 0; i < 2; ++i) {
+              const f32x4 cnt = mfma16<T>(x, vis[i], f32x4{});
+#pragma unroll
+              for (int dd = 0; dd < DT; ++dd)
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                  if (dd == d && cnt[j] > 0.f) acc[i][dd][j] = __builtin_nanf("");
             }
-            const f32x16 cnt = mfma32<T>(x, vis, f32x16{});
-#pragma unroll
-            for (int e = 0; e < 16; ++e)
-              if (cnt[e] > 0.f) acc[d][e] = __builtin_nanf("");
           }
         }
       }
     }
 
-    // ---- store: the lane's query, d = 32 dt + 8 i + 4 g + j ----
-    const float total = sum_xor32(l);
-    seen = __shfl_xor((int)seen, 32, 64) | (int)seen;
-    if (r < rows) {
-      const size_t orow = (size_t)(rw.first + tok) * a.n_q + head;
-      const bool none = total == 0.f && !seen;
+    // ---- store: the lane's query, d = 16 dt + 4 g + j ----
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const float total = sum_xor32(sum_xor16(l[i]));
+      const bool met = any_group(seen[i]);
+      if (32 * wave + 16 * i + r16 >= rows) continue;
+      const size_t orow = (size_t)(rw.first + tok[i]) * a.n_q + head[i];
+      const bool none = total == 0.f && !met;
       if (a.splits == 1) {
         const float inv = none ? 0.f : 1.0f / total;
 #pragma unroll
         for (int d = 0; d < DT; ++d)
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-            st64(a.out + orow * D + 32 * d + 8 * i + 4 * g,
-                 u32x2{T::pack2(acc[d][4 * i] * inv, acc[d][4 * i + 1] * inv),
-                       T::pack2(acc[d][4 * i + 2] * inv, acc[d][4 * i + 3] * inv)});
+          st64(a.out + orow * D + 16 * d + 4 * g, u32x2{T::pack2(acc[i][d][0] * inv, acc[i][d][1] * inv),
+                                                        T::pack2(acc[i][d][2] * inv, acc[i][d][3] * inv)});
       } else {
         const size_t all = (size_t)a.T * a.n_q;
         float* p = a.part + ((size_t)split * all + orow) * D;
 #pragma unroll
-        for (int d = 0; d < DT; ++d)
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-            *reinterpret_cast<f32x4*>(p + 32 * d + 8 * i + 4 * g) =
-                f32x4{acc[d][4 * i], acc[d][4 * i + 1], acc[d][4 * i + 2], acc[d][4 * i + 3]};
+        for (int d = 0; d < DT; ++d) *reinterpret_cast<f32x4*>(p + 16 * d + 4 * g) = acc[i][d];
         if (g == 0) {
           float* ml = a.part + (size_t)a.splits * all * D + ((size_t)split * all + orow) * 2;
-          ml[0] = none ? -INFINITY : total == 0.f ? kNoScore : m;
+          ml[0] = none ? -INFINITY : total == 0.f ? kNoScore : m[i];
           ml[1] = total;
         }
       }
@@ -797,7 +885,7 @@ static Plan plan(int B, int T, int max_q, int max_kv, int n_q, int n_kv) {
   const long long rows = (long long)max_q * G;
   Plan p;
   p.nr = rows <= 16 ? 1 : rows <= 32 ? 2 : 0;
-  p.tiles = (int)std::min((rows + TR - 1) / TR, 65535LL);
+  p.tiles = (int)std::min((rows + 32 * KV8_TW - 1) / (32 * KV8_TW), 65535LL);
   const long long units = (long long)B * n_kv * (p.nr ? 1 : p.tiles);
   const long long want = ((p.nr ? 2048 : 256) + units - 1) / units;
   long long chunk = (max_kv + want - 1) / want;
@@ -816,19 +904,19 @@ static int launch_rows(const Args& a, hipStream_t s) {
   return MX_OK;
 }
 
-template <typename T, int D, bool WIDE>
+template <typename T, int D, int TW, bool WIDE>
 static int launch_tiles(const Args& a, const Plan& p, hipStream_t s) {
   constexpr int lds = Stage<D>::LDS;
-  MX_RETURN_IF_HIP((lds_limit_once<tile_kernel<T, D, WIDE>>(lds)));
-  hipLaunchKernelGGL((tile_kernel<T, D, WIDE>), dim3((unsigned)(a.B * a.n_kv), (unsigned)p.tiles, (unsigned)a.splits), dim3(64 * TW),
-                     lds, s, a);
+  MX_RETURN_IF_HIP((lds_limit_once<tile_kernel<T, D, TW, WIDE>>(lds)));
+  hipLaunchKernelGGL((tile_kernel<T, D, TW, WIDE>), dim3((unsigned)(a.B * a.n_kv), (unsigned)p.tiles, (unsigned)a.splits),
+                     dim3(64 * TW), lds, s, a);
   MX_RETURN_IF_HIP(hipGetLastError());
   return MX_OK;
 }
 
 template <typename T, int D>
 static int run(const Args& a, const Plan& p, hipStream_t s) {
-  const int rc = p.nr == 1 ? launch_rows<T, D, 1>(a, s) : p.nr == 2 ? launch_rows<T, D, 2>(a, s) : a.lp >= 6 ? launch_tiles<T, D, true>(a, p, s) : launch_tiles<T, D, false>(a, p, s);
+  const int rc = p.nr == 1 ? launch_rows<T, D, 1>(a, s) : p.nr == 2 ? launch_rows<T, D, 2>(a, s) : a.lp >= 6 ? launch_tiles<T, D, KV8_TW, true>(a, p, s) : launch_tiles<T, D, KV8_TW, false>(a, p, s);
   if (rc != MX_OK || p.splits == 1) return rc;
   const long long rows = (long long)a.T * a.n_q;
   hipLaunchKernelGGL((combine_kernel<T, D>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, s, a);
