@@ -88,6 +88,31 @@ __device__ __forceinline__ u32x4 nans8(uint32_t lo, uint32_t hi) {
   }
   return v;
 }
+// The NaNs among a tile's V codes that rows see, into their sums.  The lane's 16 keys begin
+// at `key`, p points at their codes of channel r16 (`there`: on a page that is one), and the
+// products have the layout of the kernels' own.
+template <typename T, int D, int NR>
+__device__ __forceinline__ void add_nans(f32x4 (&acc)[NR][D / 16], const int (&limit)[NR], const uint8_t* p, bool there,
+                                         int key, int P) {
+#pragma unroll
+  for (int u = 0; u < 2; ++u) {
+    u32x4 vis[NR];
+#pragma unroll
+    for (int i = 0; i < NR; ++i) vis[i] = visible8<T>(key + 8 * u, limit[i]);
+#pragma unroll
+    for (int d = 0; d < D / 16; ++d) {
+      const u32x2 v = there ? ld64(p + (size_t)16 * d * P + 8 * u) : u32x2{};
+      const u32x4 x = nans8<T>(v[0], v[1]);
+#pragma unroll
+      for (int i = 0; i < NR; ++i) {
+        const f32x4 cnt = mfma16<T>(x, vis[i], f32x4{});
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (cnt[j] > 0.f) acc[i][d][j] = __builtin_nanf("");
+      }
+    }
+  }
+}
 // x of any of the lanes l, l ^ 16, l ^ 32, l ^ 48
 __device__ __forceinline__ bool any_group(bool x) {
   const int v = (int)x | __shfl_xor((int)x, 16, 64);
@@ -97,7 +122,7 @@ __device__ __forceinline__ bool any_group(bool x) {
 // ---------------------------------------------------------------------------
 // Few rows per sequence (decode, a few speculated tokens): the cache is read once
 // from HBM into registers.  A workgroup takes one KV head of a sequence and one
-// chunk of its tokens; its waves take 64-key tiles in turn and meet in LDS.
+// chunk of its tokens; its NW waves take 64-key tiles in turn and meet in LDS.
 //
 // 16x16x32 MFMAs on 16 NR rows (row = token * G + head of the group).  Row r of
 // score subtile t is key 16 (r / 4) + 4 t + r % 4 of the tile: lane group g = lane / 16
@@ -106,14 +131,17 @@ __device__ __forceinline__ bool any_group(bool x) {
 // them, so a lane has one page, one ks and one vs per tile whatever the page.
 // K's rows are read 32 bytes a lane at d = 128 (16 at 64), the contraction's order
 // of channels permuted alike in Q.
+//
+// WIDE: pages of 64 tokens and more, where a tile has one page.  Its address is the
+// scalar unit's work, and a lane adds an offset that never changes.
 // ---------------------------------------------------------------------------
-constexpr int NW = 4;  // waves of a workgroup
-
-template <typename T, int D, int NR>
-__global__ __launch_bounds__(64 * NW, NR == 1 ? 2 : 1) void rows_kernel(const Args a) {
+constexpr int NW = 4;
+template <typename T, int D, int NR, bool WIDE>
+__global__ __launch_bounds__(64 * NW, 2) void rows_kernel(const Args a) {
   constexpr int KC = D / 32;   // contraction steps
   constexpr int KL = D / 64;   // 16-byte loads of a K row per lane
   constexpr int DT = D / 16;   // output fragments
+  constexpr int LD = D == 128 ? 7 : 6;
   extern __shared__ __align__(16) unsigned char smem[];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -123,22 +151,42 @@ __global__ __launch_bounds__(64 * NW, NR == 1 ? 2 : 1) void rows_kernel(const Ar
   const int split = blockIdx.y;
   const int P = 1 << a.lp;
 
+  // ---- page numbers: of the lane's K rows and of its V keys (WIDE: of the tile), raw.  Their
+  // columns do not wait for the sequence's length. ----
+  struct Ids {
+    int k, v;
+  };
+  const int* row_pages = a.table + (size_t)b * a.max_pages;
+  const int last_col = a.max_pages - 1;
+  const long long begin = (long long)split * a.chunk;
+  auto ids_of = [&](int tile) {
+    const int at = (int)min(begin + 64LL * tile, 0x7fffffc0LL);
+    if constexpr (WIDE) {
+      const int p = row_pages[min(at >> a.lp, last_col)];
+      return Ids{p, p};
+    } else {
+      return Ids{row_pages[min((at + 16 * (r16 >> 2)) >> a.lp, last_col)], row_pages[min((at + 16 * g) >> a.lp, last_col)]};
+    }
+  };
+  Ids now = ids_of(wave), next = ids_of(wave + NW);
   const Rows rw = rows_of(a.cu, b, a.T);
   const int n = rw.last - rw.first;
   const int len = cut_len(a.lens[b], a.max_pages, a.lp);
   if (n == 0) return;
-  const int t0 = min((long long)split * a.chunk, (long long)len);
-  const int t1 = split + 1 == a.splits ? len : min(len, t0 + a.chunk);
-  const int* row_pages = a.table + (size_t)b * a.max_pages;
+  const int t0 = (int)min(begin, (long long)len);
+  const int t1 = split + 1 == a.splits ? len : (int)min(begin + a.chunk, (long long)len);
   const int tiles = (t1 - t0 + 63) / 64;
   const float c = fabsf(a.c);
   const uint32_t flip = a.c < 0.f ? 0x80008000u : 0u;  // a negative scale turns q, so that larger scores stay larger
+
+  // lane offsets in a page: of K row 16 (r16 / 4) + r16 % 4, of V's channel r16
+  const int k_key = 16 * (r16 >> 2) + (r16 & 3);
+  const uint32_t k_off = (uint32_t)(k_key * D + g * (D / 4)), v_off = (uint32_t)(r16 * P + 16 * g);
 
   for (int r0 = 0; r0 < n * G; r0 += 16 * NR) {
     // ---- this block's rows ----
     u32x4 qf[NR][KC];
     int limit[NR];  // keys that the lane's row sees: t < limit
-    int low = len;  // ... that every row of the block sees
 #pragma unroll
     for (int i = 0; i < NR; ++i) {
       const int r = min(r0 + 16 * i + r16, n * G - 1);
@@ -146,9 +194,9 @@ __global__ __launch_bounds__(64 * NW, NR == 1 ? 2 : 1) void rows_kernel(const Ar
       const uint16_t* src = a.q + (size_t)(rw.first + tok) * a.q_stride + (h * G + r % G) * D + g * (D / 4);
 #pragma unroll
       for (int k = 0; k < KC; ++k) qf[i][k] = ld128(src + 8 * k) ^ u32x4{flip, flip, flip, flip};
-      limit[i] = a.causal ? max(len - n + tok + 1, 0) : len;
+      limit[i] = min(a.causal ? max(len - n + tok + 1, 0) : len, t1);
     }
-    if (a.causal) low = max(len - n + r0 / G + 1, 0);
+    const int low = min(a.causal ? max(len - n + r0 / G + 1, 0) : len, t1);  // keys that every row of the block sees
 
     f32x4 acc[NR][DT];
     float m[NR], l[NR];
@@ -162,57 +210,74 @@ __global__ __launch_bounds__(64 * NW, NR == 1 ? 2 : 1) void rows_kernel(const Ar
       for (int d = 0; d < DT; ++d) acc[i][d] = f32x4{};
     }
 
-    // ---- a tile's pages: of the lane's K rows and of its V keys ----
-    struct Ids {
-      int k, v;
-    };
-    auto ids_of = [&](int tile) {
-      const int at = t0 + 64 * tile;
-      const bool in = tile < tiles;
-      return Ids{in ? page_of(row_pages, at + 16 * (r16 >> 2), a.lp, a.max_pages, a.pages) : -1,
-                 in ? page_of(row_pages, at + 16 * g, a.lp, a.max_pages, a.pages) : -1};
-    };
+    // tiles that not every row of the block sees whole start here: at most 3, with a causal mask
+    const int first_partial = low > t0 ? (low - t0) / 64 : 0;
+    int flagged = 0;
     u32x4 kx[4][KL], vx[DT];
     float ks = 1.f, vs = 1.f;
+    // a page that is none reads page 0 and is masked
+    auto valid = [&](int p) { return (uint32_t)p < (uint32_t)a.pages; };
     auto load_k = [&](int tile, Ids id) {
-      const int at = t0 + 64 * tile + 16 * (r16 >> 2) + (r16 & 3);
-      const size_t page = (size_t)max(id.k, 0) * a.n_kv + h;  // a page that is none reads page 0 and is masked
-      const uint8_t* p = a.kc + page * (size_t)(D * P) + (size_t)(at & (P - 1)) * D + g * (D / 4);
+      const int at = t0 + 64 * tile;
+      const uint8_t* p;
+      uint32_t ph;
+      if constexpr (WIDE) {
+        const int page = __builtin_amdgcn_readfirstlane(id.k);
+        ph = (uint32_t)((valid(page) ? page : 0) * a.n_kv + h);
+        p = a.kc + ((uint64_t)ph << (a.lp + LD)) + (at & (P - 1)) * D + k_off;
+      } else {
+        const uint64_t pk = (uint32_t)((valid(id.k) ? id.k : 0) * a.n_kv + h);
+        ph = (uint32_t)((valid(id.v) ? id.v : 0) * a.n_kv + h);
+        p = a.kc + (pk << (a.lp + LD)) + (uint32_t)(((at + k_key) & (P - 1)) * D + g * (D / 4));
+      }
 #pragma unroll
       for (int t = 0; t < 4; ++t)
 #pragma unroll
         for (int u = 0; u < KL; ++u) kx[t][u] = ld128(p + 4 * t * D + 16 * u);
-      ks = a.ks[(size_t)max(id.v, 0) * a.n_kv + h];
+      ks = a.ks[ph];
     };
     auto load_v = [&](int tile, Ids id) {
-      const int at = t0 + 64 * tile + 16 * g;
-      const size_t page = (size_t)max(id.v, 0) * a.n_kv + h;
-      const uint8_t* p = a.vc + page * (size_t)(D * P) + (size_t)r16 * P + (at & (P - 1));
+      const int at = t0 + 64 * tile;
+      const uint8_t* p;
+      uint32_t ph;
+      if constexpr (WIDE) {
+        const int page = __builtin_amdgcn_readfirstlane(id.v);
+        ph = (uint32_t)((valid(page) ? page : 0) * a.n_kv + h);
+        p = a.vc + ((uint64_t)ph << (a.lp + LD)) + (at & (P - 1)) + v_off;
+      } else {
+        ph = (uint32_t)((valid(id.v) ? id.v : 0) * a.n_kv + h);
+        p = a.vc + ((uint64_t)ph << (a.lp + LD)) + (uint32_t)(r16 * P + ((at + 16 * g) & (P - 1)));
+      }
 #pragma unroll
       for (int d = 0; d < DT; ++d) vx[d] = ld128(p + (size_t)16 * d * P);
-      vs = a.vs[page];
+      vs = a.vs[ph];
     };
 
     int tile = wave;
-    Ids now = ids_of(tile), next = ids_of(tile + NW);
+    if (r0 > 0) {
+      now = ids_of(tile);
+      next = ids_of(tile + NW);
+    }
     if (tile < tiles) {
       load_k(tile, now);
       load_v(tile, now);
     }
     for (; tile < tiles; tile += NW) {
       const int key0 = t0 + 64 * tile + 16 * g;  // the lane's keys: key0 .. key0 + 15
-      const bool bad = now.v < 0;
-      const bool masked = t0 + 64 * tile + 64 > min(low, t1) || __any(bad);
+      const bool bad = !valid(now.v);
+      const bool masked = t0 + 64 * tile + 64 > low || __any(bad);
       // ---- scores ----
       f32x4 s[NR][4];
 #pragma unroll
-      for (int t = 0; t < 4; ++t)
+      for (int t = 0; t < 4; ++t) {
 #pragma unroll
         for (int k = 0; k < KC; ++k) {
           const u32x4 kf = widen8<T>(kx[t][k >> 1][2 * (k & 1)], kx[t][k >> 1][2 * (k & 1) + 1]);
 #pragma unroll
           for (int i = 0; i < NR; ++i) s[i][t] = mfma16<T>(kf, qf[i][k], k ? s[i][t] : f32x4{});
         }
+        __builtin_amdgcn_sched_barrier(0);  // or every fragment is widened before the first product
+      }
       const float cs = c * ks, lv = __builtin_amdgcn_logf(vs), iv = 1.0f / vs;
       const Ids after = ids_of(tile + 2 * NW);
       if (tile + NW < tiles) load_k(tile + NW, next);
@@ -221,42 +286,47 @@ __global__ __launch_bounds__(64 * NW, NR == 1 ? 2 : 1) void rows_kernel(const Ar
       u32x4 pf[NR][2];
 #pragma unroll
       for (int i = 0; i < NR; ++i) {
-        float y[16];
         float mx = -INFINITY;
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
-          y[e] = __builtin_fmaf(s[i][e >> 2][e & 3], cs, lv);
+          float y = __builtin_fmaf(s[i][e >> 2][e & 3], cs, lv);
           if (masked) {
-            const bool in = !bad && key0 + e < min(limit[i], t1);
+            const bool in = !bad && key0 + e < limit[i];
             seen[i] |= in;
-            y[e] = in ? y[e] : -INFINITY;
+            y = in ? y : -INFINITY;
           }
-          mx = fmaxf(mx, y[e]);
+          s[i][e >> 2][e & 3] = y;
+          mx = fmaxf(mx, y);
         }
         if (!masked) seen[i] = true;
         const float top = fmaxf(m[i], max_xor32(max_xor16(mx)));
         const float base = top == -INFINITY ? 0.f : top;
-        const float corr = m[i] == top ? 1.f : __builtin_amdgcn_exp2f(m[i] - top);
-        m[i] = top;
+        if (__any(m[i] != top)) {
+          const float corr = m[i] == top ? 1.f : __builtin_amdgcn_exp2f(m[i] - top);
+          l[i] *= corr;
+#pragma unroll
+          for (int d = 0; d < DT; ++d) acc[i][d] *= corr;
+          m[i] = top;
+        }
         float sum = 0.f;
 #pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          y[e] = __builtin_amdgcn_exp2f(y[e] - base);
-          sum += y[e];
+        for (int t = 0; t < 4; ++t) {
+          f32x4 p;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) p[j] = __builtin_amdgcn_exp2f(s[i][t][j] - base);
+          sum += (p[0] + p[1]) + (p[2] + p[3]);
+          pf[i][t >> 1][2 * (t & 1)] = T::pack2(p[0], p[1]);
+          pf[i][t >> 1][2 * (t & 1) + 1] = T::pack2(p[2], p[3]);
         }
-        // masked keys of a page that is none have its vs of garbage
-        l[i] = l[i] * corr + (bad ? 0.f : sum * iv);
-#pragma unroll
-        for (int d = 0; d < DT; ++d) acc[i][d] *= corr;
-#pragma unroll
-        for (int u = 0; u < 2; ++u)
-          pf[i][u] = u32x4{T::pack2(y[8 * u], y[8 * u + 1]), T::pack2(y[8 * u + 2], y[8 * u + 3]),
-                           T::pack2(y[8 * u + 4], y[8 * u + 5]), T::pack2(y[8 * u + 6], y[8 * u + 7])};
+        l[i] += bad ? 0.f : sum * iv;  // a page that is none has no scale
       }
 
-      // ---- codes of V that a row does not see must not reach it: 0 * NaN ----
+      // ---- codes of V that a row does not see must not reach it: 0 * NaN.  Those past the
+      // last token or of no page become 0; so do NaNs that only some rows see, which are
+      // looked at again behind the loop. ----
       if (masked) {
-        uint32_t any_nan = 0;
+        const bool partial = a.causal && t0 + 64 * tile + 64 > low;
+        bool nan = false;
 #pragma unroll
         for (int d = 0; d < DT; ++d)
 #pragma unroll
@@ -264,43 +334,36 @@ __global__ __launch_bounds__(64 * NW, NR == 1 ? 2 : 1) void rows_kernel(const Ar
 #pragma unroll
             for (int j = 0; j < 4; ++j)
               if (bad || key0 + 4 * w + j >= t1) vx[d][w] &= ~(0xffu << (8 * j));
-            any_nan |= nan_bytes(vx[d][w]);
-          }
-        if (a.causal && __any(any_nan != 0)) {
-          // some row may not see it: count, for every row and channel, the NaNs it does
-          // see, and take them out of the product
-#pragma unroll
-          for (int i = 0; i < NR; ++i) {
-            const u32x4 vis[2] = {visible8<T>(key0, limit[i]), visible8<T>(key0 + 8, limit[i])};
-#pragma unroll
-            for (int d = 0; d < DT; ++d) {
-              f32x4 cnt{};
-#pragma unroll
-              for (int u = 0; u < 2; ++u) cnt = mfma16<T>(nans8<T>(vx[d][2 * u], vx[d][2 * u + 1]), vis[u], cnt);
-#pragma unroll
-              for (int j = 0; j < 4; ++j)
-                if (cnt[j] > 0.f) acc[i][d][j] = __builtin_nanf("");
+            if (partial) {
+              const uint32_t bits = nan_bytes(vx[d][w]);
+              nan |= bits != 0;
+              vx[d][w] &= ~spread(bits);
             }
           }
-#pragma unroll
-          for (int d = 0; d < DT; ++d)
-#pragma unroll
-            for (int w = 0; w < 4; ++w) vx[d][w] &= ~spread(nan_bytes(vx[d][w]));
-        }
+        if (__any(nan)) flagged |= 1 << (tile - first_partial);
       }
 
       // ---- O^T += V^T P'^T ----
 #pragma unroll
-      for (int d = 0; d < DT; ++d)
+      for (int d = 0; d < DT; ++d) {
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
           const u32x4 vf = widen8<T>(vx[d][2 * u], vx[d][2 * u + 1]);
 #pragma unroll
           for (int i = 0; i < NR; ++i) acc[i][d] = mfma16<T>(vf, pf[i][u], acc[i][d]);
         }
+        if (d & 1) __builtin_amdgcn_sched_barrier(0);
+      }
       if (tile + NW < tiles) load_v(tile + NW, next);
       now = next;
       next = after;
+    }
+
+    for (; flagged; flagged &= flagged - 1) {
+      const int key = t0 + 64 * (first_partial + __builtin_ctz(flagged)) + 16 * g;
+      const int page = key < t1 ? page_of(row_pages, key, a.lp, a.max_pages, a.pages) : -1;
+      add_nans<T, D, NR>(acc, limit, a.vc + ((size_t)max(page, 0) * a.n_kv + h) * (size_t)(D * P) + r16 * P + (key & (P - 1)),
+                         page >= 0, key, P);
     }
 
     // ---- the waves' states meet: m and the denominator, then the sums ----
@@ -368,9 +431,8 @@ __global__ __launch_bounds__(64 * NW, NR == 1 ? 2 : 1) void rows_kernel(const Ar
 // 16x16x32 MFMAs: for the same products 32x32x16 ones read and write twice the
 // accumulator registers, and the power that takes costs clock.
 // ---------------------------------------------------------------------------
-#ifndef KV8_TW
-#define KV8_TW 8
-#endif
+constexpr int TW = 8;           // waves
+constexpr int TR = 32 * TW;     // rows of a workgroup
 constexpr int BN = 64;          // keys of a tile
 constexpr float kLazy = 8.0f;   // log2 units that a score may pass the running maximum by before it moves
 
@@ -393,11 +455,11 @@ __device__ __forceinline__ int v_slot(int row, int slot) { return slot ^ ((row >
 
 // WIDE: pages of 64 tokens and more.  A tile then has one page, whose address the scalar unit
 // works out; its threads add an offset that never changes.
-template <typename T, int D, int TW, bool WIDE>
+template <typename T, int D, bool WIDE>
 __global__ __launch_bounds__(64 * TW, 2) void tile_kernel(const Args a) {
   using L = Stage<D>;
   constexpr int KC = D / 32, DT = D / 16;
-  constexpr int NT = 64 * TW, TR = 32 * TW;
+  constexpr int NT = 64 * TW;
   constexpr int U = D * 8 / NT;  // 16-byte units of a tile (K, then V) per thread
   static_assert(U >= 1 && U * NT == D * 8, "units");
   extern __shared__ __align__(1024) unsigned char smem[];
@@ -782,26 +844,8 @@ __global__ __launch_bounds__(64 * TW, 2) void tile_kernel(const Args a) {
       for (int flagged = *flags; flagged; flagged &= flagged - 1) {
         const int key = s0 + BN * (first_masked + __builtin_ctz(flagged)) + 16 * g;  // the lane's keys
         const int page = key < high ? page_of(row_pages, key, a.lp, a.max_pages, a.pages) : -1;
-        const uint8_t* p = a.vc + ((size_t)max(page, 0) * a.n_kv + h) * (size_t)(D * P) + (size_t)r16 * P + (key & (P - 1));
-#pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          u32x4 vis[2];
-#pragma unroll
-          for (int i = 0; i < 2; ++i) vis[i] = visible8<T>(key + 8 * u, limit[i]);
-          for (int d = 0; d < DT; ++d) {
-            const u32x2 v = page < 0 ? u32x2{} : ld64(p + (size_t)16 * d * P + 8 * u);
-            const u32x4 x = nans8<T>(v[0], v[1]);
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-              const f32x4 cnt = mfma16<T>(x, vis[i], f32x4{});
-#pragma unroll
-              for (int dd = 0; dd < DT; ++dd)
-#pragma unroll
-                for (int j = 0; j < 4; ++j)
-                  if (dd == d && cnt[j] > 0.f) acc[i][dd][j] = __builtin_nanf("");
-            }
-          }
-        }
+        add_nans<T, D, 2>(acc, limit, a.vc + ((size_t)max(page, 0) * a.n_kv + h) * (size_t)(D * P) + r16 * P + (key & (P - 1)),
+                          page >= 0, key, P);
       }
     }
 
@@ -835,40 +879,53 @@ __global__ __launch_bounds__(64 * TW, 2) void tile_kernel(const Args a) {
 }
 
 // ---------------------------------------------------------------------------
-// The splits' partial results of a row meet: one wave per row.
+// The splits' partial results of a row meet: one workgroup per row, D / 4 lanes per
+// split, so that the splits' loads are under way together.
 // ---------------------------------------------------------------------------
 template <typename T, int D>
 __global__ __launch_bounds__(256) void combine_kernel(const Args a) {
-  const int lane = threadIdx.x & 63;
-  const long long r = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
-  const size_t rows = (size_t)a.T * a.n_q;
-  if (r >= (long long)rows) return;
+  constexpr int LANES = D / 4, GROUPS = 256 / LANES;
+  __shared__ f32x4 sums[GROUPS][LANES];
+  __shared__ float2 state[GROUPS];  // m and the denominator
+  const int grp = threadIdx.x / LANES, c = threadIdx.x % LANES;
+  const size_t r = blockIdx.x, rows = (size_t)a.T * a.n_q;
   if (a.cu) {
     const int tok = (int)(r / a.n_q);
     if (tok < a.cu[0] || tok >= a.cu[a.B]) return;  // no sequence's row
   }
-  const float* ml = a.part + (size_t)a.splits * rows * D;
-  float top = -INFINITY;
-  for (int s = lane; s < a.splits; s += 64) top = fmaxf(top, ml[((size_t)s * rows + r) * 2]);
-#pragma unroll
-  for (int off = 1; off < 64; off <<= 1) top = fmaxf(top, __shfl_xor(top, off, 64));
-  constexpr int V = D / 64;  // channels of a lane
-  float o[V] = {}, total = 0.f;
-  for (int s = 0; s < a.splits; ++s) {
-    const float m = ml[((size_t)s * rows + r) * 2];
-    if (m == -INFINITY) continue;
-    const float w = __builtin_amdgcn_exp2f(m - top);
-    total += w * ml[((size_t)s * rows + r) * 2 + 1];
-    const float* p = a.part + ((size_t)s * rows + r) * D + lane * V;
-#pragma unroll
-    for (int v = 0; v < V; ++v) o[v] += w * p[v];
+  const float2* ml = reinterpret_cast<const float2*>(a.part + (size_t)a.splits * rows * D);
+  float top = -INFINITY, total = 0.f;
+  f32x4 o{};
+#pragma unroll 4
+  for (int s = grp; s < a.splits; s += GROUPS) {
+    const float2 x = ml[(size_t)s * rows + r];
+    const f32x4 v = *reinterpret_cast<const f32x4*>(a.part + ((size_t)s * rows + r) * D + 4 * c);
+    if (x.x == -INFINITY) continue;  // no visible token: nothing was summed
+    const float up = fmaxf(top, x.x);
+    const float w0 = top == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(top - up), w1 = __builtin_amdgcn_exp2f(x.x - up);
+    total = total * w0 + x.y * w1;
+    o = o * w0 + v * w1;
+    top = up;
   }
-  const float inv = top == -INFINITY ? 0.f : 1.0f / total;
-  uint16_t* out = a.out + (size_t)r * D + lane * V;
-  if constexpr (V == 2)
-    *reinterpret_cast<uint32_t*>(out) = top == -INFINITY ? 0u : T::pack2(o[0] * inv, o[1] * inv);
-  else
-    *out = top == -INFINITY ? (uint16_t)0 : (uint16_t)T::pack2(o[0] * inv, 0.f);
+  sums[grp][c] = o;
+  if (c == 0) state[grp] = float2{top, total};
+  __syncthreads();
+  if (grp > 0) return;
+  float most = -INFINITY;
+#pragma unroll
+  for (int k = 0; k < GROUPS; ++k) most = fmaxf(most, state[k].x);
+  total = 0.f;
+  o = f32x4{};
+#pragma unroll
+  for (int k = 0; k < GROUPS; ++k) {
+    const float2 x = state[k];
+    if (x.x == -INFINITY) continue;
+    const float w = __builtin_amdgcn_exp2f(x.x - most);
+    total += w * x.y;
+    o += w * sums[k][c];
+  }
+  o *= most == -INFINITY ? 0.f : 1.0f / total;
+  st64(a.out + r * D + 4 * c, u32x2{T::pack2(o[0], o[1]), T::pack2(o[2], o[3])});
 }
 
 // ---------------------------------------------------------------------------
@@ -880,35 +937,47 @@ struct Plan {
   int splits, chunk;
 };
 
+static long long up(long long x, long long to) { return (x + to - 1) / to; }
+
+// The rows kernel up to 32 rows a KV head, else the tile kernel.  The keys are split
+// where there are fewer workgroups than CUs.  A split costs its workgroup's start and
+// end, some 250 tokens' worth, and the combine's launch, so chunks are as long as the GPU
+// stays filled: rows kernel, one workgroup per CU while sequences times KV heads are
+// few, two from 128 on (chunks of 256, 512, 1024, 2048 and 4096 tokens: B4 of 4096 tokens 14.6, 13.8,
+// 16.8, 23.1, 33.8 us; B32 59, 47, 42, 38, 41), and at most 4096 tokens, which keeps sequences of
+// different lengths apart (B64 of up to 8192: 218, 174, 154, 147, 149).
 static Plan plan(int B, int T, int max_q, int max_kv, int n_q, int n_kv) {
-  const int G = n_q / n_kv;
-  const long long rows = (long long)max_q * G;
+  const long long rows = (long long)(max_q < T ? max_q : T) * (n_q / n_kv), heads = (long long)B * n_kv;
   Plan p;
   p.nr = rows <= 16 ? 1 : rows <= 32 ? 2 : 0;
-  p.tiles = (int)std::min((rows + 32 * KV8_TW - 1) / (32 * KV8_TW), 65535LL);
-  const long long units = (long long)B * n_kv * (p.nr ? 1 : p.tiles);
-  const long long want = ((p.nr ? 2048 : 256) + units - 1) / units;
-  long long chunk = (max_kv + want - 1) / want;
-  chunk = (chunk + 255) / 256 * 256;
-  p.splits = (int)((max_kv + chunk - 1) / chunk);
-  p.chunk = (int)chunk;
+  p.tiles = (int)std::min(up(rows, TR), 65535LL);
+  long long chunk;
+  if (p.nr) {
+    chunk = up(up(heads * max_kv, heads >= 128 ? 512 : 256), 256) * 256;
+    chunk = std::min(chunk, 4096LL);
+  } else {
+    chunk = up(max_kv, up(256, heads * p.tiles));
+    chunk = up(chunk, 256) * 256;
+  }
+  p.splits = (int)std::min(up(max_kv, chunk), 65535LL);
+  p.chunk = (int)std::min(chunk, 0x40000000LL);
   return p;
 }
 
-template <typename T, int D, int NR>
+template <typename T, int D, int NR, bool WIDE>
 static int launch_rows(const Args& a, hipStream_t s) {
   constexpr int lds = NW * NR * (16 * 2 * 4 + (D / 16) * 64 * 16);
-  MX_RETURN_IF_HIP((lds_limit_once<rows_kernel<T, D, NR>>(lds)));
-  hipLaunchKernelGGL((rows_kernel<T, D, NR>), dim3((unsigned)(a.B * a.n_kv), (unsigned)a.splits), dim3(64 * NW), lds, s, a);
+  MX_RETURN_IF_HIP((lds_limit_once<rows_kernel<T, D, NR, WIDE>>(lds)));
+  hipLaunchKernelGGL((rows_kernel<T, D, NR, WIDE>), dim3((unsigned)(a.B * a.n_kv), (unsigned)a.splits), dim3(64 * NW), lds, s, a);
   MX_RETURN_IF_HIP(hipGetLastError());
   return MX_OK;
 }
 
-template <typename T, int D, int TW, bool WIDE>
+template <typename T, int D, bool WIDE>
 static int launch_tiles(const Args& a, const Plan& p, hipStream_t s) {
   constexpr int lds = Stage<D>::LDS;
-  MX_RETURN_IF_HIP((lds_limit_once<tile_kernel<T, D, TW, WIDE>>(lds)));
-  hipLaunchKernelGGL((tile_kernel<T, D, TW, WIDE>), dim3((unsigned)(a.B * a.n_kv), (unsigned)p.tiles, (unsigned)a.splits),
+  MX_RETURN_IF_HIP((lds_limit_once<tile_kernel<T, D, WIDE>>(lds)));
+  hipLaunchKernelGGL((tile_kernel<T, D, WIDE>), dim3((unsigned)(a.B * a.n_kv), (unsigned)p.tiles, (unsigned)a.splits),
                      dim3(64 * TW), lds, s, a);
   MX_RETURN_IF_HIP(hipGetLastError());
   return MX_OK;
@@ -916,10 +985,14 @@ static int launch_tiles(const Args& a, const Plan& p, hipStream_t s) {
 
 template <typename T, int D>
 static int run(const Args& a, const Plan& p, hipStream_t s) {
-  const int rc = p.nr == 1 ? launch_rows<T, D, 1>(a, s) : p.nr == 2 ? launch_rows<T, D, 2>(a, s) : a.lp >= 6 ? launch_tiles<T, D, KV8_TW, true>(a, p, s) : launch_tiles<T, D, KV8_TW, false>(a, p, s);
+  const bool wide = a.lp >= 6;
+  const int rc = p.nr == 1   ? (wide ? launch_rows<T, D, 1, true>(a, s) : launch_rows<T, D, 1, false>(a, s))
+                 : p.nr == 2 ? (wide ? launch_rows<T, D, 2, true>(a, s) : launch_rows<T, D, 2, false>(a, s))
+                 : wide      ? launch_tiles<T, D, true>(a, p, s)
+                             : launch_tiles<T, D, false>(a, p, s);
   if (rc != MX_OK || p.splits == 1) return rc;
   const long long rows = (long long)a.T * a.n_q;
-  hipLaunchKernelGGL((combine_kernel<T, D>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, s, a);
+  hipLaunchKernelGGL((combine_kernel<T, D>), dim3((unsigned)rows), dim3(256), 0, s, a);
   MX_RETURN_IF_HIP(hipGetLastError());
   return MX_OK;
 }
