@@ -13,7 +13,7 @@
 // Both kernels compute C^T = B . A^T with 16x16x64 MFMAs: a lane of the result
 // then holds one row m and 4 consecutive n per fragment, its sA is one value
 // and its stores run along C's rows.
-#include "mx_common.h"
+#include "int8_common.h"
 
 namespace mx {
 namespace gemmi8 {
@@ -351,6 +351,178 @@ __global__ __launch_bounds__(64 * RW) void gemm_int8_rows_kernel(
 }
 
 // ---------------------------------------------------------------------------
+// A linear layer for up to 4 rows in one kernel: every workgroup quantises the rows for
+// itself (in LDS, while its rows of B are on the way), and the second launch, the codes'
+// way through memory and the workspace fall away.  Otherwise as the kernel above.
+// ---------------------------------------------------------------------------
+constexpr int FEW_ROWS = 4, FEW_VALUES = 16384;  // rows, rows times K
+template <int FB>
+struct Few {
+  static constexpr int X = FEW_VALUES * 2;  // the rows as they come, then their codes
+  static constexpr int SLOT = 16 * FB * KS, LPW = 2 * FB;
+  static constexpr int NS = 48 * 1024 / RW / SLOT;
+  static constexpr int LDS = X + RW * NS * SLOT;
+  static_assert(LDS <= 80 * 1024 && RW * FB * 64 * 16 <= RW * NS * SLOT, "two workgroups on a CU");
+};
+
+template <int FB, typename T>
+__global__ __launch_bounds__(64 * RW, 2) void linear_int8_few_kernel(const uint16_t* __restrict__ X,
+                                                                    const uint8_t* __restrict__ B,
+                                                                    const float* __restrict__ sB,
+                                                                    uint16_t* __restrict__ C, int M, int N, int K, int ldx) {
+  using F = Few<FB>;
+  constexpr int NT = 64 * RW;
+  extern __shared__ __align__(1024) unsigned char smem[];
+  const int t = threadIdx.x, lane = t & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(t >> 6);
+  const int r16 = lane & 15, g = lane >> 4;
+  const int n0 = blockIdx.x * 16 * FB;
+  const int steps = (K + KS - 1) / KS;
+  const int k0 = steps * wave / RW, k1 = steps * (wave + 1) / RW;
+  const uint32_t x0 = lds_addr(smem);
+
+  // X's rows, 8 values a lane and load, one behind the other in LDS
+  const int eighths = K / 8, pieces = M * eighths;
+  for (int i = 64 * wave; i < pieces; i += NT) {
+    const int p = min(i + lane, pieces - 1);
+    dma16(X, (uint32_t)(p / eighths * ldx + p % eighths * 8) * 2, x0 + 16 * i);
+  }
+  // the wave's ring of B's rows
+  const uint32_t ring = x0 + F::X + wave * F::NS * F::SLOT;
+  const int lr = lane >> 3;
+  uint32_t off[F::LPW];
+#pragma unroll
+  for (int n = 0; n < F::LPW; ++n) off[n] = (uint32_t)(min(n0 + 8 * n + lr, N - 1) - n0) * (uint32_t)K;
+  const uint8_t* b_rows = B + (size_t)n0 * K;
+  const int ch[2] = {(lane & 7) ^ swz_a(lr), (lane & 7) ^ swz_a(8 + lr)};
+  auto issue = [&](int k, int slot) {
+    const int last = (K - k * KS) / 16 - 1;
+#pragma unroll
+    for (int n = 0; n < F::LPW; ++n)
+      dma16(b_rows + (size_t)k * KS, off[n] + 16 * min(ch[n & 1], last), ring + slot * F::SLOT + n * 1024);
+  };
+#pragma unroll
+  for (int s = 0; s < F::NS; ++s)
+    if (k0 + s < k1) issue(k0 + s, s);
+  land_args(C, sB);
+
+  // ---- codes: units of 16 values, at most 4 a thread; those of a row are K / 16 ----
+  if (k1 - k0 >= F::NS)
+    wait_vmcnt<F::NS * F::LPW>();  // X is there, B may be on the way
+  else
+    wait_vmcnt<0>();
+  lds_barrier();
+  constexpr int U = FEW_VALUES / 16 / NT;
+  const int per = K / 16, units = M * per;
+  u32x4 lo[U], hi[U];
+  uint32_t mx[FEW_ROWS] = {};
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const int i = t + u * NT;
+    lo[u] = hi[u] = u32x4{};
+    if (i < units) {
+      lo[u] = lds_ld128(x0 + 32 * i);
+      hi[u] = lds_ld128(x0 + 32 * i + 16);
+    }
+    uint32_t v = 0;
+    quant8::take_magnitudes<T>(v, lo[u]);
+    quant8::take_magnitudes<T>(v, hi[u]);
+    v = max(v & 0xffffu, v >> 16);
+#pragma unroll
+    for (int m = 0; m < FEW_ROWS; ++m)
+      if (i / per == m) mx[m] = max(mx[m], v);
+  }
+  auto meet = [] {  // LDS reads and writes done, B's loads still on the way
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    lds_barrier();
+  };
+  meet();  // X is in registers: its place takes the waves' maxima, then the codes
+  uint32_t* most = reinterpret_cast<uint32_t*>(smem);  // [RW][FEW_ROWS]
+#pragma unroll
+  for (int m = 0; m < FEW_ROWS; ++m) {
+    if (m >= M) break;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) mx[m] = max(mx[m], (uint32_t)__shfl_xor((int)mx[m], o, 64));
+    if (lane == 0) most[wave * FEW_ROWS + m] = mx[m];
+  }
+  meet();
+  float sa[FEW_ROWS];
+#pragma unroll
+  for (int m = 0; m < FEW_ROWS; ++m) {
+    uint32_t v = 0;
+    if (m < M) {
+#pragma unroll
+      for (int w = 0; w < RW; ++w) v = max(v, most[w * FEW_ROWS + m]);
+    }
+    sa[m] = quant8::scale_of<T>(v);
+  }
+  meet();
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const int i = t + u * NT;
+    if (i < units) {
+      const int m = i / per;
+      const float s = m == 0 ? sa[0] : m == 1 ? sa[1] : m == 2 ? sa[2] : sa[3];
+      st128(smem + 16 * i, quant8::encode<T>(lo[u], hi[u], s, 1.0f / s));
+    }
+  }
+  meet();
+
+  // ---- the product: lane's row of A r16 (the last one again past M: never stored) ----
+  const uint32_t a_at = x0 + min(r16, M - 1) * K + 16 * g;
+  uint32_t b_at[2];
+#pragma unroll
+  for (int h = 0; h < 2; ++h) b_at[h] = ring + r16 * KS + 16 * ((4 * h + g) ^ swz_a(r16));
+  i32x4 acc[FB];
+#pragma unroll
+  for (int f = 0; f < FB; ++f) acc[f] = i32x4{};
+  int slot = 0;
+  for (int k = k0; k < k1; ++k) {
+    if (k + F::NS <= k1)
+      wait_vmcnt<(F::NS - 1) * F::LPW>();
+    else
+      wait_vmcnt<0>();
+    asm volatile("" ::: "memory");  // no read before the wait
+    const uint32_t so = slot * F::SLOT;
+    u32x4 a[2], b[2][FB];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      a[h] = u32x4{};
+      if (k * KS + 64 * h + 16 * g < K) a[h] = lds_ld128(a_at + k * KS + 64 * h);
+#pragma unroll
+      for (int f = 0; f < FB; ++f) b[h][f] = lds_ld128(b_at[h] + so + 16 * f * KS);
+    }
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int f = 0; f < FB; ++f) acc[f] = mfma_i8(b[h][f], a[h], acc[f]);
+    __builtin_amdgcn_sched_barrier(0);  // the slot's reads have arrived: it can be filled again
+    if (k + F::NS < k1) issue(k + F::NS, slot);
+    slot = slot + 1 == F::NS ? 0 : slot + 1;
+  }
+  __syncthreads();
+  i32x4* red = reinterpret_cast<i32x4*>(smem + F::X);  // [RW][FB][64]
+#pragma unroll
+  for (int f = 0; f < FB; ++f) red[(wave * FB + f) * 64 + lane] = acc[f];
+  __syncthreads();
+  for (int f = wave; f < FB; f += RW) {
+    i32x4 c = red[f * 64 + lane];
+#pragma unroll
+    for (int w = 1; w < RW; ++w) c += red[(w * FB + f) * 64 + lane];
+    const int n = n0 + 16 * f + 4 * g;
+    if (r16 < M && n < N) {
+      const float s = r16 == 0 ? sa[0] : r16 == 1 ? sa[1] : r16 == 2 ? sa[2] : sa[3];
+      const u32x2 v = scaled4<T>(c, s, scales4(sB, n, N));
+      uint16_t* out = C + (size_t)r16 * N + n;
+      if ((N & 3) == 0)
+        st64(out, v);
+      else
+        store4(out, v, N - n);
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------
 // Launch choice.  What bounds every variant short of the largest products is the rate
 // at which a CU takes operand lines in, near 46 GB/s for one workgroup of a CU and 61 for two
 // side by side (measured from 1x1024x1024 to 8192^3; about 37 for the 256x256 tile,
@@ -421,6 +593,18 @@ static int run(int variant, const uint8_t* A, const float* sA, const uint8_t* B,
 #undef TILE
 }
 
+static bool few(int M, int K) { return M <= FEW_ROWS && (long long)M * K <= FEW_VALUES; }
+
+template <int FB, typename T>
+static int launch_few(const void* X, const void* B, const float* sB, void* C, int M, int N, int K, int ldx, hipStream_t s) {
+  constexpr auto kern = linear_int8_few_kernel<FB, T>;
+  MX_RETURN_IF_HIP(lds_limit_once<kern>(Few<FB>::LDS));
+  hipLaunchKernelGGL(kern, dim3((unsigned)((N + 16 * FB - 1) / (16 * FB))), dim3(64 * RW), Few<FB>::LDS, s,
+                     (const uint16_t*)X, (const uint8_t*)B, sB, (uint16_t*)C, M, N, K, ldx);
+  MX_RETURN_IF_HIP(hipGetLastError());
+  return MX_OK;
+}
+
 static int check(const void* A, const float* sA, const void* B, const float* sB, const void* C, int M, int N, int K,
                  int dtype) {
   if (!A || !sA || !B || !sB || !C) return MX_ERR_NULL;
@@ -450,19 +634,31 @@ extern "C" int mx_gemm_int8(const void* A, const float* sA, const void* B, const
 static size_t linear_codes(int M, int K) { return ((size_t)M * K + 255) / 256 * 256; }
 
 extern "C" size_t mx_linear_int8_workspace(int M, int K) {
-  if (M <= 0 || K <= 0 || K % 16) return 0;
+  if (M <= 0 || K <= 0 || K % 16 || mx::gemmi8::few(M, K)) return 0;
   return linear_codes(M, K) + (size_t)M * sizeof(float);
 }
 
 extern "C" int mx_linear_int8(const void* X, const void* W, const float* sW, void* C, int M, int N, int K, int ldx,
                               int dtype, void* workspace, size_t ws_bytes, void* stream) {
-  if (!X || !workspace) return MX_ERR_NULL;
-  float* sx = (float*)((unsigned char*)workspace + linear_codes(M > 0 ? M : 1, K > 0 ? K : 1));
-  const int rc = mx::gemmi8::check(workspace, sx, W, sW, C, M, N, K, dtype);
+  using namespace mx::gemmi8;
+  if (!X) return MX_ERR_NULL;
+  // X, the scales sW in place of the rows' own, for the checks that the product makes
+  const int rc = check(X, sW, W, sW, C, M, N, K, dtype);
   if (rc != MX_OK) return rc;
   if (ldx < K) return MX_ERR_SHAPE;
-  if (ldx % 8 || ((uintptr_t)X & 15)) return MX_ERR_ALIGN;
-  if (ws_bytes < mx_linear_int8_workspace(M, K)) return MX_ERR_WORKSPACE;
+  if (ldx % 8) return MX_ERR_ALIGN;
+  hipStream_t s = (hipStream_t)stream;
+  if (few(M, K) && (long long)M * ldx < (1LL << 30)) {
+    // 16 rows of B a workgroup while two on every CU hold all of N
+    const bool one = N <= 8192;
+    if (dtype == MX_DTYPE_BF16)
+      return one ? launch_few<1, mx::BF16>(X, W, sW, C, M, N, K, ldx, s) : launch_few<2, mx::BF16>(X, W, sW, C, M, N, K, ldx, s);
+    return one ? launch_few<1, mx::F16>(X, W, sW, C, M, N, K, ldx, s) : launch_few<2, mx::F16>(X, W, sW, C, M, N, K, ldx, s);
+  }
+  if (!workspace) return MX_ERR_NULL;
+  if ((uintptr_t)workspace & 15) return MX_ERR_ALIGN;
+  if (ws_bytes < linear_codes(M, K) + (size_t)M * sizeof(float)) return MX_ERR_WORKSPACE;
+  float* sx = (float*)((unsigned char*)workspace + linear_codes(M, K));
   const int q = mx_quant_int8(X, workspace, sx, M, K, ldx, dtype, stream);
   if (q != MX_OK) return q;
   return mx_gemm_int8(workspace, sx, W, sW, C, M, N, K, dtype, stream);

@@ -470,6 +470,8 @@ def mla_decode_absorbed(q_nope, q_rope, kv, w_uk, w_uv, scale, out=None, workspa
 # ---------------------------------------------------------------------------
 def _rows(t, name, dtypes, inner):
     """Checks of a tensor whose rows (first dimension) may lie apart, each of them contiguous; its row stride."""
+    if type(t) is _Tensor and t.dtype in dtypes and t.is_cuda and t.dim() == inner + 1 and t.is_contiguous():
+        return t.stride(0)
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{name} must be a torch.Tensor")
     if t.dtype not in dtypes:
@@ -478,8 +480,6 @@ def _rows(t, name, dtypes, inner):
         raise ValueError(f"{name} must be on a HIP device (got {t.device})")
     if t.dim() != inner + 1:
         raise ValueError(f"{name} must be {inner + 1}-D (got shape {tuple(t.shape)})")
-    if t.is_contiguous():
-        return t.numel() // t.shape[0] if t.shape[0] else 0
     want = 1
     for d in range(inner, 0, -1):
         if t.shape[d] != 1 and t.stride(d) != want:
@@ -498,6 +498,19 @@ def _launch(fn, t, *args):
     else:
         with torch.cuda.device(d):
             _lib.call(fn, *args, _C._cuda_getCurrentRawStream(d))
+
+
+def _workspace(workspace, need, t):
+    """(pointer, bytes) of the caller's workspace, or of a new one on t's device where the call needs one.  A new one
+    may go once the call has returned: what the allocator gives its memory to next runs behind it on the stream."""
+    if workspace is None:
+        if not need:
+            return None, 0
+        workspace = torch.empty(need, dtype=torch.uint8, device=t.device)
+    else:
+        _require(workspace, "workspace", (torch.uint8,))
+        _same_device(t, workspace)
+    return workspace.data_ptr(), workspace.numel()
 
 
 def quant_int8(x, q=None, scales=None):
@@ -582,13 +595,10 @@ def linear_int8(x, w, sw, out=None, workspace=None):
         _require(out, "out", (x.dtype,), 2)
         if out.shape != (M, N):
             raise ValueError(f"out must be {(M, N)}, got {tuple(out.shape)}")
-    if workspace is None:
-        workspace = torch.empty(linear_int8_workspace_bytes(M, K), dtype=torch.uint8, device=x.device)
-    else:
-        _require(workspace, "workspace", (torch.uint8,))
-    _same_device(x, w, sw, out, workspace)
+    ws, ws_bytes = _workspace(workspace, linear_int8_workspace_bytes(M, K), x)
+    _same_device(x, w, sw, out)
     _launch("mx_linear_int8", x, x.data_ptr(), w.data_ptr(), sw.data_ptr(), out.data_ptr(), M, N, K, ldx,
-            _IO_DTYPES[x.dtype], workspace.data_ptr(), workspace.numel())
+            _IO_DTYPES[x.dtype], ws, ws_bytes)
     return out
 
 
@@ -756,14 +766,7 @@ def gqa_kv8(q, cache, page_table, kv_lens, cu_q=None, max_q=None, max_kv=None, c
             raise ValueError(f"out must be {tuple(q.shape)}")
     if q.get_device() != cache._device or out.get_device() != cache._device:
         raise ValueError("all tensors must be on the cache's device")
-    need = gqa_kv8_workspace_bytes(B, T, max_q, max_kv, n_q, n_kv, d)
-    if workspace is None:
-        if need:
-            workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
-    else:
-        _require(workspace, "workspace", (torch.uint8,))
-        _same_device(q, workspace)
-    ws, ws_bytes = (None, 0) if workspace is None else (workspace.data_ptr(), workspace.numel())
+    ws, ws_bytes = _workspace(workspace, gqa_kv8_workspace_bytes(B, T, max_q, max_kv, n_q, n_kv, d), q)
     _launch("mx_gqa_kv8", q, q.data_ptr(), *cache._args, page_table.data_ptr(), kv_lens.data_ptr(), cu, out.data_ptr(),
             B, T, max_q, max_kv, n_q, n_kv, d, page, pages, most, qs, float(scale), int(bool(causal)),
             _IO_DTYPES[q.dtype], ws, ws_bytes)

@@ -323,11 +323,12 @@ int mx_gemm_int8(const void* A, const float* sA, const void* B, const float* sB,
                  int dtype, void* stream);
 
 /*
- * An int8 linear layer: mx_quant_int8 of X[M,K] into the workspace, then
- * mx_gemm_int8 with the weight W[N,K] and its scales sW[N].  C has X's type.
- * The workspace (mx_linear_int8_workspace(M, K) bytes, 16-byte aligned; 0 for
- * invalid sizes) holds the codes and the scales; calls that may overlap each
- * need their own.
+ * An int8 linear layer: mx_quant_int8 of X[M,K], then mx_gemm_int8 with the
+ * weight W[N,K] and its scales sW[N].  C has X's type.
+ * The workspace (mx_linear_int8_workspace(M, K) bytes, 16-byte aligned) holds
+ * the codes and the scales; calls that may overlap each need their own.  It is 0
+ * for up to 4 rows of together up to 16384 values, which one kernel does, and for
+ * invalid sizes.
  */
 int mx_linear_int8(const void* X, const void* W, const float* sW, void* C, int M, int N, int K, int ldx, int dtype,
                    void* workspace, size_t ws_bytes, void* stream);

@@ -13,11 +13,12 @@ DTYPES = [torch.bfloat16, torch.float16]
 
 
 def bound(exact: torch.Tensor, dtype) -> torch.Tensor:
-    """How far the product may be off: its rounding to `dtype` (half a step relative to the value, or half
-    the smallest f16 subnormal), after three fp32 roundings (the int32 sum's conversion, two scales)."""
+    """How far the product may be off: its rounding to `dtype` (half a step relative to the value), after three
+    fp32 roundings (the int32 sum's conversion, two scales); among the subnormals half of the type's step (f16 2^-24,
+    bf16 2^-133) after two roundings of half fp32's (2^-149), the first of them times a scale below 1."""
     fp32 = 3 * 2.0 ** -24
-    return exact.abs() * ((1 + fp32) * torch.finfo(dtype).eps / 2 + fp32 * 1.0001) + (
-        2.0 ** -25 if dtype == torch.float16 else 0.0)
+    least = 2.0 ** -25 if dtype == torch.float16 else 2.0 ** -134
+    return exact.abs() * ((1 + fp32) * torch.finfo(dtype).eps / 2 + fp32 * 1.0001) + least + 2.0 ** -149
 
 
 def rows(m, k, dtype, seed):
@@ -104,7 +105,8 @@ def test_product_of_extremes(ops):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
-@pytest.mark.parametrize("m,n,k", [(1, 40, 256), (37, 300, 1040), (130, 260, 512)])
+@pytest.mark.parametrize("m,n,k", [(1, 40, 256), (37, 300, 1040), (130, 260, 512), (1, 17, 16), (1, 8200, 16384), (2, 33, 8192),
+                                   (3, 1, 5456), (4, 70, 4096), (4, 8211, 2064), (3, 100, 144), (4, 64, 4112), (5, 64, 256)])
 def test_linear(ops, dtype, m, n, k):
     """Against the oracle's quantiser and product, with the caller's workspace, on rows that lie apart."""
     announce(f"linear_int8 {m}x{n}x{k} {dtype}")
@@ -112,19 +114,33 @@ def test_linear(ops, dtype, m, n, k):
     w, sw = oracle.quantize_rows(rows(n, k, dtype, 12))
     q, sx = oracle.quantize_rows(x[:, k:].contiguous())
     exact = oracle.product(q, sx, w, sw)
-    ws = torch.empty(ops.linear_int8_workspace_bytes(m, k), dtype=torch.uint8, device="cuda")
+    ws = torch.empty(max(1, ops.linear_int8_workspace_bytes(m, k)), dtype=torch.uint8, device="cuda")
     y = ops.linear_int8(x.cuda()[:, k:], w.cuda(), sw.cuda(), workspace=ws)
     assert y.dtype == dtype
     assert bool(((y.cpu().double() - exact).abs() <= bound(exact, dtype)).all())
 
 
-def test_linear_poisoned_row(ops):
-    announce("linear_int8 NaN row")
-    x = rows(5, 256, torch.bfloat16, 1)
-    x[2, 9], x[4, 0] = float("nan"), float("-inf")
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_linear_special_rows(ops, dtype):
+    """In either kernel (one for few rows, quantiser and product for more): rows of NaN or infinity poison themselves
+    alone, zero rows give zeros, tiny and exactly tied values what the oracle gives."""
+    announce(f"linear_int8 special rows {dtype}")
+    x = rows(8, 256, dtype, 1)
+    x[1, 9], x[3, 0] = float("nan"), float("-inf")
+    x[2] = 0
+    x[4] = torch.finfo(dtype).smallest_normal / 8
+    x[5] = (torch.arange(256) - 127.5) * 0.5
+    x[5, 0] = 127
+    x[6] = torch.finfo(dtype).max
     w, sw = oracle.quantize_rows(rows(48, 256, torch.bfloat16, 2))
-    y = ops.linear_int8(x.cuda(), w.cuda(), sw.cuda()).cpu()
-    assert y.isnan().all(1).tolist() == [False, False, True, False, True] and not y[[0, 1, 3]].isnan().any()
+    q, sx = oracle.quantize_rows(x)
+    exact = oracle.product(q, sx, w, sw)
+    for a, b in ((0, 8), (0, 4), (4, 8), (1, 2), (2, 4), (5, 7)):
+        y = ops.linear_int8(x[a:b].cuda(), w.cuda(), sw.cuda()).cpu().double()
+        assert torch.equal(y.isnan(), exact[a:b].isnan())
+        over = exact[a:b].abs() > torch.finfo(dtype).max
+        ok = ((y - exact[a:b]).abs() <= bound(exact[a:b], dtype)) | y.isnan() | over
+        assert bool(ok.all()) and bool((y[over].abs() >= torch.finfo(dtype).max).all())
 
 
 def test_streams_and_capture(ops):
@@ -132,10 +148,10 @@ def test_streams_and_capture(ops):
     announce("linear_int8 graphs on two streams")
     w, sw = oracle.quantize_rows(rows(320, 512, torch.bfloat16, 5))
     w, sw = w.cuda(), sw.cuda()
-    xs = [rows(m, 512, torch.bfloat16, m).cuda() for m in (3, 90)]
+    xs = [rows(m, 512, torch.bfloat16, m).cuda() for m in (6, 90)]
     want = [ops.linear_int8(x, w, sw) for x in xs]
     outs = [torch.empty_like(y) for y in want]
-    spaces = [torch.empty(ops.linear_int8_workspace_bytes(*x.shape), dtype=torch.uint8, device="cuda") for x in xs]
+    spaces = [torch.empty(max(1, ops.linear_int8_workspace_bytes(*x.shape)), dtype=torch.uint8, device="cuda") for x in xs]
     torch.cuda.synchronize()
     graphs = []
     for x, y, ws in zip(xs, outs, spaces):

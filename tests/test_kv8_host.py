@@ -41,11 +41,11 @@ BAD = [
         *[({i: U}, _lib.MX_ERR_ALIGN) for i in (0, 2, 4)], *[({i: V}, _lib.MX_ERR_ALIGN) for i in (1, 3)],
         ({8: 3}, _lib.MX_ERR_DTYPE)]),
     # X, W, sW, C, M, N, K, ldx, dtype, workspace, bytes, stream
-    *_calls("mx_linear_int8", [P, P, P, P, 4, 8, 64, 64, 0, P, 1 << 20, None], [
+    *_calls("mx_linear_int8", [P, P, P, P, 40, 8, 64, 64, 0, P, 1 << 20, None], [
         *[({i: None}, _lib.MX_ERR_NULL) for i in (0, 1, 2, 3, 9)], *[({i: 0}, _lib.MX_ERR_SHAPE) for i in (4, 5, 6)],
         ({4: -5}, _lib.MX_ERR_SHAPE), ({6: 72}, _lib.MX_ERR_SHAPE), ({7: 56}, _lib.MX_ERR_SHAPE),
         ({7: 68}, _lib.MX_ERR_ALIGN), ({0: U}, _lib.MX_ERR_ALIGN), ({9: U}, _lib.MX_ERR_ALIGN),
-        ({8: 7}, _lib.MX_ERR_DTYPE), ({10: 271}, _lib.MX_ERR_WORKSPACE)]),
+        ({8: 7}, _lib.MX_ERR_DTYPE), ({10: 2719}, _lib.MX_ERR_WORKSPACE)]),
     # k, v, kc, vc, ks, vs, table, lens, cu, B, T, max_q, n_kv, d, page, pages, max_pages, ldk, ldv, dtype, stream
     *_calls("mx_kv8_append", [P] * 9 + [2, 5, 4, 2, 64, 16, 9, 3, 128, 128, 0, None], [
         *[({i: None}, _lib.MX_ERR_NULL) for i in range(8)], ({8: None}, _lib.MX_ERR_SHAPE),
@@ -78,7 +78,9 @@ def test_entry_points_refuse(name, args, code):
 
 def test_workspaces():
     lib = _lib.load()
-    assert lib.mx_linear_int8_workspace(3, 48) == 256 + 12
+    assert lib.mx_linear_int8_workspace(30, 48) == 1536 + 120
+    assert lib.mx_linear_int8_workspace(4, 4096) == 0  # one kernel
+    assert lib.mx_linear_int8_workspace(4, 4112) > 0 and lib.mx_linear_int8_workspace(5, 16) > 0
     assert [lib.mx_linear_int8_workspace(*a) for a in ((0, 48), (3, 0), (3, 40), (-1, 16))] == [0] * 4
     assert lib.mx_gqa_kv8_workspace(64, 64, 1, 64, 32, 8, 128) == 0  # one short chunk: no partial results
     assert lib.mx_gqa_kv8_workspace(1, 1, 1, 100000, 32, 8, 128) > 0
