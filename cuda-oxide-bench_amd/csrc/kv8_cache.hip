@@ -35,10 +35,59 @@ __device__ __forceinline__ uint32_t codes2(float a, float b) {
   return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false) & 0xffffu;
 }
 
+// Four codes of packed values x, y of the 16-bit type, divided by s = a power of two: one
+// instruction for two (all finite values of both types at scales from 2^-32 to 2^120 give
+// the codes of the exact quotient).
+template <typename T>
+__device__ __forceinline__ uint32_t codes4(uint32_t x, uint32_t y, float s);
+typedef short i16x2_t __attribute__((ext_vector_type(2)));
+template <>
+__device__ __forceinline__ uint32_t codes4<BF16>(uint32_t x, uint32_t y, float s) {
+  const i16x2_t lo = __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(i16x2_t{}, __builtin_bit_cast(bf16x2_t, x), s, false);
+  return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(lo, __builtin_bit_cast(bf16x2_t, y), s, true));
+}
+template <>
+__device__ __forceinline__ uint32_t codes4<F16>(uint32_t x, uint32_t y, float s) {
+  const i16x2_t lo = __builtin_amdgcn_cvt_scalef32_pk_fp8_f16(i16x2_t{}, __builtin_bit_cast(f16x2_t, x), s, false);
+  return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_fp8_f16(lo, __builtin_bit_cast(f16x2_t, y), s, true));
+}
+// The same for any values and any scale: infinities and NaN become NaN.
+template <typename T>
+__device__ uint32_t codes4_any(uint32_t x, uint32_t y, float r) {
+  float v[4] = {T::to_f32(x & 0xffffu) * r, T::to_f32(x >> 16) * r, T::to_f32(y & 0xffffu) * r, T::to_f32(y >> 16) * r};
+  const uint32_t bits[4] = {x & 0x7fffu, (x >> 16) & 0x7fffu, y & 0x7fffu, (y >> 16) & 0x7fffu};
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    if (bits[i] >= first_nonfinite<T>()) v[i] = __builtin_nanf("");
+  return codes2(v[0], v[1]) | codes2(v[2], v[3]) << 16;
+}
+
+// max of the two 16-bit halves, each as an unsigned integer
+__device__ __forceinline__ uint32_t max_u16x2(uint32_t a, uint32_t b) {
+  typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+  return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u16x2, a), __builtin_bit_cast(u16x2, b)));
+}
+// The magnitudes of x's halves, 0 for one that is not finite.
+template <typename T>
+__device__ __forceinline__ uint32_t finite_magnitudes(uint32_t x) {
+  const uint32_t lo = x & 0x7fffu, hi = (x >> 16) & 0x7fffu;
+  return (lo < first_nonfinite<T>() ? lo : 0u) | (hi < first_nonfinite<T>() ? hi << 16 : 0u);
+}
+
 // One code at another scale; NaN stays the NaN that it is.
 __device__ __forceinline__ uint8_t moved(uint8_t code, float ratio) {
   if ((code & 0x7f) == 0x7f) return code;
   return (uint8_t)codes2(__builtin_amdgcn_cvt_f32_fp8(code, 0) * ratio, 0.f);
+}
+
+// Rows i of four words become columns: out[c] holds byte c of w[0] .. w[3].
+__device__ __forceinline__ void transpose4(const uint32_t (&w)[4], uint32_t (&out)[4]) {
+  const uint32_t a = __builtin_amdgcn_perm(w[1], w[0], 0x05010400u), b = __builtin_amdgcn_perm(w[3], w[2], 0x05010400u);
+  const uint32_t c = __builtin_amdgcn_perm(w[1], w[0], 0x07030602u), d = __builtin_amdgcn_perm(w[3], w[2], 0x07030602u);
+  out[0] = __builtin_amdgcn_perm(b, a, 0x05040100u);
+  out[1] = __builtin_amdgcn_perm(b, a, 0x07060302u);
+  out[2] = __builtin_amdgcn_perm(d, c, 0x05040100u);
+  out[3] = __builtin_amdgcn_perm(d, c, 0x07060302u);
 }
 
 // One workgroup per (page that new tokens reach, head): it reads them once, 4 tokens
@@ -70,54 +119,71 @@ __global__ __launch_bounds__(256) void append_kernel(const uint16_t* __restrict_
   const int start = len - n;  // position of the first new token; below 0 where there are more rows than tokens
   const int j_end = (len - 1) >> LP;
   for (int j = (max(start, 0) >> LP) + blockIdx.y; j <= j_end; j += gridDim.y) {
-    const int page = page_of(table + (size_t)b * max_pages, j << LP, LP, max_pages, pages);
-    if (page < 0) continue;
     const int lo = max(start - (j << LP), 0), hi = min(len - (j << LP), P);  // the new tokens' slots
     const int row0 = rows.first + (j << LP) - start;                       // the row of slot 0
-    const size_t at = (size_t)page * n_kv + h;
 
     u32x4 x[2][U][4];
-    uint32_t mx[2] = {0, 0};
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const int unit = t + u * NT, s0 = unit / (D / 8) * 4, c0 = unit % (D / 8) * 8;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const bool in = unit < UNITS && s0 + i >= lo && s0 + i < hi;
         x[0][u][i] = x[1][u][i] = u32x4{};
-        if (in) {
+        if (unit < UNITS && s0 + i >= lo && s0 + i < hi) {
           x[0][u][i] = ld128(knew + (size_t)(row0 + s0 + i) * k_stride + h * D + c0);
           x[1][u][i] = ld128(vnew + (size_t)(row0 + s0 + i) * v_stride + h * D + c0);
         }
       }
     }
+    const int page = page_of(table + (size_t)b * max_pages, j << LP, LP, max_pages, pages);
+    if (page < 0) continue;
+    const size_t at = (size_t)page * n_kv + h;
+    const float was[2] = {lo > 0 ? ks[at] : 0.f, lo > 0 ? vs[at] : 0.f};  // no tokens before: a scale of any size
+
+    // the largest magnitudes, an infinity or NaN the largest of all
+    uint32_t mx[2] = {0, 0};
 #pragma unroll
-    for (int kv = 0; kv < 2; ++kv)
+    for (int kv = 0; kv < 2; ++kv) {
 #pragma unroll
       for (int u = 0; u < U; ++u)
 #pragma unroll
         for (int i = 0; i < 4; ++i)
 #pragma unroll
-          for (int w = 0; w < 4; ++w) {
-            const uint32_t lo16 = x[kv][u][i][w] & 0x7fffu, hi16 = (x[kv][u][i][w] >> 16) & 0x7fffu;
-            if (lo16 < first_nonfinite<T>()) mx[kv] = max(mx[kv], lo16);
-            if (hi16 < first_nonfinite<T>()) mx[kv] = max(mx[kv], hi16);
-          }
-    const float was[2] = {ks[at], vs[at]};
-#pragma unroll
-    for (int kv = 0; kv < 2; ++kv) {
-#pragma unroll
-      for (int off = 1; off < 64; off <<= 1) mx[kv] = max(mx[kv], (uint32_t)__shfl_xor((int)mx[kv], off, 64));
-      if ((t & 63) == 0) red[kv][t >> 6] = mx[kv];
+          for (int w = 0; w < 4; ++w) mx[kv] = max_u16x2(mx[kv], x[kv][u][i][w] & 0x7fff7fffu);
     }
-    __syncthreads();  // also: every thread has read the page's scales
+    auto meet = [&] {  // the maxima of all threads
+#pragma unroll
+      for (int kv = 0; kv < 2; ++kv) {
+        mx[kv] = max(mx[kv] & 0xffffu, mx[kv] >> 16);
+#pragma unroll
+        for (int off = 1; off < 64; off <<= 1) mx[kv] = max(mx[kv], (uint32_t)__shfl_xor((int)mx[kv], off, 64));
+        if ((t & 63) == 0) red[kv][t >> 6] = mx[kv];
+      }
+      __syncthreads();  // also: every thread has read the page's scales
+#pragma unroll
+      for (int kv = 0; kv < 2; ++kv)
+#pragma unroll
+        for (int w = 0; w < NT / 64; ++w) mx[kv] = max(mx[kv], red[kv][w]);
+    };
+    meet();
+    const bool finite = max(mx[0], mx[1]) < first_nonfinite<T>();
+    if (!finite) {
+      mx[0] = mx[1] = 0;
+#pragma unroll
+      for (int kv = 0; kv < 2; ++kv)
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int w = 0; w < 4; ++w) mx[kv] = max_u16x2(mx[kv], finite_magnitudes<T>(x[kv][u][i][w]));
+      __syncthreads();  // red has been read
+      meet();
+    }
     float now[2];
 #pragma unroll
     for (int kv = 0; kv < 2; ++kv) {
-      uint32_t m = 0;
-#pragma unroll
-      for (int w = 0; w < NT / 64; ++w) m = max(m, red[kv][w]);
-      now[kv] = scale_for<T>(m);
+      now[kv] = scale_for<T>(mx[kv]);
       if (lo > 0) now[kv] = fmaxf(now[kv], was[kv]);
     }
     if (t == 0) {
@@ -140,34 +206,31 @@ __global__ __launch_bounds__(256) void append_kernel(const uint16_t* __restrict_
       }
     }
 
+    const bool plain = finite && ((__float_as_uint(now[0]) | __float_as_uint(now[1])) & 0x7fffffu) == 0;  // powers of two
     const float r[2] = {1.0f / now[0], 1.0f / now[1]};
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const int unit = t + u * NT, s0 = unit / (D / 8) * 4, c0 = unit % (D / 8) * 8;
       if (unit >= UNITS || s0 >= hi || s0 + 4 <= lo) continue;
-      uint32_t code[2][4][2];  // [K, V][token][8 channels]
+      uint32_t code[2][2][4];  // [K, V][4 channels][token]
 #pragma unroll
       for (int kv = 0; kv < 2; ++kv)
 #pragma unroll
         for (int i = 0; i < 4; ++i)
 #pragma unroll
-          for (int w = 0; w < 4; ++w) {
-            const uint32_t v = x[kv][u][i][w];
-            float a = T::to_f32(v & 0xffffu) * r[kv], c = T::to_f32(v >> 16) * r[kv];
-            if ((v & 0x7fffu) >= first_nonfinite<T>()) a = __builtin_nanf("");
-            if (((v >> 16) & 0x7fffu) >= first_nonfinite<T>()) c = __builtin_nanf("");
-            const uint32_t two = codes2(a, c);
-            code[kv][i][w >> 1] = (w & 1) ? code[kv][i][w >> 1] | two << 16 : two;
+          for (int w = 0; w < 2; ++w) {
+            const u32x4& v = x[kv][u][i];
+            code[kv][w][i] = plain ? codes4<T>(v[2 * w], v[2 * w + 1], now[kv]) : codes4_any<T>(v[2 * w], v[2 * w + 1], r[kv]);
           }
 #pragma unroll
       for (int i = 0; i < 4; ++i)
-        if (s0 + i >= lo && s0 + i < hi) st64(kp + (s0 + i) * D + c0, u32x2{code[0][i][0], code[0][i][1]});
+        if (s0 + i >= lo && s0 + i < hi) st64(kp + (s0 + i) * D + c0, u32x2{code[0][0][i], code[0][1][i]});
 #pragma unroll
-      for (int c = 0; c < 8; ++c) {
-        uint32_t w = 0;
+      for (int w = 0; w < 2; ++w) {
+        uint32_t four[4];
+        transpose4(code[1][w], four);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) w |= ((code[1][i][c >> 2] >> (8 * (c & 3))) & 0xffu) << (8 * i);
-        *reinterpret_cast<uint32_t*>(vt + (c0 + c) * VROW + s0) = w;
+        for (int c = 0; c < 4; ++c) *reinterpret_cast<uint32_t*>(vt + (c0 + 4 * w + c) * VROW + s0) = four[c];
       }
     }
     __syncthreads();
