@@ -351,25 +351,25 @@ __global__ __launch_bounds__(64 * RW) void gemm_int8_rows_kernel(
 }
 
 // ---------------------------------------------------------------------------
-// A linear layer for up to 4 rows in one kernel: every workgroup quantises the rows for
-// itself (in LDS, while its rows of B are on the way), and the second launch, the codes'
+// A linear layer for one to a few rows in one kernel: every workgroup quantises the rows
+// for itself (in LDS, while its rows of B are on the way), and the second launch, the codes'
 // way through memory and the workspace fall away.  Otherwise as the kernel above.
 // ---------------------------------------------------------------------------
-constexpr int FEW_ROWS = 4, FEW_VALUES = 16384;  // rows, rows times K
+constexpr int FEW_ROWS = 8, FEW_VALUES = 8192;  // the most rows, the most rows times K
 template <int FB>
 struct Few {
   static constexpr int X = FEW_VALUES * 2;  // the rows as they come, then their codes
+  static constexpr int SCALES = X, RING = X + 1024;
   static constexpr int SLOT = 16 * FB * KS, LPW = 2 * FB;
-  static constexpr int NS = 48 * 1024 / RW / SLOT;
-  static constexpr int LDS = X + RW * NS * SLOT;
-  static_assert(LDS <= 80 * 1024 && RW * FB * 64 * 16 <= RW * NS * SLOT, "two workgroups on a CU");
+  static constexpr int NS = (80 * 1024 - RING) / RW / SLOT;  // two workgroups on a CU
+  static constexpr int LDS = RING + RW * NS * SLOT;
+  static_assert(NS >= 2 && NS * LPW < 64 && FB * 64 * 16 <= NS * SLOT, "rings");
 };
 
 template <int FB, typename T>
-__global__ __launch_bounds__(64 * RW, 2) void linear_int8_few_kernel(const uint16_t* __restrict__ X,
-                                                                    const uint8_t* __restrict__ B,
-                                                                    const float* __restrict__ sB,
-                                                                    uint16_t* __restrict__ C, int M, int N, int K, int ldx) {
+__global__ __launch_bounds__(64 * RW, 2) void linear_int8_few_kernel(
+    const uint16_t* __restrict__ X, const uint8_t* __restrict__ B, const float* __restrict__ sB, uint16_t* __restrict__ C,
+    int M, int N, int K, int ldx) {
   using F = Few<FB>;
   constexpr int NT = 64 * RW;
   extern __shared__ __align__(1024) unsigned char smem[];
@@ -382,13 +382,13 @@ __global__ __launch_bounds__(64 * RW, 2) void linear_int8_few_kernel(const uint1
   const uint32_t x0 = lds_addr(smem);
 
   // X's rows, 8 values a lane and load, one behind the other in LDS
-  const int eighths = K / 8, pieces = M * eighths;
-  for (int i = 64 * wave; i < pieces; i += NT) {
-    const int p = min(i + lane, pieces - 1);
-    dma16(X, (uint32_t)(p / eighths * ldx + p % eighths * 8) * 2, x0 + 16 * i);
+  const uint32_t eighths = K / 8, pieces = M * eighths;
+  for (uint32_t i = 64 * wave; i < pieces; i += NT) {
+    const uint32_t p = min(i + lane, pieces - 1);
+    dma16(X, (p / eighths * ldx + p % eighths * 8) * 2, x0 + 16 * i);
   }
   // the wave's ring of B's rows
-  const uint32_t ring = x0 + F::X + wave * F::NS * F::SLOT;
+  const uint32_t ring = x0 + F::RING + wave * F::NS * F::SLOT;
   const int lr = lane >> 3;
   uint32_t off[F::LPW];
 #pragma unroll
@@ -406,19 +406,26 @@ __global__ __launch_bounds__(64 * RW, 2) void linear_int8_few_kernel(const uint1
     if (k0 + s < k1) issue(k0 + s, s);
   land_args(C, sB);
 
-  // ---- codes: units of 16 values, at most 4 a thread; those of a row are K / 16 ----
+  uint32_t* most = reinterpret_cast<uint32_t*>(smem + F::SCALES);  // the rows' maxima, then their scales
+  if (t < FEW_ROWS) most[t] = 0;
+  auto meet = [] {  // LDS reads and writes done, B's loads still on the way
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    lds_barrier();
+  };
   if (k1 - k0 >= F::NS)
     wait_vmcnt<F::NS * F::LPW>();  // X is there, B may be on the way
   else
     wait_vmcnt<0>();
-  lds_barrier();
+  meet();
+
+  // ---- codes: units of 16 values, those of a row are K / 16 ----
   constexpr int U = FEW_VALUES / 16 / NT;
-  const int per = K / 16, units = M * per;
+  const uint32_t per = K / 16, units = M * per;
   u32x4 lo[U], hi[U];
-  uint32_t mx[FEW_ROWS] = {};
 #pragma unroll
   for (int u = 0; u < U; ++u) {
-    const int i = t + u * NT;
+    const uint32_t i = t + u * NT;
+    if (i - lane >= units) break;  // the wave's units all lie behind the last
     lo[u] = hi[u] = u32x4{};
     if (i < units) {
       lo[u] = lds_ld128(x0 + 32 * i);
@@ -428,41 +435,25 @@ __global__ __launch_bounds__(64 * RW, 2) void linear_int8_few_kernel(const uint1
     quant8::take_magnitudes<T>(v, lo[u]);
     quant8::take_magnitudes<T>(v, hi[u]);
     v = max(v & 0xffffu, v >> 16);
+    const uint32_t m = min(i, units - 1) / per;
+    if (__all(m == (uint32_t)__builtin_amdgcn_readfirstlane((int)m))) {  // one row: one lane for all
 #pragma unroll
-    for (int m = 0; m < FEW_ROWS; ++m)
-      if (i / per == m) mx[m] = max(mx[m], v);
-  }
-  auto meet = [] {  // LDS reads and writes done, B's loads still on the way
-    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-    lds_barrier();
-  };
-  meet();  // X is in registers: its place takes the waves' maxima, then the codes
-  uint32_t* most = reinterpret_cast<uint32_t*>(smem);  // [RW][FEW_ROWS]
-#pragma unroll
-  for (int m = 0; m < FEW_ROWS; ++m) {
-    if (m >= M) break;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) mx[m] = max(mx[m], (uint32_t)__shfl_xor((int)mx[m], o, 64));
-    if (lane == 0) most[wave * FEW_ROWS + m] = mx[m];
-  }
-  meet();
-  float sa[FEW_ROWS];
-#pragma unroll
-  for (int m = 0; m < FEW_ROWS; ++m) {
-    uint32_t v = 0;
-    if (m < M) {
-#pragma unroll
-      for (int w = 0; w < RW; ++w) v = max(v, most[w * FEW_ROWS + m]);
+      for (int o = 1; o < 64; o <<= 1) v = max(v, (uint32_t)__shfl_xor((int)v, o, 64));
+      if (lane == 0) atomicMax(most + m, v);
+    } else {
+      atomicMax(most + m, v);
     }
-    sa[m] = quant8::scale_of<T>(v);
   }
+  meet();  // the maxima are whole, and X is in registers: the codes take its place
+  float* scales = reinterpret_cast<float*>(most);
+  const float own = t < M ? quant8::scale_of<T>(most[t]) : 0.f;
+  if (t < M) scales[t] = own;  // a thread reads and writes its own row's
   meet();
 #pragma unroll
   for (int u = 0; u < U; ++u) {
-    const int i = t + u * NT;
+    const uint32_t i = t + u * NT;
     if (i < units) {
-      const int m = i / per;
-      const float s = m == 0 ? sa[0] : m == 1 ? sa[1] : m == 2 ? sa[2] : sa[3];
+      const float s = scales[i / per];
       st128(smem + 16 * i, quant8::encode<T>(lo[u], hi[u], s, 1.0f / s));
     }
   }
@@ -501,7 +492,7 @@ __global__ __launch_bounds__(64 * RW, 2) void linear_int8_few_kernel(const uint1
     slot = slot + 1 == F::NS ? 0 : slot + 1;
   }
   __syncthreads();
-  i32x4* red = reinterpret_cast<i32x4*>(smem + F::X);  // [RW][FB][64]
+  i32x4* red = reinterpret_cast<i32x4*>(smem + F::RING);  // [RW][FB][64]
 #pragma unroll
   for (int f = 0; f < FB; ++f) red[(wave * FB + f) * 64 + lane] = acc[f];
   __syncthreads();
@@ -511,8 +502,7 @@ __global__ __launch_bounds__(64 * RW, 2) void linear_int8_few_kernel(const uint1
     for (int w = 1; w < RW; ++w) c += red[(w * FB + f) * 64 + lane];
     const int n = n0 + 16 * f + 4 * g;
     if (r16 < M && n < N) {
-      const float s = r16 == 0 ? sa[0] : r16 == 1 ? sa[1] : r16 == 2 ? sa[2] : sa[3];
-      const u32x2 v = scaled4<T>(c, s, scales4(sB, n, N));
+      const u32x2 v = scaled4<T>(c, scales[r16], scales4(sB, n, N));
       uint16_t* out = C + (size_t)r16 * N + n;
       if ((N & 3) == 0)
         st64(out, v);
@@ -528,8 +518,8 @@ __global__ __launch_bounds__(64 * RW, 2) void linear_int8_few_kernel(const uint1
 // side by side (measured from 1x1024x1024 to 8192^3; about 37 for the 256x256 tile,
 // whose ring holds two slots), so a variant costs
 //     start + (workgroups per CU) * (rows of A and B of a workgroup) * K / rate
-// and no less than HBM takes for the operands.  Against the best variant of each of 37
-// measured products the choice loses 2% on average.
+// and no less than HBM takes for the operands.  Against the best variant of each of 52
+// measured products the choice loses 1.4% on average.
 // ---------------------------------------------------------------------------
 struct Variant {
   int bm, bn;
@@ -570,6 +560,7 @@ static int run(int variant, const uint8_t* A, const float* sA, const uint8_t* B,
                int N, int K, hipStream_t s) {
   const Variant& v = kVariants[variant];
   const long long tm = (M + v.bm - 1) / v.bm, tn = (N + v.bn - 1) / v.bn;
+  if (tm * tn >= (1 << 23)) return MX_ERR_SHAPE;  // fewer than 2^32 threads
 #define ROWS(FM, FB, PER)                                                                                         \
   launch(gemm_int8_rows_kernel<FM, FB, PER, T>, lds_limit_once<gemm_int8_rows_kernel<FM, FB, PER, T>>(Rows<FM, FB, PER>::LDS), \
          Rows<FM, FB, PER>::LDS, 64 * RW, dim3((unsigned)(tm * tn)), A, sA, B, sB, C, M, N, K, s)
@@ -593,14 +584,25 @@ static int run(int variant, const uint8_t* A, const float* sA, const uint8_t* B,
 #undef TILE
 }
 
-static bool few(int M, int K) { return M <= FEW_ROWS && (long long)M * K <= FEW_VALUES; }
+// One kernel where the codes that every workgroup makes again cost less than the launch and
+// the codes' way that it saves, against the quantiser and the best product (K x N, us):
+//   rows  512x4096  1024x4096  2048x4096  4096x4096  4096x16384  8192x4096
+//   1      4.3/5.3    4.8/5.8    5.8/6.8    6.3/8.0   15.3/18.1  10.3/11.5
+//   2      4.2/5.7    5.2/6.2    6.6/7.4    7.8/8.5   15.9/18.7  13.5/12.9
+//   4      4.4/5.8    5.6/6.4    7.6/7.4   10.6/8.8   17.7/18.7
+//   8      5.1/6.2    7.3/6.6   10.4/7.7
+static bool few(int M, int K) {
+  const long long values = (long long)M * K;
+  return M <= 2 ? values <= FEW_VALUES : M <= FEW_ROWS && values <= FEW_VALUES / 2;
+}
 
 template <int FB, typename T>
 static int launch_few(const void* X, const void* B, const float* sB, void* C, int M, int N, int K, int ldx, hipStream_t s) {
+  using F = Few<FB>;
   constexpr auto kern = linear_int8_few_kernel<FB, T>;
-  MX_RETURN_IF_HIP(lds_limit_once<kern>(Few<FB>::LDS));
-  hipLaunchKernelGGL(kern, dim3((unsigned)((N + 16 * FB - 1) / (16 * FB))), dim3(64 * RW), Few<FB>::LDS, s,
-                     (const uint16_t*)X, (const uint8_t*)B, sB, (uint16_t*)C, M, N, K, ldx);
+  MX_RETURN_IF_HIP(lds_limit_once<kern>(F::LDS));
+  hipLaunchKernelGGL(kern, dim3((unsigned)((N + 16 * FB - 1) / (16 * FB))), dim3(64 * RW), F::LDS, s, (const uint16_t*)X,
+                     (const uint8_t*)B, sB, (uint16_t*)C, M, N, K, ldx);
   MX_RETURN_IF_HIP(hipGetLastError());
   return MX_OK;
 }
@@ -612,7 +614,7 @@ static int check(const void* A, const float* sA, const void* B, const float* sB,
   if (((uintptr_t)A | (uintptr_t)B | (uintptr_t)C) & 15) return MX_ERR_ALIGN;
   if (((uintptr_t)sA | (uintptr_t)sB) & 3) return MX_ERR_ALIGN;
   if (dtype != MX_DTYPE_BF16 && dtype != MX_DTYPE_F16) return MX_ERR_DTYPE;
-  if ((long long)((M + 63) / 64) * ((N + 63) / 64) > 0x7fffffffLL) return MX_ERR_SHAPE;
+  if (M > 0x7fffff00 || N > 0x7fffff00) return MX_ERR_SHAPE;
   return MX_OK;
 }
 
@@ -648,7 +650,9 @@ extern "C" int mx_linear_int8(const void* X, const void* W, const float* sW, voi
   if (ldx < K) return MX_ERR_SHAPE;
   if (ldx % 8) return MX_ERR_ALIGN;
   hipStream_t s = (hipStream_t)stream;
-  if (few(M, K) && (long long)M * ldx < (1LL << 30)) {
+  if (few(M, K)) {
+    if (M == 1) ldx = K;
+    if ((long long)M * ldx >= (1LL << 30) || N >= (1 << 27)) return MX_ERR_SHAPE;  // 32-bit offsets; threads
     // 16 rows of B a workgroup while two on every CU hold all of N
     const bool one = N <= 8192;
     if (dtype == MX_DTYPE_BF16)

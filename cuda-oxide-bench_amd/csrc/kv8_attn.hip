@@ -879,50 +879,55 @@ __global__ __launch_bounds__(64 * TW, 2) void tile_kernel(const Args a) {
 }
 
 // ---------------------------------------------------------------------------
-// The splits' partial results of a row meet: one workgroup per row, D / 4 lanes per
-// split, so that the splits' loads are under way together.
+// The splits' partial results of a row meet: WAVES waves per row, D / 4 lanes per split, so
+// that the splits' loads are under way together.
 // ---------------------------------------------------------------------------
-template <typename T, int D>
-__global__ __launch_bounds__(256) void combine_kernel(const Args a) {
-  constexpr int LANES = D / 4, GROUPS = 256 / LANES;
-  __shared__ f32x4 sums[GROUPS][LANES];
-  __shared__ float2 state[GROUPS];  // m and the denominator
-  const int grp = threadIdx.x / LANES, c = threadIdx.x % LANES;
-  const size_t r = blockIdx.x, rows = (size_t)a.T * a.n_q;
-  if (a.cu) {
+constexpr int CT = 256;  // threads
+template <typename T, int D, int WAVES>
+__global__ __launch_bounds__(CT) void combine_kernel(const Args a) {
+  constexpr int LANES = D / 4, GROUPS = 64 * WAVES / LANES, ROWS = CT / 64 / WAVES;
+  __shared__ f32x4 sums[ROWS][GROUPS][LANES];
+  __shared__ float2 state[ROWS][GROUPS];  // m and the denominator
+  const int own = threadIdx.x / (64 * WAVES), grp = threadIdx.x / LANES % GROUPS, c = threadIdx.x % LANES;
+  const size_t rows = (size_t)a.T * a.n_q, at = (size_t)blockIdx.x * ROWS + own;
+  const size_t r = at < rows ? at : rows - 1;
+  bool live = at < rows;
+  if (a.cu) {  // else no sequence's row
     const int tok = (int)(r / a.n_q);
-    if (tok < a.cu[0] || tok >= a.cu[a.B]) return;  // no sequence's row
+    live = live && tok >= a.cu[0] && tok < a.cu[a.B];
   }
   const float2* ml = reinterpret_cast<const float2*>(a.part + (size_t)a.splits * rows * D);
   float top = -INFINITY, total = 0.f;
   f32x4 o{};
+  if (live) {
 #pragma unroll 4
-  for (int s = grp; s < a.splits; s += GROUPS) {
-    const float2 x = ml[(size_t)s * rows + r];
-    const f32x4 v = *reinterpret_cast<const f32x4*>(a.part + ((size_t)s * rows + r) * D + 4 * c);
-    if (x.x == -INFINITY) continue;  // no visible token: nothing was summed
-    const float up = fmaxf(top, x.x);
-    const float w0 = top == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(top - up), w1 = __builtin_amdgcn_exp2f(x.x - up);
-    total = total * w0 + x.y * w1;
-    o = o * w0 + v * w1;
-    top = up;
+    for (int s = grp; s < a.splits; s += GROUPS) {
+      const float2 x = ml[(size_t)s * rows + r];
+      const f32x4 v = *reinterpret_cast<const f32x4*>(a.part + ((size_t)s * rows + r) * D + 4 * c);
+      if (x.x == -INFINITY) continue;  // no visible token: nothing was summed
+      const float up = fmaxf(top, x.x);
+      const float w0 = top == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(top - up), w1 = __builtin_amdgcn_exp2f(x.x - up);
+      total = total * w0 + x.y * w1;
+      o = o * w0 + v * w1;
+      top = up;
+    }
   }
-  sums[grp][c] = o;
-  if (c == 0) state[grp] = float2{top, total};
+  sums[own][grp][c] = o;
+  if (c == 0) state[own][grp] = float2{top, total};
   __syncthreads();
-  if (grp > 0) return;
+  if (grp > 0 || !live) return;
   float most = -INFINITY;
 #pragma unroll
-  for (int k = 0; k < GROUPS; ++k) most = fmaxf(most, state[k].x);
+  for (int k = 0; k < GROUPS; ++k) most = fmaxf(most, state[own][k].x);
   total = 0.f;
   o = f32x4{};
 #pragma unroll
   for (int k = 0; k < GROUPS; ++k) {
-    const float2 x = state[k];
+    const float2 x = state[own][k];
     if (x.x == -INFINITY) continue;
     const float w = __builtin_amdgcn_exp2f(x.x - most);
     total += w * x.y;
-    o += w * sums[k][c];
+    o += w * sums[own][k][c];
   }
   o *= most == -INFINITY ? 0.f : 1.0f / total;
   st64(a.out + r * D + 4 * c, u32x2{T::pack2(o[0], o[1]), T::pack2(o[2], o[3])});
@@ -945,7 +950,9 @@ static long long up(long long x, long long to) { return (x + to - 1) / to; }
 // stays filled: rows kernel, one workgroup per CU while sequences times KV heads are
 // few, two from 128 on (chunks of 256, 512, 1024, 2048 and 4096 tokens: B4 of 4096 tokens 14.6, 13.8,
 // 16.8, 23.1, 33.8 us; B32 59, 47, 42, 38, 41), and at most 4096 tokens, which keeps sequences of
-// different lengths apart (B64 of up to 8192: 218, 174, 154, 147, 149).
+// different lengths apart (B64 of up to 8192: 218, 174, 154, 147, 149).  Tile kernel: one per
+// CU, chunks a multiple of 128 (256: 512 rows on 4096 tokens 63.6 us, not 61.7; 64 on 1024
+// 25.8, not 23.4; 64: as 128).
 static Plan plan(int B, int T, int max_q, int max_kv, int n_q, int n_kv) {
   const long long rows = (long long)(max_q < T ? max_q : T) * (n_q / n_kv), heads = (long long)B * n_kv;
   Plan p;
@@ -957,7 +964,7 @@ static Plan plan(int B, int T, int max_q, int max_kv, int n_q, int n_kv) {
     chunk = std::min(chunk, 4096LL);
   } else {
     chunk = up(max_kv, up(256, heads * p.tiles));
-    chunk = up(chunk, 256) * 256;
+    chunk = up(chunk, 128) * 128;
   }
   p.splits = (int)std::min(up(max_kv, chunk), 65535LL);
   p.chunk = (int)std::min(chunk, 0x40000000LL);
@@ -992,14 +999,20 @@ static int run(const Args& a, const Plan& p, hipStream_t s) {
                              : launch_tiles<T, D, false>(a, p, s);
   if (rc != MX_OK || p.splits == 1) return rc;
   const long long rows = (long long)a.T * a.n_q;
-  hipLaunchKernelGGL((combine_kernel<T, D>), dim3((unsigned)rows), dim3(256), 0, s, a);
+  // few rows: the splits of a row side by side; many: few splits each (of 16384 rows in 2
+  // splits 17 us with 4 waves a row, 8.8 with one)
+  if (rows < 2048)
+    hipLaunchKernelGGL((combine_kernel<T, D, 4>), dim3((unsigned)rows), dim3(CT), 0, s, a);
+  else
+    hipLaunchKernelGGL((combine_kernel<T, D, 1>), dim3((unsigned)up(rows, 4)), dim3(CT), 0, s, a);
   MX_RETURN_IF_HIP(hipGetLastError());
   return MX_OK;
 }
 
+// A launch has fewer than 2^32 threads in x: 512 a workgroup here, 64 a row in the combine.
 static bool sizes_ok(int B, int T, int max_q, int max_kv, int n_q, int n_kv, int d) {
   return B > 0 && T > 0 && max_q > 0 && max_kv > 0 && n_q > 0 && n_kv > 0 && n_q % n_kv == 0 && (d == 64 || d == 128) &&
-         (long long)B * n_kv <= (1 << 24) && (long long)T * n_q <= 0x7fffffffLL;
+         (long long)B * n_kv <= (1 << 22) && (long long)T * n_q <= (1 << 25) && (long long)n_q * d <= 0x7fffffffLL;
 }
 
 }  // namespace kv8
@@ -1021,7 +1034,8 @@ extern "C" int mx_gqa_kv8(const void* q, const void* k_cache, const void* v_cach
   if (!q || !O || !page_table || !kv_lens) return MX_ERR_NULL;
   const int rc = check_cache(k_cache, v_cache, k_scale, v_scale, n_kv, d, page, pages);
   if (rc != MX_OK) return rc;
-  if (!sizes_ok(B, T, max_q, max_kv, n_q, n_kv, d) || max_pages <= 0 || (!cu && T != B)) return MX_ERR_SHAPE;
+  if (!sizes_ok(B, T, max_q, max_kv, n_q, n_kv, d) || (!cu && T != B)) return MX_ERR_SHAPE;
+  if (max_pages <= 0 || (long long)max_pages * page > kMostTokens) return MX_ERR_SHAPE;
   if (q_stride < n_q * d) return MX_ERR_SHAPE;
   if (q_stride % 8 || (((uintptr_t)q | (uintptr_t)O) & 15)) return MX_ERR_ALIGN;
   if (dtype != MX_DTYPE_BF16 && dtype != MX_DTYPE_F16) return MX_ERR_DTYPE;

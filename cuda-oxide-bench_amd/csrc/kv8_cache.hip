@@ -295,9 +295,10 @@ extern "C" int mx_kv8_append(const void* k, const void* v, void* k_cache, void* 
   if (!k || !v || !page_table || !kv_lens) return MX_ERR_NULL;
   const int rc = check_cache(k_cache, v_cache, k_scale, v_scale, n_kv, d, page, pages);
   if (rc != MX_OK) return rc;
-  if (B <= 0 || T <= 0 || max_q <= 0 || max_pages <= 0 || (!cu && T != B)) return MX_ERR_SHAPE;
-  if ((long long)B * n_kv > (1 << 24)) return MX_ERR_SHAPE;
-  if (k_stride < n_kv * d || v_stride < n_kv * d) return MX_ERR_SHAPE;
+  if (B <= 0 || T <= 0 || max_q <= 0 || (!cu && T != B)) return MX_ERR_SHAPE;
+  if (max_pages <= 0 || (long long)max_pages * page > kMostTokens) return MX_ERR_SHAPE;
+  if ((long long)B * n_kv > (1 << 22)) return MX_ERR_SHAPE;  // fewer than 2^32 threads in x
+  if (k_stride < (long long)n_kv * d || v_stride < (long long)n_kv * d) return MX_ERR_SHAPE;
   if (k_stride % 8 || v_stride % 8 || (((uintptr_t)k | (uintptr_t)v) & 15)) return MX_ERR_ALIGN;
   if (dtype != MX_DTYPE_BF16 && dtype != MX_DTYPE_F16) return MX_ERR_DTYPE;
   const int lp = log2_page(page);
@@ -323,7 +324,7 @@ extern "C" int mx_kv8_copy_pages(void* k_cache, void* v_cache, float* k_scale, f
   if (n <= 0) return MX_ERR_SHAPE;
   const long long bytes = (long long)n_kv * page * d;
   const long long pieces = (bytes + PIECE - 1) / PIECE;
-  if (bytes > 0x7fffffffLL || 2 * pieces * n > 0x7fffffffLL) return MX_ERR_SHAPE;
+  if (bytes > 0x7fffffffLL || 2 * pieces * n > (1 << 23)) return MX_ERR_SHAPE;  // fewer than 2^32 threads
   hipLaunchKernelGGL(copy_kernel, dim3((unsigned)(2 * pieces * n)), dim3(COPY_NT), 0, (hipStream_t)stream,
                      (uint8_t*)k_cache, (uint8_t*)v_cache, k_scale, v_scale, src, dst, n_kv, (uint32_t)bytes, (int)pieces,
                      pages);

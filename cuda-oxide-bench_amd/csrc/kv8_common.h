@@ -10,6 +10,10 @@ namespace kv8 {
 
 #define KV8_HD __host__ __device__ __forceinline__
 
+// The most tokens that a row of the page table may hold: token numbers, a tile past the
+// last among them, are ints.
+constexpr long long kMostTokens = 1LL << 30;
+
 // Tokens of a sequence in the cache: kv_lens[b], at least 0 and at most what its
 // row of the page table can hold.
 KV8_HD int cut_len(int len, int max_pages, int lp) {

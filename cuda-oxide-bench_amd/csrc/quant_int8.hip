@@ -77,15 +77,19 @@ __global__ __launch_bounds__(NT) void quant_int8_kernel(const uint16_t* __restri
 
 template <typename T>
 static int launch(const void* X, void* Q, float* S, int M, int K, int ldx, hipStream_t s) {
+  constexpr int MOST = 1 << 23;  // rows of a launch: fewer than 2^32 threads
   const int per = (K / 16 + NT - 1) / NT;
-  auto go = [&](auto kern) {
-    hipLaunchKernelGGL(kern, dim3((unsigned)M), dim3(NT), 0, s, (const uint16_t*)X, (uint8_t*)Q, S, K, ldx);
-  };
-  if (per <= 1) go(quant_int8_kernel<T, 1>);
-  else if (per <= 2) go(quant_int8_kernel<T, 2>);
-  else if (per <= 4) go(quant_int8_kernel<T, 4>);
-  else go(quant_int8_kernel<T, 0>);
-  MX_RETURN_IF_HIP(hipGetLastError());
+  for (long long m = 0; m < M; m += MOST) {
+    auto go = [&](auto kern) {
+      hipLaunchKernelGGL(kern, dim3((unsigned)(M - m < MOST ? M - m : MOST)), dim3(NT), 0, s, (const uint16_t*)X + m * ldx,
+                         (uint8_t*)Q + m * K, S + m, K, ldx);
+    };
+    if (per <= 1) go(quant_int8_kernel<T, 1>);
+    else if (per <= 2) go(quant_int8_kernel<T, 2>);
+    else if (per <= 4) go(quant_int8_kernel<T, 4>);
+    else go(quant_int8_kernel<T, 0>);
+    MX_RETURN_IF_HIP(hipGetLastError());
+  }
   return MX_OK;
 }
 

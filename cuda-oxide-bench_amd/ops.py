@@ -468,9 +468,13 @@ def mla_decode_absorbed(q_nope, q_rope, kv, w_uk, w_uv, scale, out=None, workspa
 # ---------------------------------------------------------------------------
 # 8-bit serving: int8 linear layers, the paged e4m3 cache and its attention
 # ---------------------------------------------------------------------------
+_INT = 1 << 31
+
+
 def _rows(t, name, dtypes, inner):
     """Checks of a tensor whose rows (first dimension) may lie apart, each of them contiguous; its row stride."""
-    if type(t) is _Tensor and t.dtype in dtypes and t.is_cuda and t.dim() == inner + 1 and t.is_contiguous():
+    if (type(t) is _Tensor and t.dtype in dtypes and t.is_cuda and t.dim() == inner + 1 and t.is_contiguous()
+            and 1 < t.shape[0] < _INT and t.stride(0) < _INT):
         return t.stride(0)
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{name} must be a torch.Tensor")
@@ -487,7 +491,12 @@ def _rows(t, name, dtypes, inner):
         want *= t.shape[d]
     if t.shape[0] > 1 and t.stride(0) < want:
         raise ValueError(f"rows of {name} overlap (strides {t.stride()})")
-    return t.stride(0) if t.shape[0] > 1 else want
+    if t.shape[0] > 1:
+        want = t.stride(0)
+    if t.shape[0] >= _INT or want >= _INT:
+        raise ValueError(f"{name} is too large (shape {tuple(t.shape)}, strides {t.stride()}): rows and their stride "
+                         "must be below 2**31")
+    return want
 
 
 def _launch(fn, t, *args):
@@ -546,7 +555,7 @@ def _check_weight(w, sw, K):
         raise ValueError(f"inner dimensions differ: {K} vs w {tuple(w.shape)}")
     if sw.shape[0] != N:
         raise ValueError(f"sw must be {(N,)}, got {tuple(sw.shape)}")
-    if N < 1 or K < 16 or K % 16 or K > 131071:
+    if not 1 <= N < _INT or K < 16 or K % 16 or K > 131071:
         raise ValueError(f"w must be [N, K] with K a multiple of 16 up to 131071, got {tuple(w.shape)}")
     return N
 
@@ -559,7 +568,7 @@ def gemm_int8(a, sa, w, sw, out=None, dtype=torch.bfloat16):
     _require(sa, "sa", (torch.float32,), 1)
     M, K = a.shape
     N = _check_weight(w, sw, K)
-    if M < 1 or sa.shape[0] != M:
+    if not 1 <= M < _INT or sa.shape[0] != M:
         raise ValueError(f"a must have rows and sa one scale for each, got {tuple(a.shape)} and {tuple(sa.shape)}")
     if out is None:
         if dtype not in _IO_DTYPES:
@@ -667,6 +676,9 @@ def _check_sequences(cache, T, page_table, kv_lens, cu_q, max_q):
     if B < 1 or most < 1 or kv_lens.shape[0] != B:
         raise ValueError(f"page_table must be [B, pages of a sequence] and kv_lens [B], got {tuple(page_table.shape)} "
                          f"and {tuple(kv_lens.shape)}")
+    if B * cache._sizes[1] > 1 << 22 or most * cache._sizes[2] > 1 << 30:
+        raise ValueError(f"page_table is too large ({tuple(page_table.shape)}): up to 2**22 sequences times KV heads, "
+                         "rows of up to 2**30 tokens")
     d = cache._device
     if page_table.get_device() != d or kv_lens.get_device() != d:
         raise ValueError("all tensors must be on the cache's device")
@@ -723,6 +735,8 @@ def kv8_copy_pages(cache, src, dst):
         raise ValueError(f"src and dst must be of one length, got {n} and {dst.shape[0]}")
     if src.get_device() != cache._device or dst.get_device() != cache._device:
         raise ValueError("all tensors must be on the cache's device")
+    if n >= _INT:
+        raise ValueError(f"src has too many pages ({n})")
     if n:
         pages, n_kv, page, d = cache._sizes
         _launch("mx_kv8_copy_pages", src, *cache._args, src.data_ptr(), dst.data_ptr(), n, n_kv, d, page, pages)

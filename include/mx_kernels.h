@@ -314,8 +314,8 @@ int mx_quant_int8(const void* X, void* Q, float* scales, int M, int K, int ldx, 
  *   C[m,n] = (sum_k A[m,k] * B[n,k]) * sA[m] * sB[n]
  * A[M,K] and B[N,K] row-major int8 (B as a linear layer stores its weight),
  * sA[M], sB[N] fp32, C[M,N] row-major bf16 or f16 (`dtype`).  The sum is
- * exact (int32), converted to fp32, scaled and rounded once.  Any M and N;
- * requires K % 16 == 0, K <= 131071 (the sum of K products of -128 fits
+ * exact (int32), converted to fp32, scaled and rounded once.  Any M and N (fewer
+ * than 2^23 workgroups: N < 2^27 for a few rows); requires K % 16 == 0, K <= 131071 (the sum of K products of -128 fits
  * int32) and 16-byte aligned A, B, C.
  * No counterpart in the reference, as above.
  */
@@ -327,8 +327,8 @@ int mx_gemm_int8(const void* A, const float* sA, const void* B, const float* sB,
  * weight W[N,K] and its scales sW[N].  C has X's type.
  * The workspace (mx_linear_int8_workspace(M, K) bytes, 16-byte aligned) holds
  * the codes and the scales; calls that may overlap each need their own.  It is 0
- * for up to 4 rows of together up to 16384 values, which one kernel does, and for
- * invalid sizes.
+ * where one kernel does all (up to 8 rows of together up to 4096 values, up to
+ * 2 of 8192; there M * ldx < 2^30), and for invalid sizes.
  */
 int mx_linear_int8(const void* X, const void* W, const float* sW, void* C, int M, int N, int K, int ldx, int dtype,
                    void* workspace, size_t ws_bytes, void* stream);
@@ -341,7 +341,8 @@ size_t mx_linear_int8_workspace(int M, int K);
  *   V codes  [pages, n_kv, d, page]   e4m3fn, each page transposed: the
  *            attention reads consecutive keys of one channel
  *   K, V scales [pages, n_kv]         fp32: value = code * scale
- * d is 64 or 128, page (tokens a page) 16, 32, 64 or 128.  Token t of sequence
+ * d is 64 or 128, page (tokens a page) 16, 32, 64 or 128; a row of the page table
+ * holds at most 2^30 tokens (max_pages * page).  Token t of sequence
  * b lies on page page_table[b * max_pages + t / page], slot t % page; kv_lens[b]
  * counts sequence b's tokens with the new ones, which are its last.  The new
  * rows (queries, keys, values) of all B sequences lie one behind the other:
@@ -362,13 +363,15 @@ size_t mx_linear_int8_workspace(int M, int K);
  *       scale, unless the new tokens begin at slot 0
  *   codes already on the page move to s: e4m3fn(RNE(code * s_old / s))
  *   new codes = e4m3fn(RNE(x / s)); an infinity or a NaN becomes NaN
+ * (A present scale that is no power of two serves as it is; the quotients are then
+ * rounded to fp32 before they become codes.)
  * Powers of two: e4m3 is a floating format, so another scale gains no
  * precision, and moving codes to a larger one then rounds nothing but the
  * smallest codes.  Slots behind the new tokens keep what they hold.
  * max_q: the most new tokens of a sequence, or an estimate (it sizes the
  * launch; a sequence with more is still written whole).  No page that a
  * sequence writes may be in another sequence's reach in the same call.
- * Requires n_kv * B <= 2^24, strides % 8 == 0 and >= n_kv * d, 16-byte aligned
+ * Requires n_kv * B <= 2^22, strides % 8 == 0 and >= n_kv * d, 16-byte aligned
  * k, v and codes.
  * No counterpart in the reference (it has no cache of keys and values beyond
  * the latent one of cutile-attn-mla).
@@ -382,7 +385,8 @@ int mx_kv8_append(const void* k, const void* v, void* k_cache, void* v_cache, fl
  * page src[i], i < n (int32 on the device; a pair with a number outside
  * 0..pages-1 is skipped).  For forked sequences (the shared prefix's last,
  * partly filled page) and compactions.  The copies run side by side: a page
- * is at most once a destination, and no destination is a source.
+ * is at most once a destination, and no destination is a source.  At most 2^34
+ * bytes of K (and as many of V) in a call.
  */
 int mx_kv8_copy_pages(void* k_cache, void* v_cache, float* k_scale, float* v_scale, const int* src, const int* dst,
                       int n, int n_kv, int d, int page, int pages, void* stream);
@@ -402,8 +406,8 @@ int mx_kv8_copy_pages(void* k_cache, void* v_cache, float* k_scale, float* v_sca
  * computed.  The workspace (mx_gqa_kv8_workspace bytes for the same sizes, may
  * be 0; 16-byte aligned) holds partial results; calls that may overlap each
  * need their own.
- * n_q % n_kv == 0; requires q_stride % 8 == 0 and >= n_q * d, 16-byte aligned q,
- * O and codes.
+ * n_q % n_kv == 0; requires B * n_kv <= 2^22, T * n_q <= 2^25, q_stride % 8 == 0 and
+ * >= n_q * d, 16-byte aligned q, O and codes.
  * No counterpart in the reference: its attention kernels read bf16 or f16 keys and
  * values of one length (cutile-attn-gqa/main.py:64-170).
  */

@@ -88,6 +88,28 @@ def test_product(ops, dtype, m, n, k):
     assert bool(out[m:].isnan().all())  # nothing behind the last row is touched
 
 
+# Each launch variant once (mx_gemm_int8 chooses by the sizes), with ragged rows, columns and inner dimensions; the
+# tiles with columns that store wide, in pairs and one by one.
+VARIANTS = [
+    (0, 129, 100, 16), (1, 129, 776, 400), (2, 1025, 98, 144), (3, 255, 2050, 144), (4, 511, 1023, 144), (5, 324, 1381, 16),
+    (6, 1024, 1023, 2064), (6, 1024, 1016, 2064), (6, 2001, 258, 4112), (7, 1925, 811, 400), (7, 1925, 816, 400),
+    (7, 1925, 810, 400), (8, 300, 6001, 400), (8, 300, 6008, 400), (9, 513, 6001, 144), (9, 513, 6008, 144), (9, 513, 6002, 144),
+    (10, 4017, 4015, 144), (10, 4017, 4016, 144), (10, 4017, 4018, 144)]
+
+
+@pytest.mark.parametrize("variant,m,n,k", VARIANTS)
+def test_product_of_every_variant(ops, variant, m, n, k):
+    announce(f"gemm_int8 variant {variant} {m}x{n}x{k}")
+    dtype = DTYPES[(variant + n) % 2]
+    a, sa = codes(m, k, m + k)
+    w, sw = codes(n, k, n + k)
+    exact = oracle.product(a, sa, w, sw)
+    out = torch.full((m + 2, n), float("nan"), dtype=dtype, device="cuda")
+    ops.gemm_int8(a.cuda(), sa.cuda(), w.cuda(), sw.cuda(), out=out[:m])
+    assert bool(((out[:m].cpu().double() - exact).abs() <= bound(exact, dtype)).all())
+    assert bool(out[m:].isnan().all())
+
+
 def test_product_of_extremes(ops):
     """The longest sum of the largest products: 131056 * 128 * 128 lies 2^18 below 2^31."""
     announce("gemm_int8 largest sum")
@@ -106,7 +128,9 @@ def test_product_of_extremes(ops):
 
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("m,n,k", [(1, 40, 256), (37, 300, 1040), (130, 260, 512), (1, 17, 16), (1, 8200, 16384), (2, 33, 8192),
-                                   (3, 1, 5456), (4, 70, 4096), (4, 8211, 2064), (3, 100, 144), (4, 64, 4112), (5, 64, 256)])
+                                   (3, 1, 5456), (4, 70, 4096), (4, 8211, 2064), (3, 100, 144), (4, 64, 4112), (5, 64, 256),
+                                   (1, 8200, 8192), (2, 8195, 4096), (2, 50, 4080), (3, 70, 1360), (8, 33, 512),
+                                   (8, 8204, 496), (7, 90, 576), (9, 64, 256), (1, 64, 8208)])
 def test_linear(ops, dtype, m, n, k):
     """Against the oracle's quantiser and product, with the caller's workspace, on rows that lie apart."""
     announce(f"linear_int8 {m}x{n}x{k} {dtype}")
@@ -135,12 +159,52 @@ def test_linear_special_rows(ops, dtype):
     w, sw = oracle.quantize_rows(rows(48, 256, torch.bfloat16, 2))
     q, sx = oracle.quantize_rows(x)
     exact = oracle.product(q, sx, w, sw)
-    for a, b in ((0, 8), (0, 4), (4, 8), (1, 2), (2, 4), (5, 7)):
-        y = ops.linear_int8(x[a:b].cuda(), w.cuda(), sw.cuda()).cpu().double()
+    for a, b, more in ((0, 8, 0), (0, 4, 0), (4, 8, 0), (1, 2, 0), (2, 4, 0), (5, 7, 0), (0, 8, 1), (0, 8, 40)):
+        xs = torch.cat([x[a:b], x[:1].expand(more, -1)])
+        y = ops.linear_int8(xs.cuda(), w.cuda(), sw.cuda()).cpu().double()[:b - a]
         assert torch.equal(y.isnan(), exact[a:b].isnan())
         over = exact[a:b].abs() > torch.finfo(dtype).max
         ok = ((y - exact[a:b]).abs() <= bound(exact[a:b], dtype)) | y.isnan() | over
         assert bool(ok.all()) and bool((y[over].abs() >= torch.finfo(dtype).max).all())
+
+
+def test_rows_of_any_stride(ops):
+    """One row has no stride that could matter; strides past 2^31 elements are refused, not cut."""
+    announce("int8 strides of one row and of far rows")
+    x = rows(1, 512, torch.bfloat16, 9)
+    w, sw = oracle.quantize_rows(rows(40, 512, torch.bfloat16, 8))
+    w, sw = w.cuda(), sw.cuda()
+    want = ops.linear_int8(x.cuda(), w, sw)
+    for stride in (0, 3, 511, 513, 10 ** 10):
+        y = x.cuda().as_strided((1, 512), (stride, 1))
+        q, s = ops.quant_int8(y)
+        same(q, s, x)
+        assert torch.equal(ops.linear_int8(y, w, sw), want)
+    big = torch.empty(2 ** 31 + 512, dtype=torch.bfloat16, device="cuda")
+    for stride in (2 ** 31, 2 ** 30):
+        far = big.as_strided((2, 512), (stride, 1))
+        far.copy_(x.expand(2, -1))
+        with pytest.raises((ValueError, RuntimeError)):
+            ops.linear_int8(far, w, sw)
+    q, s = ops.quant_int8(far)
+    same(q, s, x.expand(2, -1))
+    far = big.as_strided((2, 512), (2 ** 31, 1))
+    with pytest.raises(ValueError):
+        ops.quant_int8(far)
+    del big, far
+
+
+def test_quantiser_of_many_rows(ops):
+    """More rows than one launch takes."""
+    announce("quant_int8 of 2^23 + 3 rows")
+    m = 2 ** 23 + 3
+    x = torch.zeros((m, 16), dtype=torch.bfloat16, device="cuda")
+    x[:, 5] = 2
+    x[-2:, 3] = 4
+    q, s = ops.quant_int8(x)
+    assert bool((s[:-2] == torch.tensor(2.0) / 127).all()) and bool((s[-2:] == torch.tensor(4.0) / 127).all())
+    assert bool((q[:, 5] == torch.tensor([127] * (m - 2) + [64, 64], dtype=torch.int8, device="cuda")).all())
+    assert int(q.count_nonzero()) == m + 2
 
 
 def test_streams_and_capture(ops):
@@ -148,7 +212,7 @@ def test_streams_and_capture(ops):
     announce("linear_int8 graphs on two streams")
     w, sw = oracle.quantize_rows(rows(320, 512, torch.bfloat16, 5))
     w, sw = w.cuda(), sw.cuda()
-    xs = [rows(m, 512, torch.bfloat16, m).cuda() for m in (6, 90)]
+    xs = [rows(m, 512, torch.bfloat16, m).cuda() for m in (12, 90)]
     want = [ops.linear_int8(x, w, sw) for x in xs]
     outs = [torch.empty_like(y) for y in want]
     spaces = [torch.empty(max(1, ops.linear_int8_workspace_bytes(*x.shape)), dtype=torch.uint8, device="cuda") for x in xs]

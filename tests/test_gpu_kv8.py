@@ -178,6 +178,68 @@ def test_append_strides_hints_and_bad_numbers(ops):
     assert_cache(cache, want)
 
 
+def test_append_to_other_scales(ops):
+    """Pages whose present scale is no power of two: it stays where it is large enough, and every code, kept or
+    new, is the nearest one up to fp32's rounding of the quotient (the scale's reciprocal, the product: 2^-23 of it)."""
+    announce("kv8_append to scales that are no powers of two")
+    n_kv, d, page = 2, 64, 32
+    for dtype, loud in itertools.product((BF16, F16), (8, 1)):
+        cache = filled(ops, 6, n_kv, d, page, 9)
+        s = torch.rand((2, 6, n_kv), generator=torch.Generator().manual_seed(1)) * 0.02 + 0.001
+        cache.k_scale.copy_(s[0])
+        cache.v_scale.copy_(s[1])
+        want = oracle.Cache(cache.k, cache.v, cache.k_scale, cache.v_scale)
+        was = [want.k * s[0][:, :, None, None], want.v * s[1][:, :, None, None]]
+        table, lens, cu = [[0], [1], [2], [3]], [20, 32, 9, 4], [0, 3, 10, 11, 15]
+        k, v = randn((15, n_kv, d), 3, dtype), randn((15, n_kv, d), 4, dtype, loud)
+        want.append(k, v, table, lens, cu)
+        ops.kv8_append(k.cuda(), v.cuda(), cache, i32(table), i32(lens), i32(cu), 7)
+        for code, exp, scale, exp_s, x, old in ((cache.k, want.k, cache.k_scale, want.ks, k, was[0]),
+                                                (cache.v.transpose(2, 3), want.v, cache.v_scale, want.vs, v, was[1])):
+            assert torch.equal(scale.cpu().double(), exp_s)
+            assert bool((exp_s[3].log2().frac() == 0).all())
+            if x is k or loud == 1:
+                assert bool((exp_s[:3].log2().frac() != 0).any())
+            for b in range(4):
+                n = cu[b + 1] - cu[b]
+                true = old[b].clone()
+                true[:, lens[b] - n:lens[b]] = x[cu[b]:cu[b + 1]].double().transpose(0, 1)
+                step = exp_s[b][:, None, None]
+                err = (code[b].cpu().double() * step - true)[:, :lens[b]].abs()
+                best = (exp[b] * step - true)[:, :lens[b]].abs()
+                assert bool((err <= best + 2 * 2.0 ** -23 * true[:, :lens[b]].abs()).all())
+                behind = torch.equal(code[b].cpu().double()[:, lens[b]:], exp[b][:, lens[b]:])
+                assert behind
+
+
+def test_one_row_of_any_stride(ops):
+    announce("kv8 one row of any stride")
+    cache, other = (filled(ops, 4, 2, 64, 16, 1) for _ in range(2))
+    table, lens = i32([[2, 1]]), i32([20])
+    q, k, v = (randn((1, n, 64), n, BF16, 0.1).cuda() for n in (4, 2, 2))
+    ops.kv8_append(k, v, other, table, lens)
+    want = ops.gqa_kv8(q, other, table, lens)
+    for stride in (0, 7, 10 ** 10):
+        far = [t.as_strided(t.shape, (stride, 64, 1)) for t in (q, k, v)]
+        ops.kv8_append(far[1], far[2], cache, table, lens)
+        assert torch.equal(cache.k.view(torch.uint8), other.k.view(torch.uint8))
+        assert torch.equal(cache.v.view(torch.uint8), other.v.view(torch.uint8))
+        assert torch.equal(ops.gqa_kv8(far[0], cache, table, lens), want)
+
+
+def test_tables_too_large_are_refused(ops):
+    announce("kv8 table of more than 2^30 tokens")
+    cache = filled(ops, 4, 1, 64, 16, 1)
+    q = randn((1, 1, 64), 1, BF16).cuda()
+    table = torch.zeros((1, 2 ** 26 + 1), dtype=torch.int32, device="cuda")
+    for call in (lambda: ops.kv8_append(q, q, cache, table, i32([5])), lambda: ops.gqa_kv8(q, cache, table, i32([5]))):
+        with pytest.raises(ValueError, match="too large"):
+            call()
+    # the widest one, all of it the same page: as many tokens as are there count
+    table = table[:, :2 ** 26].contiguous()
+    assert torch.equal(ops.gqa_kv8(q, cache, table, i32([5])), ops.gqa_kv8(q, cache, i32([[0]]), i32([5])))
+
+
 # ---- attention ------------------------------------------------------------
 ATTEND = [
     # d, page, n_kv, group, dtype, lens, news

@@ -45,12 +45,14 @@ BAD = [
         *[({i: None}, _lib.MX_ERR_NULL) for i in (0, 1, 2, 3, 9)], *[({i: 0}, _lib.MX_ERR_SHAPE) for i in (4, 5, 6)],
         ({4: -5}, _lib.MX_ERR_SHAPE), ({6: 72}, _lib.MX_ERR_SHAPE), ({7: 56}, _lib.MX_ERR_SHAPE),
         ({7: 68}, _lib.MX_ERR_ALIGN), ({0: U}, _lib.MX_ERR_ALIGN), ({9: U}, _lib.MX_ERR_ALIGN),
-        ({8: 7}, _lib.MX_ERR_DTYPE), ({10: 2719}, _lib.MX_ERR_WORKSPACE)]),
+        ({8: 7}, _lib.MX_ERR_DTYPE), ({10: 2719}, _lib.MX_ERR_WORKSPACE), ({4: 8, 7: 2 ** 27}, _lib.MX_ERR_SHAPE),
+        ({4: 1, 5: 2 ** 27}, _lib.MX_ERR_SHAPE)]),
     # k, v, kc, vc, ks, vs, table, lens, cu, B, T, max_q, n_kv, d, page, pages, max_pages, ldk, ldv, dtype, stream
     *_calls("mx_kv8_append", [P] * 9 + [2, 5, 4, 2, 64, 16, 9, 3, 128, 128, 0, None], [
         *[({i: None}, _lib.MX_ERR_NULL) for i in range(8)], ({8: None}, _lib.MX_ERR_SHAPE),
         *[({i: 0}, _lib.MX_ERR_SHAPE) for i in range(9, 17)], ({13: 96}, _lib.MX_ERR_SHAPE), ({14: 48}, _lib.MX_ERR_SHAPE),
-        ({14: 256}, _lib.MX_ERR_SHAPE), ({9: 2 ** 23 + 1}, _lib.MX_ERR_SHAPE), ({15: 2 ** 31 - 1}, _lib.MX_ERR_SHAPE),
+        ({14: 256}, _lib.MX_ERR_SHAPE), ({16: 2 ** 26 + 1}, _lib.MX_ERR_SHAPE), ({12: 2 ** 20, 9: 8}, _lib.MX_ERR_SHAPE),
+        ({9: 2 ** 23 + 1}, _lib.MX_ERR_SHAPE), ({15: 2 ** 31 - 1}, _lib.MX_ERR_SHAPE),
         ({17: 120}, _lib.MX_ERR_SHAPE), ({18: 64}, _lib.MX_ERR_SHAPE), ({17: 132}, _lib.MX_ERR_ALIGN),
         ({18: 130}, _lib.MX_ERR_ALIGN), *[({i: U}, _lib.MX_ERR_ALIGN) for i in range(4)],
         *[({i: V}, _lib.MX_ERR_ALIGN) for i in (4, 5)], ({19: 2}, _lib.MX_ERR_DTYPE)]),
@@ -67,7 +69,7 @@ BAD = [
         ({16: 8}, _lib.MX_ERR_SHAPE), ({19: 248}, _lib.MX_ERR_SHAPE), ({19: 260}, _lib.MX_ERR_ALIGN),
         ({0: U}, _lib.MX_ERR_ALIGN), ({8: U}, _lib.MX_ERR_ALIGN), ({2: U}, _lib.MX_ERR_ALIGN), ({23: U}, _lib.MX_ERR_ALIGN),
         ({22: 2}, _lib.MX_ERR_DTYPE), ({23: None}, _lib.MX_ERR_WORKSPACE), ({24: 1000}, _lib.MX_ERR_WORKSPACE),
-        ({10: 2 ** 30}, _lib.MX_ERR_SHAPE)]),
+        ({10: 2 ** 30}, _lib.MX_ERR_SHAPE), ({18: 2 ** 26 + 1}, _lib.MX_ERR_SHAPE), ({9: 2 ** 22}, _lib.MX_ERR_SHAPE)]),
 ]
 
 
@@ -79,12 +81,49 @@ def test_entry_points_refuse(name, args, code):
 def test_workspaces():
     lib = _lib.load()
     assert lib.mx_linear_int8_workspace(30, 48) == 1536 + 120
-    assert lib.mx_linear_int8_workspace(4, 4096) == 0  # one kernel
-    assert lib.mx_linear_int8_workspace(4, 4112) > 0 and lib.mx_linear_int8_workspace(5, 16) > 0
+    for m, k in ((1, 8192), (2, 4096), (3, 1360), (8, 512), (5, 16)):  # one kernel
+        assert lib.mx_linear_int8_workspace(m, k) == 0
+    for m, k in ((1, 8208), (2, 4112), (3, 1376), (8, 528), (9, 16)):
+        assert lib.mx_linear_int8_workspace(m, k) >= m * (k + 4)
     assert [lib.mx_linear_int8_workspace(*a) for a in ((0, 48), (3, 0), (3, 40), (-1, 16))] == [0] * 4
     assert lib.mx_gqa_kv8_workspace(64, 64, 1, 64, 32, 8, 128) == 0  # one short chunk: no partial results
     assert lib.mx_gqa_kv8_workspace(1, 1, 1, 100000, 32, 8, 128) > 0
     assert lib.mx_gqa_kv8_workspace(1, 1, 1, 100000, 31, 8, 128) == 0
+
+
+def test_launches_choose(tmp_path):
+    """The GPU tests reach every variant of the product; the attention's kernel, its splits and its chunks over many
+    sizes: no split starts behind the last token, up to 32 rows per KV head never take the tiles."""
+    from test_gpu_int8 import VARIANTS
+    sizes = ", ".join(f"{{{v}, {m}, {n}, {k}}}" for v, m, n, k in VARIANTS)
+    out = query(tmp_path, "gemm_int8.hip", r"""
+  using namespace mx::gemmi8;
+  const int sizes[][4] = {SIZES};
+  for (auto& s : sizes) printf("%d\n", pick(s[1], s[2], s[3]) == s[0] ? s[0] : -1);
+  printf("%d\n", kNumVariants);""".replace("SIZES", sizes))
+    assert set(out[:-1]) == {str(v) for v in range(int(out[-1]))}
+    out = query(tmp_path, "kv8_attn.hip", r"""
+  using namespace mx::kv8;
+  long long n = 0;
+  for (int B : {1, 3, 64, 4096})
+    for (int T : {1, 16, 17, 32, 33, 1000, 100000})
+      for (int kv : {1, 255, 256, 257, 8192, 131072, 1 << 30})
+        for (int n_kv : {1, 8, 32})
+          for (int G : {1, 4, 16, 48})
+            for (int max_q : {1, T}) {
+              const Plan p = plan(B, T, max_q, kv, n_kv * G, n_kv);
+              const long long rows = (long long)std::min(max_q, T) * G;
+              const bool kernel = rows <= 16 ? p.nr == 1 : rows <= 32 ? p.nr == 2 : p.nr == 0;
+              const bool whole = p.splits >= 1 && p.splits <= 65535 && p.chunk >= 1 && p.tiles >= 1;
+              const bool useful = p.splits == 1 || (long long)(p.splits - 1) * p.chunk < kv;
+              if (!kernel || !whole || !useful) {
+                printf("plan(%d, %d, %d, %d, %d, %d)\n", B, T, max_q, kv, n_kv * G, n_kv);
+                return 0;
+              }
+              ++n;
+            }
+  printf("ok %d\n", n > 1000);""")
+    assert out == ["ok 1"]
 
 
 def test_operators_refuse_before_the_device():
