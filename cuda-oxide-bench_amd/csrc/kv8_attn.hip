@@ -175,7 +175,6 @@ __global__ __launch_bounds__(64 * NW, 2) void rows_kernel(const Args a) {
   if (n == 0) return;
   const int t0 = (int)min(begin, (long long)len);
   const int t1 = split + 1 == a.splits ? len : (int)min(begin + a.chunk, (long long)len);
-  const int tiles = (t1 - t0 + 63) / 64;
   const float c = fabsf(a.c);
   const uint32_t flip = a.c < 0.f ? 0x80008000u : 0u;  // a negative scale turns q, so that larger scores stay larger
 
@@ -196,7 +195,10 @@ __global__ __launch_bounds__(64 * NW, 2) void rows_kernel(const Args a) {
       for (int k = 0; k < KC; ++k) qf[i][k] = ld128(src + 8 * k) ^ u32x4{flip, flip, flip, flip};
       limit[i] = min(a.causal ? max(len - n + tok + 1, 0) : len, t1);
     }
-    const int low = min(a.causal ? max(len - n + r0 / G + 1, 0) : len, t1);  // keys that every row of the block sees
+    // keys that every row of the block sees, and those that any does
+    const int low = min(a.causal ? max(len - n + r0 / G + 1, 0) : len, t1);
+    const int high = min(a.causal ? max(len - n + min(r0 + 16 * NR - 1, n * G - 1) / G + 1, 0) : len, t1);
+    const int tiles = high > t0 ? (high - t0 + 63) / 64 : 0;
 
     f32x4 acc[NR][DT];
     float m[NR], l[NR];
@@ -950,10 +952,13 @@ static long long up(long long x, long long to) { return (x + to - 1) / to; }
 // stays filled: rows kernel, one workgroup per CU while sequences times KV heads are
 // few, two from 128 on (chunks of 256, 512, 1024, 2048 and 4096 tokens: B4 of 4096 tokens 14.6, 13.8,
 // 16.8, 23.1, 33.8 us; B32 59, 47, 42, 38, 41), and at most 4096 tokens, which keeps sequences of
-// different lengths apart (B64 of up to 8192: 218, 174, 154, 147, 149).  Tile kernel: one per
+// different lengths apart (B64 of up to 8192: 218, 174, 154, 147, 149).  Up to 512 tokens of
+// 128, 1024 of 64, one workgroup is as fast as two and the combine (B1..16, us: d = 128, 512
+// tokens 9.1..10.9 and 10.0..12.0, 768 tokens 10.7..12.6 and 10.0..14.0; d = 64, 512 tokens
+// 6.4..7.5 and 8.3..9.6, 1001 tokens 9.3..9.5 and 9.2..10.5).  Tile kernel: one per
 // CU, chunks a multiple of 128 (256: 512 rows on 4096 tokens 63.6 us, not 61.7; 64 on 1024
 // 25.8, not 23.4; 64: as 128).
-static Plan plan(int B, int T, int max_q, int max_kv, int n_q, int n_kv) {
+static Plan plan(int B, int T, int max_q, int max_kv, int n_q, int n_kv, int d) {
   const long long rows = (long long)(max_q < T ? max_q : T) * (n_q / n_kv), heads = (long long)B * n_kv;
   Plan p;
   p.nr = rows <= 16 ? 1 : rows <= 32 ? 2 : 0;
@@ -962,6 +967,7 @@ static Plan plan(int B, int T, int max_q, int max_kv, int n_q, int n_kv) {
   if (p.nr) {
     chunk = up(up(heads * max_kv, heads >= 128 ? 512 : 256), 256) * 256;
     chunk = std::min(chunk, 4096LL);
+    if ((long long)max_kv * d <= 65536) chunk = max_kv;
   } else {
     chunk = up(max_kv, up(256, heads * p.tiles));
     chunk = up(chunk, 128) * 128;
@@ -1021,7 +1027,7 @@ static bool sizes_ok(int B, int T, int max_q, int max_kv, int n_q, int n_kv, int
 extern "C" size_t mx_gqa_kv8_workspace(int B, int T, int max_q, int max_kv, int n_q, int n_kv, int d) {
   using namespace mx::kv8;
   if (!sizes_ok(B, T, max_q, max_kv, n_q, n_kv, d)) return 0;
-  const Plan p = plan(B, T, max_q, max_kv, n_q, n_kv);
+  const Plan p = plan(B, T, max_q, max_kv, n_q, n_kv, d);
   return p.splits == 1 ? 0 : (size_t)p.splits * T * n_q * (d + 2) * sizeof(float);
 }
 
@@ -1039,7 +1045,7 @@ extern "C" int mx_gqa_kv8(const void* q, const void* k_cache, const void* v_cach
   if (q_stride < n_q * d) return MX_ERR_SHAPE;
   if (q_stride % 8 || (((uintptr_t)q | (uintptr_t)O) & 15)) return MX_ERR_ALIGN;
   if (dtype != MX_DTYPE_BF16 && dtype != MX_DTYPE_F16) return MX_ERR_DTYPE;
-  const Plan p = plan(B, T, max_q, max_kv, n_q, n_kv);
+  const Plan p = plan(B, T, max_q, max_kv, n_q, n_kv, d);
   if (p.splits > 1) {
     if (!workspace || ws_bytes < mx_gqa_kv8_workspace(B, T, max_q, max_kv, n_q, n_kv, d)) return MX_ERR_WORKSPACE;
     if ((uintptr_t)workspace & 15) return MX_ERR_ALIGN;

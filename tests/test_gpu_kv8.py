@@ -387,6 +387,20 @@ def test_attend_hints_only_choose(ops, news):
     assert torch.equal(out, same)
 
 
+@pytest.mark.parametrize("causal", [True, False])
+def test_attend_more_rows_than_hinted(ops, causal):
+    """2300 rows of one sequence where max_q says 1: blocks of rows far from the last token, NaN codes here and there,
+    which only the rows that see them may show."""
+    announce(f"gqa_kv8 2300 rows, hint 1, causal={causal}")
+    n, page = 2300, 64
+    cache = filled(ops, 40, 1, 64, page, 5)
+    table = tables([n + 7], page, 40, 6)
+    for t in (60, 700, 2111, 2290) if causal else (700,):
+        cache.v.view(torch.uint8)[table[0][t // page], 0, t % 64, t % page] = 0x7F
+    q = randn((n, 1, 64), 7, BF16, 0.05)
+    check_attend(ops, cache, q, table, [n + 7], [n], causal, max_q=1)
+
+
 def test_far_pages(ops):
     """Codes past 2^32 bytes of each of the cache's tensors, written, copied and read."""
     announce("kv8 pages past 2^32 bytes")

@@ -111,7 +111,7 @@ def test_launches_choose(tmp_path):
         for (int n_kv : {1, 8, 32})
           for (int G : {1, 4, 16, 48})
             for (int max_q : {1, T}) {
-              const Plan p = plan(B, T, max_q, kv, n_kv * G, n_kv);
+              const Plan p = plan(B, T, max_q, kv, n_kv * G, n_kv, T % 2 ? 64 : 128);
               const long long rows = (long long)std::min(max_q, T) * G;
               const bool kernel = rows <= 16 ? p.nr == 1 : rows <= 32 ? p.nr == 2 : p.nr == 0;
               const bool whole = p.splits >= 1 && p.splits <= 65535 && p.chunk >= 1 && p.tiles >= 1;
