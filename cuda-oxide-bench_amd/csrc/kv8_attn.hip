@@ -136,8 +136,11 @@ __device__ __forceinline__ bool any_group(bool x) {
 // scalar unit's work, and a lane adds an offset that never changes.
 // ---------------------------------------------------------------------------
 constexpr int NW = 4;
+// Workgroups on a CU.  32 rows of 128 channels need some 430 registers a lane: with two workgroups
+// they spill (32 rows on 4096 tokens, B4 26.6 and 19.6 us, B16 47 and 36).
+constexpr int rows_per_cu(int nr, int d) { return nr * d == 256 ? 1 : 2; }
 template <typename T, int D, int NR, bool WIDE>
-__global__ __launch_bounds__(64 * NW, 2) void rows_kernel(const Args a) {
+__global__ __launch_bounds__(64 * NW, rows_per_cu(NR, D)) void rows_kernel(const Args a) {
   constexpr int KC = D / 32;   // contraction steps
   constexpr int KL = D / 64;   // 16-byte loads of a K row per lane
   constexpr int DT = D / 16;   // output fragments
@@ -965,7 +968,7 @@ static Plan plan(int B, int T, int max_q, int max_kv, int n_q, int n_kv, int d) 
   p.tiles = (int)std::min(up(rows, TR), 65535LL);
   long long chunk;
   if (p.nr) {
-    chunk = up(up(heads * max_kv, heads >= 128 ? 512 : 256), 256) * 256;
+    chunk = up(up(heads * max_kv, heads >= 128 && rows_per_cu(p.nr, d) == 2 ? 512 : 256), 256) * 256;
     chunk = std::min(chunk, 4096LL);
     if ((long long)max_kv * d <= 65536) chunk = max_kv;
   } else {
