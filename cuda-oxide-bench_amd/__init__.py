@@ -1,5 +1,6 @@
 """MI355X (gfx950) quant-inference kernel path: bf16 / fp8 block-scaled GEMM,
-fused causal GQA forward, MLA absorbed decode and GDN decode.
+fused causal GQA forward, MLA absorbed decode and GDN decode; int8 linear
+layers and a paged 8-bit cache of keys and values with its attention.
 
 The package directory name is not a Python identifier; import it with
 ``importlib.import_module("cuda-oxide-bench_amd")`` after putting the repo
