@@ -4,10 +4,10 @@
 // the scales ks, vs those of t's page and head.  The codes go through the 16-bit
 // MFMAs (e4m3 -> bf16 / f16 is exact), the scales around them:
 //     y[t]  = scale log2(e) ks (q . k8[t]) + log2(vs)
-//     P'[t] = 2^(y[t] - m),   m = the running maximum of y
+//     P'[t] = 2^(y[t] - m),   m = the running maximum of y (f16: less a constant)
 //     O     = (sum_t P'[t] v8[t]) / (sum_t P'[t] / vs)
 // so a page's two scales cost one FMA constant per score and one product per page in
-// the denominator, P' carries vs and stays within 0..1 in either 16-bit type, and any positive
+// the denominator, P' carries vs and stays within either 16-bit type's range, and any positive
 // scales serve.  (m - max y of a page is at most the spread of log2 vs, so the
 // denominator's terms stay in fp32's range while the vs of a sequence lie within 2^100.)
 //
@@ -61,6 +61,14 @@ __device__ __forceinline__ u32x4 widen8(uint32_t a, uint32_t b) {
 template <typename T>
 __device__ __forceinline__ constexpr uint32_t one_bits() {
   return std::is_same<T, BF16>::value ? 0x3f80u : 0x3c00u;
+}
+
+// log2 of the largest P'.  f16 has no more than 24 binades below one, and a page whose vs is that
+// far below the largest may hold all of a channel: P' then fills the range up to 2^15.
+// tile_kernel, whose maximum may lag by kLazy, leaves room for that.
+template <typename T>
+__device__ __forceinline__ constexpr float lift() {
+  return std::is_same<T, BF16>::value ? 0.f : 15.f;
 }
 
 // A dword with 0x80 in each byte of x that is a NaN code.
@@ -305,7 +313,7 @@ __global__ __launch_bounds__(64 * NW, rows_per_cu(NR, D)) void rows_kernel(const
         }
         if (!masked) seen[i] = true;
         const float top = fmaxf(m[i], max_xor32(max_xor16(mx)));
-        const float base = top == -INFINITY ? 0.f : top;
+        const float base = top == -INFINITY ? 0.f : top - lift<T>();
         if (__any(m[i] != top)) {
           const float corr = m[i] == top ? 1.f : __builtin_amdgcn_exp2f(m[i] - top);
           l[i] *= corr;
@@ -466,6 +474,7 @@ __global__ __launch_bounds__(64 * TW, 2) void tile_kernel(const Args a) {
   constexpr int KC = D / 32, DT = D / 16;
   constexpr int NT = 64 * TW;
   constexpr int U = D * 8 / NT;  // 16-byte units of a tile (K, then V) per thread
+  constexpr float LEVEL = lift<T>() > kLazy ? lift<T>() - kLazy : 0.f;  // where a moved maximum puts log2 P'
   static_assert(U >= 1 && U * NT == D * 8, "units");
   extern __shared__ __align__(1024) unsigned char smem[];
   const int tid = threadIdx.x, lane = tid & 63;
@@ -763,7 +772,7 @@ __global__ __launch_bounds__(64 * TW, 2) void tile_kernel(const Args a) {
       }
       __builtin_amdgcn_sched_barrier(0);
 
-      const bool moved = __any(fmaxf(mx[0], mx[1]) > kLazy);
+      const bool moved = __any(fmaxf(mx[0], mx[1]) > LEVEL + kLazy);
       if (moved || open) {
 #pragma unroll
         for (int k = 0; k < KC; ++k)
@@ -780,7 +789,7 @@ __global__ __launch_bounds__(64 * TW, 2) void tile_kernel(const Args a) {
           mx[i] = exponents(i);
           mx[i] = max_xor32(max_xor16(mx[i]));
           const bool empty = open && sum_xor32(sum_xor16(l[i])) == 0.f, met = mx[i] > -INFINITY;
-          const float shift = empty ? (met ? mx[i] : 0.f) : mx[i] > kLazy ? mx[i] : 0.f;
+          const float shift = empty ? (met ? mx[i] - LEVEL : 0.f) : mx[i] > LEVEL + kLazy ? mx[i] - LEVEL : 0.f;
           still |= empty && !met;
           seen[i] |= cst[1] > -INFINITY && at + 16 * g < limit[i];
           m[i] += shift;

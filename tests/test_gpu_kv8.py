@@ -293,6 +293,32 @@ def test_attend_scales_far_apart_and_negative(ops, news):
         check_attend(ops, cache, q, tables(lens, 16, 25, 6), lens, news, scale=scale)
 
 
+@pytest.mark.parametrize("news", [[1], [20], [100]])
+def test_attend_channel_on_quiet_pages(ops, news):
+    """f16: a channel that only pages with a scale 2^22 below the others' hold.  Its weights P' there lie within f16's
+    range, so the channel has the relative error of any other: the roundings of P' and of the output, 2^-11 each, what
+    the fp32 steps add (2^-15 is ample: scores to 2, some 200 terms), and half of f16's least step, 2^-25."""
+    announce(f"gqa_kv8 quiet pages {news}")
+    n, page = 300, 64
+    cache = filled(ops, 5, 1, 64, page, 3)
+    table = [[4, 0, 2, 1, 3]]
+    cache.v_scale.fill_(1.0)
+    cache.k_scale.fill_(2.0 ** -9)
+    cache.v_scale[2] = cache.v_scale[3] = 2.0 ** -22
+    v = cache.v.view(torch.uint8)
+    for p in (0, 1, 4):
+        v[p, :, 0] = 0
+    for p in (2, 3):
+        v[p, :, 0] = 0x70 + (torch.arange(page, device="cuda") % 14).to(torch.uint8)
+    q = randn((news[0], 2, 64), 5, F16, 0.2)
+    exp, _, _ = oracle.Cache(cache.k, cache.v, cache.k_scale, cache.v_scale).attend(q, table, [n], prefix(news), False)
+    more = {} if news == [1] else {"cu_q": i32(prefix(news)), "max_q": news[0]}
+    got = ops.gqa_kv8(q.cuda(), cache, i32(table), i32([n]), causal=False, **more).cpu().double()[..., 0]
+    exp = exp[..., 0]
+    assert bool((exp > 2.0 ** -20).all())
+    assert bool(((got - exp).abs() <= exp * (2 * 2.0 ** -11 + 2.0 ** -15) + 2.0 ** -25).all())
+
+
 @pytest.mark.parametrize("news", [[1], [4], [9], [100]])
 def test_attend_nan_and_inf(ops, news):
     """NaN codes of K and V reach the rows that see their token and no others; a query with an infinity gives what
