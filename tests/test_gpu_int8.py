@@ -40,7 +40,8 @@ def same(q, s, x):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
-@pytest.mark.parametrize("m,k", [(1, 16), (3, 48), (5, 4096), (2, 4112), (7, 8208), (2, 16400), (300, 1040)])
+@pytest.mark.parametrize("m,k", [(1, 16), (3, 48), (5, 4096), (2, 4112), (7, 8208), (2, 16400), (300, 1040),
+                                 (2047, 1024), (2048, 16), (2051, 496), (2050, 1024), (2049, 1040)])
 def test_quantiser(ops, dtype, m, k):
     announce(f"quant_int8 {m}x{k} {dtype}")
     x = rows(m, k, dtype, m + k)
