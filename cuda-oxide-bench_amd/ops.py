@@ -473,9 +473,11 @@ _INT = 1 << 31
 
 def _rows(t, name, dtypes, inner):
     """Checks of a tensor whose rows (first dimension) may lie apart, each of them contiguous; its row stride."""
-    if (type(t) is _Tensor and t.dtype in dtypes and t.is_cuda and t.dim() == inner + 1 and t.is_contiguous()
-            and 1 < t.shape[0] < _INT and t.stride(0) < _INT):
-        return t.stride(0)
+    if type(t) is _Tensor and t.dtype in dtypes and t.is_cuda and t.dim() == inner + 1 and t.is_contiguous():
+        rows = t.shape[0]
+        stride = t.numel() if rows == 1 else t.stride(0)  # one row may have any stride
+        if rows < _INT and stride < _INT:
+            return stride
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{name} must be a torch.Tensor")
     if t.dtype not in dtypes:

@@ -497,6 +497,46 @@ def test_graphs_and_streams(ops, news):
             assert torch.equal(out, want)
 
 
+def test_a_captured_step_follows_the_device(ops):
+    """One captured step of decoding, replayed while lengths, table, tokens and queries change in place: as eager calls
+    on a cache of their own, from a first token to lengths past the hint."""
+    announce("kv8 captured step, other lengths at each replay")
+    n_kv, d, page, most = 2, 128, 16, 60
+    caches = [filled(ops, 2 * most, n_kv, d, page, 3) for _ in range(2)]
+    table = i32(tables([most * page, most * page], page, 2 * most, 4))
+    lens = i32([0, 1])
+    k, v, q = (torch.empty((2, n, d), dtype=BF16, device="cuda") for n in (n_kv, n_kv, 8))
+    out, x = torch.empty_like(q), [randn((2, 12, d), s, BF16, 0.3) for s in range(6)]
+    ws = torch.empty(ops.gqa_kv8_workspace_bytes(2, 2, 1, 700, 8, n_kv, d), dtype=torch.uint8, device="cuda")
+    assert ws.numel()
+
+    def step():
+        ops.kv8_append(k, v, caches[0], table, lens)
+        ops.gqa_kv8(q, caches[0], table, lens, max_kv=700, out=out, workspace=ws)
+
+    k.zero_(), v.zero_(), q.zero_()
+    step()  # sequence 0 has no token yet, sequence 1 its first
+    ops.kv8_append(k, v, caches[1], table, lens)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        step()
+    for i, n in enumerate(([1, 2], [2, 300], [17, 301], [700, 959], [701, 960], [5, 16])):
+        lens.copy_(i32(n))
+        if i == 3:
+            table.copy_(table.flip(0))
+        k.copy_(x[i][:, :2]), v.copy_(x[i][:, 2:4]), q.copy_(x[i][:, 4:])
+        out.fill_(float("nan"))
+        g.replay()
+        ops.kv8_append(k, v, caches[1], table, lens)
+        want = ops.gqa_kv8(q, caches[1], table, lens, max_kv=700)
+        torch.cuda.synchronize()
+        assert torch.equal(out, want)
+        for a, b in ((caches[0].k, caches[1].k), (caches[0].v, caches[1].v)):
+            assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
+        assert torch.equal(caches[0].k_scale, caches[1].k_scale)
+
+
 # ---- pages ----------------------------------------------------------------
 @pytest.mark.parametrize("d,page,n_kv", [(64, 16, 1), (128, 64, 8), (64, 128, 3)])
 def test_copy_pages(ops, d, page, n_kv):
