@@ -236,22 +236,22 @@ __global__ __launch_bounds__(64 * NW, (NW / 4 * Tile<BM, BN, NW, NS>::PER_CU)) v
 // which the L1 takes one at a time (64x4096x7168: 21 us, and 11.5 this way).
 // ---------------------------------------------------------------------------
 constexpr int RW = 4;  // waves
-template <int FM, int FB, int PER_CU>
+template <int FM, int FB>
 struct Rows {
   static constexpr int SLOT = 16 * (FM + FB) * KS;
   static constexpr int LPW = 2 * (FM + FB);  // 1 KB loads of a step
-  static constexpr int FIT = 160 * 1024 / PER_CU / RW / SLOT;
+  static constexpr int FIT = 80 * 1024 / RW / SLOT;  // two workgroups on a CU
   static constexpr int NS = FIT > 8 ? 8 : FIT;
   static constexpr int LDS = RW * NS * SLOT;
   static_assert(NS >= 2 && (NS - 1) * LPW < 64, "vmcnt");
   static_assert(FM * FB * 64 * 16 <= NS * SLOT, "the sums meet in the rings");
 };
 
-template <int FM, int FB, int PER_CU, typename T>
+template <int FM, int FB, typename T>
 __global__ __launch_bounds__(64 * RW) void gemm_int8_rows_kernel(
     const uint8_t* __restrict__ A, const float* __restrict__ sA, const uint8_t* __restrict__ B,
     const float* __restrict__ sB, uint16_t* __restrict__ C, int M, int N, int K) {
-  using R = Rows<FM, FB, PER_CU>;
+  using R = Rows<FM, FB>;
   extern __shared__ __align__(1024) unsigned char smem[];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -514,22 +514,24 @@ __global__ __launch_bounds__(64 * RW, 2) void linear_int8_few_kernel(
 
 // ---------------------------------------------------------------------------
 // Launch choice.  What bounds every variant short of the largest products is the rate
-// at which a CU takes operand lines in, near 46 GB/s for one workgroup of a CU and 61 for two
-// side by side (measured from 1x1024x1024 to 8192^3; about 37 for the 256x256 tile,
-// whose ring holds two slots), so a variant costs
-//     start + (workgroups per CU) * (rows of A and B of a workgroup) * K / rate
-// and no less than HBM takes for the operands.  Against the best variant of each of 52
-// measured products the choice loses 1.4% on average.
+// at which a CU takes operand lines in (44 to 82 GB/s with one workgroup on the CU, 58 to 71
+// with more; the 256x256 tile, whose ring holds two slots, 40), and where K is short a
+// workgroup's begin and end.  So a variant costs
+//     start + next * (n - 1) + n * (rows of A and B of a workgroup) * K / rate
+// for n workgroups on a CU.  The constants are fits to the times of all variants over 158 products
+// (1x64x16 to 8192^3); over these and 84 others the choice loses 1.5% on average against the best
+// variant of each, and 27% at most (3034x964x4480: 33 us, 26 with 64x128 tiles).  Without `next` it
+// lost 8%, and 5267x830x16 took 27.9 us in place of 7.6.  Rows kernels of 64x32 and 32x64 gained
+// 0.2% where they were best, and are not kept.
 // ---------------------------------------------------------------------------
 struct Variant {
   int bm, bn;
-  float start, one, many;  // us; bytes per us with one workgroup on a CU, with more
+  float start, next, one, many;  // us; bytes per us with one workgroup on a CU, with more
 };
 constexpr Variant kVariants[] = {
-    {16, 16, 2.3f, 46e3f, 61e3f},  {16, 32, 2.3f, 46e3f, 61e3f},  {32, 16, 2.3f, 46e3f, 61e3f},
-    {32, 32, 2.3f, 48e3f, 61e3f},  {64, 32, 2.3f, 50e3f, 50e3f},  {32, 64, 2.3f, 50e3f, 50e3f},
-    {64, 64, 3.3f, 46e3f, 61e3f},  {128, 64, 3.3f, 46e3f, 64e3f}, {64, 128, 3.3f, 46e3f, 62e3f},
-    {128, 128, 3.3f, 44e3f, 60e3f}, {256, 256, 3.3f, 37e3f, 37e3f},
+    {16, 16, 2.6f, 0.5f, 68e3f, 65e3f},    {16, 32, 2.7f, 0.6f, 64e3f, 71e3f},   {32, 16, 2.7f, 0.6f, 82e3f, 68e3f},
+    {32, 32, 2.9f, 0.8f, 71e3f, 68e3f},    {64, 64, 3.8f, 1.4f, 51e3f, 71e3f},   {128, 64, 4.6f, 1.8f, 55e3f, 70e3f},
+    {64, 128, 4.8f, 1.9f, 51e3f, 71e3f},   {128, 128, 5.1f, 2.8f, 44e3f, 61e3f}, {256, 256, 11.8f, 10.4f, 47e3f, 40e3f},
 };
 constexpr int kNumVariants = sizeof(kVariants) / sizeof(kVariants[0]);
 
@@ -540,7 +542,7 @@ static int pick(int M, int N, int K) {
     const Variant& v = kVariants[i];
     const double wgs = (double)((M + v.bm - 1) / v.bm) * ((N + v.bn - 1) / v.bn);
     const double n = wgs <= 256 ? 1 : wgs <= 8192 ? (double)(((long long)wgs + 255) / 256) : wgs / 256;
-    const double us = v.start + n * (v.bm + v.bn) * K / (n > 1 ? v.many : v.one);
+    const double us = v.start + v.next * (n - 1) + n * (v.bm + v.bn) * K / (n > 1 ? v.many : v.one);
     if (us < least) least = us, best = i;
   }
   return best;
@@ -561,23 +563,21 @@ static int run(int variant, const uint8_t* A, const float* sA, const uint8_t* B,
   const Variant& v = kVariants[variant];
   const long long tm = (M + v.bm - 1) / v.bm, tn = (N + v.bn - 1) / v.bn;
   if (tm * tn >= (1 << 23)) return MX_ERR_SHAPE;  // fewer than 2^32 threads
-#define ROWS(FM, FB, PER)                                                                                         \
-  launch(gemm_int8_rows_kernel<FM, FB, PER, T>, lds_limit_once<gemm_int8_rows_kernel<FM, FB, PER, T>>(Rows<FM, FB, PER>::LDS), \
-         Rows<FM, FB, PER>::LDS, 64 * RW, dim3((unsigned)(tm * tn)), A, sA, B, sB, C, M, N, K, s)
+#define ROWS(FM, FB)                                                                                               \
+  launch(gemm_int8_rows_kernel<FM, FB, T>, lds_limit_once<gemm_int8_rows_kernel<FM, FB, T>>(Rows<FM, FB>::LDS),    \
+         Rows<FM, FB>::LDS, 64 * RW, dim3((unsigned)(tm * tn)), A, sA, B, sB, C, M, N, K, s)
 #define TILE(BM, BN, NW, NS)                                                                                      \
   launch(gemm_int8_kernel<BM, BN, NW, NS, T>, lds_limit_once<gemm_int8_kernel<BM, BN, NW, NS, T>>(Tile<BM, BN, NW, NS>::LDS), \
          Tile<BM, BN, NW, NS>::LDS, 64 * NW, dim3((unsigned)(tm * tn)), A, sA, B, sB, C, M, N, K, s)
   switch (variant) {
-    case 0: return ROWS(1, 1, 2);
-    case 1: return ROWS(1, 2, 2);
-    case 2: return ROWS(2, 1, 2);
-    case 3: return ROWS(2, 2, 2);
-    case 4: return ROWS(4, 2, 1);
-    case 5: return ROWS(2, 4, 1);
-    case 6: return TILE(64, 64, 4, 4);
-    case 7: return TILE(128, 64, 4, 3);
-    case 8: return TILE(64, 128, 4, 3);
-    case 9: return TILE(128, 128, 8, 2);
+    case 0: return ROWS(1, 1);
+    case 1: return ROWS(1, 2);
+    case 2: return ROWS(2, 1);
+    case 3: return ROWS(2, 2);
+    case 4: return TILE(64, 64, 4, 4);
+    case 5: return TILE(128, 64, 4, 3);
+    case 6: return TILE(64, 128, 4, 3);
+    case 7: return TILE(128, 128, 8, 2);
     default: return TILE(256, 256, 8, 2);
   }
 #undef ROWS

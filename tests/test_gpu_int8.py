@@ -92,10 +92,10 @@ def test_product(ops, dtype, m, n, k):
 # Each launch variant once (mx_gemm_int8 chooses by the sizes), with ragged rows, columns and inner dimensions; the
 # tiles with columns that store wide, in pairs and one by one.
 VARIANTS = [
-    (0, 129, 100, 16), (1, 129, 776, 400), (2, 1025, 98, 144), (3, 255, 2050, 144), (4, 511, 1023, 144), (5, 324, 1381, 16),
-    (6, 1024, 1023, 2064), (6, 1024, 1016, 2064), (6, 2001, 258, 4112), (7, 1925, 811, 400), (7, 1925, 816, 400),
-    (7, 1925, 810, 400), (8, 300, 6001, 400), (8, 300, 6008, 400), (9, 513, 6001, 144), (9, 513, 6008, 144), (9, 513, 6002, 144),
-    (10, 4017, 4015, 144), (10, 4017, 4016, 144), (10, 4017, 4018, 144)]
+    (0, 129, 100, 16), (1, 34, 5242, 144), (2, 1025, 98, 144), (2, 129, 776, 400), (3, 292, 418, 144), (3, 324, 1381, 16),
+    (4, 255, 2050, 144), (4, 1024, 1023, 2064), (4, 1024, 1016, 2064), (4, 2001, 258, 4112), (5, 1925, 811, 400),
+    (5, 1925, 816, 400), (5, 1925, 810, 400), (6, 300, 6001, 400), (6, 300, 6008, 400), (7, 513, 6001, 144),
+    (7, 513, 6008, 144), (7, 513, 6002, 144), (8, 4017, 4015, 144), (8, 4017, 4016, 144), (8, 4017, 4018, 144)]
 
 
 @pytest.mark.parametrize("variant,m,n,k", VARIANTS)
