@@ -275,7 +275,9 @@ __global__ __launch_bounds__(64 * NW, rows_per_cu(NR, D)) void rows_kernel(const
       load_k(tile, now);
       load_v(tile, now);
     }
-    for (; tile < tiles; tile += NW) {
+    // (as a lambda the compiler schedules it better than in the loop: 33 sequences of up to
+    // 2000 tokens, d = 64: 25.0 -> 23.5 us)
+    auto step = [&](int tile) {
       const int key0 = t0 + 64 * tile + 16 * g;  // the lane's keys: key0 .. key0 + 15
       const bool bad = !valid(now.v);
       const bool masked = t0 + 64 * tile + 64 > low || __any(bad);
@@ -370,7 +372,8 @@ __global__ __launch_bounds__(64 * NW, rows_per_cu(NR, D)) void rows_kernel(const
       if (tile + NW < tiles) load_v(tile + NW, next);
       now = next;
       next = after;
-    }
+    };
+    for (; tile < tiles; tile += NW) step(tile);
 
     for (; flagged; flagged &= flagged - 1) {
       const int key = t0 + 64 * (first_partial + __builtin_ctz(flagged)) + 16 * g;
