@@ -61,23 +61,43 @@ class KVPages:
         Returns the page copies, (from, to), to carry out before they are
         written: of a last page that is partly filled and shared, which the sequence
         then holds alone.  MemoryError where the pool has too few pages."""
-        if tokens < 0:
-            raise ValueError(f"tokens ({tokens}) must not be negative")
-        entry = self._of(seq)
-        pages, old = entry
-        if tokens == 0:
-            return []
-        split = old % self.page != 0 and self._users[pages[-1]] > 1
-        need = -(-(old + tokens) // self.page) - len(pages)
-        if need + split > len(self._free):
-            raise MemoryError(f"{need + split} pages are needed and {len(self._free)} are free")
+        return self.extend_all([(seq, tokens)])
+
+    def extend_all(self, wants) -> list[tuple[int, int]]:
+        """extend() for each (sequence, tokens) of a step, or for none: where the pool has too few
+        pages for all of them, MemoryError, and no sequence has moved to a page whose copy is lost
+        with the call.  The copies returned are one list for ops.kv8_copy_pages."""
+        more: dict[int, int] = {}
+        for seq, tokens in wants:
+            if tokens < 0:
+                raise ValueError(f"tokens ({tokens}) must not be negative")
+            self._of(seq)
+            more[seq] = more.get(seq, 0) + tokens
+        plan, users, need = [], {}, 0
+        for seq, tokens in more.items():
+            pages, old = self._seqs[seq]
+            if tokens == 0:
+                continue
+            split = False
+            if old % self.page:
+                last = pages[-1]
+                left = users.get(last, self._users[last])  # who holds it once those before have their own
+                split = left > 1
+                users[last] = left - split
+            fresh = -(-(old + tokens) // self.page) - len(pages)
+            plan.append((self._seqs[seq], split, fresh, old + tokens))
+            need += fresh + split
+        if need > len(self._free):
+            raise MemoryError(f"{need} pages are needed and {len(self._free)} are free")
         copies = []
-        if split:
-            copies.append((pages[-1], self._take()))
-            self._users[pages[-1]] -= 1
-            pages[-1] = copies[0][1]
-        pages.extend(self._take() for _ in range(need))
-        entry[1] = old + tokens
+        for entry, split, fresh, tokens in plan:
+            pages = entry[0]
+            if split:
+                copies.append((pages[-1], self._take()))
+                self._users[pages[-1]] -= 1
+                pages[-1] = copies[-1][1]
+            pages.extend(self._take() for _ in range(fresh))
+            entry[1] = tokens
         return copies
 
     def truncate(self, seq: int, tokens: int) -> None:

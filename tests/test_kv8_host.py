@@ -246,3 +246,80 @@ def test_pages_refuse():
     assert table.tolist() == [[0, 1, -1], [-1, -1, -1]] and lens.tolist() == [17, 0]
     src, dst = kv_pages.copy_lists([], device="cpu")
     assert src.shape == dst.shape == (0,) and src.dtype == torch.int32
+
+
+def test_pages_of_a_whole_step_or_of_none():
+    """extend_all(): where a later sequence of a step finds no page, the ones before it keep theirs, so that no copy is
+    lost; a shared last page is split once for each of its users but one; a sequence may be named twice."""
+    pool = kv_pages.KVPages(3, 16)
+    a = pool.new()
+    pool.extend(a, 20)
+    c = pool.fork(a)
+    before = [(pool.pages_of(s), pool.length(s)) for s in (a, c)]
+    with pytest.raises(MemoryError):
+        pool.extend_all([(a, 1), (c, 14)])
+    with pytest.raises(KeyError):
+        pool.extend_all([(a, 1), (9, 1)])
+    with pytest.raises(ValueError):
+        pool.extend_all([(a, 1), (c, -1)])
+    assert before == [(pool.pages_of(s), pool.length(s)) for s in (a, c)] and pool.free_pages == 1
+    assert pool.extend_all(iter([(a, 1), (c, 12)])) == [(1, 2)]
+    assert (pool.pages_of(a), pool.pages_of(c)) == ((0, 2), (0, 1))
+    assert pool.extend_all([]) == pool.extend_all([(a, 0)]) == []
+
+    pool = kv_pages.KVPages(9, 16)
+    a = pool.new()
+    pool.extend(a, 5)
+    forks = [a] + [pool.fork(a) for _ in range(3)]
+    assert pool.extend_all([(s, 1) for s in forks]) == [(0, 1), (0, 2), (0, 3)]
+    assert [pool.pages_of(s) for s in forks] == [(1,), (2,), (3,), (0,)]
+    d = pool.fork(a)
+    assert pool.extend_all([(d, 10), (d, 3)]) == [(1, 4)]
+    assert pool.pages_of(d) == (4, 5) and pool.length(d) == 19 and pool.pages_of(a) == (1,)
+
+
+def test_pages_of_steps_against_a_model():
+    """Random steps of several sequences, forks and ends, in pools that are often full: a step that fails changes
+    nothing, one that succeeds gives copies whose targets are new, and what was written stays readable."""
+    failed = 0
+    for seed in range(40):
+        rng = random.Random(seed)
+        page = rng.choice([1, 4, 16])
+        pool = kv_pages.KVPages(rng.randint(2, 14), page)
+        memory = [[None] * page for _ in range(pool.pages)]
+        truth, stamp = {}, 0
+        for _ in range(150):
+            what = rng.choice(["new", "step", "step", "step", "fork", "free"])
+            if what == "new" or not truth:
+                truth[pool.new()] = []
+            elif what == "fork":
+                s = rng.choice(list(truth))
+                truth[pool.fork(s)] = list(truth[s])
+            elif what == "free":
+                s = rng.choice(list(truth))
+                pool.free(s)
+                del truth[s]
+            else:
+                step = [(rng.choice(list(truth)), rng.randint(0, page + 1)) for _ in range(rng.randint(1, 5))]
+                before = ({s: (pool.pages_of(s), pool.length(s)) for s in truth}, pool.free_pages)
+                used = {p for s in truth for p in pool.pages_of(s)}
+                try:
+                    copies = pool.extend_all(step)
+                except MemoryError:
+                    failed += 1
+                    assert before == ({s: (pool.pages_of(s), pool.length(s)) for s in truth}, pool.free_pages)
+                    continue
+                targets = [b for _, b in copies]
+                assert len(set(targets)) == len(targets) and not set(targets) & used
+                for a, b in copies:
+                    memory[b] = list(memory[a])
+                for s, n in step:
+                    for _ in range(n):
+                        stamp += 1
+                        t = len(truth[s])
+                        memory[pool.pages_of(s)[t // page]][t % page] = stamp
+                        truth[s].append(stamp)
+            for s, tokens in truth.items():
+                assert pool.length(s) == len(tokens)
+                assert [memory[pool.pages_of(s)[t // page]][t % page] for t in range(len(tokens))] == tokens
+    assert failed > 100
