@@ -7,6 +7,8 @@ sequences, whose prefix it holds; it is written only while it belongs to one.
 """
 from __future__ import annotations
 
+from operator import index
+
 import torch
 
 
@@ -69,6 +71,7 @@ class KVPages:
         with the call.  The copies returned are one list for ops.kv8_copy_pages."""
         more: dict[int, int] = {}
         for seq, tokens in wants:
+            tokens = index(tokens)
             if tokens < 0:
                 raise ValueError(f"tokens ({tokens}) must not be negative")
             self._of(seq)

@@ -323,3 +323,17 @@ def test_pages_of_steps_against_a_model():
                 assert pool.length(s) == len(tokens)
                 assert [memory[pool.pages_of(s)[t // page]][t % page] for t in range(len(tokens))] == tokens
     assert failed > 100
+
+
+def test_pages_take_whole_numbers_of_tokens():
+    """A count that is no whole number is refused before anything has changed; numpy's and torch's integers count."""
+    pool = kv_pages.KVPages(6, 16)
+    a = pool.new()
+    pool.extend(a, 20)
+    c = pool.fork(a)
+    for tokens in (17.0, float("nan"), "3", None, torch.tensor(2.0)):
+        with pytest.raises(TypeError):
+            pool.extend(c, tokens)
+    assert pool.pages_of(c) == pool.pages_of(a) == (0, 1) and pool.length(c) == 20 and pool.free_pages == 4
+    assert pool.extend(c, torch.tensor([3, 17], dtype=torch.int32)[1]) == [(1, 2)]
+    assert pool.length(c) == 37 and type(pool.length(c)) is int
