@@ -279,7 +279,9 @@ __global__ __launch_bounds__(64 * NW, rows_per_cu(NR, D)) void rows_kernel(const
     // 2000 tokens, d = 64: 25.0 -> 23.5 us)
     auto step = [&](int tile) {
       const int key0 = t0 + 64 * tile + 16 * g;  // the lane's keys: key0 .. key0 + 15
-      const bool bad = !valid(now.v);
+      // also bad: a page behind the sequence's last, whose scales may be anything (WIDE: a tile's
+      // one page always holds a token)
+      const bool bad = !valid(now.v) || (!WIDE && key0 >= t1);
       const bool masked = t0 + 64 * tile + 64 > low || __any(bad);
       // ---- scores ----
       f32x4 s[NR][4];
@@ -333,7 +335,7 @@ __global__ __launch_bounds__(64 * NW, rows_per_cu(NR, D)) void rows_kernel(const
           pf[i][t >> 1][2 * (t & 1)] = T::pack2(p[0], p[1]);
           pf[i][t >> 1][2 * (t & 1) + 1] = T::pack2(p[2], p[3]);
         }
-        l[i] += bad ? 0.f : sum * iv;  // a page that is none has no scale
+        l[i] += bad ? 0.f : sum * iv;  // 0 * inf: such a page has no scale
       }
 
       // ---- codes of V that a row does not see must not reach it: 0 * NaN.  Those past the

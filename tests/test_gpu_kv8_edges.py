@@ -1,0 +1,40 @@
+"""The paged 8-bit cache on the GPU at its edges: pages without tokens, queries that are no numbers, every 16-bit value,
+split launches of each kernel form, scales far apart."""
+from __future__ import annotations
+
+import pytest
+import torch
+
+from conftest import announce
+from oracle import kv8 as oracle
+from test_gpu_kv8 import BF16, F16, check_attend, filled, i32, prefix, randn, tables
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("news", [[1, 1], [6, 2], [70, 30]])
+@pytest.mark.parametrize("d,page", [(64, 16), (128, 16), (64, 32), (128, 32), (64, 64), (128, 64), (128, 128)])
+def test_pages_of_no_token_do_not_count(ops, d, page, news, dtype):
+    """Pages that the table names behind a sequence's last token, not written yet: whatever their codes and scales
+    are, zeros, infinities or NaN, the outputs are bit for bit those with ordinary ones."""
+    announce(f"gqa_kv8 pages behind the last token d{d} page{page} {news} {dtype}")
+    lens = [max(20, news[0]), 1090]
+    pages = sum(-(-n // page) for n in lens) + 9
+    cache = filled(ops, pages, 2, d, page, 1)
+    table = tables(lens, page, pages - 8, 2, columns=-(-lens[1] // page) + 4)
+    for row in table:
+        first = row.index(-1)
+        row[first:] = [pages - 8 + i % 8 for i in range(len(row) - first)]
+    q = randn((sum(news), 8, d), 3, dtype, 0.1).cuda()
+    more = () if news == [1, 1] else (i32(prefix(news)), max(news))
+    args = (q, cache, i32(table), i32(lens), *more)
+    want = [ops.gqa_kv8(*args, causal=causal) for causal in (True, False)]
+    assert all(bool(w.isfinite().all()) for w in want)
+    cache.k.view(torch.uint8)[-8:] = 0x7F
+    cache.v.view(torch.uint8)[-8:] = 0x7F
+    for bad in (0.0, float("inf"), float("nan")):
+        cache.k_scale[-8:] = bad
+        cache.v_scale[-8:] = bad
+        for causal, w in zip((True, False), want):
+            assert torch.equal(ops.gqa_kv8(*args, causal=causal), w)
