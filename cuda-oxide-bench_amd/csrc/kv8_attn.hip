@@ -452,6 +452,7 @@ __global__ __launch_bounds__(64 * NW, rows_per_cu(NR, D)) void rows_kernel(const
 constexpr int TW = 8;           // waves
 constexpr int TR = 32 * TW;     // rows of a workgroup
 constexpr int BN = 64;          // keys of a tile
+constexpr int kOdd = 1 << 30;   // in a row's token number: its query holds an infinity or a NaN
 constexpr float kLazy = 8.0f;   // log2 units that a score may pass the running maximum by before it moves
 
 template <int D>
@@ -678,6 +679,25 @@ __global__ __launch_bounds__(64 * TW, 2) void tile_kernel(const Args a) {
       for (int i = tid; i < L::V / 16; i += NT) st128(smem + L::V_OFF + 2 * L::V + 16 * i, u32x4{});
       find(0);
       load(0);
+      // A query with an infinity or a NaN: all its scores are infinite or NaN, and its output is NaN if it
+      // sees a token, 0 if not.  A page that is none does not hold such scores back (0 * inf), so zeros
+      // take the query's place, and kOdd in tok tells the store.  0 times the query, summed, is NaN in
+      // each of the row's four lanes.  (Here the tile's codes are waited for anyway: up to 0.4% of a
+      // large prompt's time, behind find(1) up to 1.8%.)
+      f32x4 x[2] = {};
+#pragma unroll
+      for (int k = 0; k < KC; ++k)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) x[i] = mfma16<T>(u32x4{}, qf[i][k], x[i]);
+      if (__any(x[0][0] + x[1][0] != 0.f)) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const bool odd = x[i][0] != 0.f;
+          tok[i] |= odd ? kOdd : 0;
+#pragma unroll
+          for (int k = 0; k < KC; ++k) qf[i][k] = odd ? u32x4{} : qf[i][k];
+        }
+      }
       find(1);
     }
     if (a.causal) __syncthreads();
@@ -877,11 +897,12 @@ __global__ __launch_bounds__(64 * TW, 2) void tile_kernel(const Args a) {
     // ---- store: the lane's query, d = 16 dt + 4 g + j ----
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      const float total = sum_xor32(sum_xor16(l[i]));
+      float total = sum_xor32(sum_xor16(l[i]));
       const bool met = any_group(seen[i]);
       if (32 * wave + 16 * i + r16 >= rows) continue;
-      const size_t orow = (size_t)(rw.first + tok[i]) * a.n_q + head[i];
+      const size_t orow = (size_t)(rw.first + (tok[i] & ~kOdd)) * a.n_q + head[i];
       const bool none = total == 0.f && !met;
+      if ((tok[i] & kOdd) && !none) total = __builtin_nanf("");
       if (a.splits == 1) {
         const float inv = none ? 0.f : 1.0f / total;
 #pragma unroll

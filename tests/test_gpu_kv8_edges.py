@@ -38,3 +38,28 @@ def test_pages_of_no_token_do_not_count(ops, d, page, news, dtype):
         cache.v_scale[-8:] = bad
         for causal, w in zip((True, False), want):
             assert torch.equal(ops.gqa_kv8(*args, causal=causal), w)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("d,page", [(64, 16), (128, 32), (128, 64), (128, 128)])
+@pytest.mark.parametrize("news", [[1, 1, 1], [5, 3, 4], [90, 40, 70]])
+def test_queries_that_are_no_numbers_and_see_nothing(ops, news, d, page, dtype):
+    """Queries with a NaN or an infinity: zeros where every page of what they could see is none, NaN where one is
+    there (all scores of such a query are infinite or NaN)."""
+    announce(f"gqa_kv8 queries of NaN d{d} page{page} {news} {dtype}")
+    lens = [500, 300, 420]
+    pages = 80
+    cache = filled(ops, pages, 2, d, page, 4)
+    table = tables(lens, page, pages, 5)
+    table[0] = [-1, pages] * (len(table[0]) // 2) + [-7] * (len(table[0]) % 2)   # none at all
+    table[1][0] = -1                                                             # some
+    table[2] = [-1 if page * (j + 1) <= lens[2] - news[2] // 2 else p for j, p in enumerate(table[2])]
+    q = randn((sum(news), 4, d), 6, dtype, 0.1)
+    for b, first in enumerate(prefix(news)[:-1]):
+        q[first, 0, 3] = float("nan")
+        q[first + news[b] - 1, 1, d - 1] = float("inf")
+        q[first + news[b] // 2, 2, d // 2] = float("-inf")
+        q[first + news[b] // 3, 3, ::7] = float("nan")
+    for causal in (True, False):
+        exp, _, _ = check_attend(ops, cache, q, table, lens, news, causal)
+        assert bool((exp[:news[0]] == 0).all()) and bool(exp[news[0]:].isnan().any())
