@@ -724,11 +724,15 @@ def kv8_append(k, v, cache, page_table, kv_lens, cu_q=None, max_q=None):
             B, T, max_q, n_kv, d, page, pages, most, ks, vs, _IO_DTYPES[k.dtype])
 
 
+_COPIES = 1 << 22  # pieces of 4096 bytes of K that mx_kv8_copy_pages takes at once
+
+
 def kv8_copy_pages(cache, src, dst):
     """Page dst[i] of the cache becomes page src[i], all heads, codes and scales
     (src, dst [n] int32): a forked sequence's last page, the moves of a compaction
     (KVPages gives both).  A page is at most once a destination, and no
-    destination is a source; pairs with numbers that are no pages are skipped."""
+    destination is a source; pairs with numbers that are no pages are skipped.  Lists of
+    any length: more pages than a launch takes (16 GiB of K) go in several."""
     _check_cache(cache)
     _require(src, "src", _I32, 1)
     _require(dst, "dst", _I32, 1)
@@ -739,9 +743,11 @@ def kv8_copy_pages(cache, src, dst):
         raise ValueError("all tensors must be on the cache's device")
     if n >= _INT:
         raise ValueError(f"src has too many pages ({n})")
-    if n:
-        pages, n_kv, page, d = cache._sizes
-        _launch("mx_kv8_copy_pages", src, *cache._args, src.data_ptr(), dst.data_ptr(), n, n_kv, d, page, pages)
+    pages, n_kv, page, d = cache._sizes
+    most = max(1, _COPIES // -(-n_kv * page * d // 4096))  # pairs of a launch
+    for i in range(0, n, most):
+        _launch("mx_kv8_copy_pages", src, *cache._args, src.data_ptr() + 4 * i, dst.data_ptr() + 4 * i, min(most, n - i),
+                n_kv, d, page, pages)
 
 
 def gqa_kv8_workspace_bytes(B: int, T: int, max_q: int, max_kv: int, n_q: int, n_kv: int, d: int) -> int:

@@ -385,8 +385,9 @@ int mx_kv8_append(const void* k, const void* v, void* k_cache, void* v_cache, fl
  * page src[i], i < n (int32 on the device; a pair with a number outside
  * 0..pages-1 is skipped).  For forked sequences (the shared prefix's last,
  * partly filled page) and compactions.  The copies run side by side: a page
- * is at most once a destination, and no destination is a source.  At most 2^34
- * bytes of K (and as many of V) in a call.
+ * is at most once a destination, and no destination is a source.  At most 2^22 pieces of
+ * 4096 bytes of K (and as many of V) in a call, a page being a whole number of pieces: n <= 2^22
+ * for pages of up to 4 KB, 2^34 bytes of K for larger ones.
  */
 int mx_kv8_copy_pages(void* k_cache, void* v_cache, float* k_scale, float* v_scale, const int* src, const int* dst,
                       int n, int n_kv, int d, int page, int pages, void* stream);

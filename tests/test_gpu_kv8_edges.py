@@ -63,3 +63,19 @@ def test_queries_that_are_no_numbers_and_see_nothing(ops, news, d, page, dtype):
     for causal in (True, False):
         exp, _, _ = check_attend(ops, cache, q, table, lens, news, causal)
         assert bool((exp[:news[0]] == 0).all()) and bool(exp[news[0]:].isnan().any())
+
+
+def test_copies_of_more_pages_than_one_launch_takes(ops):
+    """2^22 + 3 pairs of 1 KB pages: all but some near both ends name no page and are skipped."""
+    announce("kv8_copy_pages of 2^22 + 3 pairs")
+    cache = filled(ops, 40, 1, 64, 16, 1)
+    was = [t.clone() for t in (cache.k.view(torch.uint8), cache.v.view(torch.uint8), cache.k_scale, cache.v_scale)]
+    n = 2 ** 22 + 3
+    src, dst = (torch.full((n,), -1, dtype=torch.int32, device="cuda") for _ in range(2))
+    for i, (a, b) in {0: (3, 20), 7: (4, 21), 2 ** 22 - 1: (5, 22), 2 ** 22: (6, 23), n - 1: (3, 24)}.items():
+        src[i], dst[i] = a, b
+        for t in was:
+            t[b] = t[a]
+    ops.kv8_copy_pages(cache, src, dst)
+    for t, e in zip((cache.k.view(torch.uint8), cache.v.view(torch.uint8), cache.k_scale, cache.v_scale), was):
+        assert torch.equal(t, e)
