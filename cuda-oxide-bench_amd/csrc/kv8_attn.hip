@@ -65,7 +65,7 @@ __device__ __forceinline__ constexpr uint32_t one_bits() {
 
 // log2 of the largest P'.  f16 has no more than 24 binades below one, and a page whose vs is that
 // far below the largest may hold all of a channel: P' then fills the range up to 2^15.
-// tile_kernel, whose maximum may lag by kLazy, leaves room for that.
+// tile_kernel, whose maximum may lag by lazy(), leaves room for that.
 template <typename T>
 __device__ __forceinline__ constexpr float lift() {
   return std::is_same<T, BF16>::value ? 0.f : 15.f;
@@ -453,7 +453,12 @@ constexpr int TW = 8;           // waves
 constexpr int TR = 32 * TW;     // rows of a workgroup
 constexpr int BN = 64;          // keys of a tile
 constexpr int kOdd = 1 << 30;   // in a row's token number: its query holds an infinity or a NaN
-constexpr float kLazy = 8.0f;   // log2 units that a score may pass the running maximum by before it moves
+// Log2 units that a score may pass the running maximum by before it moves.  f16: what P' has of its
+// range above 2^10, so that weights 2^24 below the row's largest are still normal numbers.
+template <typename T>
+__device__ __forceinline__ constexpr float lazy() {
+  return std::is_same<T, BF16>::value ? 8.f : 5.f;
+}
 
 template <int D>
 struct Stage {
@@ -481,7 +486,8 @@ __global__ __launch_bounds__(64 * TW, 2) void tile_kernel(const Args a) {
   constexpr int KC = D / 32, DT = D / 16;
   constexpr int NT = 64 * TW;
   constexpr int U = D * 8 / NT;  // 16-byte units of a tile (K, then V) per thread
-  constexpr float LEVEL = lift<T>() > kLazy ? lift<T>() - kLazy : 0.f;  // where a moved maximum puts log2 P'
+  constexpr float TOP = lift<T>() > 0.f ? lift<T>() : lazy<T>();  // a larger log2 P' moves the maximum,
+  constexpr float LEVEL = TOP - lazy<T>();                        // to here
   static_assert(U >= 1 && U * NT == D * 8, "units");
   extern __shared__ __align__(1024) unsigned char smem[];
   const int tid = threadIdx.x, lane = tid & 63;
@@ -803,7 +809,7 @@ __global__ __launch_bounds__(64 * TW, 2) void tile_kernel(const Args a) {
       __builtin_amdgcn_sched_barrier(0);
       __builtin_amdgcn_s_setprio(0);
 
-      const bool moved = __any(fmaxf(mx[0], mx[1]) > LEVEL + kLazy);
+      const bool moved = __any(fmaxf(mx[0], mx[1]) > TOP);
       if (moved || open) {
 #pragma unroll
         for (int k = 0; k < KC; ++k)
@@ -820,7 +826,7 @@ __global__ __launch_bounds__(64 * TW, 2) void tile_kernel(const Args a) {
           mx[i] = exponents(i);
           mx[i] = max_xor32(max_xor16(mx[i]));
           const bool empty = open && sum_xor32(sum_xor16(l[i])) == 0.f, met = mx[i] > -INFINITY;
-          const float shift = empty ? (met ? mx[i] - LEVEL : 0.f) : mx[i] > LEVEL + kLazy ? mx[i] - LEVEL : 0.f;
+          const float shift = empty ? (met ? mx[i] - LEVEL : 0.f) : mx[i] > TOP ? mx[i] - LEVEL : 0.f;
           still |= empty && !met;
           seen[i] |= cst[1] > -INFINITY && at + 16 * g < limit[i];
           m[i] += shift;

@@ -65,6 +65,34 @@ def test_queries_that_are_no_numbers_and_see_nothing(ops, news, d, page, dtype):
         assert bool((exp[:news[0]] == 0).all()) and bool(exp[news[0]:].isnan().any())
 
 
+@pytest.mark.parametrize("news,apart", [([1], 27), ([16], 27), ([20], 23), ([100], 23)])
+def test_attend_one_token_on_a_quiet_page(ops, news, apart):
+    """f16: a channel that a single token holds, whose page's scale lies 2^27 below the others' (2^23 where a KV head has
+    more than 32 rows, here two a token).  The row's largest P' is put at 2^15 (2^10 or above) and scores are
+    below 1/8, so the token's P' is 2^(15 - 27 - 1/2) or 2^(10 - 23 - 1/2), more than 2^-14: a normal f16, and so is the
+    output.  The channel then has the relative error of any other: the roundings of P' and of the output, 2^-11 each, and
+    what the fp32 steps add (2^-15 is ample)."""
+    announce(f"gqa_kv8 one quiet token {news}")
+    n, page, d = 100, 16, 64
+    cache = filled(ops, 7, 1, d, page, 3)
+    table = [[4, 0, 2, 1, 3, 6, 5]]
+    loud = 2.0 ** (apart - 9)
+    cache.k_scale.fill_(2.0 ** -9)
+    cache.v_scale.fill_(loud)
+    cache.v_scale[2] = 2.0 ** -9                       # tokens 32 .. 47
+    v = cache.v.view(torch.uint8)
+    v.copy_((torch.arange(v.numel()) % 4).reshape(v.shape).to(torch.uint8))    # 0 .. 3 * 2^-9
+    v[:, :, 0] = 0
+    v[2, :, 0, 5] = 0x7E                               # 448: 0.875 with its scale, about 0.00875 in the output
+    q = randn((news[0], 2, d), 5, F16, 0.002)
+    exp, _, score = oracle.Cache(cache.k, cache.v, cache.k_scale, cache.v_scale).attend(q, table, [n], prefix(news), False)
+    assert float(score.max()) < 1 / 8 and bool((exp[..., 0] > 2.0 ** -8).all()) and bool((exp[..., 0] < 2.0 ** -6).all())
+    more = {} if news == [1] else {"cu_q": i32(prefix(news)), "max_q": news[0]}
+    got = ops.gqa_kv8(q.cuda(), cache, i32(table), i32([n]), causal=False, **more).cpu().double()[..., 0]
+    exp = exp[..., 0]
+    assert bool(((got - exp).abs() <= exp * (2 * 2.0 ** -11 + 2.0 ** -15)).all())
+
+
 def test_copies_of_more_pages_than_one_launch_takes(ops):
     """2^22 + 3 pairs of 1 KB pages: all but some near both ends name no page and are skipped."""
     announce("kv8_copy_pages of 2^22 + 3 pairs")
