@@ -7,9 +7,10 @@
 //     P'[t] = 2^(y[t] - m),   m = the running maximum of y (f16: less a constant)
 //     O     = (sum_t P'[t] v8[t]) / (sum_t P'[t] / vs)
 // so a page's two scales cost one FMA constant per score and one product per page in
-// the denominator, P' carries vs and stays within either 16-bit type's range, and any positive
-// scales serve.  (m - max y of a page is at most the spread of log2 vs, so the
-// denominator's terms stay in fp32's range while the vs of a sequence lie within 2^100.)
+// the denominator, and P' carries vs and stays within either 16-bit type's range.  (m - max y of a
+// page is at most the spread of log2 vs, so no term of the denominator that counts is lost in fp32
+// while the vs of a sequence lie within 2^100; a term is at most 2^8 / vs (f16: 2^15, where a vs
+// below 2^-40 gives outputs of 0 anyway), so that the sum of 2^30 stays finite from vs = 2^-90 on.)
 //
 // S^T = K . Q^T and O^T = V^T . P'^T: a lane of the score tile holds one query and its
 // keys, which is the layout that the second product takes P' in.

@@ -400,8 +400,9 @@ int mx_kv8_copy_pages(void* k_cache, void* v_cache, float* k_scale, float* v_sca
  * t <= kv_lens[b] - n_b + i.  q: [T, n_q, d] bf16 or f16, rows q_stride elements
  * apart; O: [T, n_q, d] contiguous, same type.  fp32 scores, softmax and sums;
  * P is rounded to the I/O type for the product with V.  A row that sees no
- * token gives zeros.  The scales of K and V may be any positive finite
- * numbers, those of V within 2^100 of each other.  (f16: P' of a token keeps its precision
+ * token gives zeros.  The scales of K may be any positive finite numbers, those of V
+ * 2^-90 to 2^120 (the denominator sums P' / scale in fp32) and within 2^100 of each other.
+ * Pages that none of the sequence's tokens lies on may hold anything.  (f16: P' of a token keeps its precision
  * while exp(score) times its page's V scale is at least 2^-24 of the row's largest.)
  * max_q and max_kv: the largest number of rows and of tokens of a sequence, or
  * estimates: they choose the kernel and its split of the keys, not what is

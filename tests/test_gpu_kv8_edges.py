@@ -93,6 +93,26 @@ def test_attend_one_token_on_a_quiet_page(ops, news, apart):
     assert bool(((got - exp).abs() <= exp * (2 * 2.0 ** -11 + 2.0 ** -15)).all())
 
 
+@pytest.mark.parametrize("news", [[1], [20], [100]])
+@pytest.mark.parametrize("e", [-90, 119])
+def test_attend_scales_of_any_size(ops, e, news):
+    """V's scales around 2^-90 or 2^119 (bf16, whose outputs reach as far)."""
+    announce(f"gqa_kv8 V scales around 2^{e} {news}")
+    n, page = 700, 32
+    cache = filled(ops, 24, 1, 64, page, 7)
+    cache.v_scale.copy_(torch.exp2(torch.rand((24, 1), generator=torch.Generator().manual_seed(3)) + e).cuda())
+    q = randn((news[0], 2, 64), 5, BF16, 0.1)
+    table = tables([n], page, 24, 2)
+    exp, weight, score = oracle.Cache(cache.k, cache.v, cache.k_scale, cache.v_scale).attend(q, table, [n], prefix(news))
+    more = {} if news == [1] else {"cu_q": i32(prefix(news)), "max_q": news[0]}
+    got = ops.gqa_kv8(q.cuda(), cache, i32(table), i32([n]), **more).cpu().double()
+    half = 2.0 ** -8
+    delta = 2.0 ** -24 * ((64 + 16) * score + 64) + 2.0 ** -21
+    rel = half * 1.01 + 2 * delta[..., None] + 2 * (n + 8) * 2.0 ** -24
+    # sums of P' v8 vanish below 2^-126 times the scale of the largest, as the P' do: 2^-126 of 448 a token
+    assert bool(((got - exp).abs() <= weight * rel + exp.abs() * half + 2.0 ** -126 * n * 448 * 2.0 ** (e + 1)).all())
+
+
 def test_copies_of_more_pages_than_one_launch_takes(ops):
     """2^22 + 3 pairs of 1 KB pages: all but some near both ends name no page and are skipped."""
     announce("kv8_copy_pages of 2^22 + 3 pairs")
