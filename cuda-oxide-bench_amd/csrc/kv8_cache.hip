@@ -36,7 +36,7 @@ __device__ __forceinline__ uint32_t codes2(float a, float b) {
 }
 
 // Four codes of packed values x, y of the 16-bit type, divided by s = a power of two: one
-// instruction for two (all finite values of both types at scales from 2^-32 to 2^120 give
+// instruction for two (all finite values of both types at scales from 2^-32 to 2^127 give
 // the codes of the exact quotient).
 template <typename T>
 __device__ __forceinline__ uint32_t codes4(uint32_t x, uint32_t y, float s);

@@ -65,6 +65,76 @@ def test_queries_that_are_no_numbers_and_see_nothing(ops, news, d, page, dtype):
         assert bool((exp[:news[0]] == 0).all()) and bool(exp[news[0]:].isnan().any())
 
 
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_append_every_value(ops, dtype):
+    """Every finite 16-bit value that fits, as keys and as values of a page with a present scale from 2^-32 to 2^127
+    (one token before keeps it): the nearest code of the exact quotient, ties to even."""
+    announce(f"kv8_append every value {dtype}")
+    d = page = 128
+    exps = [-32, -31, -20, -9, -1, 0, 1, 7, 30, 60, 119, 120, 121, 126, 127]
+    bits = torch.arange(-2 ** 15, 2 ** 15, dtype=torch.int32).to(torch.int16).view(dtype)
+    bits = bits[bits.isfinite()]
+    n_kv = -(-bits.numel() // ((page - 1) * d))
+    x = torch.zeros(n_kv * (page - 1) * d, dtype=dtype)
+    x[:bits.numel()] = bits
+    x = x.reshape(page - 1, n_kv, d)
+    cache = ops.KV8Cache.empty(len(exps), n_kv, d, page)
+    scale = torch.tensor([2.0 ** e for e in exps])
+    cache.k_scale.copy_(scale[:, None].expand(-1, n_kv))
+    cache.v_scale.copy_(scale[:, None].expand(-1, n_kv))
+    parts = [torch.where(x.double().abs() <= 448 * 2.0 ** e, x, torch.zeros_like(x)) for e in exps]
+    k = torch.cat(parts).cuda()
+    table, lens = i32([[b] for b in range(len(exps))]), i32([page] * len(exps))
+    ops.kv8_append(k, -k, cache, table, lens, i32([b * (page - 1) for b in range(len(exps) + 1)]), page - 1)
+    for got in (cache.k_scale, cache.v_scale):
+        assert torch.equal(got.cpu(), scale[:, None].expand(-1, n_kv))
+    for b, (e, part) in enumerate(zip(exps, parts)):
+        want = oracle.nearest_e4m3(part.double() * 2.0 ** -e).transpose(0, 1)
+        got = cache.k[b].cpu().float().double()[:, 1:], -cache.v[b].cpu().float().double().transpose(1, 2)[:, 1:]
+        for g in got:
+            assert torch.equal(g, want), f"scale 2^{e}: {int((g != want).sum())} codes"
+
+
+# d, page, n_kv, group, lens, news: see test_split_launches_cover_each_kernel in test_kv8_host.py
+SPLIT = [
+    (128, 16, 1, 4, [600, 530], [1, 1]),
+    (64, 32, 3, 1, [1200, 40], [1, 1]),
+    (128, 64, 1, 7, [700, 515], [2, 1]),
+    (64, 128, 2, 5, [1100, 1030], [3, 2]),
+    (128, 32, 2, 8, [700, 520], [3, 4]),
+    (128, 16, 1, 5, [550, 1030], [4, 5]),
+    (64, 16, 2, 12, [1100, 1050], [2, 2]),
+    (128, 64, 1, 7, [1030, 600], [4, 3]),
+    (64, 128, 1, 10, [1300, 90], [3, 1]),
+    (128, 16, 1, 3, [300, 700], [40, 90]),
+    (64, 32, 2, 2, [290, 500], [130, 61]),
+    (128, 128, 2, 2, [300, 500], [150, 61]),
+    (64, 64, 1, 4, [300, 640], [150, 300]),
+]
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("case", range(len(SPLIT)))
+def test_attend_split(ops, case, causal, dtype):
+    """Every kernel form with its keys split: NaN codes of V among the last tokens and, without a causal mask, one
+    that every row sees; codes behind the last token and pages behind the last one are NaN."""
+    d, page, n_kv, group, lens, news = SPLIT[case]
+    announce(f"gqa_kv8 split d{d} page{page} n_kv{n_kv} group{group} {lens} {news} causal={causal} {dtype}")
+    pages = sum(-(-n // page) for n in lens) + 2
+    cache = filled(ops, pages, n_kv, d, page, case)
+    table = tables(lens, page, pages, case)
+    v = cache.v.view(torch.uint8)
+    for row, n in zip(table, lens):
+        if n % page:
+            cache.k.view(torch.uint8)[row[n // page], :, n % page:] = 0x7F
+            v[row[n // page], :, :, n % page:] = 0xFF
+        for t, c in ((n - 1, 5), (n - 2, d - 1), (n - 9, 17)) if causal else ((n // 2, 5),):
+            v[row[t // page], n_kv - 1, c, t % page] = 0x7F
+    q = randn((sum(news), n_kv * group, d), 100 + case, dtype, 0.02)
+    check_attend(ops, cache, q, table, lens, news, causal)
+
+
 @pytest.mark.parametrize("news,apart", [([1], 27), ([16], 27), ([20], 23), ([100], 23)])
 def test_attend_one_token_on_a_quiet_page(ops, news, apart):
     """f16: a channel that a single token holds, whose page's scale lies 2^27 below the others' (2^23 where a KV head has

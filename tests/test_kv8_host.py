@@ -337,3 +337,22 @@ def test_pages_take_whole_numbers_of_tokens():
     assert pool.pages_of(c) == pool.pages_of(a) == (0, 1) and pool.length(c) == 20 and pool.free_pages == 4
     assert pool.extend(c, torch.tensor([3, 17], dtype=torch.int32)[1]) == [(1, 2)]
     assert pool.length(c) == 37 and type(pool.length(c)) is int
+
+
+def test_split_launches_cover_each_kernel(tmp_path):
+    """The cases of test_attend_split: each kernel (16 rows, 32 rows, tiles) with pages of less than 64 tokens and of
+    more, at d = 64 and 128, has its keys split in one at least."""
+    from test_gpu_kv8_edges import SPLIT
+    sizes = ", ".join("{%d, %d, %d, %d, %d, %d}" % (len(lens), sum(news), max(news), -(-max(lens) // page) * page, n_kv * group, n_kv)
+                      for d, page, n_kv, group, lens, news in SPLIT)
+    ds = ", ".join(str(case[0]) for case in SPLIT)
+    out = query(tmp_path, "kv8_attn.hip", r"""
+  using namespace mx::kv8;
+  const int s[][6] = {SIZES}, ds[] = {DS};
+  int i = 0;
+  for (auto& c : s) {
+    const Plan p = plan(c[0], c[1], c[2], c[3], c[4], c[5], ds[i++]);
+    printf("%d %d\n", p.nr, p.splits > 1);
+  }""".replace("SIZES", sizes).replace("DS", ds))
+    got = {(line.split()[0], case[1] >= 64, case[0]) for line, case in zip(out, SPLIT) if line.endswith(" 1")}
+    assert got == {(nr, wide, d) for nr in "120" for wide in (False, True) for d in (64, 128)}, out
