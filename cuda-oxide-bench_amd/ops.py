@@ -765,8 +765,9 @@ def gqa_kv8(q, cache, page_table, kv_lens, cu_q=None, max_q=None, max_kv=None, c
     left as they are.  max_q and max_kv (the most rows and tokens of a sequence; T and
     the table's width without them) choose the launch, not what is computed: give
     max_kv where the table is wider than the sequences are long.  scale defaults to
-    1/sqrt(d).  Pass `workspace` (uint8, contiguous, at least gqa_kv8_workspace_bytes)
-    to allocate nothing but the result; calls that may overlap each need their own."""
+    1/sqrt(d).  Pass `workspace` (uint8, contiguous, at least gqa_kv8_workspace_bytes for
+    the same hints: fewer tokens can need more) to allocate nothing but the result; calls
+    that may overlap each need their own."""
     _check_cache(cache)
     qs = _rows(q, "q", _IO_DTYPES, 2)
     T = q.shape[0]
@@ -775,7 +776,10 @@ def gqa_kv8(q, cache, page_table, kv_lens, cu_q=None, max_q=None, max_kv=None, c
     n_q = q.shape[1]
     if T < 1 or q.shape[2] != d or n_q < 1 or n_q % n_kv:
         raise ValueError(f"q must be [T, a multiple of {n_kv}, {d}], got {tuple(q.shape)}")
-    max_kv = most * page if max_kv is None else min(int(max_kv), most * page)
+    if max_kv is None:
+        max_kv = most * page
+    else:  # a workspace was sized for the caller's own hint: another one may need more
+        max_kv = min(int(max_kv), most * page if workspace is None else 1 << 30)
     if max_kv < 1:
         raise ValueError(f"max_kv ({max_kv}) must be positive")
     if scale is None:

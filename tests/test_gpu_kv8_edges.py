@@ -197,3 +197,18 @@ def test_copies_of_more_pages_than_one_launch_takes(ops):
     ops.kv8_copy_pages(cache, src, dst)
     for t, e in zip((cache.k.view(torch.uint8), cache.v.view(torch.uint8), cache.k_scale, cache.v_scale), was):
         assert torch.equal(t, e)
+
+
+@pytest.mark.parametrize("wide", [2048, 2100, 100000])
+def test_a_workspace_of_the_calls_own_hints(ops, wide):
+    """A workspace of gqa_kv8_workspace_bytes' size for the hints of the call, max_kv among them, is enough, also where
+    max_kv is more than the table holds."""
+    announce(f"gqa_kv8 workspace of its own hints, max_kv {wide}")
+    cache = filled(ops, 130, 8, 128, 64, 1)
+    lens = [2048, 1900, 700, 64]
+    table = tables(lens, 64, 130, 2, columns=32)
+    q = randn((4, 32, 128), 3, BF16, 0.02)
+    need = ops.gqa_kv8_workspace_bytes(4, 4, 1, wide, 32, 8, 128)
+    assert need
+    ws = torch.empty(need, dtype=torch.uint8, device="cuda")
+    check_attend(ops, cache, q, table, lens, [1] * 4, max_kv=wide, workspace=ws)
