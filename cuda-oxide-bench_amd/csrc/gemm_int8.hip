@@ -26,10 +26,26 @@ __device__ __forceinline__ i32x4 mfma_i8(const u32x4& a, const u32x4& b, const i
   return __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(i32x4, a), __builtin_bit_cast(i32x4, b), c, 0, 0, 0);
 }
 
+// c sa sb, rounded.  c sa may leave fp32's normal range where the result does not: FAR takes an sa that far
+// from one in two parts.
+__device__ __forceinline__ bool far_from_one(float sa) { return fabsf(sa) >= 0x1p96f || fabsf(sa) < 0x1p-96f; }
+template <typename T, bool FAR>
+__device__ __forceinline__ u32x2 scaled4(const i32x4& c, float sa, const f32x4& sb) {
+  f32x4 y;
+  if constexpr (FAR) {
+    const bool large = fabsf(sa) >= 0x1p96f, small = fabsf(sa) < 0x1p-96f;
+    const float part = large ? 0x1p64f : small ? 0x1p-64f : 1.f, rest = sa * (large ? 0x1p-64f : small ? 0x1p64f : 1.f);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) y[i] = (float)c[i] * rest * sb[i] * part;
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) y[i] = (float)c[i] * sa * sb[i];
+  }
+  return u32x2{T::pack2(y[0], y[1]), T::pack2(y[2], y[3])};
+}
 template <typename T>
 __device__ __forceinline__ u32x2 scaled4(const i32x4& c, float sa, const f32x4& sb) {
-  return u32x2{T::pack2((float)c[0] * sa * sb[0], (float)c[1] * sa * sb[1]),
-               T::pack2((float)c[2] * sa * sb[2], (float)c[3] * sa * sb[3])};
+  return __any(far_from_one(sa)) ? scaled4<T, true>(c, sa, sb) : scaled4<T, false>(c, sa, sb);
 }
 __device__ __forceinline__ void store4(uint16_t* p, const u32x2& v, int left) {
 #pragma unroll
@@ -187,16 +203,30 @@ __global__ __launch_bounds__(64 * NW, (NW / 4 * Tile<BM, BN, NW, NS>::PER_CU)) v
   const bool wide = (N & 7) == 0;
   if (!wide) __syncthreads();  // the rings are free
   unsigned char* stage = smem + wave * 2048;
+  float sa[FM];
+  bool far = false;
+#pragma unroll
+  for (int i = 0; i < FM; ++i) {
+    sa[i] = sA[min(m0 + wm * CF::TM + 16 * i + r16, M - 1)];
+    far |= far_from_one(sa[i]);
+  }
+  far = __any(far);
 #pragma unroll
   for (int i = 0; i < FM; ++i) {
     const int m = m0 + wm * CF::TM + 16 * i + r16;
-    const float sa = sA[min(m, M - 1)];
     u32x4 row[2];
+    auto scale = [&](auto far_tag) {
 #pragma unroll
-    for (int f = 0; f < 2; ++f) {
-      const u32x2 lo = scaled4<T>(acc[i][2 * f], sa, sb[2 * f]), hi = scaled4<T>(acc[i][2 * f + 1], sa, sb[2 * f + 1]);
-      row[f] = u32x4{lo[0], lo[1], hi[0], hi[1]};
-    }
+      for (int f = 0; f < 2; ++f) {
+        const u32x2 lo = scaled4<T, decltype(far_tag)::value>(acc[i][2 * f], sa[i], sb[2 * f]);
+        const u32x2 hi = scaled4<T, decltype(far_tag)::value>(acc[i][2 * f + 1], sa[i], sb[2 * f + 1]);
+        row[f] = u32x4{lo[0], lo[1], hi[0], hi[1]};
+      }
+    };
+    if (far)
+      scale(std::true_type{});
+    else
+      scale(std::false_type{});
     if (wide) {
       uint16_t* out = C + (size_t)m * N + n;
 #pragma unroll

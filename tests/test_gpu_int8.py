@@ -237,3 +237,35 @@ def test_streams_and_capture(ops):
         assert torch.equal(eager, want[0])
         for y, e in zip(outs, want):
             assert torch.equal(y, e)
+
+
+@pytest.mark.parametrize("m", [1, 3, 20, 300])
+def test_scales_far_from_one(ops, m):
+    """Products whose sum times the token's scale leaves fp32's normal range, though the result does not: rows near
+    bf16's largest value through every kernel, and scales from 2^-140 to 2^120 with the other one at the far end."""
+    announce(f"int8 scales far from one, {m} rows")
+    n, k = 40, 256
+    x = torch.zeros((m, k))
+    x[:, 3], x[:, 7] = 3e38, 1e38
+    x[m // 2] = -x[m // 2]
+    x = x.to(torch.bfloat16)
+    w = torch.zeros((n, k))
+    w[:, 3], w[:, 7] = torch.linspace(-0.7, 0.7, n), 0.3
+    w, sw = oracle.quantize_rows(w.to(torch.bfloat16))
+    q, sx = oracle.quantize_rows(x)
+    exact = oracle.product(q, sx, w, sw)
+    assert bool((exact.abs() < torch.finfo(torch.bfloat16).max).all())
+    y = ops.linear_int8(x.cuda(), w.cuda(), sw.cuda())
+    assert bool(((y.cpu().double() - exact).abs() <= bound(exact, torch.bfloat16)).all())
+    a, _ = codes(m, k, 5)
+    b, _ = codes(n, k, 6)
+    for e, f in ((120, -120), (100, -30), (-140, 120), (-100, 110), (96, 10), (-97, -20), (0, -120)):
+        g = torch.Generator().manual_seed(e + 200)
+        sa, sb = ((1 + torch.rand(r, generator=g)) * 2.0 ** x for r, x in ((m, e), (n, f)))
+        sa[::3] = 1.5 * 2.0 ** -f  # rows of ordinary size beside them
+        exact = oracle.product(a, sa, b, sb)
+        for dtype in DTYPES:
+            out = ops.gemm_int8(a.cuda(), sa.cuda(), b.cuda(), sb.cuda(), dtype=dtype)
+            over = exact.abs() > torch.finfo(dtype).max * (1 - 2.0 ** -10)
+            ok = ((out.cpu().double() - exact).abs() <= bound(exact, dtype)) | over
+            assert bool(ok.all()), f"scales 2^{e}, 2^{f}, {dtype}: {int((~ok).sum())} outputs"
