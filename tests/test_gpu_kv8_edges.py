@@ -7,7 +7,7 @@ import torch
 
 from conftest import announce
 from oracle import kv8 as oracle
-from test_gpu_kv8 import BF16, F16, check_attend, filled, i32, prefix, randn, tables
+from test_gpu_kv8 import BF16, F16, bound, check_attend, filled, i32, prefix, randn, tables
 
 pytestmark = pytest.mark.gpu
 
@@ -212,3 +212,39 @@ def test_a_workspace_of_the_calls_own_hints(ops, wide):
     assert need
     ws = torch.empty(need, dtype=torch.uint8, device="cuda")
     check_attend(ops, cache, q, table, lens, [1] * 4, max_kv=wide, workspace=ws)
+
+
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("d,page,news", [(128, 64, [3, 0, 2, 5, 1]), (64, 16, [4, 0, 3, 1, 6]), (128, 16, [7, 0, 5, 8, 2]),
+                                         (64, 64, [90, 0, 40, 70, 33]), (128, 32, [90, 0, 40, 70, 33])])
+def test_rows_of_none_with_split_keys(ops, d, page, news, dtype, causal):
+    """Keys split over workgroups: rows before the first and behind the last sequence stay as they are, sequences of no
+    rows and of no tokens, more rows than tokens, lengths past the table, pages that are none."""
+    announce(f"gqa_kv8 rows of none, split keys, d{d} page{page} {news} {dtype} causal={causal}")
+    lens = [1200, 900, 0, 1100, 17 if news[4] > 17 else 1]
+    pages = sum(-(-n // page) for n in lens) + 2
+    cache = filled(ops, pages, 2, d, page, 3)
+    table = tables(lens, page, pages, 4)
+    for j in range(5, 12):
+        table[0][j] = -1 if j % 2 else pages
+    cu = [4 + c for c in prefix(news)]
+    q = randn((cu[-1] + 5, 6, d), 5, dtype, 0.05)
+    oc = oracle.Cache(cache.k, cache.v, cache.k_scale, cache.v_scale)
+    exp, weight, score = oc.attend(q, table, lens, cu, causal)
+    out = torch.full(q.shape, 7.0, dtype=dtype, device="cuda")
+    asked = ops.gqa_kv8_workspace_bytes(5, q.shape[0], max(news), len(table[0]) * page, 6, 2, d)
+    assert asked, "the keys are split"
+    ops.gqa_kv8(q.cuda(), cache, i32(table), i32([2 ** 31 - 1 if n == 1200 and 1200 % page == 0 else n for n in lens]), i32(cu),
+                max_q=max(news), causal=causal, out=out)
+    got = out.cpu().double()
+    assert bool((got[:cu[0]] == 7).all()) and bool((got[cu[-1]:] == 7).all())
+    rows = slice(cu[0], cu[-1])
+    limit = bound(exp, weight, score, lens, d, dtype, cache.v_scale)
+    assert bool(((got - exp).abs() <= limit)[rows].all())
+    assert bool((got[cu[2]:cu[3]] == 0).all())
+    # ranges that begin below 0 and end past the rows: cut
+    wild = [-5, *cu[1:-1], q.shape[0] + 9]
+    cut = [0, *cu[1:-1], q.shape[0]]
+    a, b = (ops.gqa_kv8(q.cuda(), cache, i32(table), i32(lens), i32(c), max_q=max(news) + 14, causal=causal) for c in (wild, cut))
+    assert torch.equal(a, b)
