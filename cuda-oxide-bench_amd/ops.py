@@ -622,7 +622,7 @@ class KV8Cache:
     tensors; the constructor takes those that the caller has.  The checks run
     here, once, and the tensors cannot be exchanged afterwards."""
 
-    __slots__ = ("_k", "_v", "_k_scale", "_v_scale", "_args", "_sizes", "_device")
+    __slots__ = ("_k", "_v", "_k_scale", "_v_scale", "_args", "_sizes", "_device", "_copies")
 
     def __init__(self, k, v, k_scale, v_scale):
         f8, f32 = (torch.float8_e4m3fn,), (torch.float32,)
@@ -643,6 +643,8 @@ class KV8Cache:
         self._args = (k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr())
         self._sizes = (pages, n_kv, page, d)
         self._device = k.get_device()
+        # pages that mx_kv8_copy_pages takes at once: 2^22 pieces of 4096 bytes
+        self._copies = max(1, (1 << 22) // -(-n_kv * page * d // 4096))
 
     @classmethod
     def empty(cls, pages, n_kv, d, page=64, device="cuda"):
@@ -724,9 +726,6 @@ def kv8_append(k, v, cache, page_table, kv_lens, cu_q=None, max_q=None):
             B, T, max_q, n_kv, d, page, pages, most, ks, vs, _IO_DTYPES[k.dtype])
 
 
-_COPIES = 1 << 22  # pieces of 4096 bytes of K that mx_kv8_copy_pages takes at once
-
-
 def kv8_copy_pages(cache, src, dst):
     """Page dst[i] of the cache becomes page src[i], all heads, codes and scales
     (src, dst [n] int32): a forked sequence's last page, the moves of a compaction
@@ -744,7 +743,7 @@ def kv8_copy_pages(cache, src, dst):
     if n >= _INT:
         raise ValueError(f"src has too many pages ({n})")
     pages, n_kv, page, d = cache._sizes
-    most = max(1, _COPIES // -(-n_kv * page * d // 4096))  # pairs of a launch
+    most = cache._copies
     for i in range(0, n, most):
         _launch("mx_kv8_copy_pages", src, *cache._args, src.data_ptr() + 4 * i, dst.data_ptr() + 4 * i, min(most, n - i),
                 n_kv, d, page, pages)
