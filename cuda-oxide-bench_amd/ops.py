@@ -593,8 +593,9 @@ def linear_int8_workspace_bytes(M: int, K: int) -> int:
 def linear_int8(x, w, sw, out=None, workspace=None):
     """An int8 linear layer: quant_int8(x), then gemm_int8 with the weight w [N,K]
     and its channel scales sw [N].  x [M,K] bf16/f16, rows may lie apart; the
-    result [M,N] has x's type.  Pass `workspace` (uint8, contiguous, at least
-    linear_int8_workspace_bytes) to allocate nothing but the result."""
+    result [M,N] has x's type.  Where one kernel does all (no workspace is asked for),
+    M times the row stride must stay below 2**30.  Pass `workspace` (uint8, contiguous,
+    at least linear_int8_workspace_bytes) to allocate nothing but the result."""
     ldx = _rows(x, "x", _IO_DTYPES, 1)
     M, K = x.shape
     N = _check_weight(w, sw, K)
