@@ -776,10 +776,8 @@ def gqa_kv8(q, cache, page_table, kv_lens, cu_q=None, max_q=None, max_kv=None, c
     n_q = q.shape[1]
     if T < 1 or q.shape[2] != d or n_q < 1 or n_q % n_kv:
         raise ValueError(f"q must be [T, a multiple of {n_kv}, {d}], got {tuple(q.shape)}")
-    if max_kv is None:
-        max_kv = most * page
-    else:  # a workspace was sized for the caller's own hint: another one may need more
-        max_kv = min(int(max_kv), most * page if workspace is None else 1 << 30)
+    hint = most * page if max_kv is None else int(max_kv)
+    max_kv = min(hint, most * page)
     if max_kv < 1:
         raise ValueError(f"max_kv ({max_kv}) must be positive")
     if scale is None:
@@ -792,7 +790,10 @@ def gqa_kv8(q, cache, page_table, kv_lens, cu_q=None, max_q=None, max_kv=None, c
             raise ValueError(f"out must be {tuple(q.shape)}")
     if q.get_device() != cache._device or out.get_device() != cache._device:
         raise ValueError("all tensors must be on the cache's device")
-    ws, ws_bytes = _workspace(workspace, gqa_kv8_workspace_bytes(B, T, max_q, max_kv, n_q, n_kv, d), q)
+    need = gqa_kv8_workspace_bytes(B, T, max_q, max_kv, n_q, n_kv, d)
+    ws, ws_bytes = _workspace(workspace, need, q)
+    if ws_bytes < need:  # sized for the hint as it is, which can need less than the table's width
+        max_kv = min(hint, 1 << 30)
     _launch("mx_gqa_kv8", q, q.data_ptr(), *cache._args, page_table.data_ptr(), kv_lens.data_ptr(), cu, out.data_ptr(),
             B, T, max_q, max_kv, n_q, n_kv, d, page, pages, most, qs, float(scale), int(bool(causal)),
             _IO_DTYPES[q.dtype], ws, ws_bytes)

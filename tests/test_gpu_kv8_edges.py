@@ -248,3 +248,21 @@ def test_rows_of_none_with_split_keys(ops, d, page, news, dtype, causal):
     cut = [0, *cu[1:-1], q.shape[0]]
     a, b = (ops.gqa_kv8(q.cuda(), cache, i32(table), i32(lens), i32(c), max_q=max(news) + 14, causal=causal) for c in (wild, cut))
     assert torch.equal(a, b)
+
+
+def test_a_workspace_of_the_tables_width(ops):
+    """max_kv past the table's width: a workspace for either serves, one that is too small for both is refused."""
+    announce("gqa_kv8 max_kv past the table, workspaces")
+    cache = filled(ops, 130, 8, 128, 64, 1)
+    lens = [2048, 1900, 700, 64]
+    table = tables(lens, 64, 130, 2, columns=32)
+    q = randn((4, 32, 128), 3, BF16, 0.02)
+    size = {n: ops.gqa_kv8_workspace_bytes(4, 4, 1, n, 32, 8, 128) for n in (2048, 2100, 4096)}
+    assert size[2100] < size[2048]
+    for hint, ws in ((2100, size[2100]), (2100, size[2048]), (4096, size[2048]), (4096, size[4096])):
+        ws = torch.empty(ws, dtype=torch.uint8, device="cuda")
+        check_attend(ops, cache, q, table, lens, [1] * 4, max_kv=hint, workspace=ws)
+    small = torch.empty(size[2100] - 16, dtype=torch.uint8, device="cuda")
+    for hint in (2048, 2100, None):
+        with pytest.raises(RuntimeError, match="workspace"):
+            ops.gqa_kv8(q.cuda(), cache, i32(table), i32(lens), max_kv=hint, workspace=small)
