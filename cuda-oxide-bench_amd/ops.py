@@ -798,3 +798,122 @@ def gqa_kv8(q, cache, page_table, kv_lens, cu_q=None, max_q=None, max_kv=None, c
             B, T, max_q, max_kv, n_q, n_kv, d, page, pages, most, qs, float(scale), int(bool(causal)),
             _IO_DTYPES[q.dtype], ws, ws_bytes)
     return out
+
+
+# ---------------------------------------------------------------------------
+# A served step before and behind the attention: norm and rotation of the heads, log probabilities
+# ---------------------------------------------------------------------------
+def rope_table(positions: int, rot: int, theta: float = 10000.0, device="cuda") -> torch.Tensor:
+    """The table of qk_norm_rope for positions 0 .. positions-1: [positions, rot] fp32, the cosines of
+    position * theta^(-2 i / rot), i < rot / 2, then the sines.  Angles in 64 bits.  Scaled or
+    otherwise changed frequencies: a table of the same form, made by the caller."""
+    if positions < 1 or rot < 16 or rot % 16:
+        raise ValueError(f"positions ({positions}) must be positive and rot ({rot}) a multiple of 16")
+    freq = theta ** (-torch.arange(0, rot, 2, dtype=torch.float64, device=device) / rot)
+    angle = torch.arange(positions, dtype=torch.float64, device=device)[:, None] * freq
+    return torch.cat([angle.cos(), angle.sin()], 1).float()
+
+
+def qk_norm_rope(q, k, q_weight, k_weight, table, positions, eps=1e-6, neighbours=False, q_out=None, k_out=None):
+    """RMS norm of each query and key head, and its rotation by the token's position, in one
+    pass -> (q_out, k_out), ready for kv8_append and the attention.
+
+    q [T, n_q, d], k [T, n_kv, d] bf16/f16, rows may lie apart (views of a fused projection);
+    q_weight, k_weight [d] of the same type; table [rows, rot] fp32 (rope_table): channels from rot
+    on are normed and not turned.  Channel i is turned with i + rot/2, with neighbours=True 2 i with
+    2 i + 1.  positions [T] int32; a token whose position is no row of the table (padding: -1) is left
+    as it is in the outputs.  q_out, k_out: rows may lie apart; q itself as q_out and k as k_out
+    work in place.  d and rot multiples of 16, d up to 256."""
+    qs, ks = _rows(q, "q", _IO_DTYPES, 2), _rows(k, "k", (q.dtype,), 2)
+    T, n_q, d = q.shape
+    n_kv = k.shape[1]
+    if T < 1 or n_q < 1 or n_kv < 1 or k.shape != (T, n_kv, d):
+        raise ValueError(f"q must be [T, n_q, d] and k [T, n_kv, d], got {tuple(q.shape)} and {tuple(k.shape)}")
+    if d < 16 or d > 256 or d % 16:
+        raise ValueError(f"d ({d}) must be a multiple of 16 up to 256")
+    for w, name in ((q_weight, "q_weight"), (k_weight, "k_weight")):
+        _require(w, name, (q.dtype,), 1)
+        if w.shape[0] != d:
+            raise ValueError(f"{name} must be {(d,)}, got {tuple(w.shape)}")
+    _require(table, "table", (torch.float32,), 2)
+    _require(positions, "positions", _I32, 1)
+    rows, rot = table.shape
+    if not 1 <= rows < _INT or rot < 16 or rot > d or rot % 16:
+        raise ValueError(f"table must be [positions, rot] with rot a multiple of 16 up to {d}, got {tuple(table.shape)}")
+    if positions.shape[0] != T:
+        raise ValueError(f"positions must be {(T,)}, got {tuple(positions.shape)}")
+    if q_out is None:
+        q_out, qos = torch.empty((T, n_q, d), dtype=q.dtype, device=q.device), n_q * d
+    else:
+        qos = _rows(q_out, "q_out", (q.dtype,), 2)
+    if k_out is None:
+        k_out, kos = torch.empty((T, n_kv, d), dtype=q.dtype, device=q.device), n_kv * d
+    else:
+        kos = _rows(k_out, "k_out", (q.dtype,), 2)
+    if q_out.shape != q.shape or k_out.shape != k.shape:
+        raise ValueError(f"q_out must be {tuple(q.shape)} and k_out {tuple(k.shape)}")
+    _same_device(q, k, q_weight, k_weight, table, positions, q_out, k_out)
+    _launch("mx_qk_norm_rope", q, q.data_ptr(), k.data_ptr(), q_weight.data_ptr(), k_weight.data_ptr(), table.data_ptr(),
+            positions.data_ptr(), q_out.data_ptr(), k_out.data_ptr(), T, n_q, n_kv, d, rot, rows, qs, ks, qos, kos,
+            float(eps), int(bool(neighbours)), _IO_DTYPES[q.dtype])
+    return q_out, k_out
+
+
+_LOGIT_DTYPES = {**_IO_DTYPES, torch.float32: _lib.MX_DTYPE_F32}
+
+
+def token_logprobs_workspace_bytes(T: int, V: int, top: int, dtype: torch.dtype) -> int:
+    return int(_lib.load().mx_token_logprobs_workspace(T, V, top, _LOGIT_DTYPES[dtype]))
+
+
+def token_logprobs(logits, tokens=None, top=0, out=None, workspace=None):
+    """(logprobs, entropy, top_ids, top_logprobs) of rows of logits, in one pass over them.
+
+    logits [T, V] bf16/f16/fp32, rows may lie apart (a padded vocabulary's slice).  tokens [T] or [T, m] int32
+    (one token a row, or several: a tree node's children): logprobs, fp32 of their shape, are
+    log softmax(row)[token], NaN where a number is no token (padding: -1); None without tokens.
+    entropy [T] fp32, natural logarithms.  top_ids int32 and top_logprobs fp32 [T, top], top up to 32 and V:
+    the most probable tokens, ties by the lowest id.  A row without a distribution (a
+    NaN, +infinity, nothing but -infinity) gives NaN and ids of -1.  Pass `out`, the four tensors (None for
+    logprobs without tokens), and `workspace` (uint8, contiguous, at least token_logprobs_workspace_bytes) to
+    allocate nothing; calls that may overlap each need their own."""
+    stride = _rows(logits, "logits", _LOGIT_DTYPES, 1)
+    T, V = logits.shape
+    if T < 1 or not 1 <= V <= 1 << 30:
+        raise ValueError(f"logits must have rows, of up to 2**30 tokens (got {tuple(logits.shape)})")
+    if not 0 <= top <= min(32, V):
+        raise ValueError(f"top ({top}) must be 0 to {min(32, V)}")
+    given = 0
+    if tokens is not None:
+        _require(tokens, "tokens", _I32)
+        if tokens.dim() not in (1, 2) or tokens.shape[0] != T:
+            raise ValueError(f"tokens must be {(T,)} or [{T}, m], got {tuple(tokens.shape)}")
+        given = tokens.numel() // T
+    if T * max(given, top) >= _INT:
+        raise ValueError(f"too many results: {T} rows of {max(given, top)}")
+    f32, dev = torch.float32, logits.device
+    if out is None:
+        logprobs = None if tokens is None else torch.empty(tokens.shape, dtype=f32, device=dev)
+        entropy = torch.empty((T,), dtype=f32, device=dev)
+        ids = torch.empty((T, top), dtype=torch.int32, device=dev)
+        best = torch.empty((T, top), dtype=f32, device=dev)
+    else:
+        logprobs, entropy, ids, best = out
+        if (logprobs is None) != (tokens is None):
+            raise ValueError("out must hold log probabilities where there are tokens, None where there are none")
+        if tokens is not None:
+            _require(logprobs, "logprobs", (f32,))
+        _require(entropy, "entropy", (f32,), 1)
+        _require(ids, "top_ids", _I32, 2)
+        _require(best, "top_logprobs", (f32,), 2)
+        if (tokens is not None and logprobs.shape != tokens.shape) or entropy.shape != (T,) or ids.shape != (T, top) or \
+                best.shape != (T, top):
+            raise ValueError(f"out must be log probabilities shaped as the tokens, {(T,)}, {(T, top)} and {(T, top)}")
+        _same_device(logits, entropy, ids, best)
+    if tokens is not None:
+        _same_device(logits, tokens, logprobs)
+    ws, ws_bytes = _workspace(workspace, token_logprobs_workspace_bytes(T, V, top, logits.dtype), logits)
+    _launch("mx_token_logprobs", logits, logits.data_ptr(), tokens.data_ptr() if given else None,
+            logprobs.data_ptr() if given else None, entropy.data_ptr(), ids.data_ptr() if top else None,
+            best.data_ptr() if top else None, T, V, stride, given, top, _LOGIT_DTYPES[logits.dtype], ws, ws_bytes)
+    return logprobs, entropy, ids, best

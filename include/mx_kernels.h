@@ -40,9 +40,10 @@ extern "C" {
 #define MX_ERR_LAUNCH (-7)      /* the HIP runtime rejected the kernel launch    */
 #define MX_ERR_UNSUPPORTED (-8) /* valid request this build has no kernel for    */
 
-/* ---- element-type codes for the 16-bit I/O tensors --------------------- */
+/* ---- element-type codes for the I/O tensors ---------------------------- */
 #define MX_DTYPE_BF16 0
 #define MX_DTYPE_F16 1
+#define MX_DTYPE_F32 2 /* logits only (mx_token_logprobs) */
 
 /* Human-readable name of a status code (static storage, never NULL). */
 const char* mx_strerror(int code);
@@ -419,6 +420,46 @@ int mx_gqa_kv8(const void* q, const void* k_cache, const void* v_cache, const fl
                int n_q, int n_kv, int d, int page, int pages, int max_pages, int q_stride, float scale, int causal,
                int dtype, void* workspace, size_t ws_bytes, void* stream);
 size_t mx_gqa_kv8_workspace(int B, int T, int max_q, int max_kv, int n_q, int n_kv, int d);
+
+/*
+ * RMS norm of every query and key head and the position rotation, in one pass: head x of
+ * token t (of T), with w = q_weight or k_weight [d] and p = positions[t],
+ *   y = x * rsqrt(mean(x^2) + eps) * w
+ *   (y_a, y_b) <- (y_a c - y_b s, y_b c + y_a s),  c = table[p, i], s = table[p, rot/2 + i]
+ * for each pair i < rot/2 of channels: (i, i + rot/2), or with neighbours != 0 (2i, 2i + 1);
+ * channels from rot on are not turned.  fp32 throughout, rounded once.  q, q_out: [T, n_q, d],
+ * k, k_out: [T, n_kv, d], bf16 or f16, rows at strides of their own (views of a fused
+ * projection); weights of the same type; table [rows, rot] fp32; positions [T] int32 on
+ * the device.  A token whose position is outside 0..rows-1 is left as it is (in q_out and k_out).
+ * q_out may be q and k_out k (same pointer and stride); any other overlap of an
+ * output with an input or the other output returns MX_ERR_ALIAS.  x^2 is summed in fp32: a head whose
+ * squares pass 2^128 becomes zeros (NaN where it holds an infinity or a NaN).
+ * d a multiple of 16 up to 256, rot a multiple of 16 up to d; strides % 8 == 0, 16-byte
+ * aligned pointers (positions: 4).
+ * No counterpart in the reference (its attention takes rotated queries and keys).
+ */
+int mx_qk_norm_rope(const void* q, const void* k, const void* q_weight, const void* k_weight, const float* table,
+                    const int* positions, void* q_out, void* k_out, int T, int n_q, int n_kv, int d, int rot, int rows,
+                    int q_stride, int k_stride, int qo_stride, int ko_stride, float eps, int neighbours, int dtype,
+                    void* stream);
+
+/*
+ * Log probabilities, entropy and top alternatives of rows of logits: for row x of T (V logits,
+ * rows `stride` elements apart; bf16, f16 or fp32), p = softmax(x):
+ *   logprob[t, i]  = log p[tokens[t, i]], i < given;  NaN where that is no token (0..V-1)
+ *   entropy[t]     = -sum p log p (natural logarithms; p = 0 adds nothing)
+ *   top_ids[t, j], top_logprob[t, j], j < top: the most probable tokens, ties by the lowest id
+ * Sums in fp32.  -inf is a logit like any other (p = 0).  A row without a distribution (a
+ * NaN, +infinity, nothing but -infinity) gives NaN and ids of -1.  given >= 0 (tokens and logprob may be NULL at 0), 0 <= top <= 32 and <= V (top_*
+ * may be NULL at 0), V <= 2^30, stride < 2^31.
+ * Logits at any alignment of their type; 16-byte aligned workspace (mx_token_logprobs_workspace bytes for
+ * the same sizes, may be 0; calls that may overlap each need their own).
+ * No counterpart in the reference, which ends at attention and products.
+ */
+int mx_token_logprobs(const void* logits, const int* tokens, float* logprob, float* entropy, int* top_ids,
+                      float* top_logprob, int T, int V, long long stride, int given, int top, int dtype, void* workspace,
+                      size_t ws_bytes, void* stream);
+size_t mx_token_logprobs_workspace(int T, int V, int top, int dtype);
 
 #ifdef __cplusplus
 }

@@ -1,0 +1,74 @@
+"""Host side of the operators before and behind the attention, without a GPU: refusals and launch rules."""
+from __future__ import annotations
+
+import ctypes
+
+import pytest
+
+from conftest import import_submodule
+from host_query import query
+
+_lib = import_submodule("_lib")
+
+BASE = 1 << 24
+P = [ctypes.c_void_p(BASE * (i + 1)) for i in range(10)]  # never dereferenced: every call below fails validation
+U, V = ctypes.c_void_p(BASE + 4), ctypes.c_void_p(BASE + 2)
+
+
+def _calls(name, good, bad):
+    for change, code in bad:
+        args = list(good)
+        for i, v in change.items():
+            args[i] = v
+        yield pytest.param(name, args, code, id=f"{name}-{change}")
+
+
+BAD = [
+    # q, k, wq, wk, table, positions, qo, ko, T, n_q, n_kv, d, rot, rows, strides q k qo ko, eps, neighbours, dtype, stream
+    *_calls("mx_qk_norm_rope", [*P[:8], 5, 4, 2, 64, 32, 100, 512, 512, 256, 128, 1e-6, 0, 0, None], [
+        *[({i: None}, _lib.MX_ERR_NULL) for i in range(8)], *[({i: 0}, _lib.MX_ERR_SHAPE) for i in range(8, 14)],
+        ({11: 40}, _lib.MX_ERR_SHAPE), ({11: 272, 12: 16}, _lib.MX_ERR_SHAPE), ({12: 80}, _lib.MX_ERR_SHAPE),
+        ({12: 24}, _lib.MX_ERR_SHAPE), ({14: 248}, _lib.MX_ERR_SHAPE), ({15: 120}, _lib.MX_ERR_SHAPE),
+        ({16: 248}, _lib.MX_ERR_SHAPE), ({17: 120}, _lib.MX_ERR_SHAPE), ({9: 2 ** 26}, _lib.MX_ERR_SHAPE),
+        *[({i: 516}, _lib.MX_ERR_ALIGN) for i in (14, 15, 16, 17)],
+        *[({i: U}, _lib.MX_ERR_ALIGN) for i in (0, 1, 2, 3, 4, 6, 7)], ({5: V}, _lib.MX_ERR_ALIGN),
+        ({20: 2}, _lib.MX_ERR_DTYPE), ({6: P[1]}, _lib.MX_ERR_ALIAS), ({7: P[0]}, _lib.MX_ERR_ALIAS),
+        ({6: P[0]}, _lib.MX_ERR_ALIAS),  # q's memory at another stride
+        ({7: P[6]}, _lib.MX_ERR_ALIAS)]),
+    # logits, tokens, logprob, entropy, ids, top_logprob, T, V, stride, given, top, dtype, workspace, bytes, stream
+    *_calls("mx_token_logprobs", [*P[:6], 3, 50000, 50000, 2, 5, 0, P[6], 1 << 24, None], [
+        *[({i: None}, _lib.MX_ERR_NULL) for i in range(6)], ({6: 0}, _lib.MX_ERR_SHAPE), ({7: 0}, _lib.MX_ERR_SHAPE),
+        ({7: 2 ** 30 + 1, 8: 2 ** 30 + 1}, _lib.MX_ERR_SHAPE), ({8: 49999}, _lib.MX_ERR_SHAPE), ({8: 2 ** 31}, _lib.MX_ERR_SHAPE),
+        ({9: -1}, _lib.MX_ERR_SHAPE), ({10: -1}, _lib.MX_ERR_SHAPE), ({10: 33}, _lib.MX_ERR_SHAPE),
+        ({7: 4, 8: 4}, _lib.MX_ERR_SHAPE), ({6: 2 ** 30}, _lib.MX_ERR_SHAPE), ({11: 3}, _lib.MX_ERR_DTYPE),
+        ({0: ctypes.c_void_p(BASE + 1)}, _lib.MX_ERR_ALIGN), ({0: V, 11: 2}, _lib.MX_ERR_ALIGN),
+        *[({i: V}, _lib.MX_ERR_ALIGN) for i in range(1, 6)], ({12: None}, _lib.MX_ERR_WORKSPACE),
+        ({13: 100}, _lib.MX_ERR_WORKSPACE), ({12: U}, _lib.MX_ERR_ALIGN)]),
+]
+
+
+@pytest.mark.parametrize("name,args,code", BAD)
+def test_entry_points_refuse(name, args, code):
+    assert getattr(_lib.load(), name)(*args) == code
+
+
+def test_logprob_slices(tmp_path):
+    """Every block of a row, at whichever alignment, lies in one slice; no slice is empty; a wave's lanes hold them all."""
+    out = query(tmp_path, "token_logprobs.hip", r"""
+  using namespace mx::logprobs;
+  for (int T : {1, 2, 17, 64, 511, 512, 100000, 1 << 30})
+    for (int V : {1, 3, 8, 4095, 4096, 32000, 100003, 200000, 1 << 30})
+      for (int dtype : {MX_DTYPE_BF16, MX_DTYPE_F32}) {
+        const Plan p = plan(T, V, dtype);
+        const long long blocks = V / (dtype == MX_DTYPE_F32 ? 4 : 8);
+        const bool whole = (long long)p.slices * p.per >= blocks, used = p.slices == 1 || (p.slices - 1LL) * p.per < blocks;
+        if (!whole || !used || p.slices < 1 || p.slices > kMostSlices || p.per < 1) printf("plan(%d, %d, %d)\n", T, V, dtype);
+      }
+  printf("%d\n", plan(1, 32000, MX_DTYPE_BF16).slices > 1);""")
+    assert out == ["1"]
+
+
+def test_workspaces():
+    f = _lib.load().mx_token_logprobs_workspace
+    assert f(1000, 50000, 5, 0) == 0 and f(1, 100, 5, 0) == 0 and f(2, 50000, 5, 0) > 0
+    assert [f(*a) for a in ((0, 50000, 5, 0), (1, 0, 0, 0), (1, 50000, 33, 0), (1, 50000, 5, 4))] == [0] * 4
