@@ -64,6 +64,10 @@ SIGNATURES: dict[str, tuple] = {
     "mx_kv8_copy_pages": (_i, [_vp] * 6 + [_i] * 5 + [_vp]),
     "mx_gqa_kv8": (_i, [_vp] * 9 + [_i] * 11 + [_f, _i, _i, _vp, _sz, _vp]),
     "mx_gqa_kv8_workspace": (_sz, [_i] * 7),
+    "mx_gqa_kv8_window": (_i, [_vp] * 9 + [_i] * 11 + [_f, _i, _i, _i, _vp, _sz, _vp]),
+    "mx_gqa_kv8_window_workspace": (_sz, [_i] * 9),
+    "mx_gqa_kv8_tree": (_i, [_vp] * 10 + [_i] * 11 + [_f, _i, _i, _vp, _sz, _vp]),
+    "mx_gqa_kv8_tree_workspace": (_sz, [_i] * 7),
     "mx_qk_norm_rope": (_i, [_vp] * 8 + [_i] * 10 + [_f, _i, _i, _vp]),
     "mx_token_logprobs": (_i, [_vp] * 6 + [_i, _i, _ll, _i, _i, _i, _vp, _sz, _vp]),
     "mx_token_logprobs_workspace": (_sz, [_i] * 4),

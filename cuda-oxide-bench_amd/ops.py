@@ -800,6 +800,97 @@ def gqa_kv8(q, cache, page_table, kv_lens, cu_q=None, max_q=None, max_kv=None, c
     return out
 
 
+def _check_attend(q, cache, page_table, kv_lens, cu_q, max_q, max_kv, scale, out):
+    """The checks that gqa_kv8_window and gqa_kv8_tree share: what their calls are made of."""
+    _check_cache(cache)
+    qs = _rows(q, "q", _IO_DTYPES, 2)
+    T, n_q = q.shape[:2]
+    B, most, cu, max_q = _check_sequences(cache, T, page_table, kv_lens, cu_q, max_q)
+    pages, n_kv, page, d = cache._sizes
+    if T < 1 or q.shape[2] != d or n_q < 1 or n_q % n_kv:
+        raise ValueError(f"q must be [T, a multiple of {n_kv}, {d}], got {tuple(q.shape)}")
+    hint = most * page if max_kv is None else int(max_kv)
+    if hint < 1:
+        raise ValueError(f"max_kv ({hint}) must be positive")
+    if out is None:
+        out = torch.empty((T, n_q, d), dtype=q.dtype, device=q.device)
+    else:
+        _require(out, "out", (q.dtype,), 3)
+        if out.shape != q.shape:
+            raise ValueError(f"out must be {tuple(q.shape)}")
+    if q.get_device() != cache._device or out.get_device() != cache._device:
+        raise ValueError("all tensors must be on the cache's device")
+    return out, B, T, n_q, cu, max_q, hint, most, qs, 1.0 / math.sqrt(d) if scale is None else float(scale)
+
+
+def _fit(need, workspace, q, hint, width):
+    """(workspace pointer, bytes, max_kv) of a call whose workspace size for a max_kv is need(max_kv): one that is too
+    small for the table's width may have been sized for the hint as it is, which can need less."""
+    most = min(hint, width)
+    want = need(most)
+    ws, ws_bytes = _workspace(workspace, want, q)
+    return ws, ws_bytes, most if ws_bytes >= want else min(hint, 1 << 30)
+
+
+def gqa_kv8_window_workspace_bytes(B: int, T: int, max_q: int, max_kv: int, n_q: int, n_kv: int, d: int, window: int,
+                                   sinks: int = 0) -> int:
+    return int(_lib.load().mx_gqa_kv8_window_workspace(B, T, max_q, max_kv, n_q, n_kv, d, window, sinks))
+
+
+def gqa_kv8_window(q, cache, page_table, kv_lens, window, sinks=0, cu_q=None, max_q=None, max_kv=None, scale=None,
+                   out=None, workspace=None):
+    """gqa_kv8 with a sliding window and sinks: a row at place p (its sequence's rows are its last
+    tokens) sees the tokens t <= p with p - t < window, and the sequence's first `sinks`.  -> [T, n_q, d].
+
+    window >= 1 counts the row's own token; a window or sinks past the sequence hide nothing.  Pages on which no row
+    sees a token are not read: their numbers in the table may be -1 or another sequence's.  The other
+    arguments, and rows that see nothing, as for gqa_kv8; `workspace` at least
+    gqa_kv8_window_workspace_bytes for the same hints."""
+    window, sinks = int(window), int(sinks)
+    if not 1 <= window < _INT or not 0 <= sinks < _INT:
+        raise ValueError(f"window ({window}) must be positive and sinks ({sinks}) not negative, both below 2**31")
+    out, B, T, n_q, cu, max_q, hint, most, qs, scale = _check_attend(q, cache, page_table, kv_lens, cu_q, max_q, max_kv,
+                                                                     scale, out)
+    pages, n_kv, page, d = cache._sizes
+    ws, ws_bytes, max_kv = _fit(
+        lambda m: gqa_kv8_window_workspace_bytes(B, T, max_q, m, n_q, n_kv, d, window, sinks), workspace, q, hint, most * page)
+    _launch("mx_gqa_kv8_window", q, q.data_ptr(), *cache._args, page_table.data_ptr(), kv_lens.data_ptr(), cu,
+            out.data_ptr(), B, T, max_q, max_kv, n_q, n_kv, d, page, pages, most, qs, scale, window, sinks,
+            _IO_DTYPES[q.dtype], ws, ws_bytes)
+    return out
+
+
+def gqa_kv8_tree_workspace_bytes(B: int, T: int, max_q: int, max_kv: int, n_q: int, n_kv: int, d: int) -> int:
+    return int(_lib.load().mx_gqa_kv8_tree_workspace(B, T, max_q, max_kv, n_q, n_kv, d))
+
+
+def gqa_kv8_tree(q, cache, page_table, kv_lens, tree, cu_q=None, max_q=None, max_kv=None, scale=None, out=None,
+                 workspace=None):
+    """gqa_kv8 for drafted tokens that form a tree -> [T, n_q, d].
+
+    A sequence's rows are its last tokens, appended to the cache already.  A row sees every token before
+    them, and of them the j-th where bit j of its mask is set: tree [T] or [T, words] int64, bit j % 64 of word j // 64,
+    up to 16 words (drafts.masks makes them of the tokens' parents).  Nothing is added to a mask, and drafted
+    tokens behind its bits are not seen.  A row that sees nothing gives zeros.  The other arguments as for
+    gqa_kv8; `workspace` at least gqa_kv8_tree_workspace_bytes for the same hints.  Of the drafted tokens those that are
+    kept are appended again, from the first one's place on (kv8_append): they then lie as decoded ones do."""
+    out, B, T, n_q, cu, max_q, hint, most, qs, scale = _check_attend(q, cache, page_table, kv_lens, cu_q, max_q, max_kv,
+                                                                     scale, out)
+    _require(tree, "tree", (torch.int64,))
+    words = 1 if tree.dim() == 1 else tree.shape[-1]
+    if tree.dim() not in (1, 2) or tree.shape[0] != T or not 1 <= words <= 16:
+        raise ValueError(f"tree must be {(T,)} or [{T}, 1 to 16], got {tuple(tree.shape)}")
+    if tree.get_device() != cache._device:
+        raise ValueError("all tensors must be on the cache's device")
+    pages, n_kv, page, d = cache._sizes
+    ws, ws_bytes, max_kv = _fit(lambda m: gqa_kv8_tree_workspace_bytes(B, T, max_q, m, n_q, n_kv, d), workspace, q, hint,
+                                most * page)
+    _launch("mx_gqa_kv8_tree", q, q.data_ptr(), *cache._args, page_table.data_ptr(), kv_lens.data_ptr(), cu,
+            tree.data_ptr(), out.data_ptr(), B, T, max_q, max_kv, n_q, n_kv, d, page, pages, most, qs, scale, words,
+            _IO_DTYPES[q.dtype], ws, ws_bytes)
+    return out
+
+
 # ---------------------------------------------------------------------------
 # A served step before and behind the attention: norm and rotation of the heads, log probabilities
 # ---------------------------------------------------------------------------

@@ -422,6 +422,37 @@ int mx_gqa_kv8(const void* q, const void* k_cache, const void* v_cache, const fl
 size_t mx_gqa_kv8_workspace(int B, int T, int max_q, int max_kv, int n_q, int n_kv, int d);
 
 /*
+ * mx_gqa_kv8 where a row sees the last `window` tokens up to its own place and the sequence's first
+ * `sinks`: row i of n_b, at place p = kv_lens[b] - n_b + i, sees the tokens t <= p with p - t < window or
+ * t < sinks.  window >= 1, sinks >= 0; one that passes the sequence hides nothing.  Pages on which no
+ * row of the call sees a token are not read, and what the table and the pages hold for them does not count: a
+ * caller may have given them back.  Rows, hints, sizes, ranges, types and workspace
+ * (mx_gqa_kv8_window_workspace bytes) as for mx_gqa_kv8.
+ * No counterpart in the reference, as above.
+ */
+int mx_gqa_kv8_window(const void* q, const void* k_cache, const void* v_cache, const float* k_scale,
+                      const float* v_scale, const int* page_table, const int* kv_lens, const int* cu, void* O, int B,
+                      int T, int max_q, int max_kv, int n_q, int n_kv, int d, int page, int pages, int max_pages,
+                      int q_stride, float scale, int window, int sinks, int dtype, void* workspace, size_t ws_bytes,
+                      void* stream);
+size_t mx_gqa_kv8_window_workspace(int B, int T, int max_q, int max_kv, int n_q, int n_kv, int d, int window, int sinks);
+
+/*
+ * mx_gqa_kv8 for drafted tokens that form a tree.  Sequence b's rows are its last n_b tokens, in the cache
+ * already (mx_kv8_append).  tree: [T, words] 64-bit masks on the device; row i sees the tokens before the
+ * drafted ones, t < kv_lens[b] - n_b, and the j-th drafted one where bit j % 64 of tree[i, j / 64] is set: its
+ * ancestors' and its own, as a rule; nothing is added to the mask.  Drafted tokens from 64 * words on are
+ * seen by no row.  1 <= words <= 16, tree 8-byte aligned.  A row that sees no token gives zeros.  Rows, hints,
+ * sizes, ranges, types and workspace (mx_gqa_kv8_tree_workspace bytes) as for mx_gqa_kv8.
+ * No counterpart in the reference, as above.
+ */
+int mx_gqa_kv8_tree(const void* q, const void* k_cache, const void* v_cache, const float* k_scale, const float* v_scale,
+                    const int* page_table, const int* kv_lens, const int* cu, const void* tree, void* O, int B, int T,
+                    int max_q, int max_kv, int n_q, int n_kv, int d, int page, int pages, int max_pages, int q_stride,
+                    float scale, int words, int dtype, void* workspace, size_t ws_bytes, void* stream);
+size_t mx_gqa_kv8_tree_workspace(int B, int T, int max_q, int max_kv, int n_q, int n_kv, int d);
+
+/*
  * RMS norm of every query and key head and the position rotation, in one pass: head x of
  * token t (of T), with w = q_weight or k_weight [d] and p = positions[t],
  *   y = x * rsqrt(mean(x^2) + eps) * w

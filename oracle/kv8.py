@@ -79,10 +79,11 @@ class Cache:
                 present[t] = True
         return k, v, present
 
-    def attend(self, q, table, lens, cu, causal=True, scale=None):
+    def attend(self, q, table, lens, cu, causal=True, scale=None, seen=None):
         """(out, weight, score) [T, n_q, d] / [T, n_q]: the attention, the sum of
         p |v| for each output, and the largest sum of |scale q k| of a row (what a bound on the
-        device's roundings needs).  Rows of no sequence are NaN."""
+        device's roundings needs).  Rows of no sequence are NaN.  seen(b, i): which of the tokens
+        0 .. lens[b] - 1 the i-th row of sequence b sees, instead of the causal mask."""
         q = q.detach().cpu().double()
         T, n_q, d = q.shape
         scale = 1 / math.sqrt(d) if scale is None else scale
@@ -96,7 +97,9 @@ class Cache:
                 k, v, present = self.tokens(b, h, lens[b], table)
                 for i in range(n):
                     see = present.clone()
-                    if causal:
+                    if seen is not None:
+                        see &= seen(b, i)
+                    elif causal:
                         see[max(lens[b] - n + i + 1, 0):] = False
                     r = cu[b] + i
                     for j in range(h * (n_q // self.n_kv), (h + 1) * (n_q // self.n_kv)):
