@@ -9,10 +9,11 @@
 // product, 2^-24 of it, would pass every exponent's range for masks like -1e30.)
 //
 // The alternatives: a key per logit orders them (the value's bits, made to rise with it, above the complement of
-// its place, so that ties go to the lowest id).  A wave keeps its best 64 keys sorted across its lanes, and only a
-// chunk in which a lane's maximum reaches the k-th of them is looked at again.  What it has there is gathered
-// in LDS, sorted 64 at a time and merged in.  The first chunk would all qualify: there the k-th largest of the 64
-// lanes' maxima is the bar, which at least k logits reach.
+// its place, so that ties go to the lowest id).  A wave keeps its best 64 keys sorted across its lanes.  A logit that
+// reaches the bar, a bound on the k-th best that only rises, waits in LDS by its place; 64 of them are
+// sorted and merged in at a time, and raise the bar.  It is the k-th of the wave's list, or what the workgroup's
+// four waves know together: the largest k-th of their lists, the least (k/4)-th.  In the first chunk it is the k-th
+// largest of the lanes' maxima.
 //
 // A row is cut into slices, a workgroup each, where there are few rows; a second kernel joins them.
 #include <algorithm>
@@ -80,11 +81,21 @@ __device__ __forceinline__ float lane_xorf(float v, int lane) {
 
 // Sorted across the lanes, the largest first.  A bitonic network: a stage J meets the lane J away, and keeps the larger
 // where both its bit J and the direction of its block of SIZE say so.
+constexpr uint64_t lanes_of_larger(int size, int j) {
+  uint64_t m = 0;
+  for (int l = 0; l < 64; ++l)
+    if (((l & j) == 0) == ((l & size) == 0)) m |= 1ull << l;
+  return m;
+}
+template <int SIZE, int J>
+__device__ __forceinline__ bool keeps_larger() {  // a constant per lane: scalar registers, not kept between stages
+  constexpr uint64_t m = lanes_of_larger(SIZE, J);
+  return __builtin_amdgcn_inverse_ballot_w64(m);
+}
 template <int SIZE, int J>
 __device__ __forceinline__ void stage(uint64_t& v, int lane) {
   const uint64_t o = lane_xor64<J>(v, lane);
-  const bool larger = ((lane & J) == 0) == ((lane & SIZE) == 0);
-  v = (o > v) == larger ? o : v;
+  v = (o > v) == keeps_larger<SIZE, J>() ? o : v;
 }
 template <int SIZE, int J = SIZE / 2>
 __device__ __forceinline__ void merge(uint64_t& v, int lane) {
@@ -100,8 +111,7 @@ __device__ __forceinline__ void sort(uint64_t& v, int lane) {
 template <int SIZE = 2, int J = 1>
 __device__ __forceinline__ void sort_floats(float& v, int lane) {
   const float o = lane_xorf<J>(v, lane);
-  const bool larger = ((lane & J) == 0) == ((lane & SIZE) == 0);
-  v = larger ? fmaxf(v, o) : fminf(v, o);
+  v = keeps_larger<SIZE, J>() ? fmaxf(v, o) : fminf(v, o);
   if constexpr (J > 1) sort_floats<SIZE, J / 2>(v, lane);
   else if constexpr (SIZE < 64) sort_floats<2 * SIZE, SIZE>(v, lane);
 }
@@ -165,98 +175,135 @@ __device__ __forceinline__ void join_lanes(State& st, int lane) {
 
 // What a wave has of the alternatives.
 struct Best {
-  uint64_t list = 0;    // sorted across the lanes; 0: none
-  uint64_t kth = 0;     // the k-th of them
-  float bar = -INFINITY;  // its value
-  int waiting = 0;      // keys in LDS that are not merged yet, below 64
+  uint64_t list = 0;      // sorted across the lanes; 0: none
+  float bar = -INFINITY;  // logits below it cannot be among them
+  bool full = false;      // the list holds `top`
+  int waiting = 0;        // places in LDS that are not merged yet, below 64
+};
+// In LDS, of each wave: places that wait, and what its list says: its k-th and its (k/4)-th value.
+struct Shared {
+  int wait[NW][128];
+  float kth[NW], part[NW];
 };
 
-__device__ __forceinline__ void merge_in(Best& best, uint64_t* buf, int n, int top, int lane) {
+template <typename T>
+__device__ __forceinline__ void merge_in(Best& best, Shared& sh, int wave, int n, int top, const void* row, int lane) {
   wave_sync();
-  uint64_t v = lane < n ? buf[lane] : 0;
+  uint64_t v = 0;
+  if (lane < n) {
+    const int place = sh.wait[wave][lane];
+    v = key_of(at<T>(row, place), place);
+  }
   sort(v, lane);
   take_best(best.list, v, lane);
-  best.kth = broadcast(best.list, top - 1);
-  best.bar = best.kth ? value_of(best.kth) : -INFINITY;
+  const uint64_t kth = broadcast(best.list, top - 1), part = broadcast(best.list, (top - 1) / NW);
+  best.full = kth != 0;
+  if (best.full) {
+    // what comes has larger ids than the list: it must be above the k-th's value
+    const uint64_t above = (kth | 0xffffffffu) + 1;
+    best.bar = fmaxf(best.bar, value_of(above));
+    if (lane == 0) *(volatile float*)&sh.kth[wave] = value_of(kth);
+  }
+  if (part && lane == 0) *(volatile float*)&sh.part[wave] = value_of(part);
+}
+// The others' lists may say more.
+__device__ __forceinline__ void raise_bar(Best& best, Shared& sh) {
+  const volatile float *k = sh.kth, *p = sh.part;
+  const float most = fmaxf(fmaxf(k[0], k[1]), fmaxf(k[2], k[3])), least = fminf(fminf(p[0], p[1]), fminf(p[2], p[3]));
+  best.bar = fmaxf(best.bar, fmaxf(most, least));
 }
 
-// x[j], by a tree of selections: registers have no index.
-template <int N>
-__device__ __forceinline__ float pick(const float (&x)[N], int j) {
-  if constexpr (N == 1) {
-    return x[0];
-  } else {
-    float half[N / 2];
-#pragma unroll
-    for (int i = 0; i < N / 2; ++i) half[i] = j & 1 ? x[2 * i + 1] : x[2 * i];
-    return pick<N / 2>(half, j >> 1);
-  }
-}
-
-// The logits x of a chunk, x[j] the token first + (j / EB) * apart + j % EB of the lane where it is there.
-template <int N, int EB>
-__device__ __forceinline__ void offer(Best& best, const float (&x)[N], const bool (&there)[N / EB], float most, int first,
-                                      int apart, int top, uint64_t* buf, int lane) {
-  float bar = best.bar;
-  if (!best.kth) {  // fewer than `top` so far
-    float v = most;
-    sort_floats(v, lane);
-    bar = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(v), top - 1));
-  }
-  uint32_t good = 0;  // of the lane's
-#pragma unroll
-  for (int j = 0; j < N; ++j) good |= there[j / EB] && x[j] >= bar ? 1u << j : 0u;
-  for (; __any(good != 0); good &= good - 1) {
-    const int j = good ? __builtin_ctz(good) : 0;
-    const uint64_t key = key_of(pick<N>(x, j), first + j / EB * apart + j % EB);
-    const uint64_t who = __ballot(good && key > best.kth);
+// The lane's logits of a chunk that reach the bar are `good`, bit j the place first + j / EB * apart + j % EB.
+template <typename T, int EB>
+__device__ __forceinline__ void offer(Best& best, Shared& sh, uint32_t good, int first, int apart, int top, const void* row,
+                                      int wave, int lane) {
+  uint32_t any = good;
+  any |= lane_xor<1>(any, lane);
+  any |= lane_xor<2>(any, lane);
+  any |= lane_xor<4>(any, lane);
+  any |= lane_xor<8>(any, lane);
+  any |= lane_xor<16>(any, lane);
+  any |= lane_xor<32>(any, lane);
+  any = (uint32_t)__builtin_amdgcn_readfirstlane((int)any);
+  for (; any; any &= any - 1) {
+    const int j = __builtin_ctz(any);
+    const uint64_t who = __ballot(good >> j & 1);
     if (who >> lane & 1)
-      buf[best.waiting + __builtin_amdgcn_mbcnt_hi((uint32_t)(who >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)who, 0))] = key;
+      sh.wait[wave][best.waiting + __builtin_amdgcn_mbcnt_hi((uint32_t)(who >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)who, 0))] =
+          first + j / EB * apart + j % EB;
     best.waiting += __popcll(who);
     if (best.waiting >= 64) {
-      merge_in(best, buf, 64, top, lane);
-      const uint64_t rest = buf[64 + lane];
+      merge_in<T>(best, sh, wave, 64, top, row, lane);
+      const int rest = sh.wait[wave][64 + lane];
       best.waiting -= 64;
       wave_sync();
-      buf[lane] = rest;
+      sh.wait[wave][lane] = rest;
     }
-  }
-  if (best.waiting) {
-    merge_in(best, buf, best.waiting, top, lane);
-    best.waiting = 0;
   }
 }
 
-// One chunk into the state and the alternatives.
-template <bool TOP, int N, int EB>
-__device__ __forceinline__ void take(State& st, Best& best, const float (&x)[N], const bool (&there)[N / EB], int first,
-                                     int apart, int top, uint64_t* buf, int lane) {
-  float most = x[0];
+// One chunk, x[u] the EB logits from place first + u * apart on where there[u], into the state and the alternatives.
+template <typename T, bool TOP, int U, int EB>
+__device__ __forceinline__ void take(State& st, Best& best, Shared& sh, const float (&x)[U][EB], const bool (&there)[U],
+                                     int first, int apart, int top, const void* row, int wave, int lane) {
+  float block[U];
 #pragma unroll
-  for (int j = 1; j < N; ++j) most = fmaxf(most, x[j]);
+  for (int u = 0; u < U; ++u) {
+    block[u] = x[u][0];
+#pragma unroll
+    for (int j = 1; j < EB; ++j) block[u] = fmaxf(block[u], x[u][j]);
+  }
+  float most = block[0];
+#pragma unroll
+  for (int u = 1; u < U; ++u) most = fmaxf(most, block[u]);
   if (__any(most > st.m)) move_to(st, fmaxf(most, st.m));
   const float off = st.m == -INFINITY ? 0.f : st.m;
   float s[4] = {}, e[4] = {};
 #pragma unroll
-  for (int j = 0; j < N; ++j) {
-    const float y = x[j] - off;
-    const float p = __builtin_amdgcn_exp2f(y * kLog2e);
-    s[j % 4] += p;
-    e[j % 4] = __builtin_fmaf(p, y, e[j % 4]);
-  }
+  for (int u = 0; u < U; ++u)
+#pragma unroll
+    for (int j = 0; j < EB; ++j) {
+      const float y = x[u][j] - off;
+      const float p = __builtin_amdgcn_exp2f(y * kLog2e);
+      s[j % 4] += p;
+      e[j % 4] = __builtin_fmaf(p, y, e[j % 4]);
+    }
   float more = (e[0] + e[1]) + (e[2] + e[3]);
   if (__any(more != more)) {  // 0 times -inf: such logits add nothing (a NaN is in S)
     more = 0.f;
+    float off2 = off;
+    asm("" : "+v"(off2));  // or the exponentials above are kept for here, in as many registers
 #pragma unroll
-    for (int j = 0; j < N; ++j) {
-      const float y = x[j] - off;
-      more += y > -INFINITY ? __builtin_amdgcn_exp2f(y * kLog2e) * y : 0.f;
-    }
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int j = 0; j < EB; ++j) {
+        const float y = x[u][j] - off2;
+        more += y > -INFINITY ? __builtin_amdgcn_exp2f(y * kLog2e) * y : 0.f;
+      }
   }
   st.s += (s[0] + s[1]) + (s[2] + s[3]);
   st.e += more;
   if constexpr (TOP) {
-    if (__any(most >= best.bar)) offer<N, EB>(best, x, there, most, first, apart, top, buf, lane);
+    float bar = best.bar;
+    if (!best.full) {  // few so far: at least `top` logits reach the k-th of the lanes' maxima
+      float v = most;
+      sort_floats(v, lane);
+      bar = fmaxf(bar, __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(v), top - 1)));
+    }
+    if (__any(most >= bar)) {
+      uint32_t good = 0;
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (__any(block[u] >= bar)) {
+#pragma unroll
+          for (int j = 0; j < EB; ++j) good |= there[u] && x[u][j] >= bar ? 1u << (u * EB + j) : 0u;
+        }
+      offer<T, EB>(best, sh, good, first, apart, top, row, wave, lane);
+      if (!best.full && best.waiting) {
+        merge_in<T>(best, sh, wave, best.waiting, top, row, lane);
+        best.waiting = 0;
+      }
+    }
   }
 }
 
@@ -282,15 +329,14 @@ __device__ __forceinline__ void answer(const Args& a, const State& st, uint64_t 
 template <typename T, bool TOP>
 __global__ __launch_bounds__(NT) void rows_kernel(const Args a) {
   constexpr int EB = 16 / kBytes<T>;  // logits of a block
-  constexpr int UB = 4;               // blocks of a chunk and thread
-  __shared__ uint64_t bufs[NW][128];
+  constexpr int U = 4;                // blocks of a chunk and thread
+  __shared__ Shared sh;
   __shared__ uint64_t lists[NW][kMostTop];
   __shared__ State states[NW];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const size_t row = blockIdx.x / (unsigned)a.slices;
   const int slice = (int)(blockIdx.x % (unsigned)a.slices);
-  uint64_t* buf = bufs[wave];
   const char* x = (const char*)a.x + row * a.stride * kBytes<T>;
   // 16-byte blocks, and the logits before the first and behind the last of them
   const int head = min((int)((16 - ((uintptr_t)x & 15)) & 15) / kBytes<T>, a.V);
@@ -299,50 +345,66 @@ __global__ __launch_bounds__(NT) void rows_kernel(const Args a) {
 
   State st{-INFINITY, 0.f, 0.f};
   Best best;
-  auto widen = [&](const u32x4& r, float* v) {
+  if constexpr (TOP) {
+    if (threadIdx.x < NW) sh.kth[threadIdx.x] = sh.part[threadIdx.x] = -INFINITY;
+    __syncthreads();
+  }
+  const int begin = (int)min((long long)slice * a.per, (long long)blocks);
+  const int end = (int)min((long long)(slice + 1) * a.per, (long long)blocks);
+  u32x4 raw[U] = {};
+  auto load = [&](int at0) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      if constexpr (std::is_same<T, F32>::value) {
-        v[i] = __uint_as_float(r[i]);
-      } else {
-        v[2 * i] = T::to_f32(r[i] & 0xffffu);
-        v[2 * i + 1] = T::to_f32(r[i] >> 16);
-      }
+    for (int u = 0; u < U; ++u) {
+      raw[u] = body[min(at0 + u * NT + (int)threadIdx.x, end - 1)];  // behind the end: not used
     }
   };
-  const int end = min((int)min((long long)(slice + 1) * a.per, (long long)blocks), blocks);
-  for (int at0 = slice * a.per; at0 < end; at0 += UB * NT) {
-    u32x4 raw[UB];
-    bool there[UB];
-    float v[UB * EB];
+  if (begin < end) load(begin);
+  for (int at0 = begin; at0 < end; at0 += U * NT) {
+    bool there[U];
+    float v[U][EB];
 #pragma unroll
-    for (int u = 0; u < UB; ++u) {
-      const int i = at0 + u * NT + (int)threadIdx.x;
-      there[u] = i < end;
-      raw[u] = there[u] ? body[i] : u32x4{};
-    }
+    for (int u = 0; u < U; ++u) {
+      there[u] = at0 + u * NT + (int)threadIdx.x < end;
 #pragma unroll
-    for (int u = 0; u < UB; ++u) {
-      widen(raw[u], v + u * EB);
-      if (!there[u]) {
-#pragma unroll
-        for (int j = 0; j < EB; ++j) v[u * EB + j] = -INFINITY;
+      for (int i = 0; i < 4; ++i) {
+        if constexpr (std::is_same<T, F32>::value) {
+          v[u][i] = __uint_as_float(raw[u][i]);
+        } else {
+          v[u][2 * i] = T::to_f32(raw[u][i] & 0xffffu);
+          v[u][2 * i + 1] = T::to_f32(raw[u][i] >> 16);
+        }
       }
     }
-    take<TOP, UB * EB, EB>(st, best, v, there, head + (at0 + (int)threadIdx.x) * EB, NT * EB, a.top, buf, lane);
+    if (at0 + U * NT < end) {
+      load(at0 + U * NT);
+    } else {
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (!there[u]) {
+#pragma unroll
+          for (int j = 0; j < EB; ++j) v[u][j] = -INFINITY;
+        }
+    }
+    take<T, TOP, U, EB>(st, best, sh, v, there, head + (at0 + (int)threadIdx.x) * EB, NT * EB, a.top, x, wave, lane);
+    if constexpr (TOP) raise_bar(best, sh);
   }
   // the logits outside the blocks: the first wave of the first slice takes those before them, of the last one those behind
   for (int side = 0; wave == 0 && side < 2; ++side) {
     const int n = side ? tail : head, v = side ? a.V - tail + lane : lane;
     if (n == 0 || slice != (side ? a.slices - 1 : 0)) continue;
     const bool there[1] = {lane < n};
-    const float x1[1] = {lane < n ? at<T>(x, v) : -INFINITY};
-    take<TOP, 1, 1>(st, best, x1, there, v, 0, a.top, buf, lane);
+    const float x1[1][1] = {{lane < n ? at<T>(x, v) : -INFINITY}};
+    if constexpr (TOP) {
+      // (those before the blocks have smaller ids than the list: they may be as large as the k-th)
+      if (best.full) best.bar = fminf(best.bar, value_of(broadcast(best.list, a.top - 1)));
+    }
+    take<T, TOP, 1, 1>(st, best, sh, x1, there, v, 0, a.top, x, wave, lane);
   }
 
   join_lanes<32>(st, lane);
   if (lane == 0) states[wave] = st;
   if constexpr (TOP) {
+    if (best.waiting) merge_in<T>(best, sh, wave, best.waiting, a.top, x, lane);
     if (lane < kMostTop) lists[wave][lane] = best.list;
   }
   __syncthreads();
@@ -362,8 +424,16 @@ __global__ __launch_bounds__(NT) void rows_kernel(const Args a) {
 }
 
 // The slices of a row meet in a wave.
+template <int J, bool MOST>
+__device__ __forceinline__ uint64_t extreme(uint64_t v, int lane) {
+  const uint64_t o = lane_xor64<J>(v, lane);
+  v = (o > v) == MOST ? o : v;
+  if constexpr (J > 1) return extreme<J / 2, MOST>(v, lane);
+  else return v;
+}
 template <typename T>
 __global__ __launch_bounds__(64) void join_kernel(const Args a) {
+  __shared__ uint64_t wait[128];
   const int lane = threadIdx.x;
   const size_t row = blockIdx.x;
   State st{-INFINITY, 0.f, 0.f};
@@ -371,17 +441,39 @@ __global__ __launch_bounds__(64) void join_kernel(const Args a) {
     const float4 s = a.states[row * a.slices + lane];
     st = State{s.x, s.y, s.z};
   }
-  join_lanes<32>(st, lane);
-  // the lanes' lists are sorted: the slices' best first, then their second, until none is good enough
-  uint64_t list = 0, kth = 0;
-  const uint64_t* keys = a.keys + (row * a.slices + lane) * a.top;
-  for (int j = 0; j < a.top; ++j) {
-    uint64_t v = lane < a.slices ? keys[j] : 0;
-    if (!__any(v > kth)) break;
-    sort(v, lane);
-    take_best(list, v, lane);
-    kth = broadcast(list, a.top - 1);
+  uint64_t list = 0;
+  if (a.top) {
+    // no key below the largest of the slices' last ones counts, nor below the least of their (top / slices)-th
+    const uint64_t* keys = a.keys + row * a.slices * a.top;
+    const uint64_t last = lane < a.slices ? keys[lane * a.top + a.top - 1] : 0;
+    const uint64_t part = lane < a.slices ? keys[lane * a.top + (a.top - 1) / a.slices] : ~0ull;
+    uint64_t bar = extreme<32, true>(last, lane);
+    const uint64_t least = extreme<32, false>(part, lane);
+    bar = least > bar ? least : bar;
+    int waiting = 0;
+    auto merge_some = [&](int n) {
+      wave_sync();
+      uint64_t v = lane < n ? wait[lane] : 0;
+      sort(v, lane);
+      take_best(list, v, lane);
+    };
+    for (int i = 0; i < a.slices * a.top; i += 64) {
+      const uint64_t key = i + lane < a.slices * a.top ? keys[i + lane] : 0;
+      const uint64_t who = __ballot(key && key >= bar);
+      if (who >> lane & 1)
+        wait[waiting + __builtin_amdgcn_mbcnt_hi((uint32_t)(who >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)who, 0))] = key;
+      waiting += __popcll(who);
+      if (waiting >= 64) {
+        merge_some(64);
+        const uint64_t rest = wait[64 + lane];
+        waiting -= 64;
+        wave_sync();
+        wait[lane] = rest;
+      }
+    }
+    if (waiting) merge_some(waiting);
   }
+  join_lanes<32>(st, lane);
   answer<T>(a, st, list, row, lane, 64);
 }
 
