@@ -11,9 +11,9 @@
 // The alternatives: a key per logit orders them (the value's bits, made to rise with it, above the complement of
 // its place, so that ties go to the lowest id).  A wave keeps its best 64 keys sorted across its lanes.  A logit that
 // reaches the bar, a bound on the k-th best that only rises, waits in LDS by its place; 64 of them are
-// sorted and merged in at a time, and raise the bar.  It is the k-th of the wave's list, or what the workgroup's
-// four waves know together: the largest k-th of their lists, the least (k/4)-th.  In the first chunk it is the k-th
-// largest of the lanes' maxima.
+// sorted and merged in at a time, and raise the bar.  It is the k-th of the wave's list (before there is one, of its
+// lanes' maxima), or what the workgroup's four waves know together: the largest k-th of theirs, the least
+// (k/4)-th.  -inf never reaches it: a row with fewer than k others has its lowest ids of -inf behind them.
 //
 // A row is cut into slices, a workgroup each, where there are few rows; a second kernel joins them.
 #include <algorithm>
@@ -174,17 +174,23 @@ __device__ __forceinline__ void join_lanes(State& st, int lane) {
 }
 
 // What a wave has of the alternatives.
+constexpr float kLowest = -3.402823466e38f;
 struct Best {
-  uint64_t list = 0;      // sorted across the lanes; 0: none
-  float bar = -INFINITY;  // logits below it cannot be among them
-  bool full = false;      // the list holds `top`
-  int waiting = 0;        // places in LDS that are not merged yet, below 64
+  uint64_t list = 0;    // sorted across the lanes; 0: none
+  float bar = kLowest;  // logits below it cannot be among them
+  int waiting = 0;      // places in LDS that are not merged yet, below 64
 };
-// In LDS, of each wave: places that wait, and what its list says: its k-th and its (k/4)-th value.
+// In LDS, of each wave: places that wait, and what it knows: its k-th and its (k/4)-th value, or values below them.
 struct Shared {
   int wait[NW][128];
   float kth[NW], part[NW];
 };
+__device__ __forceinline__ void tell(Shared& sh, int wave, float kth, float part, int lane) {
+  if (lane == 0) {
+    *(volatile float*)&sh.kth[wave] = kth;
+    *(volatile float*)&sh.part[wave] = part;
+  }
+}
 
 template <typename T>
 __device__ __forceinline__ void merge_in(Best& best, Shared& sh, int wave, int n, int top, const void* row, int lane) {
@@ -196,17 +202,13 @@ __device__ __forceinline__ void merge_in(Best& best, Shared& sh, int wave, int n
   }
   sort(v, lane);
   take_best(best.list, v, lane);
-  const uint64_t kth = broadcast(best.list, top - 1), part = broadcast(best.list, (top - 1) / NW);
-  best.full = kth != 0;
-  if (best.full) {
-    // what comes has larger ids than the list: it must be above the k-th's value
-    const uint64_t above = (kth | 0xffffffffu) + 1;
-    best.bar = fmaxf(best.bar, value_of(above));
-    if (lane == 0) *(volatile float*)&sh.kth[wave] = value_of(kth);
-  }
-  if (part && lane == 0) *(volatile float*)&sh.part[wave] = value_of(part);
+  const uint64_t kth = broadcast(best.list, top - 1);
+  if (!kth) return;
+  tell(sh, wave, value_of(kth), value_of(broadcast(best.list, (top - 1) / NW)), lane);
+  // what comes has larger ids than the list: it must be above the k-th's value
+  best.bar = fmaxf(best.bar, value_of((kth | 0xffffffffu) + 1));
 }
-// The others' lists may say more.
+// The others may know more.
 __device__ __forceinline__ void raise_bar(Best& best, Shared& sh) {
   const volatile float *k = sh.kth, *p = sh.part;
   const float most = fmaxf(fmaxf(k[0], k[1]), fmaxf(k[2], k[3])), least = fminf(fminf(p[0], p[1]), fminf(p[2], p[3]));
@@ -217,18 +219,11 @@ __device__ __forceinline__ void raise_bar(Best& best, Shared& sh) {
 template <typename T, int EB>
 __device__ __forceinline__ void offer(Best& best, Shared& sh, uint32_t good, int first, int apart, int top, const void* row,
                                       int wave, int lane) {
-  uint32_t any = good;
-  any |= lane_xor<1>(any, lane);
-  any |= lane_xor<2>(any, lane);
-  any |= lane_xor<4>(any, lane);
-  any |= lane_xor<8>(any, lane);
-  any |= lane_xor<16>(any, lane);
-  any |= lane_xor<32>(any, lane);
-  any = (uint32_t)__builtin_amdgcn_readfirstlane((int)any);
-  for (; any; any &= any - 1) {
-    const int j = __builtin_ctz(any);
-    const uint64_t who = __ballot(good >> j & 1);
-    if (who >> lane & 1)
+  for (;; good &= good - 1) {  // each lane's first, then its second
+    const uint64_t who = __ballot(good != 0);
+    if (!who) break;
+    const int j = __builtin_ctz(good | 0x80000000u);
+    if (good)
       sh.wait[wave][best.waiting + __builtin_amdgcn_mbcnt_hi((uint32_t)(who >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)who, 0))] =
           first + j / EB * apart + j % EB;
     best.waiting += __popcll(who);
@@ -242,10 +237,11 @@ __device__ __forceinline__ void offer(Best& best, Shared& sh, uint32_t good, int
   }
 }
 
-// One chunk, x[u] the EB logits from place first + u * apart on where there[u], into the state and the alternatives.
+// One chunk, x[u] the EB logits from place first + u * apart on (-inf where there are none), into the state and the
+// alternatives.
 template <typename T, bool TOP, int U, int EB>
-__device__ __forceinline__ void take(State& st, Best& best, Shared& sh, const float (&x)[U][EB], const bool (&there)[U],
-                                     int first, int apart, int top, const void* row, int wave, int lane) {
+__device__ __forceinline__ void take(State& st, Best& best, Shared& sh, const float (&x)[U][EB], int first, int apart, int top,
+                                     const void* row, int wave, int lane) {
   float block[U];
 #pragma unroll
   for (int u = 0; u < U; ++u) {
@@ -266,63 +262,58 @@ __device__ __forceinline__ void take(State& st, Best& best, Shared& sh, const fl
       const float y = x[u][j] - off;
       const float p = __builtin_amdgcn_exp2f(y * kLog2e);
       s[j % 4] += p;
-      e[j % 4] = __builtin_fmaf(p, y, e[j % 4]);
+      e[j % 4] = __builtin_fmaf(p, fmaxf(y, kLowest), e[j % 4]);  // not 0 times -inf
     }
-  float more = (e[0] + e[1]) + (e[2] + e[3]);
-  if (__any(more != more)) {  // 0 times -inf: such logits add nothing (a NaN is in S)
-    more = 0.f;
-    float off2 = off;
-    asm("" : "+v"(off2));  // or the exponentials above are kept for here, in as many registers
-#pragma unroll
-    for (int u = 0; u < U; ++u)
-#pragma unroll
-      for (int j = 0; j < EB; ++j) {
-        const float y = x[u][j] - off2;
-        more += y > -INFINITY ? __builtin_amdgcn_exp2f(y * kLog2e) * y : 0.f;
-      }
-  }
   st.s += (s[0] + s[1]) + (s[2] + s[3]);
-  st.e += more;
+  st.e += (e[0] + e[1]) + (e[2] + e[3]);
   if constexpr (TOP) {
-    float bar = best.bar;
-    if (!best.full) {  // few so far: at least `top` logits reach the k-th of the lanes' maxima
+    if (best.bar == kLowest) {  // at least `top` logits reach the k-th of the lanes' maxima
       float v = most;
       sort_floats(v, lane);
-      bar = fmaxf(bar, __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(v), top - 1)));
+      const float kth = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(v), top - 1));
+      tell(sh, wave, kth, __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(v), (top - 1) / NW)), lane);
+      best.bar = fmaxf(best.bar, kth);
     }
-    if (__any(most >= bar)) {
+    if (__any(most >= best.bar)) {
       uint32_t good = 0;
 #pragma unroll
       for (int u = 0; u < U; ++u)
-        if (__any(block[u] >= bar)) {
+        if (__any(block[u] >= best.bar)) {
 #pragma unroll
-          for (int j = 0; j < EB; ++j) good |= there[u] && x[u][j] >= bar ? 1u << (u * EB + j) : 0u;
+          for (int j = 0; j < EB; ++j) good |= x[u][j] >= best.bar ? 1u << (u * EB + j) : 0u;
         }
       offer<T, EB>(best, sh, good, first, apart, top, row, wave, lane);
-      if (!best.full && best.waiting) {
-        merge_in<T>(best, sh, wave, best.waiting, top, row, lane);
-        best.waiting = 0;
-      }
     }
   }
 }
 
-// A row's answers from its state (in every thread) and its best keys (a lane's of one wave).
+// A given token's logit, read ahead of its use: NaN where the number is no token.
 template <typename T>
-__device__ __forceinline__ void answer(const Args& a, const State& st, uint64_t key, size_t row, int tid, int threads) {
-  const void* x = (const char*)a.x + row * a.stride * kBytes<T>;
+__device__ __forceinline__ float given_logit(const Args& a, const void* x, size_t row, int i) {
+  const int v = a.tokens[row * a.given + i];
+  return (uint32_t)v < (uint32_t)a.V ? at<T>(x, v) : __builtin_nanf("");
+}
+
+// A row's answers, by one wave, from its state (in every lane), its best keys and the lane's given token's logit.
+template <typename T>
+__device__ __forceinline__ void answer(const Args& a, const State& st, uint64_t key, float asked, const void* x, size_t row,
+                                       int lane) {
   const bool none = !(st.s > 0.f && st.s < INFINITY);  // a NaN, +inf, nothing but -inf: no distribution
   const float log_s = logf(st.s), nan = __builtin_nanf("");
-  auto log_p = [&](float v) { return (v - st.m) - log_s; };
-  for (int i = tid; i < a.given; i += threads) {
-    const int v = a.tokens[row * a.given + i];
-    const bool token = (uint32_t)v < (uint32_t)a.V;
-    a.logprob[row * a.given + i] = none || !token ? nan : log_p(at<T>(x, v));
+  for (int i = lane; i < a.given; i += 64) {
+    if (i >= 64) asked = given_logit<T>(a, x, row, i);
+    a.logprob[row * a.given + i] = none ? nan : (asked - st.m) - log_s;
   }
-  if (tid == 0) a.entropy[row] = none ? nan : log_s - st.e / st.s;
-  if (tid < a.top) {
-    a.ids[row * a.top + tid] = none ? -1 : (int)~(uint32_t)key;
-    a.top_logprob[row * a.top + tid] = none ? nan : log_p(value_of(key));
+  if (lane == 0) a.entropy[row] = none ? nan : log_s - st.e / st.s;
+  int n = __popcll(__ballot(key != 0));
+  if (n < a.top && !none) {  // the rest are -inf: their lowest ids, which are among the first 64
+    uint64_t who = __ballot(lane < a.V && at<T>(x, min(lane, a.V - 1)) == -INFINITY);
+    for (; n < a.top; ++n, who &= who - 1)
+      if (lane == n) key = key_of(-INFINITY, __builtin_ctzll(who));
+  }
+  if (lane < a.top) {
+    a.ids[row * a.top + lane] = none ? -1 : (int)~(uint32_t)key;
+    a.top_logprob[row * a.top + lane] = none ? nan : (value_of(key) - st.m) - log_s;
   }
 }
 
@@ -346,7 +337,7 @@ __global__ __launch_bounds__(NT) void rows_kernel(const Args a) {
   State st{-INFINITY, 0.f, 0.f};
   Best best;
   if constexpr (TOP) {
-    if (threadIdx.x < NW) sh.kth[threadIdx.x] = sh.part[threadIdx.x] = -INFINITY;
+    if (threadIdx.x < NW) sh.kth[threadIdx.x] = sh.part[threadIdx.x] = kLowest;
     __syncthreads();
   }
   const int begin = (int)min((long long)slice * a.per, (long long)blocks);
@@ -359,12 +350,11 @@ __global__ __launch_bounds__(NT) void rows_kernel(const Args a) {
     }
   };
   if (begin < end) load(begin);
+  const float asked = a.slices == 1 && wave == 0 && lane < a.given ? given_logit<T>(a, x, row, lane) : 0.f;
   for (int at0 = begin; at0 < end; at0 += U * NT) {
-    bool there[U];
     float v[U][EB];
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      there[u] = at0 + u * NT + (int)threadIdx.x < end;
+    for (int u = 0; u < U; ++u)
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         if constexpr (std::is_same<T, F32>::value) {
@@ -374,31 +364,30 @@ __global__ __launch_bounds__(NT) void rows_kernel(const Args a) {
           v[u][2 * i + 1] = T::to_f32(raw[u][i] >> 16);
         }
       }
-    }
     if (at0 + U * NT < end) {
       load(at0 + U * NT);
     } else {
 #pragma unroll
       for (int u = 0; u < U; ++u)
-        if (!there[u]) {
+        if (at0 + u * NT + (int)threadIdx.x >= end) {
 #pragma unroll
           for (int j = 0; j < EB; ++j) v[u][j] = -INFINITY;
         }
     }
-    take<T, TOP, U, EB>(st, best, sh, v, there, head + (at0 + (int)threadIdx.x) * EB, NT * EB, a.top, x, wave, lane);
     if constexpr (TOP) raise_bar(best, sh);
+    take<T, TOP, U, EB>(st, best, sh, v, head + (at0 + (int)threadIdx.x) * EB, NT * EB, a.top, x, wave, lane);
   }
   // the logits outside the blocks: the first wave of the first slice takes those before them, of the last one those behind
   for (int side = 0; wave == 0 && side < 2; ++side) {
     const int n = side ? tail : head, v = side ? a.V - tail + lane : lane;
     if (n == 0 || slice != (side ? a.slices - 1 : 0)) continue;
-    const bool there[1] = {lane < n};
     const float x1[1][1] = {{lane < n ? at<T>(x, v) : -INFINITY}};
     if constexpr (TOP) {
       // (those before the blocks have smaller ids than the list: they may be as large as the k-th)
-      if (best.full) best.bar = fminf(best.bar, value_of(broadcast(best.list, a.top - 1)));
+      const uint64_t kth = broadcast(best.list, a.top - 1);
+      if (kth) best.bar = fminf(best.bar, value_of(kth));
     }
-    take<T, TOP, 1, 1>(st, best, sh, x1, there, v, 0, a.top, x, wave, lane);
+    take<T, TOP, 1, 1>(st, best, sh, x1, v, 0, a.top, x, wave, lane);
   }
 
   join_lanes<32>(st, lane);
@@ -415,7 +404,7 @@ __global__ __launch_bounds__(NT) void rows_kernel(const Args a) {
     if constexpr (TOP) take_best(best.list, lane < kMostTop ? lists[w][lane] : 0, lane);
   }
   if (a.slices == 1) {
-    answer<T>(a, st, best.list, row, lane, 64);
+    answer<T>(a, st, best.list, asked, x, row, lane);
     return;
   }
   const size_t at = row * a.slices + slice;
@@ -436,6 +425,8 @@ __global__ __launch_bounds__(64) void join_kernel(const Args a) {
   __shared__ uint64_t wait[128];
   const int lane = threadIdx.x;
   const size_t row = blockIdx.x;
+  const char* x = (const char*)a.x + row * a.stride * kBytes<T>;
+  const float asked = lane < a.given ? given_logit<T>(a, x, row, lane) : 0.f;
   State st{-INFINITY, 0.f, 0.f};
   if (lane < a.slices) {
     const float4 s = a.states[row * a.slices + lane];
@@ -474,7 +465,7 @@ __global__ __launch_bounds__(64) void join_kernel(const Args a) {
     if (waiting) merge_some(waiting);
   }
   join_lanes<32>(st, lane);
-  answer<T>(a, st, list, row, lane, 64);
+  answer<T>(a, st, list, asked, x, row, lane);
 }
 
 struct Plan {
