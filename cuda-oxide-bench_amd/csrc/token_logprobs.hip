@@ -167,10 +167,23 @@ __device__ __forceinline__ void join(State& st, State o) {
   st.s += o.s;
   st.e += o.e;
 }
-template <int J>
+template <int J = 32>
+__device__ __forceinline__ float lanes_max(float v, int lane) {
+  v = fmaxf(v, lane_xorf<J>(v, lane));
+  if constexpr (J > 1) return lanes_max<J / 2>(v, lane);
+  else return v;
+}
+template <int J = 32>
+__device__ __forceinline__ float lanes_sum(float v, int lane) {
+  v += lane_xorf<J>(v, lane);
+  if constexpr (J > 1) return lanes_sum<J / 2>(v, lane);
+  else return v;
+}
+// The lanes' states in every lane: each moves to the largest maximum once.
 __device__ __forceinline__ void join_lanes(State& st, int lane) {
-  join(st, State{lane_xorf<J>(st.m, lane), lane_xorf<J>(st.s, lane), lane_xorf<J>(st.e, lane)});
-  if constexpr (J > 1) join_lanes<J / 2>(st, lane);
+  move_to(st, lanes_max(st.m, lane));
+  st.s = lanes_sum(st.s, lane);
+  st.e = lanes_sum(st.e, lane);
 }
 
 // What a wave has of the alternatives.
@@ -201,7 +214,8 @@ __device__ __forceinline__ void merge_in(Best& best, Shared& sh, int wave, int n
     v = key_of(at<T>(row, place), place);
   }
   sort(v, lane);
-  take_best(best.list, v, lane);
+  if (__any(best.list != 0)) take_best(best.list, v, lane);
+  else best.list = v;
   const uint64_t kth = broadcast(best.list, top - 1);
   if (!kth) return;
   tell(sh, wave, value_of(kth), value_of(broadcast(best.list, (top - 1) / NW)), lane);
@@ -390,7 +404,7 @@ __global__ __launch_bounds__(NT) void rows_kernel(const Args a) {
     take<T, TOP, 1, 1>(st, best, sh, x1, v, 0, a.top, x, wave, lane);
   }
 
-  join_lanes<32>(st, lane);
+  join_lanes(st, lane);
   if (lane == 0) states[wave] = st;
   if constexpr (TOP) {
     if (best.waiting) merge_in<T>(best, sh, wave, best.waiting, a.top, x, lane);
@@ -436,8 +450,16 @@ __global__ __launch_bounds__(64) void join_kernel(const Args a) {
   if (a.top) {
     // no key below the largest of the slices' last ones counts, nor below the least of their (top / slices)-th
     const uint64_t* keys = a.keys + row * a.slices * a.top;
+    const int all = a.slices * a.top;
+    constexpr int N = 8;  // loads under way
+    uint64_t key[N];
+    auto load = [&](int i) {
+#pragma unroll
+      for (int n = 0; n < N; ++n) key[n] = keys[min(i + 64 * n + lane, all - 1)];
+    };
     const uint64_t last = lane < a.slices ? keys[lane * a.top + a.top - 1] : 0;
     const uint64_t part = lane < a.slices ? keys[lane * a.top + (a.top - 1) / a.slices] : ~0ull;
+    load(0);
     uint64_t bar = extreme<32, true>(last, lane);
     const uint64_t least = extreme<32, false>(part, lane);
     bar = least > bar ? least : bar;
@@ -446,25 +468,32 @@ __global__ __launch_bounds__(64) void join_kernel(const Args a) {
       wave_sync();
       uint64_t v = lane < n ? wait[lane] : 0;
       sort(v, lane);
-      take_best(list, v, lane);
+      if (__any(list != 0)) take_best(list, v, lane);
+      else list = v;
     };
-    for (int i = 0; i < a.slices * a.top; i += 64) {
-      const uint64_t key = i + lane < a.slices * a.top ? keys[i + lane] : 0;
-      const uint64_t who = __ballot(key && key >= bar);
-      if (who >> lane & 1)
-        wait[waiting + __builtin_amdgcn_mbcnt_hi((uint32_t)(who >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)who, 0))] = key;
-      waiting += __popcll(who);
-      if (waiting >= 64) {
-        merge_some(64);
-        const uint64_t rest = wait[64 + lane];
-        waiting -= 64;
-        wave_sync();
-        wait[lane] = rest;
+    for (int i = 0; i < all; i += 64 * N) {
+      if (i) load(i);
+#pragma unroll 1
+      for (int n = 0; n < N && i + 64 * n < all; ++n) {
+        const bool good = i + 64 * n + lane < all && key[0] && key[0] >= bar;
+        const uint64_t who = __ballot(good);
+        if (good)
+          wait[waiting + __builtin_amdgcn_mbcnt_hi((uint32_t)(who >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)who, 0))] = key[0];
+        waiting += __popcll(who);
+        if (waiting >= 64) {
+          merge_some(64);
+          const uint64_t rest = wait[64 + lane];
+          waiting -= 64;
+          wave_sync();
+          wait[lane] = rest;
+        }
+#pragma unroll
+        for (int m = 0; m + 1 < N; ++m) key[m] = key[m + 1];
       }
     }
     if (waiting) merge_some(waiting);
   }
-  join_lanes<32>(st, lane);
+  join_lanes(st, lane);
   answer<T>(a, st, list, asked, x, row, lane);
 }
 
