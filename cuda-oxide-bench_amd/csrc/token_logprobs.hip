@@ -44,6 +44,10 @@ struct F32 {};
 template <typename T>
 constexpr int kBytes = std::is_same<T, F32>::value ? 4 : 2;
 
+// A dword of -inf.
+template <typename T>
+constexpr uint32_t kNone = std::is_same<T, F32>::value ? 0xff800000u : std::is_same<T, BF16>::value ? 0xff80ff80u : 0xfc00fc00u;
+
 template <typename T>
 __device__ __forceinline__ float at(const void* row, int v) {
   if constexpr (std::is_same<T, F32>::value) return ((const float*)row)[v];
@@ -147,6 +151,10 @@ __device__ __forceinline__ void wave_sync() {
   __builtin_amdgcn_wave_barrier();
 }
 
+__device__ __forceinline__ float uniform(float v) {
+  return __uint_as_float((uint32_t)__builtin_amdgcn_readfirstlane((int)__float_as_uint(v)));
+}
+
 // ---- the softmax's state ----
 struct State {
   float m, s, e;
@@ -196,13 +204,12 @@ struct Best {
 // In LDS, of each wave: places that wait, and what it knows: its k-th and its (k/4)-th value, or values below them.
 struct Shared {
   int wait[NW][128];
-  float kth[NW], part[NW];
+  uint64_t known[NW];  // the k-th's bits above the (k/4)-th's
 };
 __device__ __forceinline__ void tell(Shared& sh, int wave, float kth, float part, int lane) {
-  if (lane == 0) {
-    *(volatile float*)&sh.kth[wave] = kth;
-    *(volatile float*)&sh.part[wave] = part;
-  }
+  if (lane == 0)
+    __hip_atomic_store(&sh.known[wave], (uint64_t)__float_as_uint(kth) << 32 | __float_as_uint(part), __ATOMIC_RELAXED,
+                       __HIP_MEMORY_SCOPE_WORKGROUP);
 }
 
 template <typename T>
@@ -220,13 +227,18 @@ __device__ __forceinline__ void merge_in(Best& best, Shared& sh, int wave, int n
   if (!kth) return;
   tell(sh, wave, value_of(kth), value_of(broadcast(best.list, (top - 1) / NW)), lane);
   // what comes has larger ids than the list: it must be above the k-th's value
-  best.bar = fmaxf(best.bar, value_of((kth | 0xffffffffu) + 1));
+  best.bar = uniform(fmaxf(best.bar, value_of((kth | 0xffffffffu) + 1)));
 }
 // The others may know more.
 __device__ __forceinline__ void raise_bar(Best& best, Shared& sh) {
-  const volatile float *k = sh.kth, *p = sh.part;
-  const float most = fmaxf(fmaxf(k[0], k[1]), fmaxf(k[2], k[3])), least = fminf(fminf(p[0], p[1]), fminf(p[2], p[3]));
-  best.bar = fmaxf(best.bar, fmaxf(most, least));
+  float most = kLowest, least = INFINITY;
+#pragma unroll
+  for (int w = 0; w < NW; ++w) {
+    const uint64_t k = __hip_atomic_load(&sh.known[w], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+    most = fmaxf(most, __uint_as_float((uint32_t)(k >> 32)));
+    least = fminf(least, __uint_as_float((uint32_t)k));
+  }
+  best.bar = uniform(fmaxf(best.bar, fmaxf(most, least)));
 }
 
 // The lane's logits of a chunk that reach the bar are `good`, bit j the place first + j / EB * apart + j % EB.
@@ -270,7 +282,7 @@ __device__ __forceinline__ void take(State& st, Best& best, Shared& sh, const fl
   const float off = st.m == -INFINITY ? 0.f : st.m;
   float s[4] = {}, e[4] = {};
 #pragma unroll
-  for (int u = 0; u < U; ++u)
+  for (int u = 0; u < U; ++u) {
 #pragma unroll
     for (int j = 0; j < EB; ++j) {
       const float y = x[u][j] - off;
@@ -278,6 +290,8 @@ __device__ __forceinline__ void take(State& st, Best& best, Shared& sh, const fl
       s[j % 4] += p;
       e[j % 4] = __builtin_fmaf(p, fmaxf(y, kLowest), e[j % 4]);  // not 0 times -inf
     }
+    __builtin_amdgcn_sched_barrier(0);  // or the exponentials of all blocks are held at once, in registers that cost a wave
+  }
   st.s += (s[0] + s[1]) + (s[2] + s[3]);
   st.e += (e[0] + e[1]) + (e[2] + e[3]);
   if constexpr (TOP) {
@@ -286,16 +300,19 @@ __device__ __forceinline__ void take(State& st, Best& best, Shared& sh, const fl
       sort_floats(v, lane);
       const float kth = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(v), top - 1));
       tell(sh, wave, kth, __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(v), (top - 1) / NW)), lane);
-      best.bar = fmaxf(best.bar, kth);
+      best.bar = uniform(fmaxf(best.bar, kth));
     }
     if (__any(most >= best.bar)) {
       uint32_t good = 0;
 #pragma unroll
-      for (int u = 0; u < U; ++u)
+      for (int u = U - 1; u >= 0; --u) {
         if (__any(block[u] >= best.bar)) {
 #pragma unroll
-          for (int j = 0; j < EB; ++j) good |= x[u][j] >= best.bar ? 1u << (u * EB + j) : 0u;
+          for (int j = EB - 1; j >= 0; --j) good = good << 1 | (x[u][j] >= best.bar ? 1u : 0u);
+        } else {
+          good <<= EB;
         }
+      }
       offer<T, EB>(best, sh, good, first, apart, top, row, wave, lane);
     }
   }
@@ -351,7 +368,7 @@ __global__ __launch_bounds__(NT) void rows_kernel(const Args a) {
   State st{-INFINITY, 0.f, 0.f};
   Best best;
   if constexpr (TOP) {
-    if (threadIdx.x < NW) sh.kth[threadIdx.x] = sh.part[threadIdx.x] = kLowest;
+    if (threadIdx.x < NW) tell(sh, threadIdx.x, kLowest, kLowest, 0);
     __syncthreads();
   }
   const int begin = (int)min((long long)slice * a.per, (long long)blocks);
@@ -360,7 +377,7 @@ __global__ __launch_bounds__(NT) void rows_kernel(const Args a) {
   auto load = [&](int at0) {
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      raw[u] = body[min(at0 + u * NT + (int)threadIdx.x, end - 1)];  // behind the end: not used
+      raw[u] = body[min(at0 + u * NT + (int)threadIdx.x, end - 1)];  // behind the end: a line that was read
     }
   };
   if (begin < end) load(begin);
@@ -368,9 +385,11 @@ __global__ __launch_bounds__(NT) void rows_kernel(const Args a) {
   for (int at0 = begin; at0 < end; at0 += U * NT) {
     float v[U][EB];
 #pragma unroll
-    for (int u = 0; u < U; ++u)
+    for (int u = 0; u < U; ++u) {
+      const bool there = at0 + u * NT + (int)threadIdx.x < end;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
+        raw[u][i] = there ? raw[u][i] : kNone<T>;
         if constexpr (std::is_same<T, F32>::value) {
           v[u][i] = __uint_as_float(raw[u][i]);
         } else {
@@ -378,16 +397,8 @@ __global__ __launch_bounds__(NT) void rows_kernel(const Args a) {
           v[u][2 * i + 1] = T::to_f32(raw[u][i] >> 16);
         }
       }
-    if (at0 + U * NT < end) {
-      load(at0 + U * NT);
-    } else {
-#pragma unroll
-      for (int u = 0; u < U; ++u)
-        if (at0 + u * NT + (int)threadIdx.x >= end) {
-#pragma unroll
-          for (int j = 0; j < EB; ++j) v[u][j] = -INFINITY;
-        }
     }
+    load(at0 + U * NT);
     if constexpr (TOP) raise_bar(best, sh);
     take<T, TOP, U, EB>(st, best, sh, v, head + (at0 + (int)threadIdx.x) * EB, NT * EB, a.top, x, wave, lane);
   }
@@ -399,7 +410,7 @@ __global__ __launch_bounds__(NT) void rows_kernel(const Args a) {
     if constexpr (TOP) {
       // (those before the blocks have smaller ids than the list: they may be as large as the k-th)
       const uint64_t kth = broadcast(best.list, a.top - 1);
-      if (kth) best.bar = fminf(best.bar, value_of(kth));
+      if (kth) best.bar = uniform(fminf(best.bar, value_of(kth)));
     }
     take<T, TOP, 1, 1>(st, best, sh, x1, v, 0, a.top, x, wave, lane);
   }
