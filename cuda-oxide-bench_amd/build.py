@@ -55,9 +55,13 @@ def common_flags() -> list[str]:
 # already get the VGPR form.
 # mla_decode_few.hip: its kernel may use more than 256 registers (one wave per
 # SIMD), and the AGPR form would copy the accumulators on every block.
+# kv8_window.hip, kv8_tree.hip: so may those of 32 rows of 128 channels (437 registers, 314 this way; 32 sequences of
+# 2048 tokens, 8 drafted ones each: 34.7 -> 32.8 us).
 SOURCE_FLAGS = {
     "gqa_fwd.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
     "mla_decode_few.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
+    "kv8_window.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
+    "kv8_tree.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
 }
 
 
