@@ -12,10 +12,11 @@
 // its place, so that ties go to the lowest id).  A wave keeps its best 64 keys sorted across its lanes.  A logit that
 // reaches the bar, a bound on the k-th best that only rises, waits in LDS by its place; 64 of them are
 // sorted and merged in at a time, and raise the bar.  It is the k-th of the wave's list (before there is one, of its
-// lanes' maxima), or what the workgroup's four waves know together: the largest k-th of theirs, the least
-// (k/4)-th.  -inf never reaches it: a row with fewer than k others has its lowest ids of -inf behind them.
+// lanes' maxima), or what the workgroup's W waves know together: the largest k-th of theirs, the least
+// (k/W)-th.  -inf never reaches it: a row with fewer than k others has its lowest ids of -inf behind them.
 //
-// A row is cut into slices, a workgroup each, where there are few rows; a second kernel joins them.
+// A workgroup takes a row, one of 16 waves where there are few; where those few are long a row is cut into slices, which
+// a second kernel joins.
 #include <algorithm>
 
 #include "mx_common.h"
@@ -23,7 +24,6 @@
 namespace mx {
 namespace logprobs {
 
-constexpr int NT = 256, NW = NT / 64;
 constexpr int kMostTop = 32;
 constexpr int kMostSlices = 16;
 constexpr float kLog2e = 1.4426950408889634f;
@@ -201,19 +201,21 @@ struct Best {
   float bar = kLowest;  // logits below it cannot be among them
   int waiting = 0;      // places in LDS that are not merged yet, below 64
 };
-// In LDS, of each wave: places that wait, and what it knows: its k-th and its (k/4)-th value, or values below them.
+// In LDS, of each wave: places that wait, and what it knows: its k-th and its (k/NW)-th value, or values below them.
+template <int NW>
 struct Shared {
   int wait[NW][128];
-  uint64_t known[NW];  // the k-th's bits above the (k/4)-th's
+  uint64_t known[NW];  // the k-th's bits above the (k/NW)-th's
 };
-__device__ __forceinline__ void tell(Shared& sh, int wave, float kth, float part, int lane) {
+template <int NW>
+__device__ __forceinline__ void tell(Shared<NW>& sh, int wave, float kth, float part, int lane) {
   if (lane == 0)
     __hip_atomic_store(&sh.known[wave], (uint64_t)__float_as_uint(kth) << 32 | __float_as_uint(part), __ATOMIC_RELAXED,
                        __HIP_MEMORY_SCOPE_WORKGROUP);
 }
 
-template <typename T>
-__device__ __forceinline__ void merge_in(Best& best, Shared& sh, int wave, int n, int top, const void* row, int lane) {
+template <typename T, int NW>
+__device__ __forceinline__ void merge_in(Best& best, Shared<NW>& sh, int wave, int n, int top, const void* row, int lane) {
   wave_sync();
   uint64_t v = 0;
   if (lane < n) {
@@ -230,20 +232,17 @@ __device__ __forceinline__ void merge_in(Best& best, Shared& sh, int wave, int n
   best.bar = uniform(fmaxf(best.bar, value_of((kth | 0xffffffffu) + 1)));
 }
 // The others may know more.
-__device__ __forceinline__ void raise_bar(Best& best, Shared& sh) {
-  float most = kLowest, least = INFINITY;
-#pragma unroll
-  for (int w = 0; w < NW; ++w) {
-    const uint64_t k = __hip_atomic_load(&sh.known[w], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
-    most = fmaxf(most, __uint_as_float((uint32_t)(k >> 32)));
-    least = fminf(least, __uint_as_float((uint32_t)k));
-  }
+template <int NW>
+__device__ __forceinline__ void raise_bar(Best& best, Shared<NW>& sh, int lane) {
+  const uint64_t k = __hip_atomic_load(&sh.known[lane % NW], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+  const float most = lanes_max<NW / 2>(__uint_as_float((uint32_t)(k >> 32)), lane);
+  const float least = -lanes_max<NW / 2>(-__uint_as_float((uint32_t)k), lane);
   best.bar = uniform(fmaxf(best.bar, fmaxf(most, least)));
 }
 
 // The lane's logits of a chunk that reach the bar are `good`, bit j the place first + j / EB * apart + j % EB.
-template <typename T, int EB>
-__device__ __forceinline__ void offer(Best& best, Shared& sh, uint32_t good, int first, int apart, int top, const void* row,
+template <typename T, int EB, int NW>
+__device__ __forceinline__ void offer(Best& best, Shared<NW>& sh, uint32_t good, int first, int apart, int top, const void* row,
                                       int wave, int lane) {
   for (;; good &= good - 1) {  // each lane's first, then its second
     const uint64_t who = __ballot(good != 0);
@@ -265,8 +264,8 @@ __device__ __forceinline__ void offer(Best& best, Shared& sh, uint32_t good, int
 
 // One chunk, x[u] the EB logits from place first + u * apart on (-inf where there are none), into the state and the
 // alternatives.
-template <typename T, bool TOP, int U, int EB>
-__device__ __forceinline__ void take(State& st, Best& best, Shared& sh, const float (&x)[U][EB], int first, int apart, int top,
+template <typename T, bool TOP, int U, int EB, int NW>
+__device__ __forceinline__ void take(State& st, Best& best, Shared<NW>& sh, const float (&x)[U][EB], int first, int apart, int top,
                                      const void* row, int wave, int lane) {
   float block[U];
 #pragma unroll
@@ -348,12 +347,68 @@ __device__ __forceinline__ void answer(const Args& a, const State& st, uint64_t 
   }
 }
 
-template <typename T, bool TOP>
+template <int J, bool MOST>
+__device__ __forceinline__ uint64_t extreme(uint64_t v, int lane) {
+  const uint64_t o = lane_xor64<J>(v, lane);
+  v = (o > v) == MOST ? o : v;
+  if constexpr (J > 1) return extreme<J / 2, MOST>(v, lane);
+  else return v;
+}
+// The best of `lists` sorted lists of `top` keys each (up to 64 lists), by one wave; wait: 128 keys of LDS.
+__device__ __forceinline__ uint64_t join_lists(const uint64_t* keys, int lists, int top, uint64_t* wait, int lane) {
+  const int all = lists * top;
+  constexpr int N = 8;  // reads under way
+  uint64_t key[N], list = 0;
+  auto load = [&](int i) {
+#pragma unroll
+    for (int n = 0; n < N; ++n) key[n] = keys[min(i + 64 * n + lane, all - 1)];
+  };
+  // no key below the largest of the lists' last ones counts, nor below the least of their (top / lists)-th
+  const uint64_t last = lane < lists ? keys[lane * top + top - 1] : 0;
+  const uint64_t part = lane < lists ? keys[lane * top + (top - 1) / lists] : ~0ull;
+  load(0);
+  uint64_t bar = extreme<32, true>(last, lane);
+  const uint64_t least = extreme<32, false>(part, lane);
+  bar = least > bar ? least : bar;
+  int waiting = 0;
+  auto merge_some = [&](int n) {
+    wave_sync();
+    uint64_t v = lane < n ? wait[lane] : 0;
+    sort(v, lane);
+    if (__any(list != 0)) take_best(list, v, lane);
+    else list = v;
+  };
+  for (int i = 0; i < all; i += 64 * N) {
+    if (i) load(i);
+#pragma unroll 1
+    for (int n = 0; n < N && i + 64 * n < all; ++n) {
+      const bool good = i + 64 * n + lane < all && key[0] && key[0] >= bar;
+      const uint64_t who = __ballot(good);
+      if (good)
+        wait[waiting + __builtin_amdgcn_mbcnt_hi((uint32_t)(who >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)who, 0))] = key[0];
+      waiting += __popcll(who);
+      if (waiting >= 64) {
+        merge_some(64);
+        const uint64_t rest = wait[64 + lane];
+        waiting -= 64;
+        wave_sync();
+        wait[lane] = rest;
+      }
+#pragma unroll
+      for (int m = 0; m + 1 < N; ++m) key[m] = key[m + 1];
+    }
+  }
+  if (waiting) merge_some(waiting);
+  return list;
+}
+
+template <typename T, bool TOP, int NT>
 __global__ __launch_bounds__(NT) void rows_kernel(const Args a) {
+  constexpr int NW = NT / 64;
   constexpr int EB = 16 / kBytes<T>;  // logits of a block
   constexpr int U = 4;                // blocks of a chunk and thread
-  __shared__ Shared sh;
-  __shared__ uint64_t lists[NW][kMostTop];
+  __shared__ Shared<NW> sh;
+  __shared__ uint64_t lists[NW * kMostTop], joined[NW > 4 ? 128 : 1];
   __shared__ State states[NW];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -399,7 +454,7 @@ __global__ __launch_bounds__(NT) void rows_kernel(const Args a) {
       }
     }
     load(at0 + U * NT);
-    if constexpr (TOP) raise_bar(best, sh);
+    if constexpr (TOP) raise_bar(best, sh, lane);
     take<T, TOP, U, EB>(st, best, sh, v, head + (at0 + (int)threadIdx.x) * EB, NT * EB, a.top, x, wave, lane);
   }
   // the logits outside the blocks: the first wave of the first slice takes those before them, of the last one those behind
@@ -419,14 +474,18 @@ __global__ __launch_bounds__(NT) void rows_kernel(const Args a) {
   if (lane == 0) states[wave] = st;
   if constexpr (TOP) {
     if (best.waiting) merge_in<T>(best, sh, wave, best.waiting, a.top, x, lane);
-    if (lane < kMostTop) lists[wave][lane] = best.list;
+    if (lane < a.top) lists[wave * a.top + lane] = best.list;
   }
   __syncthreads();
   if (wave != 0) return;
+  st = states[lane % NW];
+  if (lane >= NW) st.s = st.e = 0.f;
+  join_lanes(st, lane);
+  if constexpr (TOP && NW > 4) {
+    best.list = join_lists(lists, NW, a.top, joined, lane);
+  } else if constexpr (TOP) {  // (so few one after the other: 4096 rows of 32000 62 us, 66 the other way)
 #pragma unroll
-  for (int w = 1; w < NW; ++w) {
-    join(st, states[w]);
-    if constexpr (TOP) take_best(best.list, lane < kMostTop ? lists[w][lane] : 0, lane);
+    for (int w = 1; w < NW; ++w) take_best(best.list, lane < a.top ? lists[w * a.top + lane] : 0, lane);
   }
   if (a.slices == 1) {
     answer<T>(a, st, best.list, asked, x, row, lane);
@@ -438,13 +497,6 @@ __global__ __launch_bounds__(NT) void rows_kernel(const Args a) {
 }
 
 // The slices of a row meet in a wave.
-template <int J, bool MOST>
-__device__ __forceinline__ uint64_t extreme(uint64_t v, int lane) {
-  const uint64_t o = lane_xor64<J>(v, lane);
-  v = (o > v) == MOST ? o : v;
-  if constexpr (J > 1) return extreme<J / 2, MOST>(v, lane);
-  else return v;
-}
 template <typename T>
 __global__ __launch_bounds__(64) void join_kernel(const Args a) {
   __shared__ uint64_t wait[128];
@@ -457,76 +509,30 @@ __global__ __launch_bounds__(64) void join_kernel(const Args a) {
     const float4 s = a.states[row * a.slices + lane];
     st = State{s.x, s.y, s.z};
   }
-  uint64_t list = 0;
-  if (a.top) {
-    // no key below the largest of the slices' last ones counts, nor below the least of their (top / slices)-th
-    const uint64_t* keys = a.keys + row * a.slices * a.top;
-    const int all = a.slices * a.top;
-    constexpr int N = 8;  // loads under way
-    uint64_t key[N];
-    auto load = [&](int i) {
-#pragma unroll
-      for (int n = 0; n < N; ++n) key[n] = keys[min(i + 64 * n + lane, all - 1)];
-    };
-    const uint64_t last = lane < a.slices ? keys[lane * a.top + a.top - 1] : 0;
-    const uint64_t part = lane < a.slices ? keys[lane * a.top + (a.top - 1) / a.slices] : ~0ull;
-    load(0);
-    uint64_t bar = extreme<32, true>(last, lane);
-    const uint64_t least = extreme<32, false>(part, lane);
-    bar = least > bar ? least : bar;
-    int waiting = 0;
-    auto merge_some = [&](int n) {
-      wave_sync();
-      uint64_t v = lane < n ? wait[lane] : 0;
-      sort(v, lane);
-      if (__any(list != 0)) take_best(list, v, lane);
-      else list = v;
-    };
-    for (int i = 0; i < all; i += 64 * N) {
-      if (i) load(i);
-#pragma unroll 1
-      for (int n = 0; n < N && i + 64 * n < all; ++n) {
-        const bool good = i + 64 * n + lane < all && key[0] && key[0] >= bar;
-        const uint64_t who = __ballot(good);
-        if (good)
-          wait[waiting + __builtin_amdgcn_mbcnt_hi((uint32_t)(who >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)who, 0))] = key[0];
-        waiting += __popcll(who);
-        if (waiting >= 64) {
-          merge_some(64);
-          const uint64_t rest = wait[64 + lane];
-          waiting -= 64;
-          wave_sync();
-          wait[lane] = rest;
-        }
-#pragma unroll
-        for (int m = 0; m + 1 < N; ++m) key[m] = key[m + 1];
-      }
-    }
-    if (waiting) merge_some(waiting);
-  }
+  const uint64_t list = a.top ? join_lists(a.keys + row * a.slices * a.top, a.slices, a.top, wait, lane) : 0;
   join_lanes(st, lane);
   answer<T>(a, st, list, asked, x, row, lane);
 }
 
 struct Plan {
-  int slices, per;
+  int threads, slices, per;
 };
 
-// A workgroup takes at least a block a thread.  512 workgroups, up to 16 a row: the join takes longer with more (rows
-// of 128000 with 20 alternatives, us: one row of 200000 12.0, with 64 slices 16.2; 16 rows 11.7 and 14.2; 64 rows of fp32
-// 17.9, with 256 workgroups 18.5, 1024 19.3; 256 rows of 100003 23.9, 23.5, 25.7).
+// Few rows of up to 64 KB: one workgroup of 16 waves each, and no second launch (one row of 32000 bf16 9.5 us, as in 15
+// slices; one of 50000 fp32 13.8, in 12 slices 9.5).  Longer ones: 512 workgroups of 4 waves, up to 16 a row: the join takes longer
+// with more (with 20 alternatives, us: one row of 200000 bf16 12.0, with 64 slices 16.2; 16 rows of 128000 11.7 and
+// 14.2; 64 rows of 128000 fp32 17.9, with 256 workgroups 18.5, 1024 19.3; 256 rows of 100003 bf16 23.9, 23.5, 25.7).
 static Plan plan(int T, int V, int dtype) {
+  constexpr int THREADS = 256;
   const int eb = dtype == MX_DTYPE_F32 ? 4 : 8;
   const long long blocks = V / eb;
-  long long slices = T >= 512 ? 1 : (512 + T - 1) / T;
-  const long long most = blocks / NT > 0 ? blocks / NT : 1;
-  slices = slices < most ? slices : most;
-  slices = slices < kMostSlices ? slices : kMostSlices;
+  const bool one = T >= 512 || blocks <= 4096;
   Plan p;
-  const long long per = (blocks + slices - 1) / slices;
-  p.per = (int)(per > 0 ? per : 1);
-  p.slices = (int)((blocks + p.per - 1) / p.per);
-  if (p.slices < 1) p.slices = 1;
+  p.threads = T <= 256 && blocks > THREADS && one ? 1024 : THREADS;
+  long long slices = one ? 1 : std::min((512LL + T - 1) / T, blocks / THREADS);  // a block a thread at least
+  slices = std::min<long long>(slices, kMostSlices);
+  p.per = (int)std::max(1LL, (blocks + slices - 1) / slices);
+  p.slices = (int)std::max(1LL, (blocks + p.per - 1) / p.per);
   return p;
 }
 
@@ -537,8 +543,8 @@ static bool sizes_ok(int T, int V, int given, int top, int dtype) {
 }
 
 template <typename T>
-static int run(Args a, int rows, hipStream_t s) {
-  const int most = (1 << 23) / a.slices;  // rows of a launch: fewer than 2^32 threads
+static int run(Args a, int rows, int threads, hipStream_t s) {
+  const int most = (1 << 21) / a.slices;  // rows of a launch: fewer than 2^32 threads
   for (long long first = 0; first < rows; first += most) {
     const int n = (int)std::min<long long>(rows - first, most);
     const dim3 grid((unsigned)(n * a.slices));
@@ -549,10 +555,13 @@ static int run(Args a, int rows, hipStream_t s) {
     b.entropy = a.entropy + first;
     b.ids = a.ids + (size_t)first * a.top;
     b.top_logprob = a.top_logprob + (size_t)first * a.top;
-    if (a.top)
-      hipLaunchKernelGGL((rows_kernel<T, true>), grid, dim3(NT), 0, s, b);
-    else
-      hipLaunchKernelGGL((rows_kernel<T, false>), grid, dim3(NT), 0, s, b);
+    if (threads == 1024) {
+      if (a.top) hipLaunchKernelGGL((rows_kernel<T, true, 1024>), grid, dim3(1024), 0, s, b);
+      else hipLaunchKernelGGL((rows_kernel<T, false, 1024>), grid, dim3(1024), 0, s, b);
+    } else {
+      if (a.top) hipLaunchKernelGGL((rows_kernel<T, true, 256>), grid, dim3(256), 0, s, b);
+      else hipLaunchKernelGGL((rows_kernel<T, false, 256>), grid, dim3(256), 0, s, b);
+    }
     MX_RETURN_IF_HIP(hipGetLastError());
     if (a.slices > 1) {
       hipLaunchKernelGGL(join_kernel<T>, dim3((unsigned)n), dim3(64), 0, s, b);
@@ -593,7 +602,7 @@ extern "C" int mx_token_logprobs(const void* logits, const int* tokens, float* l
   const Args a{logits, tokens, logprob, entropy, top_ids, top_logprob, (float4*)workspace,
                (uint64_t*)((float4*)workspace + (size_t)T * p.slices), V, given, top, p.slices, p.per, stride};
   hipStream_t s = (hipStream_t)stream;
-  if (dtype == MX_DTYPE_BF16) return run<mx::BF16>(a, T, s);
-  if (dtype == MX_DTYPE_F16) return run<mx::F16>(a, T, s);
-  return run<F32>(a, T, s);
+  if (dtype == MX_DTYPE_BF16) return run<mx::BF16>(a, T, p.threads, s);
+  if (dtype == MX_DTYPE_F16) return run<mx::F16>(a, T, p.threads, s);
+  return run<F32>(a, T, p.threads, s);
 }

@@ -800,34 +800,58 @@ def gqa_kv8(q, cache, page_table, kv_lens, cu_q=None, max_q=None, max_kv=None, c
     return out
 
 
+def _is(t, dtype, ndim, device):
+    """Whether t is a contiguous tensor as named: the common path of the checks below, in one expression."""
+    return (type(t) is _Tensor and t.dtype is dtype and t.dim() == ndim and t.get_device() == device
+            and t.is_contiguous())
+
+
+def _new(shape, dtype, device):
+    """torch.empty, by the binding that takes 1.2 us and not 1.6."""
+    strides, step = [], 1
+    for n in reversed(shape):
+        strides.append(step)
+        step *= n
+    return torch.empty_strided(shape, strides[::-1], dtype=dtype, device=device)
+
+
 def _check_attend(q, cache, page_table, kv_lens, cu_q, max_q, max_kv, scale, out):
     """The checks that gqa_kv8_window and gqa_kv8_tree share: what their calls are made of."""
     _check_cache(cache)
-    qs = _rows(q, "q", _IO_DTYPES, 2)
-    T, n_q = q.shape[:2]
-    B, most, cu, max_q = _check_sequences(cache, T, page_table, kv_lens, cu_q, max_q)
     pages, n_kv, page, d = cache._sizes
-    if T < 1 or q.shape[2] != d or n_q < 1 or n_q % n_kv:
+    dev, i32 = cache._device, torch.int32
+    qs = _rows(q, "q", _IO_DTYPES, 2)
+    T, n_q, qd = q.shape
+    if cu_q is not None and _is(page_table, i32, 2, dev) and _is(kv_lens, i32, 1, dev) and _is(cu_q, i32, 1, dev) and \
+            kv_lens.shape[0] == page_table.shape[0] == cu_q.shape[0] - 1 and (max_q is None or 1 <= max_q <= T) and \
+            0 < page_table.shape[0] * n_kv <= 1 << 22 and 0 < page_table.shape[1] * page <= 1 << 30:
+        B, most = page_table.shape
+        cu, max_q = cu_q.data_ptr(), max_q or T
+    else:
+        B, most, cu, max_q = _check_sequences(cache, T, page_table, kv_lens, cu_q, max_q)
+    if T < 1 or qd != d or n_q < 1 or n_q % n_kv:
         raise ValueError(f"q must be [T, a multiple of {n_kv}, {d}], got {tuple(q.shape)}")
     hint = most * page if max_kv is None else int(max_kv)
     if hint < 1:
         raise ValueError(f"max_kv ({hint}) must be positive")
     if out is None:
-        out = torch.empty((T, n_q, d), dtype=q.dtype, device=q.device)
+        out = _new((T, n_q, d), q.dtype, q.device)
     else:
         _require(out, "out", (q.dtype,), 3)
         if out.shape != q.shape:
             raise ValueError(f"out must be {tuple(q.shape)}")
-    if q.get_device() != cache._device or out.get_device() != cache._device:
+    if q.get_device() != dev or out.get_device() != dev:
         raise ValueError("all tensors must be on the cache's device")
-    return out, B, T, n_q, cu, max_q, hint, most, qs, 1.0 / math.sqrt(d) if scale is None else float(scale)
+    return out, B, T, n_q, cu, int(max_q), hint, most, qs, 1.0 / math.sqrt(d) if scale is None else float(scale)
 
 
-def _fit(need, workspace, q, hint, width):
-    """(workspace pointer, bytes, max_kv) of a call whose workspace size for a max_kv is need(max_kv): one that is too
-    small for the table's width may have been sized for the hint as it is, which can need less."""
+def _fit(need, sizes, workspace, q, hint, width):
+    """(workspace pointer, bytes, max_kv) of a call whose workspace size is need(*sizes) with max_kv for sizes[3]: one
+    that is too small for the table's width may have been sized for the hint as it is, which can need less."""
     most = min(hint, width)
-    want = need(most)
+    want = need(*sizes[:3], most, *sizes[3:])
+    if workspace is None and not want:
+        return None, 0, most
     ws, ws_bytes = _workspace(workspace, want, q)
     return ws, ws_bytes, most if ws_bytes >= want else min(hint, 1 << 30)
 
@@ -852,8 +876,8 @@ def gqa_kv8_window(q, cache, page_table, kv_lens, window, sinks=0, cu_q=None, ma
     out, B, T, n_q, cu, max_q, hint, most, qs, scale = _check_attend(q, cache, page_table, kv_lens, cu_q, max_q, max_kv,
                                                                      scale, out)
     pages, n_kv, page, d = cache._sizes
-    ws, ws_bytes, max_kv = _fit(
-        lambda m: gqa_kv8_window_workspace_bytes(B, T, max_q, m, n_q, n_kv, d, window, sinks), workspace, q, hint, most * page)
+    ws, ws_bytes, max_kv = _fit(gqa_kv8_window_workspace_bytes, (B, T, max_q, n_q, n_kv, d, window, sinks), workspace, q,
+                                hint, most * page)
     _launch("mx_gqa_kv8_window", q, q.data_ptr(), *cache._args, page_table.data_ptr(), kv_lens.data_ptr(), cu,
             out.data_ptr(), B, T, max_q, max_kv, n_q, n_kv, d, page, pages, most, qs, scale, window, sinks,
             _IO_DTYPES[q.dtype], ws, ws_bytes)
@@ -876,15 +900,15 @@ def gqa_kv8_tree(q, cache, page_table, kv_lens, tree, cu_q=None, max_q=None, max
     kept are appended again, from the first one's place on (kv8_append): they then lie as decoded ones do."""
     out, B, T, n_q, cu, max_q, hint, most, qs, scale = _check_attend(q, cache, page_table, kv_lens, cu_q, max_q, max_kv,
                                                                      scale, out)
-    _require(tree, "tree", (torch.int64,))
+    if not _is(tree, torch.int64, 2, cache._device):
+        _require(tree, "tree", (torch.int64,))
     words = 1 if tree.dim() == 1 else tree.shape[-1]
     if tree.dim() not in (1, 2) or tree.shape[0] != T or not 1 <= words <= 16:
         raise ValueError(f"tree must be {(T,)} or [{T}, 1 to 16], got {tuple(tree.shape)}")
     if tree.get_device() != cache._device:
         raise ValueError("all tensors must be on the cache's device")
     pages, n_kv, page, d = cache._sizes
-    ws, ws_bytes, max_kv = _fit(lambda m: gqa_kv8_tree_workspace_bytes(B, T, max_q, m, n_q, n_kv, d), workspace, q, hint,
-                                most * page)
+    ws, ws_bytes, max_kv = _fit(gqa_kv8_tree_workspace_bytes, (B, T, max_q, n_q, n_kv, d), workspace, q, hint, most * page)
     _launch("mx_gqa_kv8_tree", q, q.data_ptr(), *cache._args, page_table.data_ptr(), kv_lens.data_ptr(), cu,
             tree.data_ptr(), out.data_ptr(), B, T, max_q, max_kv, n_q, n_kv, d, page, pages, most, qs, scale, words,
             _IO_DTYPES[q.dtype], ws, ws_bytes)
@@ -917,36 +941,40 @@ def qk_norm_rope(q, k, q_weight, k_weight, table, positions, eps=1e-6, neighbour
     work in place.  d and rot multiples of 16, d up to 256."""
     qs, ks = _rows(q, "q", _IO_DTYPES, 2), _rows(k, "k", (q.dtype,), 2)
     T, n_q, d = q.shape
-    n_kv = k.shape[1]
+    n_kv, dtype, dev = k.shape[1], q.dtype, q.get_device()
     if T < 1 or n_q < 1 or n_kv < 1 or k.shape != (T, n_kv, d):
         raise ValueError(f"q must be [T, n_q, d] and k [T, n_kv, d], got {tuple(q.shape)} and {tuple(k.shape)}")
     if d < 16 or d > 256 or d % 16:
         raise ValueError(f"d ({d}) must be a multiple of 16 up to 256")
-    for w, name in ((q_weight, "q_weight"), (k_weight, "k_weight")):
-        _require(w, name, (q.dtype,), 1)
-        if w.shape[0] != d:
-            raise ValueError(f"{name} must be {(d,)}, got {tuple(w.shape)}")
-    _require(table, "table", (torch.float32,), 2)
-    _require(positions, "positions", _I32, 1)
+    if not (_is(q_weight, dtype, 1, dev) and _is(k_weight, dtype, 1, dev) and _is(table, torch.float32, 2, dev)
+            and _is(positions, torch.int32, 1, dev) and k.get_device() == dev):
+        for w, name in ((q_weight, "q_weight"), (k_weight, "k_weight")):
+            _require(w, name, (dtype,), 1)
+        _require(table, "table", (torch.float32,), 2)
+        _require(positions, "positions", _I32, 1)
+        _same_device(q, k, q_weight, k_weight, table, positions)
+    if q_weight.shape[0] != d or k_weight.shape[0] != d:
+        raise ValueError(f"q_weight and k_weight must be {(d,)}, got {tuple(q_weight.shape)} and {tuple(k_weight.shape)}")
     rows, rot = table.shape
     if not 1 <= rows < _INT or rot < 16 or rot > d or rot % 16:
         raise ValueError(f"table must be [positions, rot] with rot a multiple of 16 up to {d}, got {tuple(table.shape)}")
     if positions.shape[0] != T:
         raise ValueError(f"positions must be {(T,)}, got {tuple(positions.shape)}")
     if q_out is None:
-        q_out, qos = torch.empty((T, n_q, d), dtype=q.dtype, device=q.device), n_q * d
+        q_out, qos = _new((T, n_q, d), dtype, q.device), n_q * d
     else:
-        qos = _rows(q_out, "q_out", (q.dtype,), 2)
+        qos = _rows(q_out, "q_out", (dtype,), 2)
+        _same_device(q, q_out)
     if k_out is None:
-        k_out, kos = torch.empty((T, n_kv, d), dtype=q.dtype, device=q.device), n_kv * d
+        k_out, kos = _new((T, n_kv, d), dtype, q.device), n_kv * d
     else:
-        kos = _rows(k_out, "k_out", (q.dtype,), 2)
+        kos = _rows(k_out, "k_out", (dtype,), 2)
+        _same_device(q, k_out)
     if q_out.shape != q.shape or k_out.shape != k.shape:
         raise ValueError(f"q_out must be {tuple(q.shape)} and k_out {tuple(k.shape)}")
-    _same_device(q, k, q_weight, k_weight, table, positions, q_out, k_out)
     _launch("mx_qk_norm_rope", q, q.data_ptr(), k.data_ptr(), q_weight.data_ptr(), k_weight.data_ptr(), table.data_ptr(),
             positions.data_ptr(), q_out.data_ptr(), k_out.data_ptr(), T, n_q, n_kv, d, rot, rows, qs, ks, qos, kos,
-            float(eps), int(bool(neighbours)), _IO_DTYPES[q.dtype])
+            float(eps), int(bool(neighbours)), _IO_DTYPES[dtype])
     return q_out, k_out
 
 
@@ -974,20 +1002,25 @@ def token_logprobs(logits, tokens=None, top=0, out=None, workspace=None):
         raise ValueError(f"logits must have rows, of up to 2**30 tokens (got {tuple(logits.shape)})")
     if not 0 <= top <= min(32, V):
         raise ValueError(f"top ({top}) must be 0 to {min(32, V)}")
-    given = 0
+    given, dev = 0, logits.get_device()
     if tokens is not None:
-        _require(tokens, "tokens", _I32)
+        if not _is(tokens, torch.int32, 2, dev):
+            _require(tokens, "tokens", _I32)
+            _same_device(logits, tokens)
         if tokens.dim() not in (1, 2) or tokens.shape[0] != T:
             raise ValueError(f"tokens must be {(T,)} or [{T}, m], got {tuple(tokens.shape)}")
         given = tokens.numel() // T
     if T * max(given, top) >= _INT:
         raise ValueError(f"too many results: {T} rows of {max(given, top)}")
-    f32, dev = torch.float32, logits.device
-    if out is None:
-        logprobs = None if tokens is None else torch.empty(tokens.shape, dtype=f32, device=dev)
-        entropy = torch.empty((T,), dtype=f32, device=dev)
-        ids = torch.empty((T, top), dtype=torch.int32, device=dev)
-        best = torch.empty((T, top), dtype=f32, device=dev)
+    f32 = torch.float32
+    if out is None:  # pieces of one tensor
+        whole = _new((T * (1 + given + 2 * top),), f32, logits.device)
+        entropy, at = whole.as_strided((T,), (1,), 0), T
+        ids = whole.view(torch.int32).as_strided((T, top), (top, 1), at)
+        best, at = whole.as_strided((T, top), (top, 1), at + T * top), at + 2 * T * top
+        logprobs = None
+        if tokens is not None:
+            logprobs = whole.as_strided(tokens.shape, (1,) if tokens.dim() == 1 else (given, 1), at)
     else:
         logprobs, entropy, ids, best = out
         if (logprobs is None) != (tokens is None):
@@ -1000,10 +1033,9 @@ def token_logprobs(logits, tokens=None, top=0, out=None, workspace=None):
         if (tokens is not None and logprobs.shape != tokens.shape) or entropy.shape != (T,) or ids.shape != (T, top) or \
                 best.shape != (T, top):
             raise ValueError(f"out must be log probabilities shaped as the tokens, {(T,)}, {(T, top)} and {(T, top)}")
-        _same_device(logits, entropy, ids, best)
-    if tokens is not None:
-        _same_device(logits, tokens, logprobs)
-    ws, ws_bytes = _workspace(workspace, token_logprobs_workspace_bytes(T, V, top, logits.dtype), logits)
+        _same_device(logits, entropy, ids, best, *(() if tokens is None else (logprobs,)))
+    need = token_logprobs_workspace_bytes(T, V, top, logits.dtype)
+    ws, ws_bytes = (None, 0) if workspace is None and not need else _workspace(workspace, need, logits)
     _launch("mx_token_logprobs", logits, logits.data_ptr(), tokens.data_ptr() if given else None,
             logprobs.data_ptr() if given else None, entropy.data_ptr(), ids.data_ptr() if top else None,
             best.data_ptr() if top else None, T, V, stride, given, top, _LOGIT_DTYPES[logits.dtype], ws, ws_bytes)

@@ -12,17 +12,15 @@ def norm_rope(x, w, table, positions, eps, neighbours=False):
     on the device's roundings needs).  Tokens whose position is no row of the table are NaN."""
     x, w, table = x.detach().cpu().double(), w.detach().cpu().double(), table.detach().cpu().double()
     half = table.shape[1] // 2
-    out = torch.full(x.shape, float("nan"), dtype=torch.float64)
-    weight = torch.zeros_like(x)
-    for t, p in enumerate(positions):
-        if not 0 <= p < table.shape[0]:
-            continue
-        y = x[t] / torch.sqrt((x[t] ** 2).mean(1, keepdim=True) + eps) * w
-        out[t], weight[t] = y, y.abs()
-        for i in range(half):
-            a, b = (2 * i, 2 * i + 1) if neighbours else (i, i + half)
-            c, s = table[p, i], table[p, half + i]
-            out[t, :, a], out[t, :, b] = y[:, a] * c - y[:, b] * s, y[:, b] * c + y[:, a] * s
-            weight[t, :, a] = (y[:, a] * c).abs() + (y[:, b] * s).abs()
-            weight[t, :, b] = (y[:, b] * c).abs() + (y[:, a] * s).abs()
+    there = torch.tensor([0 <= p < table.shape[0] for p in positions])
+    at = table[torch.tensor([p if 0 <= p < table.shape[0] else 0 for p in positions])]
+    y = x / torch.sqrt((x ** 2).mean(2, keepdim=True) + eps) * w
+    out, weight = y.clone(), y.abs()
+    for i in range(half):
+        a, b = (2 * i, 2 * i + 1) if neighbours else (i, i + half)
+        c, s = at[:, None, i], at[:, None, half + i]
+        out[..., a], out[..., b] = y[..., a] * c - y[..., b] * s, y[..., b] * c + y[..., a] * s
+        weight[..., a] = (y[..., a] * c).abs() + (y[..., b] * s).abs()
+        weight[..., b] = (y[..., b] * c).abs() + (y[..., a] * s).abs()
+    out[~there] = float("nan")
     return out, weight

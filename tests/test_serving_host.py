@@ -64,8 +64,8 @@ def test_logprob_slices(tmp_path):
         const bool whole = (long long)p.slices * p.per >= blocks, used = p.slices == 1 || (p.slices - 1LL) * p.per < blocks;
         if (!whole || !used || p.slices < 1 || p.slices > kMostSlices || p.per < 1) printf("plan(%d, %d, %d)\n", T, V, dtype);
       }
-  printf("%d\n", plan(1, 32000, MX_DTYPE_BF16).slices > 1);""")
-    assert out == ["1"]
+  printf("%d %d\n", plan(1, 32000, MX_DTYPE_BF16).threads, plan(1, 50000, MX_DTYPE_BF16).slices > 1);""")
+    assert out == ["1024 1"]
 
 
 def test_workspaces():
