@@ -557,8 +557,7 @@ __global__ __launch_bounds__(64 * NW, rows_per_cu(NR, D)) void rows_kernel(const
 // 16x16x32 MFMAs: for the same products 32x32x16 ones read and write twice the
 // accumulator registers, and the power that takes costs clock.
 // ---------------------------------------------------------------------------
-constexpr int TW = 8;           // waves
-constexpr int TR = 32 * TW;     // rows of a workgroup
+constexpr int TR = 32 * 8;      // rows of a workgroup of 8 waves
 constexpr int BN = 64;          // keys of a tile
 constexpr int kOdd = 1 << 30;   // in a row's token number: its query holds an infinity or a NaN
 // Log2 units that a score may pass the running maximum by before it moves.  f16: what P' has of its
@@ -588,11 +587,11 @@ __device__ __forceinline__ int v_slot(int row, int slot) { return slot ^ ((row >
 // WIDE: pages of 64 tokens and more.  A tile then has one page, whose address the scalar unit
 // works out; its threads add an offset that never changes (3 x 2048 rows on 4096 tokens 281 us,
 // 290 with pages of 16).  For d = 64 the other form serves every page: 209..212 us, 216..219 this way.
-template <typename T, int D, bool WIDE, Mode MODE>
+template <typename T, int D, bool WIDE, Mode MODE, int TW>
 __global__ __launch_bounds__(64 * TW, 2) void tile_kernel(const Args a) {
   using L = Stage<D>;
   constexpr int KC = D / 32, DT = D / 16;
-  constexpr int NT = 64 * TW;
+  constexpr int NT = 64 * TW, TR = 32 * TW;
   constexpr int U = D * 8 / NT;  // 16-byte units of a tile (K, then V) per thread
   constexpr float TOP = lift<T>() > 0.f ? lift<T>() : lazy<T>();  // a larger log2 P' moves the maximum,
   constexpr float LEVEL = TOP - lazy<T>();                        // to here
@@ -1184,6 +1183,7 @@ struct Plan {
   int nr;       // 16-row blocks of the rows kernel; 0: the tile kernel
   int tiles;    // 256-row tiles of the tile kernel
   int splits, chunk;
+  int waves = 8;  // of a workgroup of the tile kernel
 };
 
 static long long up(long long x, long long to) { return (x + to - 1) / to; }
@@ -1229,16 +1229,31 @@ static int launch_rows(const Args& a, hipStream_t s) {
 }
 
 constexpr int kMostWords = 32;  // 32-bit words of a TREE's mask
-template <typename T, int D, bool WIDE, Mode MODE>
+template <typename T, int D, bool WIDE, Mode MODE, int TW>
 static int launch_tiles(const Args& a, const Plan& p, hipStream_t s) {
-  // TREE: with the masks of the tokens that TR rows may belong to
-  constexpr int most = Stage<D>::LDS + (MODE == TREE ? TR * kMostWords * 4 : 0);
-  const int lds = Stage<D>::LDS + (MODE == TREE ? ((TR - 2) / (a.n_q / a.n_kv) + 2) * a.words * 4 : 0);
-  MX_RETURN_IF_HIP((lds_limit_once<tile_kernel<T, D, WIDE, MODE>>(most)));
-  hipLaunchKernelGGL((tile_kernel<T, D, WIDE, MODE>), dim3((unsigned)(a.B * a.n_kv), (unsigned)p.tiles, (unsigned)a.splits),
+  // TREE: with the masks of the tokens that the rows may belong to
+  constexpr int most = Stage<D>::LDS + (MODE == TREE ? 32 * TW * kMostWords * 4 : 0);
+  const int lds = Stage<D>::LDS + (MODE == TREE ? ((32 * TW - 2) / (a.n_q / a.n_kv) + 2) * a.words * 4 : 0);
+  MX_RETURN_IF_HIP((lds_limit_once<tile_kernel<T, D, WIDE, MODE, TW>>(most)));
+  hipLaunchKernelGGL((tile_kernel<T, D, WIDE, MODE, TW>), dim3((unsigned)(a.B * a.n_kv), (unsigned)p.tiles, (unsigned)a.splits),
                      dim3(64 * TW), (unsigned)lds, s, a);
   MX_RETURN_IF_HIP(hipGetLastError());
   return MX_OK;
+}
+
+// The plan of a tree: up to 256 rows of 64 channels take workgroups of 4 waves, two of which a CU holds (33 sequences of up to
+// 2000 tokens, 16 heads with up to 100 rows each 87 -> 62 us, with up to 50 83 -> 53; 128 channels' stages fill a CU with one:
+// one workgroup of 8 waves).
+static Plan tree_plan(int B, int T, int max_q, int max_kv, int n_q, int n_kv, int d) {
+  Plan p = plan(B, T, max_q, max_kv, n_q, n_kv, d);
+  const long long rows = (long long)(max_q < T ? max_q : T) * (n_q / n_kv), heads = (long long)B * n_kv;
+  if (p.nr || rows > 256 || d != 64) return p;
+  p.waves = 4;
+  p.tiles = (int)up(rows, 128);
+  const long long chunk = up(up(max_kv, up(512, heads * p.tiles)), 128) * 128;
+  p.splits = (int)std::min(up(max_kv, chunk), 65535LL);
+  p.chunk = (int)std::min(chunk, 0x40000000LL);
+  return p;
 }
 
 template <typename T, int D, Mode MODE>
@@ -1246,8 +1261,9 @@ static int run(const Args& a, const Plan& p, hipStream_t s) {
   const bool wide = a.lp >= 6;
   const int rc = p.nr == 1   ? (wide ? launch_rows<T, D, 1, true, MODE>(a, s) : launch_rows<T, D, 1, false, MODE>(a, s))
                  : p.nr == 2 ? (wide ? launch_rows<T, D, 2, true, MODE>(a, s) : launch_rows<T, D, 2, false, MODE>(a, s))
-                 : wide && D == 128 ? launch_tiles<T, D, D == 128, MODE>(a, p, s)
-                                    : launch_tiles<T, D, false, MODE>(a, p, s);
+                 : p.waves == 4     ? launch_tiles<T, D, false, MODE, MODE == TREE && D == 64 ? 4 : 8>(a, p, s)
+                 : wide && D == 128 ? launch_tiles<T, D, D == 128, MODE, 8>(a, p, s)
+                                    : launch_tiles<T, D, false, MODE, 8>(a, p, s);
   if (rc != MX_OK || p.splits == 1) return rc;
   const long long rows = (long long)a.T * a.n_q;
   // few rows: the splits of a row side by side; many: few splits each (of 16384 rows in 2

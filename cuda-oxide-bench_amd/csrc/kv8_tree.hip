@@ -5,7 +5,7 @@
 extern "C" size_t mx_gqa_kv8_tree_workspace(int B, int T, int max_q, int max_kv, int n_q, int n_kv, int d) {
   using namespace mx::kv8;
   if (!sizes_ok(B, T, max_q, max_kv, n_q, n_kv, d)) return 0;
-  return workspace_of(plan(B, T, max_q, max_kv, n_q, n_kv, d), T, n_q, d);
+  return workspace_of(tree_plan(B, T, max_q, max_kv, n_q, n_kv, d), T, n_q, d);
 }
 
 extern "C" int mx_gqa_kv8_tree(const void* q, const void* k_cache, const void* v_cache, const float* k_scale,
@@ -20,7 +20,7 @@ extern "C" int mx_gqa_kv8_tree(const void* q, const void* k_cache, const void* v
   if (rc != MX_OK) return rc;
   if (words < 1 || 2 * words > kMostWords) return MX_ERR_SHAPE;
   if ((uintptr_t)tree & 7) return MX_ERR_ALIGN;
-  const Plan p = plan(B, T, max_q, max_kv, n_q, n_kv, d);
+  const Plan p = tree_plan(B, T, max_q, max_kv, n_q, n_kv, d);
   const Args a{(const uint16_t*)q, (const uint8_t*)k_cache, (const uint8_t*)v_cache, k_scale, v_scale, page_table, kv_lens,
                cu, (uint16_t*)O, (float*)workspace, B, T, n_q, n_kv, pages, max_pages, q_stride, log2_page(page), 1,
                p.splits, p.chunk, scale * kLog2e, 0, 0, (const uint32_t*)tree, 2 * words};
