@@ -1102,10 +1102,20 @@ __global__ __launch_bounds__(64 * TW, 2) void tile_kernel(const Args a) {
       if ((tok[i] & kOdd) && !none) total = __builtin_nanf("");
       if (a.splits == 1) {
         const float inv = none ? 0.f : 1.0f / total;
+        // two fragments' channels change places between neighbouring lane groups: 16 bytes a store
 #pragma unroll
-        for (int d = 0; d < DT; ++d)
-          st64(a.out + orow * D + 16 * d + 4 * g, u32x2{T::pack2(acc[i][d][0] * inv, acc[i][d][1] * inv),
-                                                        T::pack2(acc[i][d][2] * inv, acc[i][d][3] * inv)});
+        for (int d = 0; d < DT; d += 2) {
+          u32x4 o;
+#pragma unroll
+          for (int w = 0; w < 2; ++w) {
+            const auto x = __builtin_amdgcn_permlane16_swap(T::pack2(acc[i][d][2 * w] * inv, acc[i][d][2 * w + 1] * inv),
+                                                            T::pack2(acc[i][d + 1][2 * w] * inv, acc[i][d + 1][2 * w + 1] * inv),
+                                                            false, false);
+            o[w] = x[0];
+            o[2 + w] = x[1];
+          }
+          st128(a.out + orow * D + 16 * d + 16 * (g & 1) + 8 * (g >> 1), o);
+        }
       } else {
         const size_t all = (size_t)a.T * a.n_q;
         float* p = a.part + ((size_t)split * all + orow) * D;
