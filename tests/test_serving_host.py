@@ -29,7 +29,7 @@ BAD = [
         *[({i: None}, _lib.MX_ERR_NULL) for i in range(8)], *[({i: 0}, _lib.MX_ERR_SHAPE) for i in range(8, 14)],
         ({11: 40}, _lib.MX_ERR_SHAPE), ({11: 272, 12: 16}, _lib.MX_ERR_SHAPE), ({12: 80}, _lib.MX_ERR_SHAPE),
         ({12: 24}, _lib.MX_ERR_SHAPE), ({14: 248}, _lib.MX_ERR_SHAPE), ({15: 120}, _lib.MX_ERR_SHAPE),
-        ({16: 248}, _lib.MX_ERR_SHAPE), ({17: 120}, _lib.MX_ERR_SHAPE), ({9: 2 ** 26}, _lib.MX_ERR_SHAPE),
+        ({16: 248}, _lib.MX_ERR_SHAPE), ({17: 120}, _lib.MX_ERR_SHAPE), ({9: 2 ** 26}, _lib.MX_ERR_SHAPE), ({8: 2 ** 29}, _lib.MX_ERR_SHAPE),
         *[({i: 516}, _lib.MX_ERR_ALIGN) for i in (14, 15, 16, 17)],
         *[({i: U}, _lib.MX_ERR_ALIGN) for i in (0, 1, 2, 3, 4, 6, 7)], ({5: V}, _lib.MX_ERR_ALIGN),
         ({20: 2}, _lib.MX_ERR_DTYPE), ({6: P[1]}, _lib.MX_ERR_ALIAS), ({7: P[0]}, _lib.MX_ERR_ALIAS),
