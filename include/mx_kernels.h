@@ -463,7 +463,7 @@ size_t mx_gqa_kv8_tree_workspace(int B, int T, int max_q, int max_kv, int n_q, i
  * projection); weights of the same type; table [rows, rot] fp32; positions [T] int32 on
  * the device.  A token whose position is outside 0..rows-1 is left as it is (in q_out and k_out).
  * q_out may be q and k_out k (same pointer and stride); any other overlap of an
- * output with an input or the other output returns MX_ERR_ALIAS.  x^2 is summed in fp32: a head whose
+ * output with q, k or the other output returns MX_ERR_ALIAS.  x^2 is summed in fp32: a head whose
  * squares pass 2^128 becomes zeros (NaN where it holds an infinity or a NaN).
  * d a multiple of 16 up to 256, rot a multiple of 16 up to d; T * (n_q + n_kv) < 2^31; strides % 8 == 0,
  * 16-byte aligned pointers (positions: 4).

@@ -76,18 +76,17 @@ def test_alignment(ops, dtype):
         check(ops, x.contiguous(), tokens_of(4, 4090, 1, off), 6, dev=big.cuda()[:, off:off + 4090])
 
 
-@pytest.mark.parametrize("T", [2, 600])
-def test_ties(ops, T):
-    """Rows of one value, of few values, zeros of both signs: the lowest ids first, whichever slice holds them."""
-    announce(f"token_logprobs ties T{T}")
-    V = 33000
+@pytest.mark.parametrize("T,V", [(2, 33000), (2, 32999), (2, 30001), (600, 33000)])
+def test_ties(ops, T, V):
+    """Rows of one value, of few values, zeros of both signs: the lowest ids first, whichever wave or slice holds them."""
+    announce(f"token_logprobs ties T{T} V{V}")
     x = torch.zeros((T, V), dtype=BF16)
     x[0] = -0.0
     x[0, 100::7] = 0.0
     x[1] = torch.randint(0, 3, (V,), generator=torch.Generator().manual_seed(1)).to(BF16)
     check(ops, x, tokens_of(T, V, 2, 2), 32)
     y = logits_of(2, V, BF16, 3, 0.5)
-    y[:, [0, 8191, 8192, 16384, 32767, 32999]] = 9.0
+    y[:, [0, 8191, 8192, 16384, V - 5, V - 1]] = 9.0
     check(ops, y, tokens_of(2, V, 2, 2), 9)
 
 
@@ -125,6 +124,16 @@ def test_tokens(ops):
     check(ops, x, None, 2)
     check(ops, x, torch.zeros((3, 0), dtype=torch.int32), 2)
     check(ops, x, tokens_of(3, 1000, 100, 1), 2)
+
+
+def test_rows_far_apart(ops):
+    """Offsets past 2^31 logits."""
+    announce("token_logprobs rows far apart")
+    stride = 1_200_000_007
+    big = torch.empty(2 * stride + 5000, dtype=BF16, device="cuda").as_strided((3, 5000), (stride, 1))
+    x = logits_of(3, 5000, BF16, 11)
+    big.copy_(x)
+    check(ops, x, tokens_of(3, 5000, 2, 1), 4, dev=big)
 
 
 def test_sharp_rows(ops):

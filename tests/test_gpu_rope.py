@@ -106,6 +106,21 @@ def test_special_values(ops):
     assert bool(((q[:, [1, 2, 5]].double() - exp).abs() <= bound(exp, weight, d, BF16)).all())
 
 
+def test_rows_far_apart(ops):
+    """Offsets past 2^31 values, in and out."""
+    announce("qk_norm_rope rows far apart")
+    stride = 1_200_000_000
+    big = torch.empty(2 * stride + 4096, dtype=BF16, device="cuda")
+    q, k = big.as_strided((3, 4, 64), (stride, 64, 1)), big.as_strided((3, 2, 64), (stride, 64, 1), 1024)
+    qc, kc = randn((3, 4, 64), 1, BF16), randn((3, 2, 64), 2, BF16)
+    q.copy_(qc)
+    k.copy_(kc)
+    w, table = randn((64,), 3, BF16), table_of(9, 64)
+    ops.qk_norm_rope(q, k, w.cuda(), w.cuda(), table.cuda(), i32([1, 8, 3]), q_out=q, k_out=k)
+    check(q, qc, w, table, [1, 8, 3], 1e-6, False)
+    check(k, kc, w, table, [1, 8, 3], 1e-6, False)
+
+
 def test_table(ops):
     """rope_table: angles in 64 bits, at far positions too."""
     t = ops.rope_table(100000, 32, 5000.0).cpu()

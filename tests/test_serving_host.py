@@ -35,6 +35,23 @@ BAD = [
         ({20: 2}, _lib.MX_ERR_DTYPE), ({6: P[1]}, _lib.MX_ERR_ALIAS), ({7: P[0]}, _lib.MX_ERR_ALIAS),
         ({6: P[0]}, _lib.MX_ERR_ALIAS),  # q's memory at another stride
         ({7: P[6]}, _lib.MX_ERR_ALIAS)]),
+    # q, kc, vc, ks, vs, table, lens, cu, O, B, T, max_q, max_kv, n_q, n_kv, d, page, pages, max_pages, ldq, scale, window,
+    # sinks, dtype, workspace, bytes, stream
+    *_calls("mx_gqa_kv8_window", [P[0]] * 9 + [2, 5, 4, 4096, 4, 2, 64, 16, 9, 300, 256, 0.1, 3000, 4, 0, P[0], 1 << 30, None], [
+        *[({i: None}, _lib.MX_ERR_NULL) for i in (0, 1, 2, 3, 4, 5, 6, 8)], ({7: None}, _lib.MX_ERR_SHAPE),
+        *[({i: 0}, _lib.MX_ERR_SHAPE) for i in range(9, 19)], ({13: 5}, _lib.MX_ERR_SHAPE), ({15: 96}, _lib.MX_ERR_SHAPE),
+        ({19: 248}, _lib.MX_ERR_SHAPE), ({19: 260}, _lib.MX_ERR_ALIGN), ({0: U}, _lib.MX_ERR_ALIGN),
+        ({21: 0}, _lib.MX_ERR_SHAPE), ({21: -1}, _lib.MX_ERR_SHAPE), ({22: -1}, _lib.MX_ERR_SHAPE),
+        ({23: 2}, _lib.MX_ERR_DTYPE), ({24: None}, _lib.MX_ERR_WORKSPACE), ({25: 1000}, _lib.MX_ERR_WORKSPACE),
+        ({24: U}, _lib.MX_ERR_ALIGN)]),
+    # q, kc, vc, ks, vs, table, lens, cu, tree, O, B, T, max_q, max_kv, n_q, n_kv, d, page, pages, max_pages, ldq, scale,
+    # words, dtype, workspace, bytes, stream
+    *_calls("mx_gqa_kv8_tree", [P[0]] * 10 + [2, 5, 4, 4096, 4, 2, 64, 16, 9, 300, 256, 0.1, 1, 0, P[0], 1 << 30, None], [
+        *[({i: None}, _lib.MX_ERR_NULL) for i in (0, 1, 2, 3, 4, 5, 6, 8, 9)], ({7: None}, _lib.MX_ERR_SHAPE),
+        *[({i: 0}, _lib.MX_ERR_SHAPE) for i in range(10, 20)], ({14: 5}, _lib.MX_ERR_SHAPE), ({16: 96}, _lib.MX_ERR_SHAPE),
+        ({20: 248}, _lib.MX_ERR_SHAPE), ({20: 260}, _lib.MX_ERR_ALIGN), ({8: U}, _lib.MX_ERR_ALIGN),
+        ({22: 0}, _lib.MX_ERR_SHAPE), ({22: 17}, _lib.MX_ERR_SHAPE), ({23: 2}, _lib.MX_ERR_DTYPE),
+        ({24: None}, _lib.MX_ERR_WORKSPACE), ({25: 1000}, _lib.MX_ERR_WORKSPACE), ({24: U}, _lib.MX_ERR_ALIGN)]),
     # logits, tokens, logprob, entropy, ids, top_logprob, T, V, stride, given, top, dtype, workspace, bytes, stream
     *_calls("mx_token_logprobs", [*P[:6], 3, 50000, 50000, 2, 5, 0, P[6], 1 << 24, None], [
         *[({i: None}, _lib.MX_ERR_NULL) for i in range(6)], ({6: 0}, _lib.MX_ERR_SHAPE), ({7: 0}, _lib.MX_ERR_SHAPE),
@@ -68,7 +85,50 @@ def test_logprob_slices(tmp_path):
     assert out == ["1024 1"]
 
 
+def test_attention_plans(tmp_path):
+    """Windows and trees over many sizes: the splits cover what a block of rows may visit and none starts behind it, a chunk is
+    whole tiles where there are several, and a tree's workgroups hold its rows."""
+    window = query(tmp_path, "kv8_window.hip", r"""
+  using namespace mx::kv8;
+  for (int B : {1, 3, 64, 4096})
+    for (int T : {1, 17, 33, 1000, 100000})
+      for (int kv : {1, 255, 1000, 8192, 1 << 30})
+        for (int G : {1, 4, 48})
+          for (int w : {1, 64, 1000, 4096, 2147483647})
+            for (int s : {0, 4, 200, 2147483647}) {
+              const int d = T % 2 ? 64 : 128;
+              const Plan p = window_plan(B, T, T, kv, 2 * G, 2, d, w, s);
+              const long long view = std::min<long long>(kv, 64 * (up(s, 64) + up((long long)w + std::min(T, 32) + 62, 64)));
+              const bool whole = p.splits >= 1 && p.splits <= 65535 && p.chunk >= 1 && (p.splits == 1 || p.chunk % 64 == 0);
+              if (!whole || (p.splits > 1 && (long long)(p.splits - 1) * p.chunk >= view))
+                printf("window_plan(%d, %d, %d, %d, %d, %d)\n", B, T, kv, G, w, s);
+            }
+  printf("ok\n");""")
+    tree = query(tmp_path, "kv8_tree.hip", r"""
+  using namespace mx::kv8;
+  for (int B : {1, 3, 64, 4096})
+    for (int T : {1, 17, 33, 64, 100, 257, 100000})
+      for (int kv : {1, 255, 1000, 8192, 1 << 30})
+        for (int G : {1, 4, 48})
+          for (int d : {64, 128}) {
+            const Plan p = tree_plan(B, T, T, kv, 2 * G, 2, d);
+            const long long rows = (long long)T * G;
+            const bool fits = p.nr ? rows <= 16 * p.nr : p.tiles == std::min(up(rows, 32 * p.waves), 65535LL);
+            const bool whole = p.splits >= 1 && p.splits <= 65535 && p.chunk >= 1 && (p.splits == 1 || p.chunk % 64 == 0);
+            if (!fits || !whole || (p.splits > 1 && (long long)(p.splits - 1) * p.chunk >= kv) || (p.waves == 4 && d != 64))
+              printf("tree_plan(%d, %d, %d, %d, %d)\n", B, T, kv, G, d);
+          }
+  printf("ok\n");""")
+    assert window == ["ok"] and tree == ["ok"]
+
+
 def test_workspaces():
-    f = _lib.load().mx_token_logprobs_workspace
+    lib = _lib.load()
+    assert lib.mx_gqa_kv8_window_workspace(1, 1, 1, 100000, 32, 8, 128, 512, 4) > 0
+    assert lib.mx_gqa_kv8_window_workspace(1, 1, 1, 100000, 32, 8, 64, 1000, 4) == 0  # one workgroup
+    assert lib.mx_gqa_kv8_window_workspace(1, 1, 1, 100000, 32, 8, 128, 0, 4) == 0
+    assert lib.mx_gqa_kv8_tree_workspace(1, 13, 13, 1001, 32, 8, 128) > 0
+    assert lib.mx_gqa_kv8_tree_workspace(1, 13, 13, 1001, 31, 8, 128) == 0
+    f = lib.mx_token_logprobs_workspace
     assert f(1000, 50000, 5, 0) == 0 and f(1, 100, 5, 0) == 0 and f(2, 50000, 5, 0) > 0
     assert [f(*a) for a in ((0, 50000, 5, 0), (1, 0, 0, 0), (1, 50000, 33, 0), (1, 50000, 5, 4))] == [0] * 4
