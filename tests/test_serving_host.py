@@ -4,6 +4,7 @@ from __future__ import annotations
 import ctypes
 
 import pytest
+import torch
 
 from conftest import import_submodule
 from host_query import query
@@ -132,3 +133,26 @@ def test_workspaces():
     f = lib.mx_token_logprobs_workspace
     assert f(1000, 50000, 5, 0) == 0 and f(1, 100, 5, 0) == 0 and f(2, 50000, 5, 0) > 0
     assert [f(*a) for a in ((0, 50000, 5, 0), (1, 0, 0, 0), (1, 50000, 33, 0), (1, 50000, 5, 4))] == [0] * 4
+
+
+def test_operators_refuse_before_the_device():
+    """Types and devices that the operators check by themselves: CPU tensors reach no kernel."""
+    ops = import_submodule("ops")
+    q, k, w = torch.zeros(2, 4, 64), torch.zeros(2, 1, 64), torch.ones(64)
+    table, places = ops.rope_table(8, 32, device="cpu"), torch.zeros(2, dtype=torch.int32)
+    bf = torch.bfloat16
+    for call in (lambda: ops.qk_norm_rope(q.to(bf), k.to(bf), w.to(bf), w.to(bf), table, places),
+                 lambda: ops.token_logprobs(w[None]), lambda: ops.token_logprobs(w[None].to(bf), places[:1], top=3)):
+        with pytest.raises(ValueError, match="HIP device"):
+            call()
+    for call in (lambda: ops.qk_norm_rope(q, k, w, w, table, places), lambda: ops.token_logprobs(places[None]),
+                 lambda: ops.token_logprobs([1.0]), lambda: ops.gqa_kv8_window(q.to(bf), None, places, places, 4),
+                 lambda: ops.gqa_kv8_tree(q.to(bf), None, places, places, places)):
+        with pytest.raises(TypeError):
+            call()
+    for window, sinks in ((0, 0), (-1, 0), (1 << 31, 0), (4, -1), (4, 1 << 31)):
+        with pytest.raises(ValueError, match="window"):
+            ops.gqa_kv8_window(q.to(bf), None, places, places, window, sinks)
+    for positions, rot in ((0, 32), (8, 24), (8, 0)):
+        with pytest.raises(ValueError, match="multiple of 16"):
+            ops.rope_table(positions, rot, device="cpu")
