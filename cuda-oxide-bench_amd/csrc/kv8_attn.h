@@ -249,7 +249,9 @@ __global__ __launch_bounds__(64 * NW, rows_per_cu(NR, D)) void rows_kernel(const
   const int k_key = 16 * (r16 >> 2) + (r16 & 3);
   const uint32_t k_off = (uint32_t)(k_key * D + g * (D / 4)), v_off = (uint32_t)(r16 * P + 16 * g);
 
-  for (int r0 = 0; r0 < n * G; r0 += 16 * NR) {
+  // with masks the grid may have workgroups for blocks of rows side by side
+  const int r_first = MODE != PLAIN ? (int)blockIdx.z * 16 * NR : 0, r_step = MODE != PLAIN ? (int)gridDim.z * 16 * NR : 16 * NR;
+  for (int r0 = r_first; r0 < n * G; r0 += r_step) {
     // ---- this block's rows ----
     u32x4 qf[NR][KC];
     int limit[NR];  // keys that the lane's row sees: t < limit
@@ -359,7 +361,7 @@ __global__ __launch_bounds__(64 * NW, rows_per_cu(NR, D)) void rows_kernel(const
     };
 
     int tile = first_tile + wave;
-    if (MODE == WINDOW || r0 > 0) {
+    if (MODE == WINDOW || r0 > r_first) {
       now = ids_of(tile);
       next = ids_of(tile + NW);
     }
@@ -1194,11 +1196,12 @@ struct Plan {
   int tiles;    // 256-row tiles of the tile kernel
   int splits, chunk;
   int waves = 8;  // of a workgroup of the tile kernel
+  int blocks = 1;  // of rows side by side in the rows kernel
 };
 
 static long long up(long long x, long long to) { return (x + to - 1) / to; }
 
-// The rows kernel up to 32 rows a KV head, else the tile kernel.  The keys are split
+// The rows kernel up to 32 rows a KV head, else the tile kernel (but see side_by_side).  The keys are split
 // where there are fewer workgroups than CUs.  A split costs its workgroup's start and
 // end, some 250 tokens' worth, and the combine's launch, so chunks are as long as the GPU
 // stays filled: rows kernel, one workgroup per CU while sequences times KV heads are
@@ -1229,11 +1232,32 @@ static Plan plan(int B, int T, int max_q, int max_kv, int n_q, int n_kv, int d) 
   return p;
 }
 
+// With masks, whether more than 32 rows take the rows kernel in blocks of 32 side by side, and the plan for that.  They do
+// where the blocks fit the CUs in one round, and from 512 tokens on also in two rounds (64 channels) or where there are but two
+// blocks: a tile of 256 rows then leaves waves without rows or CUs without work.  Trees, us in tiles and so: 128
+// channels, 1 sequence of 1001 tokens with 52 rows 17.4 and 15.1, of 500 with 480 rows 25.2 and 14.2, 16 of 1001 with 52
+// 28.2 and 18.9, 64 of 2000 with 52 101 and 80, but 16 of 4096 with 128 (two rounds) 66 and 84; 64 channels, 32 of 2000
+// with 128 43.7 and 37.0, 64 of 1500 with 128 (four rounds) 46 and 59, 64 of 300 with 64 17.0 and 19.4.  Windows of 2048, 64 of
+// 64 rows: 128 channels 127 and 130, 64 channels 110 and 61.
+static bool side_by_side(Plan& p, long long rows, long long heads, int max_kv, int d) {
+  const long long blocks = up(rows, 32), fit = 256 * rows_per_cu(2, d);  // workgroups that the CUs hold
+  const bool many = heads * blocks > (d == 64 ? 2 * fit : fit);
+  if (heads * blocks > fit && (max_kv < 512 || (blocks > 2 && many))) return false;
+  p.nr = 2;
+  p.blocks = (int)blocks;
+  const long long parts = std::max(fit / (heads * blocks), 1LL);
+  const long long chunk = (long long)max_kv * d <= 65536 ? max_kv : up(up(max_kv, parts), 256) * 256;
+  p.splits = (int)std::min(up(max_kv, chunk), 65535LL);
+  p.chunk = (int)std::min(chunk, 0x40000000LL);
+  return true;
+}
+
 template <typename T, int D, int NR, bool WIDE, Mode MODE>
-static int launch_rows(const Args& a, hipStream_t s) {
+static int launch_rows(const Args& a, int blocks, hipStream_t s) {
   constexpr int lds = NW * NR * (16 * 2 * 4 + (D / 16) * 64 * 16);
   MX_RETURN_IF_HIP((lds_limit_once<rows_kernel<T, D, NR, WIDE, MODE>>(lds)));
-  hipLaunchKernelGGL((rows_kernel<T, D, NR, WIDE, MODE>), dim3((unsigned)(a.B * a.n_kv), (unsigned)a.splits), dim3(64 * NW), lds, s, a);
+  hipLaunchKernelGGL((rows_kernel<T, D, NR, WIDE, MODE>), dim3((unsigned)(a.B * a.n_kv), (unsigned)a.splits, (unsigned)blocks),
+                     dim3(64 * NW), lds, s, a);
   MX_RETURN_IF_HIP(hipGetLastError());
   return MX_OK;
 }
@@ -1257,7 +1281,7 @@ static int launch_tiles(const Args& a, const Plan& p, hipStream_t s) {
 static Plan tree_plan(int B, int T, int max_q, int max_kv, int n_q, int n_kv, int d) {
   Plan p = plan(B, T, max_q, max_kv, n_q, n_kv, d);
   const long long rows = (long long)(max_q < T ? max_q : T) * (n_q / n_kv), heads = (long long)B * n_kv;
-  if (p.nr || rows > 256 || d != 64) return p;
+  if (p.nr || side_by_side(p, rows, heads, max_kv, d) || rows > 256 || d != 64) return p;
   p.waves = 4;
   p.tiles = (int)up(rows, 128);
   const long long chunk = up(up(max_kv, up(512, heads * p.tiles)), 128) * 128;
@@ -1269,8 +1293,8 @@ static Plan tree_plan(int B, int T, int max_q, int max_kv, int n_q, int n_kv, in
 template <typename T, int D, Mode MODE>
 static int run(const Args& a, const Plan& p, hipStream_t s) {
   const bool wide = a.lp >= 6;
-  const int rc = p.nr == 1   ? (wide ? launch_rows<T, D, 1, true, MODE>(a, s) : launch_rows<T, D, 1, false, MODE>(a, s))
-                 : p.nr == 2 ? (wide ? launch_rows<T, D, 2, true, MODE>(a, s) : launch_rows<T, D, 2, false, MODE>(a, s))
+  const int rc = p.nr == 1   ? (wide ? launch_rows<T, D, 1, true, MODE>(a, p.blocks, s) : launch_rows<T, D, 1, false, MODE>(a, p.blocks, s))
+                 : p.nr == 2 ? (wide ? launch_rows<T, D, 2, true, MODE>(a, p.blocks, s) : launch_rows<T, D, 2, false, MODE>(a, p.blocks, s))
                  : p.waves == 4     ? launch_tiles<T, D, false, MODE, MODE == TREE && D == 64 ? 4 : 8>(a, p, s)
                  : wide && D == 128 ? launch_tiles<T, D, D == 128, MODE, 8>(a, p, s)
                                     : launch_tiles<T, D, false, MODE, 8>(a, p, s);

@@ -47,13 +47,22 @@ def compare(cache, oc, q, table, lens, news, seen, out, scale=None):
     assert bool(ok.all()), f"{int((~ok).sum())} of {ok.numel()} outputs are off, by up to {float(off.nan_to_num().max())}"
 
 
+def crowd(table, lens, news, empty):
+    """With that many empty sequences behind them: so many more workgroups that rows past 32 a KV head go to the tile kernel."""
+    return table + [[-1] * len(table[0])] * empty, lens + [0] * empty, news + [0] * empty
+
+
 def run_window(ops, cache, q, table, lens, news, window, sinks, oc=None, scale=None, **hints):
     oc = oc or oracle.Cache(cache.k, cache.v, cache.k_scale, cache.v_scale)
     out = torch.full(q.shape, float("nan"), dtype=q.dtype, device="cuda")
     more = {} if news == [1] * len(news) else {"cu_q": i32(prefix(news)), "max_q": max(max(news), 1)}
     ops.gqa_kv8_window(q.cuda(), cache, i32(table), i32(lens), window, sinks, scale=scale, out=out, **{**more, **hints})
     compare(cache, oc, q, table, lens, news, in_window(lens, news, window, sinks), out, scale)
-    return out
+    if max(news) * q.shape[1] > 32 * cache.k.shape[1] and not hints:
+        t, l, n = crowd(table, lens, news, 600)
+        tiles = torch.full(q.shape, float("nan"), dtype=q.dtype, device="cuda")
+        ops.gqa_kv8_window(q.cuda(), cache, i32(t), i32(l), window, sinks, i32(prefix(n)), max(news), 300, scale, tiles)
+        compare(cache, oc, q, table, lens, news, in_window(lens, news, window, sinks), tiles, scale)
 
 
 def run_tree(ops, cache, q, table, lens, news, masks, words=None, oc=None, scale=None, **hints):
@@ -64,7 +73,11 @@ def run_tree(ops, cache, q, table, lens, news, masks, words=None, oc=None, scale
                      **{"max_q": max(news), **hints}, scale=scale, out=out)
     cut = [[r & (1 << 64 * words) - 1 for r in seq] for seq in masks]
     compare(cache, oc, q, table, lens, news, in_tree(lens, news, cut), out, scale)
-    return out
+    if max(news) * q.shape[1] > 32 * cache.k.shape[1] and not hints:
+        t, l, n = crowd(table, lens, news, 600)
+        tiles = torch.full(q.shape, float("nan"), dtype=q.dtype, device="cuda")
+        ops.gqa_kv8_tree(q.cuda(), cache, i32(t), i32(l), words_of(masks, words), i32(prefix(n)), max(news), 300, scale, tiles)
+        compare(cache, oc, q, table, lens, news, in_tree(lens, news, cut), tiles, scale)
 
 
 def random_masks(rng, news):
@@ -130,6 +143,29 @@ def test_window_split_keys(ops, max_q, d, page):
         run_window(ops, cache, q, table, lens, news, 4000, 130, oc, 0.02, max_q=300)
 
 
+@pytest.mark.parametrize("d,page", [(128, 64), (64, 16), (128, 32)])
+def test_split_keys_of_tiles(ops, d, page):
+    """Long contexts of 256 rows a KV head among sequences that are empty: the keys are split in the tile kernel."""
+    announce(f"window and tree split tiles d{d} page{page}")
+    lens, news, empty = [5000, 3001, 90], [64, 33, 1], 137
+    cache = filled(ops, sum(-(-n // page) for n in lens) + 2, 1, d, page, 60)
+    table = tables(lens, page, cache.pages, 61)
+    q = randn((sum(news), 4, d), 62, BF16)
+    oc = oracle.Cache(cache.k, cache.v, cache.k_scale, cache.v_scale)
+    t, l, n = crowd(table, lens, news, empty)
+    t, l, cu = i32(t), i32(l), i32(prefix(n))
+    assert ops.gqa_kv8_window_workspace_bytes(140, 98, 64, 5000, 4, 1, d, 2500, 100) > 0
+    assert ops.gqa_kv8_tree_workspace_bytes(140, 98, 64, 5000, 4, 1, d) > 0
+    for window, sinks in ((2500, 100), (4000, 0)):
+        out = torch.full(q.shape, float("nan"), dtype=BF16, device="cuda")
+        ops.gqa_kv8_window(q.cuda(), cache, t, l, window, sinks, cu, 64, 5000, 0.02, out)
+        compare(cache, oc, q, table, lens, news, in_window(lens, news, window, sinks), out, 0.02)
+    masks = random_masks(random.Random(9), news)
+    out = torch.full(q.shape, float("nan"), dtype=BF16, device="cuda")
+    ops.gqa_kv8_tree(q.cuda(), cache, t, l, words_of(masks, 1), cu, 64, 5000, 0.02, out)
+    compare(cache, oc, q, table, lens, news, in_tree(lens, news, masks), out, 0.02)
+
+
 @pytest.mark.parametrize("group,n", [(1, 1), (4, 3), (4, 70), (1, 200)])
 @pytest.mark.parametrize("page", [16, 64])
 def test_window_pages_out_of_view(ops, group, n, page):
@@ -161,13 +197,15 @@ def test_window_pages_out_of_view(ops, group, n, page):
 
 
 def test_window_as_plain_attention(ops):
-    """A window past every sequence: bit for bit what gqa_kv8 gives where the keys are not split."""
+    """A window past every sequence: bit for bit what gqa_kv8 gives where both take one kernel and the keys are not split."""
     announce("window as plain")
     for news, group in (([1, 1, 1], 4), ([3, 8, 1], 2), ([60, 100, 5], 4)):
         lens, page = [120, 300, 77], 16
         cache = filled(ops, 40, 2, 64, page, 13)
         table = tables(lens, page, 40, 14)
         q = randn((sum(news), 2 * group, 64), 15, BF16).cuda()
+        if max(news) * group > 32:
+            table, lens, news = crowd(table, lens, news, 600)
         args = (i32(prefix(news)), max(news))
         want = ops.gqa_kv8(q, cache, i32(table), i32(lens), *args)
         got = ops.gqa_kv8_window(q, cache, i32(table), i32(lens), 2 ** 31 - 1, 0, *args)
@@ -259,7 +297,7 @@ def test_tree_masks(ops, group, n):
 
 
 def test_tree_of_one_branch(ops):
-    """A chain is a causal mask: bit for bit what gqa_kv8 gives."""
+    """A chain is a causal mask: bit for bit what gqa_kv8 gives where both take one kernel."""
     announce("tree of one branch")
     for n, group in ((3, 4), (8, 4), (50, 8)):
         lens, news, page = [120, 300, n], [n, n, n], 64
@@ -267,6 +305,8 @@ def test_tree_of_one_branch(ops):
         table = tables(lens, page, 20, 30)
         q = randn((3 * n, 2 * group, 128), 31, BF16).cuda()
         tree = drafts.masks(list(range(-1, n - 1))).repeat(3, 1).cuda()
+        if n * group > 32:
+            table, lens, news = crowd(table, lens, news, 600)
         want = ops.gqa_kv8(q, cache, i32(table), i32(lens), i32(prefix(news)), n)
         assert torch.equal(ops.gqa_kv8_tree(q, cache, i32(table), i32(lens), tree, i32(prefix(news)), n), want)
         assert torch.equal(ops.gqa_kv8_tree(q, cache, i32(table), i32(lens), tree[:, 0].contiguous(), i32(prefix(news)), n), want)

@@ -114,11 +114,15 @@ def test_attention_plans(tmp_path):
           for (int d : {64, 128}) {
             const Plan p = tree_plan(B, T, T, kv, 2 * G, 2, d);
             const long long rows = (long long)T * G;
-            const bool fits = p.nr ? rows <= 16 * p.nr : p.tiles == std::min(up(rows, 32 * p.waves), 65535LL);
+            const bool fits = p.nr ? rows <= 16LL * p.nr * p.blocks && p.blocks <= 65535 : p.tiles == std::min(up(rows, 32 * p.waves), 65535LL);
             const bool whole = p.splits >= 1 && p.splits <= 65535 && p.chunk >= 1 && (p.splits == 1 || p.chunk % 64 == 0);
             if (!fits || !whole || (p.splits > 1 && (long long)(p.splits - 1) * p.chunk >= kv) || (p.waves == 4 && d != 64))
               printf("tree_plan(%d, %d, %d, %d, %d)\n", B, T, kv, G, d);
           }
+  for (int d : {64, 128}) {  // many sequences, of 300 tokens or of more blocks: tiles, which split long contexts
+    const Plan a = tree_plan(603, 98, 64, 300, 4, 1, d), b = tree_plan(140, 98, 64, 5000, 4, 1, d), c = tree_plan(1, 13, 13, 1001, 32, 8, d);
+    if (a.nr || a.splits != 1 || b.nr || b.splits < 2 || c.nr != 2 || c.blocks != 2) printf("d %d\n", d);
+  }
   printf("ok\n");""")
     assert window == ["ok"] and tree == ["ok"]
 
