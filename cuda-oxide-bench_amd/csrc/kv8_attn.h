@@ -1232,20 +1232,27 @@ static Plan plan(int B, int T, int max_q, int max_kv, int n_q, int n_kv, int d) 
   return p;
 }
 
-// With masks, whether more than 32 rows take the rows kernel in blocks of 32 side by side, and the plan for that.  They do
-// where the blocks fit the CUs in one round, and from 512 tokens on also in two rounds (64 channels) or where there are but two
-// blocks: a tile of 256 rows then leaves waves without rows or CUs without work.  Trees, us in tiles and so: 128
-// channels, 1 sequence of 1001 tokens with 52 rows 17.4 and 15.1, of 500 with 480 rows 25.2 and 14.2, 16 of 1001 with 52
-// 28.2 and 18.9, 64 of 2000 with 52 101 and 80, but 16 of 4096 with 128 (two rounds) 66 and 84; 64 channels, 32 of 2000
-// with 128 43.7 and 37.0, 64 of 1500 with 128 (four rounds) 46 and 59, 64 of 300 with 64 17.0 and 19.4.  Windows of 2048, 64 of
-// 64 rows: 128 channels 127 and 130, 64 channels 110 and 61.
+// With masks, whether more than 16 rows take the rows kernel in blocks side by side, and the plan for that.
+//
+// Blocks of 16, where each CU gets up to 1024 tokens of one: latency counts, and a step on 32 rows takes longer.  Trees, us in
+// blocks of 32 and so: 128 channels, 1 sequence of 1001 tokens with 28 rows 14.7 and 12.4, with 52 15.0 and 12.6, of 8192 with
+// 64 20.1 and 19.0, but of 32768 with 52 33.6 and 41.9, 4 of 4096 with 64 22.9 and 25.1.
+//
+// Blocks of 32, where they fit the CUs in one round, and from 512 tokens on also in two rounds (64 channels) or where
+// there are but two blocks: a tile of 256 rows then leaves waves without rows or CUs without work.  Trees, us in tiles and so: 128
+// channels, 16 sequences of 1001 tokens with 52 rows 28.2 and 18.9, 64 of 2000 with 52 101 and 80, but 16 of 4096 with 128
+// (two rounds) 66 and 84; 64 channels, 32 of 2000 with 128 43.7 and 37.0, 64 of 1500 with 128 (four rounds) 46 and 59,
+// 64 of 300 with 64 17.0 and 19.4.  Windows of 2048, 64 of 64 rows: 128 channels 127 and 130, 64 channels 110 and 61.
 static bool side_by_side(Plan& p, long long rows, long long heads, int max_kv, int d) {
   const long long blocks = up(rows, 32), fit = 256 * rows_per_cu(2, d);  // workgroups that the CUs hold
+  const long long small = heads * up(rows, 16);
+  const bool few = small <= 512 && small * max_kv <= 256 * 1024;
+  if (p.nr == 1 || (!few && p.nr)) return false;
   const bool many = heads * blocks > (d == 64 ? 2 * fit : fit);
-  if (heads * blocks > fit && (max_kv < 512 || (blocks > 2 && many))) return false;
-  p.nr = 2;
-  p.blocks = (int)blocks;
-  const long long parts = std::max(fit / (heads * blocks), 1LL);
+  if (!few && heads * blocks > fit && (max_kv < 512 || (blocks > 2 && many))) return false;
+  p.nr = few ? 1 : 2;
+  p.blocks = (int)(few ? up(rows, 16) : blocks);
+  const long long parts = std::max(few ? 256 / small : fit / (heads * blocks), 1LL);
   const long long chunk = (long long)max_kv * d <= 65536 ? max_kv : up(up(max_kv, parts), 256) * 256;
   p.splits = (int)std::min(up(max_kv, chunk), 65535LL);
   p.chunk = (int)std::min(chunk, 0x40000000LL);
@@ -1281,7 +1288,7 @@ static int launch_tiles(const Args& a, const Plan& p, hipStream_t s) {
 static Plan tree_plan(int B, int T, int max_q, int max_kv, int n_q, int n_kv, int d) {
   Plan p = plan(B, T, max_q, max_kv, n_q, n_kv, d);
   const long long rows = (long long)(max_q < T ? max_q : T) * (n_q / n_kv), heads = (long long)B * n_kv;
-  if (p.nr || side_by_side(p, rows, heads, max_kv, d) || rows > 256 || d != 64) return p;
+  if (side_by_side(p, rows, heads, max_kv, d) || p.nr || rows > 256 || d != 64) return p;
   p.waves = 4;
   p.tiles = (int)up(rows, 128);
   const long long chunk = up(up(max_kv, up(512, heads * p.tiles)), 128) * 128;

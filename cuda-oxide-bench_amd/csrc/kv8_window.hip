@@ -12,7 +12,7 @@ static Plan window_plan(int B, int T, int max_q, int max_kv, int n_q, int n_kv, 
   const long long rows = std::min(max_q, 32);
   const int kv = (int)std::min((long long)max_kv, 64 * (up(sinks, 64) + up(window + rows + 62, 64)));
   Plan p = plan(B, T, max_q, kv, n_q, n_kv, d);
-  if (!p.nr) side_by_side(p, (long long)std::min(max_q, T) * (n_q / n_kv), (long long)B * n_kv, kv, d);
+  side_by_side(p, (long long)std::min(max_q, T) * (n_q / n_kv), (long long)B * n_kv, kv, d);
   if (p.nr && (long long)kv * d <= 1152 * 64) {
     p.splits = 1;
     p.chunk = kv;

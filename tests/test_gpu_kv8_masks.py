@@ -36,48 +36,55 @@ def words_of(masks, words):
     return torch.tensor([[x - (1 << 64) if x >> 63 else x for x in r] for r in rows], dtype=torch.int64).cuda()
 
 
-def compare(cache, oc, q, table, lens, news, seen, out, scale=None):
+def compare(cache, oc, q, table, lens, news, seen, outs, scale=None):
     cu = prefix(news)
     exp, weight, score = oc.attend(q, table, lens, cu, scale=scale, seen=seen)
-    got = out.cpu().double()
-    assert torch.equal(got.isnan(), exp.isnan()), f"NaN: {int(got.isnan().sum())}, {int(exp.isnan().sum())}"
     vs = cache.v_scale[cache.v_scale.isfinite()]
-    off = (got - exp).abs()
-    ok = (off <= bound(exp, weight, score, lens, cache.d, q.dtype, vs.clamp_max(2.0 ** 30))) | exp.isnan()
-    assert bool(ok.all()), f"{int((~ok).sum())} of {ok.numel()} outputs are off, by up to {float(off.nan_to_num().max())}"
+    may = bound(exp, weight, score, lens, cache.d, q.dtype, vs.clamp_max(2.0 ** 30))
+    for out in outs:
+        got = out.cpu().double()
+        assert torch.equal(got.isnan(), exp.isnan()), f"NaN: {int(got.isnan().sum())}, {int(exp.isnan().sum())}"
+        off = (got - exp).abs()
+        ok = (off <= may) | exp.isnan()
+        assert bool(ok.all()), f"{int((~ok).sum())} of {ok.numel()} outputs are off, by up to {float(off.nan_to_num().max())}"
 
 
-def crowd(table, lens, news, empty):
-    """With that many empty sequences behind them: so many more workgroups that rows past 32 a KV head go to the tile kernel."""
-    return table + [[-1] * len(table[0])] * empty, lens + [0] * empty, news + [0] * empty
+def crowd(table, lens, news, empty, page):
+    """With that many empty sequences behind them, which choose the kernel: so many more workgroups, and a table of 1000 tokens."""
+    wide = [row + [-1] * (-(-1000 // page) - len(row)) for row in table]
+    return wide + [[-1] * len(wide[0])] * empty, lens + [0] * empty, news + [0] * empty
+
+
+def forms(cache, table, lens, news, q):
+    """(table, lens, news, max_kv) for more than 16 rows a KV head: blocks of 16 and of 32 side by side and whole tiles of rows,
+    as far as their number allows."""
+    yield table, lens, news, None
+    if max(news) * q.shape[1] > 16 * cache.k.shape[1]:
+        for empty, max_kv in ((120, 1000), (600, 300)):
+            yield *crowd(table, lens, news, empty, cache.k.shape[2]), max_kv
 
 
 def run_window(ops, cache, q, table, lens, news, window, sinks, oc=None, scale=None, **hints):
     oc = oc or oracle.Cache(cache.k, cache.v, cache.k_scale, cache.v_scale)
-    out = torch.full(q.shape, float("nan"), dtype=q.dtype, device="cuda")
-    more = {} if news == [1] * len(news) else {"cu_q": i32(prefix(news)), "max_q": max(max(news), 1)}
-    ops.gqa_kv8_window(q.cuda(), cache, i32(table), i32(lens), window, sinks, scale=scale, out=out, **{**more, **hints})
-    compare(cache, oc, q, table, lens, news, in_window(lens, news, window, sinks), out, scale)
-    if max(news) * q.shape[1] > 32 * cache.k.shape[1] and not hints:
-        t, l, n = crowd(table, lens, news, 600)
-        tiles = torch.full(q.shape, float("nan"), dtype=q.dtype, device="cuda")
-        ops.gqa_kv8_window(q.cuda(), cache, i32(t), i32(l), window, sinks, i32(prefix(n)), max(news), 300, scale, tiles)
-        compare(cache, oc, q, table, lens, news, in_window(lens, news, window, sinks), tiles, scale)
+    outs = []
+    for t, l, n, max_kv in forms(cache, table, lens, news, q):
+        outs.append(torch.full(q.shape, float("nan"), dtype=q.dtype, device="cuda"))
+        more = {} if n == [1] * len(n) else {"cu_q": i32(prefix(n)), "max_q": max(max(n), 1)}
+        ops.gqa_kv8_window(q.cuda(), cache, i32(t), i32(l), window, sinks, scale=scale, out=outs[-1],
+                           **{"max_kv": max_kv, **more, **hints})
+    compare(cache, oc, q, table, lens, news, in_window(lens, news, window, sinks), outs, scale)
 
 
 def run_tree(ops, cache, q, table, lens, news, masks, words=None, oc=None, scale=None, **hints):
     oc = oc or oracle.Cache(cache.k, cache.v, cache.k_scale, cache.v_scale)
     words = words or max(1, -(-max(news) // 64))
-    out = torch.full(q.shape, float("nan"), dtype=q.dtype, device="cuda")
-    ops.gqa_kv8_tree(q.cuda(), cache, i32(table), i32(lens), words_of(masks, words), i32(prefix(news)),
-                     **{"max_q": max(news), **hints}, scale=scale, out=out)
+    outs = []
+    for t, l, n, max_kv in forms(cache, table, lens, news, q):
+        outs.append(torch.full(q.shape, float("nan"), dtype=q.dtype, device="cuda"))
+        ops.gqa_kv8_tree(q.cuda(), cache, i32(t), i32(l), words_of(masks, words), i32(prefix(n)),
+                         **{"max_q": max(n), "max_kv": max_kv, **hints}, scale=scale, out=outs[-1])
     cut = [[r & (1 << 64 * words) - 1 for r in seq] for seq in masks]
-    compare(cache, oc, q, table, lens, news, in_tree(lens, news, cut), out, scale)
-    if max(news) * q.shape[1] > 32 * cache.k.shape[1] and not hints:
-        t, l, n = crowd(table, lens, news, 600)
-        tiles = torch.full(q.shape, float("nan"), dtype=q.dtype, device="cuda")
-        ops.gqa_kv8_tree(q.cuda(), cache, i32(t), i32(l), words_of(masks, words), i32(prefix(n)), max(news), 300, scale, tiles)
-        compare(cache, oc, q, table, lens, news, in_tree(lens, news, cut), tiles, scale)
+    compare(cache, oc, q, table, lens, news, in_tree(lens, news, cut), outs, scale)
 
 
 def random_masks(rng, news):
@@ -152,18 +159,18 @@ def test_split_keys_of_tiles(ops, d, page):
     table = tables(lens, page, cache.pages, 61)
     q = randn((sum(news), 4, d), 62, BF16)
     oc = oracle.Cache(cache.k, cache.v, cache.k_scale, cache.v_scale)
-    t, l, n = crowd(table, lens, news, empty)
+    t, l, n = crowd(table, lens, news, empty, page)
     t, l, cu = i32(t), i32(l), i32(prefix(n))
     assert ops.gqa_kv8_window_workspace_bytes(140, 98, 64, 5000, 4, 1, d, 2500, 100) > 0
     assert ops.gqa_kv8_tree_workspace_bytes(140, 98, 64, 5000, 4, 1, d) > 0
     for window, sinks in ((2500, 100), (4000, 0)):
         out = torch.full(q.shape, float("nan"), dtype=BF16, device="cuda")
         ops.gqa_kv8_window(q.cuda(), cache, t, l, window, sinks, cu, 64, 5000, 0.02, out)
-        compare(cache, oc, q, table, lens, news, in_window(lens, news, window, sinks), out, 0.02)
+        compare(cache, oc, q, table, lens, news, in_window(lens, news, window, sinks), [out], 0.02)
     masks = random_masks(random.Random(9), news)
     out = torch.full(q.shape, float("nan"), dtype=BF16, device="cuda")
     ops.gqa_kv8_tree(q.cuda(), cache, t, l, words_of(masks, 1), cu, 64, 5000, 0.02, out)
-    compare(cache, oc, q, table, lens, news, in_tree(lens, news, masks), out, 0.02)
+    compare(cache, oc, q, table, lens, news, in_tree(lens, news, masks), [out], 0.02)
 
 
 @pytest.mark.parametrize("group,n", [(1, 1), (4, 3), (4, 70), (1, 200)])
@@ -204,9 +211,9 @@ def test_window_as_plain_attention(ops):
         cache = filled(ops, 40, 2, 64, page, 13)
         table = tables(lens, page, 40, 14)
         q = randn((sum(news), 2 * group, 64), 15, BF16).cuda()
-        if max(news) * group > 32:
-            table, lens, news = crowd(table, lens, news, 600)
-        args = (i32(prefix(news)), max(news))
+        if max(news) * group > 16:
+            table, lens, news = crowd(table, lens, news, 600, page)
+        args = (i32(prefix(news)), max(news), 300)
         want = ops.gqa_kv8(q, cache, i32(table), i32(lens), *args)
         got = ops.gqa_kv8_window(q, cache, i32(table), i32(lens), 2 ** 31 - 1, 0, *args)
         assert torch.equal(got, want)
@@ -305,11 +312,12 @@ def test_tree_of_one_branch(ops):
         table = tables(lens, page, 20, 30)
         q = randn((3 * n, 2 * group, 128), 31, BF16).cuda()
         tree = drafts.masks(list(range(-1, n - 1))).repeat(3, 1).cuda()
-        if n * group > 32:
-            table, lens, news = crowd(table, lens, news, 600)
-        want = ops.gqa_kv8(q, cache, i32(table), i32(lens), i32(prefix(news)), n)
-        assert torch.equal(ops.gqa_kv8_tree(q, cache, i32(table), i32(lens), tree, i32(prefix(news)), n), want)
-        assert torch.equal(ops.gqa_kv8_tree(q, cache, i32(table), i32(lens), tree[:, 0].contiguous(), i32(prefix(news)), n), want)
+        if n * group > 16:
+            table, lens, news = crowd(table, lens, news, 600, page)
+        args = (i32(prefix(news)), n, 300)
+        want = ops.gqa_kv8(q, cache, i32(table), i32(lens), *args)
+        assert torch.equal(ops.gqa_kv8_tree(q, cache, i32(table), i32(lens), tree, *args), want)
+        assert torch.equal(ops.gqa_kv8_tree(q, cache, i32(table), i32(lens), tree[:, 0].contiguous(), *args), want)
 
 
 def test_tree_bad_numbers(ops):

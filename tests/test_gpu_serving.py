@@ -60,7 +60,7 @@ def test_a_drafted_tree_is_verified(ops, dtype, n_q, n_kv, d, page):
     q, k, v = project(sum(news), [*range(37), *range(90)], 5)
     table, lens = append(seqs, news, k, v)
     out = ops.gqa_kv8_window(q, cache, table.cuda(), lens.cuda(), window, sinks, i32(prefix(news)), max(news))
-    compare(cache, mirror, q, table.tolist(), lens.tolist(), news, in_window(lens.tolist(), news, window, sinks), out)
+    compare(cache, mirror, q, table.tolist(), lens.tolist(), news, in_window(lens.tolist(), news, window, sinks), [out])
 
     parents = [[-1, 0, 0, 1, 2, 2, 4], [-1, 0, 1, 1, 0, 4, 5, 5, 6, 6, 6, 2, 11]]
     base, news = news, [len(p) for p in parents]
@@ -71,7 +71,7 @@ def test_a_drafted_tree_is_verified(ops, dtype, n_q, n_kv, d, page):
     tree = torch.cat([drafts.masks(p) for p in parents]).cuda()
     out = ops.gqa_kv8_tree(q, cache, table.cuda(), lens.cuda(), tree, i32(prefix(news)), max(news))
     rows = [drafts.masks(p)[:, 0].tolist() for p in parents]
-    compare(cache, mirror, q, table.tolist(), lens.tolist(), news, in_tree(lens.tolist(), news, rows), out)
+    compare(cache, mirror, q, table.tolist(), lens.tolist(), news, in_tree(lens.tolist(), news, rows), [out])
     logits = ops.linear_int8(out.flatten(1), gpu[2], gpu[3])
     children = [[i for i, p in enumerate(ps) if p == t] for ps in parents for t in range(len(ps))]
     drafted = torch.randint(0, vocab, (sum(news),), generator=torch.Generator().manual_seed(7))
@@ -94,7 +94,7 @@ def test_a_drafted_tree_is_verified(ops, dtype, n_q, n_kv, d, page):
     table, lens = append(seqs, [1, 1], k, v)
     check_attend(ops, cache, q.cpu(), table.tolist(), lens.tolist(), [1, 1])
     out = ops.gqa_kv8_window(q, cache, table.cuda(), lens.cuda(), window, sinks)
-    compare(cache, mirror, q, table.tolist(), lens.tolist(), [1, 1], in_window(lens.tolist(), [1, 1], window, sinks), out)
+    compare(cache, mirror, q, table.tolist(), lens.tolist(), [1, 1], in_window(lens.tolist(), [1, 1], window, sinks), [out])
 
 
 def test_a_captured_step(ops):

@@ -119,9 +119,12 @@ def test_attention_plans(tmp_path):
             if (!fits || !whole || (p.splits > 1 && (long long)(p.splits - 1) * p.chunk >= kv) || (p.waves == 4 && d != 64))
               printf("tree_plan(%d, %d, %d, %d, %d)\n", B, T, kv, G, d);
           }
-  for (int d : {64, 128}) {  // many sequences, of 300 tokens or of more blocks: tiles, which split long contexts
-    const Plan a = tree_plan(603, 98, 64, 300, 4, 1, d), b = tree_plan(140, 98, 64, 5000, 4, 1, d), c = tree_plan(1, 13, 13, 1001, 32, 8, d);
-    if (a.nr || a.splits != 1 || b.nr || b.splits < 2 || c.nr != 2 || c.blocks != 2) printf("d %d\n", d);
+  for (int d : {64, 128}) {  // tiles, which split long contexts, blocks of 16 and of 32, one block of 32
+    const Plan a = tree_plan(603, 98, 64, 300, 4, 1, d), b = tree_plan(140, 98, 64, 5000, 4, 1, d);
+    const Plan c = tree_plan(1, 13, 13, 1001, 32, 8, d), e = tree_plan(123, 39, 13, 1000, 4, 1, d), f = tree_plan(123, 24, 8, 4000, 4, 1, d);
+    if (a.nr || a.splits != 1 || b.nr || b.splits < 2 || c.nr != 1 || c.blocks != 4 || e.nr != 2 || e.blocks != 2 || f.nr != 2 ||
+        f.blocks != 1)
+      printf("d %d\n", d);
   }
   printf("ok\n");""")
     assert window == ["ok"] and tree == ["ok"]
