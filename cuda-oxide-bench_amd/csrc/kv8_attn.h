@@ -1282,9 +1282,9 @@ static int launch_tiles(const Args& a, const Plan& p, hipStream_t s) {
   return MX_OK;
 }
 
-// The plan of a tree: up to 256 rows of 64 channels take workgroups of 4 waves, two of which a CU holds (33 sequences of up to
-// 2000 tokens, 16 heads with up to 100 rows each 87 -> 62 us, with up to 50 83 -> 53; 128 channels' stages fill a CU with one:
-// one workgroup of 8 waves).
+// The plan of a tree: in tiles, up to 256 rows of 64 channels take workgroups of 4 waves, two of which a CU holds (33 sequences
+// of 500 tokens, 16 heads with up to 100 rows each 41 -> 31 us, of 2000 with up to 200 104 -> 91; 128 channels' stages fill a CU
+// with one: one workgroup of 8 waves).
 static Plan tree_plan(int B, int T, int max_q, int max_kv, int n_q, int n_kv, int d) {
   Plan p = plan(B, T, max_q, max_kv, n_q, n_kv, d);
   const long long rows = (long long)(max_q < T ? max_q : T) * (n_q / n_kv), heads = (long long)B * n_kv;
