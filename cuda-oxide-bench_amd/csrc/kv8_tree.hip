@@ -18,7 +18,7 @@ extern "C" int mx_gqa_kv8_tree(const void* q, const void* k_cache, const void* v
   const int rc = check_call(q, k_cache, v_cache, k_scale, v_scale, page_table, kv_lens, cu, O, B, T, max_q, max_kv, n_q,
                             n_kv, d, page, pages, max_pages, q_stride, dtype);
   if (rc != MX_OK) return rc;
-  if (words < 1 || 2 * words > kMostWords) return MX_ERR_SHAPE;
+  if (words < 1 || words > kMostWords / 2) return MX_ERR_SHAPE;
   if ((uintptr_t)tree & 7) return MX_ERR_ALIGN;
   const Plan p = tree_plan(B, T, max_q, max_kv, n_q, n_kv, d);
   const Args a{(const uint16_t*)q, (const uint8_t*)k_cache, (const uint8_t*)v_cache, k_scale, v_scale, page_table, kv_lens,

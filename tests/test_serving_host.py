@@ -163,3 +163,10 @@ def test_operators_refuse_before_the_device():
     for positions, rot in ((0, 32), (8, 24), (8, 0)):
         with pytest.raises(ValueError, match="multiple of 16"):
             ops.rope_table(positions, rot, device="cpu")
+
+
+@pytest.mark.parametrize("words", [(1 << 30) + 1, (1 << 30) + 8, (1 << 31) - 1])
+def test_tree_words_past_half_of_an_int(words):
+    """Counts whose double, in words of 32 bits, leaves an int's range: refused like any other past 16."""
+    args = [P[0]] * 10 + [2, 5, 4, 4096, 4, 2, 64, 16, 9, 300, 256, 0.1, words, 0, P[0], 1 << 30, None]
+    assert _lib.load().mx_gqa_kv8_tree(*args) == _lib.MX_ERR_SHAPE
