@@ -864,6 +864,7 @@ def gqa_kv8_window(q, cache, page_table, kv_lens, window, sinks=0, cu_q=None, ma
                    out=None, workspace=None):
     """gqa_kv8 with a sliding window and sinks: a row at place p (its sequence's rows are its last
     tokens) sees the tokens t <= p with p - t < window, and the sequence's first `sinks`.  -> [T, n_q, d].
+    Places, not branches: of a drafted tree's rows it would show each those of the other branches before it.
 
     window >= 1 counts the row's own token; a window or sinks past the sequence hide nothing.  Pages on which no row
     sees a token are not read: their numbers in the table may be -1 or another sequence's.  The other

@@ -424,7 +424,8 @@ size_t mx_gqa_kv8_workspace(int B, int T, int max_q, int max_kv, int n_q, int n_
 /*
  * mx_gqa_kv8 where a row sees the last `window` tokens up to its own place and the sequence's first
  * `sinks`: row i of n_b, at place p = kv_lens[b] - n_b + i, sees the tokens t <= p with p - t < window or
- * t < sinks.  window >= 1, sinks >= 0; one that passes the sequence hides nothing.  Pages on which no
+ * t < sinks: by places, so rows must be consecutive tokens, not a tree's.  window >= 1,
+ * sinks >= 0; one that passes the sequence hides nothing.  Pages on which no
  * row of the call sees a token are not read, and what the table and the pages hold for them does not count: a
  * caller may have given them back.  Rows, hints, sizes, ranges, types and workspace
  * (mx_gqa_kv8_window_workspace bytes) as for mx_gqa_kv8.

@@ -33,3 +33,11 @@ def test_operators_with_a_workspace_are_named():
              and "workspace" in inspect.signature(f).parameters and n.startswith(("linear_int8", "gqa_kv8", "token_"))]
     assert len(takes) == 5
     assert [n for n in takes if n not in spans or f"{n}_workspace_bytes" not in spans] == []
+
+
+def test_trees_and_windows_are_apart():
+    """The windowed form's mask goes by places: rows of a drafted tree would see drafts that are not their ancestors."""
+    drafted = [code for code in BLOCKS if "ops.gqa_kv8_tree(" in code]
+    assert drafted and not any("ops.gqa_kv8_window(" in code for code in drafted)
+    assert any("ops.gqa_kv8_window(" in code for code in BLOCKS)
+    assert "tree" in import_submodule("ops").gqa_kv8_window.__doc__
