@@ -896,8 +896,11 @@ def gqa_kv8_tree(q, cache, page_table, kv_lens, tree, cu_q=None, max_q=None, max
     them, and of them the j-th where bit j of its mask is set: tree [T] or [T, words] int64, bit j % 64 of word j // 64,
     up to 16 words (drafts.masks makes them of the tokens' parents).  Nothing is added to a mask, and drafted
     tokens behind its bits are not seen.  A row that sees nothing gives zeros.  The other arguments as for
-    gqa_kv8; `workspace` at least gqa_kv8_tree_workspace_bytes for the same hints.  Of the drafted tokens those that are
-    kept are appended again, from the first one's place on (kv8_append): they then lie as decoded ones do."""
+    gqa_kv8; `workspace` at least gqa_kv8_tree_workspace_bytes for the same hints.  The drafted
+    tokens that are kept are appended again, from the first one's place on (kv8_append).  A page that held tokens
+    before the drafts keeps the scales that rejected ones raised, its tokens rounded to them: draft on a fork of the
+    sequence (KVPages.fork, whose extend copies that page) and append the kept ones to the sequence itself where it
+    must hold what decoding them would have left."""
     out, B, T, n_q, cu, max_q, hint, most, qs, scale = _check_attend(q, cache, page_table, kv_lens, cu_q, max_q, max_kv,
                                                                      scale, out)
     if not _is(tree, torch.int64, 2, cache._device):
