@@ -465,7 +465,8 @@ size_t mx_gqa_kv8_tree_workspace(int B, int T, int max_q, int max_kv, int n_q, i
  * the device.  A token whose position is outside 0..rows-1 is left as it is (in q_out and k_out).
  * q_out may be q and k_out k (same pointer and stride); any other overlap of an
  * output with q, k or the other output returns MX_ERR_ALIAS.  x^2 is summed in fp32: a head whose
- * squares pass 2^128 becomes zeros (NaN where it holds an infinity or a NaN).
+ * squares pass 2^128 becomes zeros (NaN where it holds an infinity or a NaN); small heads and an eps of 0 or
+ * below fp32's normal numbers are as by the formula (a head of zeros without eps: NaN).
  * d a multiple of 16 up to 256, rot a multiple of 16 up to d; T * (n_q + n_kv) < 2^31; strides % 8 == 0,
  * 16-byte aligned pointers (positions: 4).
  * No counterpart in the reference (its attention takes rotated queries and keys).

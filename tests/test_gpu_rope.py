@@ -172,3 +172,28 @@ def test_graph_and_streams(ops):
         g.replay()
         torch.cuda.synchronize()
         assert torch.equal(qo, want[0]) and torch.equal(ko, want[1])
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("neighbours", [False, True])
+@pytest.mark.parametrize("d", [32, 80, 256])
+@pytest.mark.parametrize("eps", [0.0, 2.0 ** -140, 2.0 ** -101, 2.0 ** -99])
+def test_small_heads(ops, dtype, neighbours, d, eps):
+    """Heads whose mean square lies below fp32's normal numbers, down to the type's smallest values, beside heads of one and
+    of zeros, with and without an eps of that size."""
+    announce(f"qk_norm_rope small heads d{d} {neighbours} eps{eps} {dtype}")
+    least = 2.0 ** -133 if dtype == BF16 else 2.0 ** -24
+    x = randn((1, 12, d), 20, dtype)
+    for h, e in enumerate([-50, -55, -62, -64, -66, -70, -80, -110, -126]):
+        x[0, h] = (x[0, h].double() * 2.0 ** e).to(dtype)
+    x[0, 9] = 0.0
+    x[0, 9, 3] = least
+    x[0, 10] = least
+    x[0, 11] = 0.0
+    w, table = randn((d,), 21, dtype), table_of(1, 16)
+    got, _ = ops.qk_norm_rope(x.cuda(), x.cuda(), w.cuda(), w.cuda(), table.cuda(), i32([0]), eps=eps, neighbours=neighbours)
+    got = got.cpu().double()
+    exp, weight = oracle.norm_rope(x, w, table, [0], eps, neighbours)  # (0 / 0 without an eps: NaN)
+    assert torch.equal(got.isnan(), exp.isnan())
+    off = (got - exp).abs()
+    assert bool((off <= bound(exp, weight, d, dtype))[~exp.isnan()].all()), float(off.nan_to_num().max())
