@@ -170,3 +170,21 @@ def test_tree_words_past_half_of_an_int(words):
     """Counts whose double, in words of 32 bits, leaves an int's range: refused like any other past 16."""
     args = [P[0]] * 10 + [2, 5, 4, 4096, 4, 2, 64, 16, 9, 300, 256, 0.1, words, 0, P[0], 1 << 30, None]
     assert _lib.load().mx_gqa_kv8_tree(*args) == _lib.MX_ERR_SHAPE
+
+
+def test_windows_of_one_workgroup(tmp_path):
+    """The rule for one workgroup on both head sizes, past what the causal form keeps to one; what a tile block visits past the
+    count that sizes the splits."""
+    out = query(tmp_path, "kv8_window.hip", r"""
+  using namespace mx::kv8;
+  for (int d : {64, 128})
+    for (int w = 1; w < 3000; ++w)
+      for (int s : {0, 4, 100}) {
+        const Plan p = window_plan(1, 1, 1, 100000, 8, 2, d, w, s);
+        const long long kv = 64 * (up(s, 64) + up(w + 63, 64));
+        if ((p.splits == 1) != (kv * d <= 65536 + 8192)) printf("d %d window %d sinks %d\n", d, w, s);
+        const long long tiles = up(w + 256 + 62, 64) - up(w + 32 + 62, 64);
+        if (tiles < 3 || tiles > 4) printf("window %d: %lld tiles\n", w, tiles);
+      }
+  printf("%d %d\n", window_plan(1, 1, 1, 100000, 8, 2, 64, 1024, 64).splits, window_plan(1, 1, 1, 100000, 8, 2, 128, 449, 64).splits);""")
+    assert out == ["1 1"]
