@@ -188,3 +188,19 @@ def test_windows_of_one_workgroup(tmp_path):
       }
   printf("%d %d\n", window_plan(1, 1, 1, 100000, 8, 2, 64, 1024, 64).splits, window_plan(1, 1, 1, 100000, 8, 2, 128, 449, 64).splits);""")
     assert out == ["1 1"]
+
+
+def test_plans_of_the_wide_forms(tmp_path):
+    """128 channels: split keys in blocks of 32 rows side by side, and tiles with and without a split (as tests on the GPU
+    take them)."""
+    window = query(tmp_path, "kv8_window.hip", r"""
+  using namespace mx::kv8;
+  const Plan a = window_plan(3, 35, 13, 8300, 32, 8, 128, 7000, 100), b = window_plan(140, 98, 64, 5000, 4, 1, 128, 2500, 100);
+  const Plan c = window_plan(602, 140, 70, 300, 4, 1, 128, 150, 20), e = window_plan(602, 400, 200, 300, 1, 1, 128, 150, 20);
+  printf("%d %d %d  %d %d  %d %d  %d %d\n", a.nr, a.blocks, a.splits > 1, b.nr, b.splits > 1, c.nr, c.splits, e.nr, e.splits);""")
+    tree = query(tmp_path, "kv8_tree.hip", r"""
+  using namespace mx::kv8;
+  const Plan a = tree_plan(3, 35, 13, 8300, 32, 8, 128), b = tree_plan(140, 98, 64, 5000, 4, 1, 128);
+  const Plan c = tree_plan(603, 180, 60, 300, 4, 1, 128), e = tree_plan(1, 13, 13, 32768, 32, 8, 128);
+  printf("%d %d %d  %d %d  %d %d  %d %d %d\n", a.nr, a.blocks, a.splits > 1, b.nr, b.splits > 1, c.nr, c.splits, e.nr, e.blocks, e.splits);""")
+    assert window == ["2 2 1  0 1  0 1  0 1"] and tree == ["2 2 1  0 1  0 1  2 2 16"]
