@@ -10,7 +10,9 @@
 // load and store), LPH lanes a head, 64 / LPH heads a wave at a time.  A wave stays with its
 // token, whose cosines and sines it keeps in registers, and with halves as pairs a lane gets the
 // other half's channels from the lane that loaded them.  Stores pass the caches (16384 tokens of 40 heads of 128
-// 59.2 us, 5.8 TB/s; with cached ones 68.4, 1024 tokens 7.5 and not 6.5).
+// 60.3 us, 5.7 TB/s; with cached ones 68.4, 1024 tokens 7.5 and not 6.5.  The append and the attention behind it read the
+// outputs at once, and the three together take as long either way: 1024 tokens 54.8 us and 55.6 with cached stores, 4096
+// 117.3 and 114.6, 16384 422 and 420).
 #include <algorithm>
 
 #include "mx_common.h"
