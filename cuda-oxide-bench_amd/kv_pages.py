@@ -104,7 +104,9 @@ class KVPages:
         return copies
 
     def truncate(self, seq: int, tokens: int) -> None:
-        """Drops the sequence's tokens from `tokens` on (rejected ones), and the pages that only they were on."""
+        """Drops the sequence's tokens from `tokens` on (rejected ones), and the pages that only they were on.  The page
+        that they shared with the tokens before them keeps the scales that they raised: extending a fork() instead
+        leaves that page as it was."""
         entry = self._of(seq)
         if not 0 <= tokens <= entry[1]:
             raise ValueError(f"tokens ({tokens}) must be 0 to {entry[1]}")
